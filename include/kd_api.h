@@ -346,6 +346,119 @@ int kd_cached_attention(int dtype, void* out, const void* q, const int64_t* q_st
                         const int64_t* k_strides, const void* v, const int64_t* v_strides, int64_t batch,
                         int64_t heads, int64_t length, int64_t keys, int64_t head_dim);
 
+/* ---- a paged key / value cache held in 8 bits (no reference counterpart) ---------------------- */
+
+/* kael keeps each layer's cached keys and values as f32 tensors of one sequence, grown by `cat`
+ * (reference src/nn/transformer.cpp:119-126). For several sequences of unlike lengths the cache is
+ * a pool of pages instead, each of `page_size` positions, which the sequences' tables hand out; a
+ * value is one signed byte times the f32 scale of its page and head.
+ *   keys          [pages][kv_heads][page_size][head_dim]
+ *   values        [pages][kv_heads][head_dim][page_size]
+ *   key_scales, value_scales  [pages][kv_heads]
+ * contiguous device memory; keys and values 16-byte aligned, the scales 4-byte. page_size is 16, 32,
+ * 64, 128 or 256 and head_dim 64 or 128 (KD_E_UNSUPPORTED otherwise). */
+typedef struct kd_paged_cache {
+    int8_t* keys;
+    int8_t* values;
+    float* key_scales;
+    float* value_scales;
+    int64_t pages;
+    int64_t kv_heads;
+    int64_t page_size;
+    int64_t head_dim;
+} kd_paged_cache;
+
+/* `sequences` ragged sequences with `tokens` rows of new tokens between them (device arrays): sequence
+ * s has the rows starts[s] .. starts[s + 1] - 1 (starts ascending, sequences + 1 entries) and, these
+ * counted, lengths[s] positions, so its row starts[s] + i stands at position
+ * lengths[s] - (starts[s + 1] - starts[s]) + i. Position p lies in page
+ * table[s * table_columns + p / page_size], slot p % page_size. The calls read these arrays when their
+ * kernels run, so a captured graph follows their contents. A table entry outside 0 .. pages - 1 is no page, and
+ * neither have positions below 0 or from table_columns * page_size on one: nothing is written there, and
+ * attention does not see it. Rows outside every sequence are left as they were. starts is clamped to
+ * 0 .. tokens. table_columns * page_size stays below 2^30, tokens * heads and the pages' number below 2^31. */
+typedef struct kd_paged_batch {
+    const int64_t* table;
+    const int64_t* starts;
+    const int64_t* lengths;
+    int64_t sequences;
+    int64_t table_columns;
+    int64_t tokens;
+} kd_paged_batch;
+
+/* The position rotation: with c and s the row of the position in cosines / sines (f32, device,
+ * [positions][features / 2]), the pair (a, b) of features becomes (a c - b s, b c + a s). Pair i is
+ * (i, i + features / 2), or (2 i, 2 i + 1) if interleaved; features from `features` on stay.
+ * features is even, 0 .. head_dim; 0 rotates nothing. A position with no row in the tables turns
+ * into NaN. */
+typedef struct kd_rotation {
+    const float* cosines;
+    const float* sines;
+    int64_t positions;
+    int64_t features;
+    int32_t interleaved;
+} kd_rotation;
+
+/* Appends the batch's new keys and values to the cache, the keys rotated, and writes the rotated
+ * queries: q_out [tokens][heads][head_dim] from q. q, k and v are f32 with element strides of (row,
+ * head) in *_strides, features contiguous (the views of a fused projection's rows, for instance).
+ * q and q_out may both be NULL. rotation may be NULL. Per page and kv head, with x the rotated
+ * values (in 64 bits) that fall into the page:
+ *   scale = max(old scale, f32(max |x| / 127)), the old scale counting as 0 when the page's slot 0 is
+ *           among the slots written now;
+ *   code  = x * (1 / scale) rounded to the nearest integer (ties to even), at most 127 in size;
+ *   codes already in the page's earlier slots become code * (old scale / scale), rounded, where the
+ *   scale grew. Slots past the sequence's end keep what they hold.
+ * A non-finite x makes the scale NaN, and with it every value of that page and head. A page that is
+ * written belongs to one sequence and is in its table once; the same page twice among the written parts
+ * of the tables gives a mixture of their contents. q_out must not overlap q, k or v. */
+int kd_paged_append(int dtype, const kd_paged_cache* cache, const kd_paged_batch* batch, const kd_rotation* rotation,
+                    void* q_out, const void* q, const int64_t* q_strides, int64_t heads, const void* k,
+                    const int64_t* k_strides, const void* v, const int64_t* v_strides);
+
+/* The cached keys and values of the batch's rows as f32, k and v [tokens][kv_heads][head_dim] (either
+ * may be NULL): code * scale, 0 where a position has no page. */
+int kd_paged_read(int dtype, void* k, void* v, const kd_paged_cache* cache, const kd_paged_batch* batch);
+
+/* Causal attention of the batch's rows against the cache, which holds their own positions already:
+ *   out[t][h] = sum over j of softmax_j(scale * q[t][h] . key[j]) * value[j]
+ * over the positions j up to the row's own that have a page; kv head h * kv_heads / heads serves head
+ * h (heads a multiple of kv_heads). A row that sees nothing is 0. q is f32 with element strides (row,
+ * head) in q_strides, features contiguous; out [tokens][heads][head_dim] contiguous, 16-byte aligned,
+ * not overlapping q. Sums and products are exact to about f32's rounding; a non-finite query or scale
+ * gives NaN where it is seen.
+ * max_keys is the largest of `lengths` as far as the host knows it, and only decides how the work is
+ * split; results are right whatever it says. Long caches are split over workgroups whose partial
+ * results pass through `workspace` (device, 16-byte aligned; kd_paged_attention_workspace says how many
+ * bytes are of use). With fewer bytes, or NULL and 0, less is split. Calls that may run at the same time
+ * (streams, graphs) need workspaces of their own. The same arguments and contents give the same bits. */
+int kd_paged_attention(int dtype, void* out, const void* q, const int64_t* q_strides, int64_t heads,
+                       const kd_paged_cache* cache, const kd_paged_batch* batch, double scale, int64_t max_keys,
+                       void* workspace, int64_t workspace_bytes);
+int kd_paged_attention_workspace(int64_t* bytes, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t sequences,
+                                 int64_t tokens, int64_t max_keys);
+
+/* ---- drafted tokens ---------------------------------------------------------------------------- */
+
+/* Verifies drafted tokens against the target model's probabilities, so that the tokens kept are
+ * distributed as the target's (no reference counterpart; the pick is kael's multinomial, src/random.cpp:
+ * 117-155). Sequence s has counts[s] (clamped to 0 .. drafts) drafted tokens x_i = drafted[s][i], drawn
+ * from the draft's probabilities q_i = draft[s][i][.], and the target's p_i = target[s][i][.] for
+ * i <= counts[s]. Draft i is accepted while u_i * q_i(x_i) < p_i(x_i), u_i = uniforms[s][i] in [0, 1).
+ * At the first that is not, a token is drawn from max(p_i - q_i, 0) (from p_i if that is 0 everywhere);
+ * if all are accepted, from p_counts[s]. That draw uses uniforms[s][drafts]: the first entry whose
+ * running sum exceeds the draw times the sum of all. draft NULL means that the drafts were certain (q_i is 1 at x_i).
+ *   target [sequences][drafts + 1][vocab], draft [sequences][drafts][vocab], drafted [sequences][drafts],
+ *   counts [sequences], uniforms [sequences][drafts + 1] (f64): device, contiguous
+ *   tokens [sequences][drafts + 1]: the accepted tokens, the drawn one, then -1
+ *   accepted [sequences]: how many drafts were accepted
+ * dtype f32 or f64; sums and comparisons in f64. A drafted token outside 0 .. vocab - 1 is never accepted
+ * (its q is 0 everywhere if certain). Where the weights have no finite positive sum the drawn token is -1. drafts may
+ * be 0. */
+int kd_verify_drafts(int dtype, int64_t* tokens, int64_t* accepted, const void* target, const void* draft,
+                     const int64_t* drafted, const int64_t* counts, const double* uniforms, int64_t sequences,
+                     int64_t drafts, int64_t vocab);
+
 /* ---- fused row kernels (extensions replacing composed device paths) ---- */
 
 /* Row softmax over `rows` contiguous rows of `cols`: max, exp(x-max), sum in double,
@@ -373,6 +486,25 @@ int kd_cross_entropy_rows(int dtype, void* losses, const void* logits, const int
  * Follows reference src/ops/nn.cpp:214-240 (CPU only in the reference). */
 int kd_cross_entropy_grad(int dtype, void* out, const void* logits, const int64_t* targets,
                           const void* row_weights, int64_t rows, int64_t cols);
+
+/* Distillation from a teacher's `kept` largest logits of each row (no reference counterpart; the draft
+ * model of kd_verify_drafts is trained with it, beside kd_cross_entropy_rows). With z = logits[r] of `cols`
+ * entries, t = teacher[r][.] and i = indices[r][.] the entries' places, T = temperature:
+ *   pi = softmax(t / T) over the row's kept entries, sigma = softmax(z / T) over all cols
+ *   losses[r] = T^2 * sum over j of pi_j * (log pi_j - log sigma_(i_j))
+ * An index outside 0 .. cols - 1 is no entry (its t is not read into the sums); a row without entries, or
+ * whose t are all -inf, has loss 0. The same index twice counts twice. stats [rows][2] receives each row's max(z) and
+ * sum exp((z - max) / T), which the gradient reads. dtype f32 or f64, rows contiguous, sums in double;
+ * 1 <= kept <= 1024, temperature > 0. */
+int kd_distill_rows(int dtype, void* losses, void* stats, const void* logits, const int64_t* indices,
+                    const void* teacher, int64_t rows, int64_t cols, int64_t kept, double temperature);
+
+/* Its gradient with respect to the logits: out = row_weights[r] * T * (sigma_c * sum(pi) - the pi_j with
+ * i_j = c), sum(pi) being 1, or 0 for a row without entries. stats from kd_distill_rows on the same logits; out may be
+ * logits. */
+int kd_distill_grad(int dtype, void* out, const void* logits, const void* stats, const int64_t* indices,
+                    const void* teacher, const void* row_weights, int64_t rows, int64_t cols, int64_t kept,
+                    double temperature);
 
 /* Backward of kd_softmax_rows over `rows` contiguous rows of `cols`: from the forward output y and
  * the incoming gradient g, out = y * (g - sum(g * y)) (softmax) or out = g - exp(y) * sum(g)

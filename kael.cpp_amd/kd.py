@@ -91,6 +91,21 @@ class AdamTensor(Structure):
                 ("count", c_int64), ("step", c_int64)]
 
 
+class PagedCache(Structure):
+    _fields_ = [("keys", c_void_p), ("values", c_void_p), ("key_scales", c_void_p), ("value_scales", c_void_p),
+                ("pages", c_int64), ("kv_heads", c_int64), ("page_size", c_int64), ("head_dim", c_int64)]
+
+
+class PagedBatch(Structure):
+    _fields_ = [("table", c_void_p), ("starts", c_void_p), ("lengths", c_void_p), ("sequences", c_int64),
+                ("table_columns", c_int64), ("tokens", c_int64)]
+
+
+class Rotation(Structure):
+    _fields_ = [("cosines", c_void_p), ("sines", c_void_p), ("positions", c_int64), ("features", c_int64),
+                ("interleaved", c_int32)]
+
+
 class GptConfig(Structure):
     _fields_ = [("vocab_size", c_int64), ("max_positions", c_int64), ("layers", c_int64), ("heads", c_int64),
                 ("dimension", c_int64), ("tanh_gelu", c_int32), ("flags", c_int32)]
@@ -105,6 +120,11 @@ def params(reals=(0.0, 0.0), integers=(0, 0)) -> ElementParameters:
     p.reals[0], p.reals[1] = float(reals[0]), float(reals[1])
     p.integers[0], p.integers[1] = int(integers[0]), int(integers[1])
     return p
+
+
+def strides(*elements):
+    """Element strides as the int64 array that the strided calls take."""
+    return (c_int64 * len(elements))(*elements)
 
 
 # name -> (restype, argtypes); shared by the backend (prefix kd_) and the oracle (oracle_).
@@ -163,6 +183,18 @@ BACKEND_ONLY = {
     "copy_d2d": (c_int, [c_void_p, c_void_p, c_int64]),
     "matmul": (c_int, [c_int, c_void_p, c_void_p, c_void_p, POINTER(MatmulSizes)]),
     "reduce_noalloc": (c_int, [c_int, c_int, c_int, c_void_p, c_void_p, c_int64, c_int64]),
+    "paged_append": (c_int, [c_int, POINTER(PagedCache), POINTER(PagedBatch), POINTER(Rotation), c_void_p, c_void_p,
+                             POINTER(c_int64), c_int64, c_void_p, POINTER(c_int64), c_void_p, POINTER(c_int64)]),
+    "paged_read": (c_int, [c_int, c_void_p, c_void_p, POINTER(PagedCache), POINTER(PagedBatch)]),
+    "paged_attention": (c_int, [c_int, c_void_p, c_void_p, POINTER(c_int64), c_int64, POINTER(PagedCache),
+                                POINTER(PagedBatch), c_double, c_int64, c_void_p, c_int64]),
+    "paged_attention_workspace": (c_int, [POINTER(c_int64), c_int64, c_int64, c_int64, c_int64, c_int64, c_int64]),
+    "verify_drafts": (c_int, [c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64,
+                              c_int64, c_int64]),
+    "distill_rows": (c_int, [c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int64,
+                             c_double]),
+    "distill_grad": (c_int, [c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int64,
+                             c_int64, c_double]),
     "event_create": (c_int, [POINTER(c_void_p)]),
     "event_destroy": (c_int, [c_void_p]),
     "event_record": (c_int, [c_void_p]),

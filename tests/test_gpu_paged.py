@@ -1,0 +1,281 @@
+"""The paged 8-bit cache (kd_paged_append, kd_paged_read, kd_paged_attention) against its definition in 64 bits
+(tests/paged.py): codes, scales and rotated queries bit for bit, attention within a tolerance derived there.
+"""
+import ctypes
+
+import numpy as np
+import pytest
+
+import kd
+import paged
+
+pytestmark = pytest.mark.gpu
+
+
+def batch_of(new, lengths, first=0, after=0):
+    starts = np.concatenate([[0], np.cumsum(new)]) + first
+    return [int(x) for x in starts], list(lengths), int(starts[-1]) + after
+
+
+def fused(rng, tokens, heads, kv_heads, dim):
+    """q, k, v as views of one projection's rows."""
+    x = rng.normal(0, 1, (tokens, heads + 2 * kv_heads, dim)).astype(np.float32)
+    return x, x[:, :heads], x[:, heads:heads + kv_heads], x[:, heads + kv_heads:]
+
+
+def run_append(kdb, cache, starts, lengths, tokens, x, heads, rotation=None, with_q=True):
+    on = paged.Device(kdb, cache, starts, lengths, tokens)
+    kv, dim = cache.kv_heads, cache.dim
+    dx = kdb.to_device(x)
+    rows = kd.strides(x.shape[1] * dim, dim)
+    q_out = kdb.to_device(np.full((max(tokens, 1), heads, dim), -777.0, np.float32))
+    turn, held = None, []
+    if rotation is not None:
+        held = [kdb.to_device(rotation[0]), kdb.to_device(rotation[1])]
+        turn = kd.Rotation(held[0].ptr, held[1].ptr, len(rotation[0]), rotation[2], int(rotation[3]))
+    size = 4 * dim
+    kdb.call("paged_append", kd.F32, on.c, on.b, turn, q_out.ptr if with_q else None, dx.ptr if with_q else None, rows,
+             heads, dx.ptr + heads * size, rows, dx.ptr + (heads + kv) * size, rows)
+    return on, q_out.numpy()[:tokens]
+
+
+def same_cache(got, want):
+    for name in paged.Cache.NAMES:
+        np.testing.assert_array_equal(getattr(got, name), getattr(want, name), err_msg=name)
+
+
+# new tokens of each sequence, its length with them, kv heads, heads, page, dim
+APPENDS = [
+    ([1], [1], 1, 1, 16, 64), ([1], [16], 1, 2, 16, 64), ([1], [17], 2, 2, 16, 128), ([16], [16], 3, 3, 16, 64),
+    ([17, 0, 5], [40, 7, 5], 2, 4, 16, 64), ([1] * 9, [1, 2, 15, 16, 17, 31, 32, 33, 48], 2, 6, 16, 64),
+    ([70, 3], [133, 64], 1, 3, 64, 128), ([130], [260], 2, 2, 128, 64), ([1, 300, 2], [256, 300, 513], 1, 1, 256, 128),
+    ([33, 31], [33, 63], 12, 12, 32, 64),
+]
+
+
+@pytest.mark.parametrize("interleaved", [False, True], ids=["halves", "pairs"])
+@pytest.mark.parametrize("case", APPENDS, ids=[f"{sum(a[0])}x{a[2]}p{a[4]}d{a[5]}" for a in APPENDS])
+def test_append_is_its_definition(kdb, case, interleaved):
+    new, lengths, kv, heads, page, dim = case
+    rng = np.random.default_rng(hash((tuple(new), kv, page)) % 1000)
+    starts, lengths, tokens = batch_of(new, lengths)
+    cache = paged.Cache(rng, len(new), -(-max(lengths) // page) + 1, kv, page, dim, spare=2)
+    x, q, k, v = fused(rng, tokens, heads, kv, dim)
+    x[:, heads:] *= rng.choice([0.1, 1, 10], (tokens, 2 * kv, 1))  # scales that grow and that stay
+    features = dim if not interleaved else dim // 2
+    rotation = (*paged.tables(max(lengths), features), features, interleaved)
+    on, q_out = run_append(kdb, cache, starts, lengths, tokens, x, heads, rotation)
+    want, want_q = paged.append(cache, starts, lengths, q, k, v, rotation)
+    np.testing.assert_array_equal(q_out, want_q)
+    same_cache(on.read_back(), want)
+    # once more with the same tokens: nothing changes
+    again = paged.Device(kdb, on.read_back(), starts, lengths, tokens)
+    same_cache(run_append(kdb, again.cache, starts, lengths, tokens, x, heads, rotation)[0].read_back(), want)
+
+
+def test_append_without_rotation_queries_or_pages(kdb):
+    """No rotation and no queries; positions without a page, before the first or past the table, are not written; rows
+    before the first and behind the last sequence are left alone."""
+    rng = np.random.default_rng(3)
+    new, lengths = [5, 20, 4, 9], [3, 40, 70, 9]
+    starts, lengths, tokens = batch_of(new, lengths, first=3, after=6)
+    cache = paged.Cache(rng, 4, 3, 2, 16, 64)
+    cache.table[1, 1] = -1
+    cache.table[3, 0] = cache.pages + 5
+    x, q, k, v = fused(rng, tokens, 4, 2, 64)
+    on, q_out = run_append(kdb, cache, starts, lengths, tokens, x, 4, with_q=False)
+    want, want_q = paged.append(cache, starts, lengths, q, k, v)
+    same_cache(on.read_back(), want)
+    assert (q_out == -777).all()
+    on, q_out = run_append(kdb, cache, starts, lengths, tokens, x, 4)
+    np.testing.assert_array_equal(q_out, want_q)
+    same_cache(on.read_back(), want)
+
+
+def test_append_of_what_is_not_finite_or_zero(kdb):
+    rng = np.random.default_rng(4)
+    starts, lengths, tokens = batch_of([20, 3, 2], [20, 19, 18])
+    cache = paged.Cache(rng, 3, 2, 2, 16, 64)
+    x, q, k, v = fused(rng, tokens, 2, 2, 64)
+    x[3, 2, 5], x[17, 5, 0] = np.inf, np.nan  # a key of head 0's first page, a value of head 1's second
+    x[20:23, 2:] = 0                          # zeros into a page that holds codes
+    x[23:25] = 1e-42                          # below the least scale's reach
+    on, _ = run_append(kdb, cache, starts, lengths, tokens, x, 2)
+    want, _ = paged.append(cache, starts, lengths, q, k, v)
+    same_cache(on.read_back(), want)
+    assert np.isnan(want.key_scales).sum() == 1 and np.isnan(want.value_scales).sum() == 1
+
+
+def test_a_position_past_the_rotation_tables_turns_into_nan(kdb):
+    rng = np.random.default_rng(5)
+    starts, lengths, tokens = batch_of([6], [20])
+    cache = paged.Cache(rng, 1, 2, 1, 16, 64)
+    x, q, k, v = fused(rng, tokens, 1, 1, 64)
+    rotation = (*paged.tables(18, 32), 32, False)
+    on, q_out = run_append(kdb, cache, starts, lengths, tokens, x, 1, rotation)
+    want, want_q = paged.append(cache, starts, lengths, q, k, v, rotation)
+    np.testing.assert_array_equal(q_out, want_q)
+    same_cache(on.read_back(), want)
+    assert np.isnan(q_out[4:, :, :32]).all() and np.isfinite(q_out[:4]).all()
+
+
+@pytest.mark.parametrize("page,dim", [(16, 64), (64, 128), (256, 64)])
+def test_read_gives_the_values(kdb, page, dim):
+    rng = np.random.default_rng(page)
+    starts, lengths, tokens = batch_of([7, 0, 90, 4], [20, 5, 90, 2], first=1, after=3)
+    cache = paged.Cache(rng, 4, -(-90 // page), 3, page, dim)
+    cache.table[0, 0] = -1 if page == 16 else cache.table[0, 0]
+    on = paged.Device(kdb, cache, starts, lengths, tokens)
+    want = {n: np.full((tokens, 3, dim), -777, np.float32) for n in ("keys", "values")}
+    for s, length in enumerate(lengths):
+        n = starts[s + 1] - starts[s]
+        for i in range(n):
+            position = length - n + i
+            at = cache.page_at(s, position)
+            row, slot = starts[s] + i, position % page
+            want["keys"][row] = cache.keys[at, :, slot] * cache.key_scales[at][:, None] if at >= 0 else 0
+            want["values"][row] = cache.values[at, :, :, slot] * cache.value_scales[at][:, None] if at >= 0 else 0
+    for skipped in (None, "keys", "values"):
+        got = {n: kdb.to_device(np.full((tokens, 3, dim), -777, np.float32)) for n in want}
+        ptr = {n: None if n == skipped else got[n].ptr for n in want}
+        kdb.call("paged_read", kd.F32, ptr["keys"], ptr["values"], on.c, on.b)
+        for n in want:
+            np.testing.assert_array_equal(got[n].numpy(), np.full_like(want[n], -777) if n == skipped else want[n])
+
+
+# ---- attention ------------------------------------------------------------------------------------
+
+
+def run_attention(kdb, on, q, scale, max_keys, workspace=None, strides=None, out=None):
+    tokens, heads, dim = q.shape
+    dq = kdb.to_device(q)
+    out = out or kdb.to_device(np.full(q.shape, -777, np.float32))
+    n = workspace.nbytes if workspace is not None else 0
+    kdb.call("paged_attention", kd.F32, out.ptr, dq.ptr, strides or kd.strides(heads * dim, dim), heads, on.c, on.b,
+             scale, max_keys, workspace.ptr if n else None, n)
+    return out.numpy()
+
+
+def workspace_for(kdb, heads, kv_heads, dim, sequences, tokens, max_keys):
+    n = ctypes.c_int64()
+    kdb.call("paged_attention_workspace", ctypes.byref(n), heads, kv_heads, dim, sequences, tokens, max_keys)
+    return kdb.empty((max(n.value, 16),), np.uint8)
+
+
+# new tokens, lengths, kv heads, heads, page, dim
+ATTENTION = [
+    ([1], [1], 1, 1, 16, 64), ([1], [64], 1, 1, 16, 64), ([1], [65], 2, 2, 32, 128), ([1], [1000], 3, 3, 16, 64),
+    ([1], [2500], 1, 8, 64, 128), ([1] * 5, [1, 63, 200, 517, 1024], 2, 2, 16, 64), ([5, 3, 1], [5, 300, 77], 2, 6, 32, 64),
+    ([16, 17], [16, 900], 1, 1, 16, 64), ([4, 4], [700, 4], 1, 4, 128, 128), ([5], [600], 1, 4, 64, 64),
+    ([100, 1, 0, 65], [100, 500, 9, 130], 1, 2, 16, 64), ([33], [33], 2, 2, 256, 128), ([257], [300], 1, 1, 64, 64),
+    ([9], [9], 1, 12, 16, 128), ([2] * 70, [2 + 7 * (s % 40) for s in range(70)], 1, 1, 16, 64),
+]
+
+
+@pytest.mark.parametrize("case", ATTENTION, ids=[f"{len(a[0])}s{sum(a[0])}t{max(a[1])}k{a[2]}of{a[3]}p{a[4]}d{a[5]}" for a in ATTENTION])
+def test_attention_is_its_definition(kdb, case):
+    new, lengths, kv, heads, page, dim = case
+    rng = np.random.default_rng(len(new) + sum(lengths))
+    starts, lengths, tokens = batch_of(new, lengths)
+    cache = paged.Cache(rng, len(new), -(-max(lengths) // page), kv, page, dim, spare=1)
+    q = rng.normal(0, 1, (tokens, heads, dim)).astype(np.float32)
+    on = paged.Device(kdb, cache, starts, lengths, tokens)
+    want, tolerance = paged.attention(cache, starts, lengths, q, dim ** -0.5)
+    space = workspace_for(kdb, heads, kv, dim, len(new), tokens, max(lengths))
+    # split as far as the call likes, on wrong hints, on less room, and not at all
+    for hint, room in ((max(lengths), space), (1, space), (1 << 20, space), (max(lengths), None),
+                       (max(lengths), kdb.empty((max(space.nbytes // 2 // 16 * 16, 16),), np.uint8))):
+        got = run_attention(kdb, on, q, dim ** -0.5, hint, room)
+        off = np.abs(got - want)
+        assert (off <= tolerance).all(), (hint, off.max(), (off / np.maximum(tolerance, 1e-30)).max())
+        np.testing.assert_array_equal(run_attention(kdb, on, q, dim ** -0.5, hint, room), got)
+
+
+def test_attention_over_views_and_rows_of_no_sequence(kdb):
+    rng = np.random.default_rng(11)
+    starts, lengths, tokens = batch_of([3, 20], [30, 50], first=2, after=5)
+    cache = paged.Cache(rng, 2, 4, 2, 16, 64)
+    x = rng.normal(0, 1, (4, tokens, 3, 64)).astype(np.float32)  # heads outside the rows, a gap between rows
+    q = np.ascontiguousarray(x[:, :, 1].transpose(1, 0, 2))
+    on = paged.Device(kdb, cache, starts, lengths, tokens)
+    want, tolerance = paged.attention(cache, starts, lengths, q, 0.3)
+    dx, out = kdb.to_device(x), kdb.to_device(np.full(q.shape, -777, np.float32))
+    kdb.call("paged_attention", kd.F32, out.ptr, dx.ptr + 64 * 4, kd.strides(3 * 64, tokens * 3 * 64), 4, on.c, on.b, 0.3,
+             50, None, 0)
+    got = out.numpy()
+    assert (np.abs(got - want) <= tolerance).all()
+    assert (got[:2] == -777).all() and (got[-5:] == -777).all()
+
+
+def test_attention_of_positions_without_a_page(kdb):
+    """Evicted pages, a sequence without any page, lengths past the table, more new tokens than positions."""
+    rng = np.random.default_rng(12)
+    starts, lengths, tokens = batch_of([1, 2, 3, 9], [100, 64, 500, 4])
+    cache = paged.Cache(rng, 4, 8, 2, 16, 64)
+    cache.table[0, [0, 2, 6]] = [-1, cache.pages, 1 << 40]
+    cache.table[1] = -1
+    q = rng.normal(0, 1, (tokens, 4, 64)).astype(np.float32)
+    on = paged.Device(kdb, cache, starts, lengths, tokens)
+    want, tolerance = paged.attention(cache, starts, lengths, q, 0.125)
+    got = run_attention(kdb, on, q, 0.125, 128, workspace_for(kdb, 4, 2, 64, 4, tokens, 128))
+    assert (np.abs(got - want) <= tolerance).all()
+    assert (got[1:3] == 0).all() and (got[6:11] == 0).all()
+
+
+def test_attention_takes_nan_from_what_it_sees_alone(kdb):
+    """A NaN scale, of a page that one row sees and another does not; a query that is not finite."""
+    rng = np.random.default_rng(13)
+    starts, lengths, tokens = batch_of([20, 20], [40, 40])
+    cache = paged.Cache(rng, 2, 3, 1, 16, 64)
+    cache.key_scales[cache.table[0, 2], 0] = np.nan     # positions 32..47: rows 12.. of the first sequence
+    cache.value_scales[cache.table[1, 2], 0] = np.nan
+    q = rng.normal(0, 1, (tokens, 2, 64)).astype(np.float32)
+    q[5, 0, 3], q[6, 1, 63] = np.inf, np.nan
+    on = paged.Device(kdb, cache, starts, lengths, tokens)
+    with np.errstate(invalid="ignore"):
+        want, tolerance = paged.attention(cache, starts, lengths, np.where(np.isfinite(q), q, 0), 0.125)
+    want[5, 0] = want[6, 1] = np.nan
+    want[12:20] = want[32:40] = np.nan
+    got = run_attention(kdb, on, q, 0.125, 40)
+    np.testing.assert_array_equal(np.isnan(got), np.isnan(want))
+    fine = ~np.isnan(want)
+    assert (np.abs(got - want)[fine] <= tolerance[fine]).all()
+
+
+@pytest.mark.parametrize("size", [1e-30, 1e-3, 30.0, 1e30])
+def test_attention_of_small_and_large_queries(kdb, size):
+    """One feature a thousand times the others', queries at both ends of the range, pages of zero and tiny scales."""
+    rng = np.random.default_rng(14)
+    starts, lengths, tokens = batch_of([3], [200])
+    cache = paged.Cache(rng, 1, 13, 1, 16, 64)
+    cache.value_scales[cache.table[0, 3]] = 0
+    cache.key_scales[cache.table[0, 4]] = 0
+    cache.value_scales[cache.table[0, 5]] = 1e-30
+    q = rng.normal(0, 1, (tokens, 2, 64)).astype(np.float32)
+    q[:, :, 7] *= 1000
+    q *= np.float32(size)
+    scale = 1 / (1000 * size)
+    on = paged.Device(kdb, cache, starts, lengths, tokens)
+    want, tolerance = paged.attention(cache, starts, lengths, q, scale)
+    got = run_attention(kdb, on, q, scale, 200)
+    assert (np.abs(got - want) <= tolerance).all()
+
+
+def test_a_prompt_drafts_and_single_tokens_in_turn(kdb):
+    """A cache built by the calls themselves, as a server runs them: prompts, then drafted tokens, then single ones, each
+    step's attention against the definition on the cache as the definition appends to it."""
+    rng = np.random.default_rng(15)
+    kv, heads, page, dim = 2, 4, 16, 64
+    cache = paged.Cache(rng, 3, 5, kv, page, dim)
+    lengths = [0, 0, 0]
+    rotation = (*paged.tables(80, dim), dim, False)
+    for new in ([37, 16, 1], [4, 4, 4], [1, 1, 1], [1, 0, 1], [5, 5, 0]):
+        starts, lengths, tokens = batch_of(new, [a + b for a, b in zip(lengths, new)])
+        x, q, k, v = fused(rng, tokens, heads, kv, dim)
+        on, q_out = run_append(kdb, cache, starts, lengths, tokens, x, heads, rotation)
+        cache, want_q = paged.append(cache, starts, lengths, q, k, v, rotation)
+        same_cache(on.read_back(), cache)
+        np.testing.assert_array_equal(q_out, want_q)
+        want, tolerance = paged.attention(cache, starts, lengths, q_out, dim ** -0.5)
+        got = run_attention(kdb, on, q_out, dim ** -0.5, max(lengths), workspace_for(kdb, heads, kv, dim, 3, tokens, 80))
+        assert (np.abs(got - want) <= tolerance).all()
