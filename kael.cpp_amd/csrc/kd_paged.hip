@@ -205,59 +205,361 @@ __global__ __launch_bounds__(256) void paged_read_kernel(Paged c, float* __restr
 }
 
 // ---- attention ------------------------------------------------------------------------------------
+//
+// Scores and weighted sums run on the signed 8-bit matrix cores, whose sums are exact: the cached codes go in as they
+// are, and the other operand as four signed digits of base 256. A query row is q = 2^(e - 30) * x with x whole, e the
+// exponent of its largest feature (x is exact for features of at least 2^-6 of that one, and off by 2^-31 of it at
+// most otherwise); a weight exp(score - max) times its value scale likewise, against the block's largest scale. Four products a
+// tile and twice bf16's rate are as many cycles as two bf16 products, where three would be needed for f32's bits, and the
+// codes need no conversion.
+//
+// A wave holds 16 rows (queries x the heads that share the kv head) as columns and takes 64 keys at a time:
+//   scores: 4 tiles of 16 keys, S^T = K . Q^T (16x16x64): lane l ends with column l % 16 and, the tiles' rows being dealt
+//     out so, the 16 keys of chunk g = l / 16; a chunk lies in one page, so a lane has one page, key scale and value scale;
+//   weights: their digits are the B operand of the second product as they stand, no lane exchanges anything;
+//   sums: O^T += V^T . P^T, the values' pages holding a feature's 16 tokens side by side.
+// The next block's codes are loaded while the present one is worked on, and the table entries of the one after it.
 
-// One workgroup a (row, head), a key a thread at a time: the scores of 256 keys, then each thread a feature's sum.
-__global__ __launch_bounds__(256) void paged_attention_kernel(Paged c, float* __restrict__ out, Strided q, int heads,
-                                                              float scale) {
-    __shared__ float qs[128], weights[256], parts[8];
-    const int64_t row = blockIdx.x / heads;
-    const int h = blockIdx.x % heads, kv = h / (heads / c.kv_heads);
-    const int s = find_sequence(row, c.sequences, [&](int at) { return int64_t{start_of(c, at)}; });
+typedef int v4i __attribute__((ext_vector_type(4)));
+
+constexpr int kAttentionWaves = 4;
+constexpr int kRowTile = 16;
+constexpr int kTileRows = kAttentionWaves * kRowTile;  // rows of a workgroup
+constexpr int kKeyBlock = 64;
+constexpr float kLog2e = 1.44269504088896341f;
+
+// Sequence s has base(s + 1) - base(s) >= ceil(count * group / 64) tiles.
+__host__ __device__ inline int64_t tile_base(int64_t start, int64_t s, int group) { return start * group / kTileRows + s; }
+
+// x of the lanes l, l ^ 16, l ^ 32 and l ^ 48 put together, in every one of them.
+template <class Op> __device__ __forceinline__ int over_chunks(int x, const Op& op) {
+    const auto near = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+    x = op(static_cast<int>(near[0]), static_cast<int>(near[1]));
+    const auto far = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+    return op(static_cast<int>(far[0]), static_cast<int>(far[1]));
+}
+__device__ __forceinline__ float chunks_max(float x) {
+    return __int_as_float(over_chunks(__float_as_int(x), [](int a, int b) {
+        return __float_as_int(fmaxf(__int_as_float(a), __int_as_float(b)));
+    }));
+}
+__device__ __forceinline__ float chunks_sum(float x) {
+    return __int_as_float(over_chunks(__float_as_int(x), [](int a, int b) {
+        return __float_as_int(__int_as_float(a) + __int_as_float(b));
+    }));
+}
+
+// The digits of four whole numbers of size at most 2^30: byte r of digits[p] is digit p of x[r], in -128 .. 127. Adding 128
+// to the lower three digits makes the bytes those of the sum; flipping their top bits takes it off again.
+__device__ __forceinline__ void digits_of(const int (&x)[4], int (&digits)[4]) {
+    uint32_t y[4];
+#pragma unroll
+    for (int r = 0; r < 4; ++r) y[r] = (static_cast<uint32_t>(x[r]) + 0x00808080u) ^ 0x00808080u;
+    const uint32_t low01 = __builtin_amdgcn_perm(y[1], y[0], 0x05010400u), low23 = __builtin_amdgcn_perm(y[3], y[2], 0x05010400u);
+    const uint32_t high01 = __builtin_amdgcn_perm(y[1], y[0], 0x07030602u), high23 = __builtin_amdgcn_perm(y[3], y[2], 0x07030602u);
+    digits[0] = static_cast<int>(__builtin_amdgcn_perm(low23, low01, 0x05040100u));
+    digits[1] = static_cast<int>(__builtin_amdgcn_perm(low23, low01, 0x07060302u));
+    digits[2] = static_cast<int>(__builtin_amdgcn_perm(high23, high01, 0x05040100u));
+    digits[3] = static_cast<int>(__builtin_amdgcn_perm(high23, high01, 0x07060302u));
+}
+
+// The digits' four sums as one number: each is below 2^21 in size, so the pairs are exact.
+__device__ __forceinline__ float joined(const v4i (&sum)[4], int r) {
+    return static_cast<float>((sum[3][r] << 8) + sum[2][r]) * 65536.f + static_cast<float>((sum[1][r] << 8) + sum[0][r]);
+}
+
+// What a lane holds of 64 keys: 4 key rows' pieces, a piece of the values of D / 16 features, and its chunk's page (-1 for
+// none) and scales.
+template <int D> struct KeyBlock {
+    v4i k[4][D / 64];
+    v4i v[D / 16];
+    const int8_t* values;
+    float key_scale, value_scale;
+    int page;
+};
+
+struct Split {
+    int count;    // parts that a row's keys are split into
+    int part;     // keys of a part, a multiple of 64; the last part goes to the end
+    float* sums;  // [row][count][D], then [row][count][2] of the maximum (base 2) and the sum
+};
+
+template <int D>
+__global__ __launch_bounds__(kAttentionWaves * 64, 2) void paged_attention_kernel(Paged c, float* __restrict__ out, Strided q,
+                                                                                  int heads, double scale, Split split) {
+    constexpr int U = D / 64;
+    constexpr int kLd = D + 4;
+    // two blocks of 128 features' keys and values do not fit the registers: their values are loaded when the scores begin
+    constexpr bool kValuesAhead = D == 64;
+    __shared__ float os[kAttentionWaves][kRowTile][kLd];
+    __shared__ float ms[kAttentionWaves][kRowTile], ls[kAttentionWaves][kRowTile];
+    const int group = heads / c.kv_heads;
+    const int wave = threadIdx.x / 64, lane = threadIdx.x % 64;
+    const int column = lane % 16, chunk = lane / 16;
+    const int part = blockIdx.x % split.count;
+    const int kv = blockIdx.x / split.count % c.kv_heads;
+    // the last rows see most keys and go first
+    const int64_t tile = tile_base(c.tokens, c.sequences, group) - 1 - blockIdx.x / split.count / c.kv_heads;
+    const int s = find_sequence(tile, c.sequences, [&](int at) { return tile_base(start_of(c, at), at, group); });
     if (s < 0) return;
     const Rows rows = rows_of(c, s);
-    if (row >= rows.row + rows.count) return;
-    const int64_t limit = min(rows.position + (row - rows.row) + 1, static_cast<int64_t>(c.columns) << c.page_shift);
-    const int size = 1 << c.page_shift, dim = c.head_dim, t = threadIdx.x;
-    if (t < dim) qs[t] = q.data[row * q.row + h * q.head + t];
-    __syncthreads();
-    float m = -INFINITY, l = 0.f, o = 0.f;
-    for (int64_t j0 = 0; j0 < limit; j0 += 256) {
-        const int64_t j = j0 + t;
-        const int64_t page = j < limit ? page_of(c, s, j >> c.page_shift) : -1;
-        float score = -INFINITY;
-        if (page >= 0) {
-            const int8_t* key = c.keys + ((page * c.kv_heads + kv) * size + (j & (size - 1))) * dim;
-            float sum = 0.f;
-            for (int d = 0; d < dim; ++d) sum += qs[d] * key[d];
-            score = sum * c.key_scales[page * c.kv_heads + kv] * scale;
+    const int64_t row0 = (tile - tile_base(rows.row, s, group)) * kTileRows, row_end = static_cast<int64_t>(rows.count) * group;
+    if (row0 < 0 || row0 >= row_end) return;
+    const int here = static_cast<int>(min(row_end - row0, int64_t{kTileRows}));
+    // row tiles of the workgroup (1, 2 or 4), and the waves that share a tile's keys
+    const int row_waves = here <= 16 ? 1 : here <= 32 ? 2 : 4, key_waves = kAttentionWaves / row_waves;
+    const int row_wave = wave % row_waves, key_wave = wave / row_waves;
+    const int64_t capacity = static_cast<int64_t>(c.columns) << c.page_shift;
+    // keys 0 .. limit - 1 are visible to row r of the sequence
+    const auto limit_of = [&](int64_t r) {
+        const int64_t limit = rows.position + r / group + 1;
+        return static_cast<int>(limit < 0 ? 0 : limit > capacity ? capacity : limit);
+    };
+    const int from = part * split.part;
+    const int all = limit_of(row0 + here - 1);
+    if (from >= all && part > 0) return;
+    const int to = part + 1 == split.count ? all : min(all, from + split.part);
+    // rows past the last one stand in for it with a query of 0 and are not written
+    const int64_t tile_row = row0 + row_wave * kRowTile;
+    const bool real = row_wave * kRowTile + column < here;
+    const int64_t r = min(tile_row + column, row0 + here - 1);
+    const int limit = limit_of(r);
+    const int least = limit_of(min(tile_row, row0 + here - 1));
+    const int most = min(to, limit_of(min(tile_row + kRowTile - 1, row0 + here - 1)));
+
+    // the row's digits: features chunk * 16 U .. + 16 U - 1 of its column's row
+    v4i digits[4][U];
+    float q_factor;
+    {
+        const float* x = q.data + (rows.row + r / group) * q.row + (kv * group + r % group) * q.head + chunk * 16 * U;
+        float f[16 * U];
+        int bits = 0;
+#pragma unroll
+        for (int d = 0; d < 16 * U; ++d) {
+            f[d] = real ? x[d] : 0.f;
+            bits = max(bits, __float_as_int(f[d]) & 0x7fffffff);
         }
-        float most = score;
-        for (int x = 32; x > 0; x /= 2) most = max_na(most, __shfl_xor(most, x));
-        if (t % 64 == 0) parts[t / 64] = most;
-        __syncthreads();
-        for (int w = 0; w < 4; ++w) most = max_na(most, parts[w]);
-        most = max_na(m, most);
-        const float p = page < 0 ? 0.f : expf(score - most);
-        weights[t] = p;
-        float sum = p;
-        for (int x = 32; x > 0; x /= 2) sum += __shfl_xor(sum, x);
-        if (t % 64 == 0) parts[4 + t / 64] = sum;
-        __syncthreads();
-        const float alpha = m == -INFINITY ? 0.f : expf(m - most);
-        l = l * alpha + (parts[4] + parts[5] + parts[6] + parts[7]);
-        m = most;
-        if (t < dim) {
-            o *= alpha;
-            for (int i = 0; i < 256 && j0 + i < limit; ++i) {
-                const int64_t value_page = page_of(c, s, (j0 + i) >> c.page_shift);
-                if (value_page < 0) continue;
-                const int64_t at = value_page * c.kv_heads + kv;
-                o += weights[i] * (c.value_scales[at] * c.values[(at * dim + t) * size + ((j0 + i) & (size - 1))]);
+        bits = over_chunks(bits, [](int a, int b) { return max(a, b); });
+        const int e = __builtin_amdgcn_frexp_expf(__int_as_float(bits));  // 0 for 0; unused where not finite
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int t = 0; t < 4; ++t) {
+                int y[4], d4[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) y[i] = static_cast<int>(rintf(ldexpf(f[16 * u + 4 * t + i], 30 - e)));
+                digits_of(y, d4);
+#pragma unroll
+                for (int p = 0; p < 4; ++p) digits[p][u][t] = d4[p];
+            }
+        q_factor = bits < 0x7f800000 ? static_cast<float>(ldexp(scale * 1.4426950408889634074, e - 30)) : NAN;
+    }
+
+    const int size = 1 << c.page_shift;
+    const int64_t* table = c.table + static_cast<int64_t>(s) * c.columns;
+    const auto page_at = [&](int key) {
+        const int at = key >> c.page_shift;
+        const int64_t page = table[min(at, c.columns - 1)];
+        return at < c.columns && page >= 0 && page < c.pages ? static_cast<int>(page) : -1;
+    };
+    // the pages of the chunk that a lane's scores belong to, and of the chunk that its piece of the keys belongs to
+    struct Pages {
+        int own, keys;
+    };
+    const int key_chunk = column / 4;
+    const auto pages_at = [&](int key) { return Pages{page_at(key + 16 * chunk), page_at(key + 16 * key_chunk)}; };
+    const auto load_values = [&](v4i (&v)[D / 16], const KeyBlock<D>& b) {
+#pragma unroll
+        for (int n = 0; n < D / 16; ++n) v[n] = *reinterpret_cast<const v4i*>(b.values + 16 * n * size);
+    };
+    const auto load = [&](KeyBlock<D>& b, int key, Pages pages) {
+        // where there is no page the first one is read, and masked
+        const int64_t own = static_cast<int64_t>(max(pages.own, 0)) * c.kv_heads + kv;
+        const int64_t other = static_cast<int64_t>(max(pages.keys, 0)) * c.kv_heads + kv;
+        const int slot = (key + 16 * key_chunk) & (size - 1), own_slot = (key + 16 * chunk) & (size - 1);
+        const int8_t* k = c.keys + (other * size + slot + lane % 4) * D + chunk * 16 * U;
+        b.values = c.values + own * size * D + column * size + own_slot;
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+            for (int u = 0; u < U; ++u) b.k[t][u] = *reinterpret_cast<const v4i*>(k + 4 * t * D + 16 * u);
+        if constexpr (kValuesAhead) load_values(b.v, b);
+        b.page = pages.own;
+        b.key_scale = c.key_scales[own];
+        b.value_scale = c.value_scales[own];
+    };
+
+    float m = -INFINITY, l = 0.f;
+    float o[D / 4] = {};
+    const auto work = [&](KeyBlock<D>& b, int key) {
+        if constexpr (!kValuesAhead) load_values(b.v, b);
+        float x[16];
+        const float factor = q_factor * b.key_scale;
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+            v4i sum[4];
+#pragma unroll
+            for (int p = 0; p < 4; ++p) {
+                sum[p] = v4i{0, 0, 0, 0};
+#pragma unroll
+                for (int u = 0; u < U; ++u)
+                    sum[p] = __builtin_amdgcn_mfma_i32_16x16x64_i8(b.k[t][u], digits[p][u], sum[p], 0, 0, 0);
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x[4 * t + i] = joined(sum, i) * factor;
+        }
+        const int first = key + 16 * chunk;  // x[i] is key first + i
+        if (key + kKeyBlock > least || __any(b.page < 0)) {
+            const int seen = b.page < 0 ? 0 : limit - first;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) x[i] = i < seen ? x[i] : -INFINITY;
+        }
+        float largest = x[0];
+#pragma unroll
+        for (int i = 1; i < 16; ++i) largest = fmaxf(largest, x[i]);
+        const float next = fmaxf(m, chunks_max(largest));
+        const float base = next == -INFINITY ? 0.f : next;  // nothing seen yet: every weight below is 0
+        const float alpha = __builtin_amdgcn_exp2f(m - base);
+        m = next;
+        // value scales against the largest that the row sees, as bits, so that NaN is the largest of all
+        const int scale_bits = __float_as_int(b.value_scale) & 0x7fffffff;
+        const int top = over_chunks(b.page >= 0 && first < limit ? scale_bits : 0, [](int a, int b) { return max(a, b); });
+        const int e = __builtin_amdgcn_frexp_expf(__int_as_float(top));
+        const float to_whole = top < 0x7f800000 ? ldexpf(b.value_scale, 30 - e) : 0.f;
+        const float from_whole = top < 0x7f800000 ? ldexpf(1.f, e - 30) : NAN;
+        float sum = 0.f;
+        v4i weights[4];
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+            int w[4], d4[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float p = __builtin_amdgcn_exp2f(x[4 * t + i] - base);
+                sum += p;
+                w[i] = static_cast<int>(rintf(p * to_whole));
+            }
+            digits_of(w, d4);
+#pragma unroll
+            for (int p = 0; p < 4; ++p) weights[p][t] = d4[p];
+        }
+        l = l * alpha + sum;
+#pragma unroll
+        for (int n = 0; n < D / 16; ++n) {
+            v4i acc[4];
+#pragma unroll
+            for (int p = 0; p < 4; ++p)
+                acc[p] = __builtin_amdgcn_mfma_i32_16x16x64_i8(b.v[n], weights[p], v4i{0, 0, 0, 0}, 0, 0, 0);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) o[4 * n + i] = o[4 * n + i] * alpha + joined(acc, i) * from_whole;
+        }
+    };
+
+    const int step = key_waves * kKeyBlock;
+    int key = from + key_wave * kKeyBlock;
+    if (key < most) {
+        KeyBlock<D> even, odd;
+        Pages pages = pages_at(key);
+        load(even, key, pages);
+        pages = pages_at(key + step);
+        while (true) {
+            if (key + step < most) load(odd, key + step, pages);
+            pages = pages_at(key + 2 * step);
+            work(even, key);
+            key += step;
+            if (key >= most) break;
+            if (key + step < most) load(even, key + step, pages);
+            pages = pages_at(key + 2 * step);
+            work(odd, key);
+            key += step;
+            if (key >= most) break;
+        }
+    }
+    l = chunks_sum(l);
+    if (chunk == 0) {
+        ms[wave][column] = m;
+        ls[wave][column] = l;
+    }
+#pragma unroll
+    for (int n = 0; n < D / 16; ++n)
+        *reinterpret_cast<float4*>(&os[wave][column][16 * n + 4 * chunk]) =
+            make_float4(o[4 * n], o[4 * n + 1], o[4 * n + 2], o[4 * n + 3]);
+    __syncthreads();
+    // the waves that shared a row's keys joined, in their order
+    for (int i = threadIdx.x; i < here * (D / 4); i += kAttentionWaves * 64) {
+        const int at = i / (D / 4), d = i % (D / 4) * 4;
+        const int w0 = at / kRowTile, col = at % kRowTile;
+        float top = -INFINITY;
+        for (int w = 0; w < key_waves; ++w) top = fmaxf(top, ms[w0 + w * row_waves][col]);
+        const float base = top == -INFINITY ? 0.f : top;
+        float sum = 0.f;
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int w = 0; w < key_waves; ++w) {
+            const int from_wave = w0 + w * row_waves;
+            const float f = __builtin_amdgcn_exp2f(ms[from_wave][col] - base);
+            const float4 add = *reinterpret_cast<const float4*>(&os[from_wave][col][d]);
+            sum += f * ls[from_wave][col];
+            v.x += f * add.x;
+            v.y += f * add.y;
+            v.z += f * add.z;
+            v.w += f * add.w;
+        }
+        const int64_t row = row0 + at;
+        const int64_t to_row = (rows.row + row / group) * heads + kv * group + row % group;
+        if (split.count == 1) {
+            const float by = sum == 0.f ? 0.f : 1.f / sum;
+            *reinterpret_cast<float4*>(out + to_row * D + d) = make_float4(v.x * by, v.y * by, v.z * by, v.w * by);
+        } else {
+            const int64_t record = to_row * split.count + part;
+            *reinterpret_cast<float4*>(split.sums + record * D + d) = v;
+            if (d == 0) {
+                float* own = split.sums + static_cast<int64_t>(c.tokens) * heads * split.count * D + record * 2;
+                own[0] = top;
+                own[1] = sum;
             }
         }
-        __syncthreads();
     }
-    if (t < dim) out[(row * heads + h) * dim + t] = l == 0.f ? 0.f : o / l;
+}
+
+// The parts of a row joined, in their order: one wave a row.
+template <int D>
+__global__ __launch_bounds__(256) void paged_join_kernel(Paged c, float* __restrict__ out, int heads, Split split) {
+    const int64_t row = static_cast<int64_t>(blockIdx.x) * 4 + threadIdx.x / 64;  // token * heads + head
+    const int lane = threadIdx.x % 64;
+    if (row >= static_cast<int64_t>(c.tokens) * heads) return;
+    const int token = static_cast<int>(row / heads);
+    const int s = find_sequence(token, c.sequences, [&](int at) { return int64_t{start_of(c, at)}; });
+    if (s < 0) return;
+    const Rows rows = rows_of(c, s);
+    if (token >= rows.row + rows.count) return;
+    const int64_t limit = min(rows.position + (token - rows.row) + 1, static_cast<int64_t>(c.columns) << c.page_shift);
+    // the parts that begin before the row's limit were worked on, and the first one always
+    const int parts = static_cast<int>(max(int64_t{1}, min(int64_t{split.count}, (limit + split.part - 1) / split.part)));
+    const float* sums = split.sums + row * split.count * D;
+    const float* ml = split.sums + static_cast<int64_t>(c.tokens) * heads * split.count * D + row * split.count * 2;
+    float top = -INFINITY;
+    for (int p = 0; p < parts; ++p) top = fmaxf(top, ml[2 * p]);
+    const float base = top == -INFINITY ? 0.f : top;
+    float sum = 0.f, v[D / 64] = {};
+    for (int p = 0; p < parts; ++p) {
+        const float f = __builtin_amdgcn_exp2f(ml[2 * p] - base);
+        sum += f * ml[2 * p + 1];
+#pragma unroll
+        for (int u = 0; u < D / 64; ++u) v[u] += f * sums[p * D + 64 * u + lane];
+    }
+#pragma unroll
+    for (int u = 0; u < D / 64; ++u) out[row * D + 64 * u + lane] = sum == 0.f ? 0.f : v[u] / sum;
+}
+
+// How a call's keys are split: into as many parts as give every CU two workgroups, none of fewer than 256 keys.
+int64_t part_bytes(int64_t rows, int64_t dim) { return rows * (dim + 2) * 4; }
+
+Split split_of(int64_t heads, int64_t kv_heads, int64_t sequences, int64_t tokens, int64_t max_keys, int64_t most) {
+    const int64_t groups = std::max<int64_t>(1, tile_base(tokens, sequences, static_cast<int>(heads / kv_heads)) * kv_heads);
+    const int64_t keys = std::min<int64_t>(std::max<int64_t>(max_keys, 1), int64_t{1} << 30);
+    int64_t count = std::min({(2 * compute_units() + groups - 1) / groups, (keys + 255) / 256, most});
+    count = std::max<int64_t>(count, 1);
+    const int64_t part = ((keys + count - 1) / count + 255) / 256 * 256;
+    return {static_cast<int>((keys + part - 1) / part), static_cast<int>(part), nullptr};
 }
 
 // ---- checks ---------------------------------------------------------------------------------------
@@ -388,10 +690,12 @@ extern "C" int kd_paged_read(int dtype, void* k, void* v, const kd_paged_cache* 
 
 extern "C" int kd_paged_attention_workspace(int64_t* bytes, int64_t heads, int64_t kv_heads, int64_t head_dim,
                                             int64_t sequences, int64_t tokens, int64_t max_keys) {
-    if (bytes == nullptr || heads < 1 || kv_heads < 1 || heads % kv_heads != 0 || head_dim < 1 || sequences < 0 ||
-        tokens < 0 || max_keys < 0)
+    if (bytes == nullptr || heads < 1 || kv_heads < 1 || heads % kv_heads != 0 || heads > 4096 ||
+        (head_dim != 64 && head_dim != 128) || sequences < 0 || sequences >= int64_t{1} << 24 || tokens < 0 ||
+        tokens >= int64_t{1} << 31 || max_keys < 0)
         return fail(KD_E_INVALID, "kd_paged_attention_workspace: bad arguments");
-    *bytes = 0;
+    const Split split = split_of(heads, kv_heads, sequences, tokens, max_keys, INT32_MAX);
+    *bytes = split.count > 1 ? split.count * part_bytes(tokens * heads, head_dim) : 0;
     return KD_OK;
 }
 
@@ -410,8 +714,22 @@ extern "C" int kd_paged_attention(int dtype, void* out, const void* q, const int
     if (int rc = check_strided(what, "q", q, q_strides, c.tokens, heads, qs)) return rc;
     if (out == nullptr || !aligned(out, 16)) return fail(KD_E_INVALID, "kd_paged_attention: out must be given, 16-byte aligned");
     if (int rc = ensure_device()) return rc;
-    hipLaunchKernelGGL(paged_attention_kernel, dim3(static_cast<uint32_t>(heads * c.tokens)), dim3(256), 0, stream(), c,
-                       static_cast<float*>(out), qs, static_cast<int>(heads), static_cast<float>(scale));
+    if (c.pages == 0) c.columns = 0;  // no position has a page
+    const int64_t rows = heads * c.tokens;
+    Split split = split_of(heads, c.kv_heads, c.sequences, c.tokens, max_keys, workspace_bytes / part_bytes(rows, c.head_dim));
+    split.sums = static_cast<float*>(workspace);
+    const int64_t groups = tile_base(c.tokens, c.sequences, static_cast<int>(heads / c.kv_heads)) * c.kv_heads * split.count;
+    if (int rc = check_grid(what, groups)) return rc;
+    const auto launch = [&](auto dim) {
+        constexpr int D = decltype(dim)::value;
+        hipLaunchKernelGGL((paged_attention_kernel<D>), dim3(static_cast<uint32_t>(groups)), dim3(kAttentionWaves * 64), 0,
+                           stream(), c, static_cast<float*>(out), qs, static_cast<int>(heads), scale, split);
+        if (split.count > 1)
+            hipLaunchKernelGGL((paged_join_kernel<D>), dim3(static_cast<uint32_t>((rows + 3) / 4)), dim3(256), 0, stream(), c,
+                               static_cast<float*>(out), static_cast<int>(heads), split);
+    };
+    if (c.head_dim == 64) launch(std::integral_constant<int, 64>{});
+    else launch(std::integral_constant<int, 128>{});
     KD_LAUNCH_CHECK();
     return KD_OK;
 }
