@@ -11,6 +11,7 @@ its whole range.
 """
 from __future__ import annotations
 
+import functools
 import math
 import sys
 from pathlib import Path
@@ -377,10 +378,9 @@ PLAIN = {"append": plain_append, "attention": plain_attention, "verify": plain_v
 # ---- the framework's calls ------------------------------------------------------------------------
 
 
+@functools.cache
 def backend():
-    package = str(Path(__file__).resolve().parents[1] / "kael.cpp_amd")
-    if package not in sys.path:
-        sys.path.insert(0, package)
+    sys.path.insert(0, str(Path(__file__).resolve().parents[1] / "kael.cpp_amd"))
     import kd
     return kd, kd.load()
 
