@@ -249,17 +249,17 @@ __device__ __forceinline__ float chunks_sum(float x) {
     }));
 }
 
-// The digits of four whole numbers of size at most 2^30: byte r of digits[p] is digit p of x[r], in -128 .. 127. Adding 128
-// to the lower three digits makes the bytes those of the sum; flipping their top bits takes it off again.
-__device__ __forceinline__ void digits_of(const int (&x)[4], int (&digits)[4]) {
-    uint32_t y[4];
-#pragma unroll
-    for (int r = 0; r < 4; ++r) y[r] = (static_cast<uint32_t>(x[r]) + 0x00808080u) ^ 0x00808080u;
-    const uint32_t low01 = __builtin_amdgcn_perm(y[1], y[0], 0x05010400u), low23 = __builtin_amdgcn_perm(y[3], y[2], 0x05010400u);
-    const uint32_t high01 = __builtin_amdgcn_perm(y[1], y[0], 0x07030602u), high23 = __builtin_amdgcn_perm(y[3], y[2], 0x07030602u);
-    digits[0] = static_cast<int>(__builtin_amdgcn_perm(low23, low01, 0x05040100u));
-    digits[1] = static_cast<int>(__builtin_amdgcn_perm(low23, low01, 0x07060302u));
-    digits[2] = static_cast<int>(__builtin_amdgcn_perm(high23, high01, 0x05040100u));
+// The digits of four whole numbers x of size at most 2^30 from x + kDigitBias: byte r of digits[p] is digit p of x[r], in
+// -128 .. 127. The bias adds 128 to the lower three digits, whose bytes then are those of the sum; flipping their top bits
+// takes it off again.
+constexpr int kDigitBias = 0x00808080;
+__device__ __forceinline__ void digits_of(const int (&biased)[4], int (&digits)[4]) {
+    const uint32_t y0 = biased[0], y1 = biased[1], y2 = biased[2], y3 = biased[3];
+    const uint32_t low01 = __builtin_amdgcn_perm(y1, y0, 0x05010400u), low23 = __builtin_amdgcn_perm(y3, y2, 0x05010400u);
+    const uint32_t high01 = __builtin_amdgcn_perm(y1, y0, 0x07030602u), high23 = __builtin_amdgcn_perm(y3, y2, 0x07030602u);
+    digits[0] = static_cast<int>(__builtin_amdgcn_perm(low23, low01, 0x05040100u) ^ 0x80808080u);
+    digits[1] = static_cast<int>(__builtin_amdgcn_perm(low23, low01, 0x07060302u) ^ 0x80808080u);
+    digits[2] = static_cast<int>(__builtin_amdgcn_perm(high23, high01, 0x05040100u) ^ 0x80808080u);
     digits[3] = static_cast<int>(__builtin_amdgcn_perm(high23, high01, 0x07060302u));
 }
 
@@ -267,16 +267,6 @@ __device__ __forceinline__ void digits_of(const int (&x)[4], int (&digits)[4]) {
 __device__ __forceinline__ float joined(const v4i (&sum)[4], int r) {
     return static_cast<float>((sum[3][r] << 8) + sum[2][r]) * 65536.f + static_cast<float>((sum[1][r] << 8) + sum[0][r]);
 }
-
-// What a lane holds of 64 keys: 4 key rows' pieces, a piece of the values of D / 16 features, and its chunk's page (-1 for
-// none) and scales.
-template <int D> struct KeyBlock {
-    v4i k[4][D / 64];
-    v4i v[D / 16];
-    const int8_t* values;
-    float key_scale, value_scale;
-    int page;
-};
 
 struct Split {
     int count;    // parts that a row's keys are split into
@@ -293,7 +283,7 @@ __global__ __launch_bounds__(kAttentionWaves * 64, 2) void paged_attention_kerne
     constexpr bool kValuesAhead = D == 64;
     __shared__ float os[kAttentionWaves][kRowTile][kLd];
     __shared__ float ms[kAttentionWaves][kRowTile], ls[kAttentionWaves][kRowTile];
-    const int group = heads / c.kv_heads;
+    const uint32_t group = static_cast<uint32_t>(heads) / c.kv_heads;
     const int wave = threadIdx.x / 64, lane = threadIdx.x % 64;
     const int column = lane % 16, chunk = lane / 16;
     const int part = blockIdx.x % split.count;
@@ -303,16 +293,19 @@ __global__ __launch_bounds__(kAttentionWaves * 64, 2) void paged_attention_kerne
     const int s = find_sequence(tile, c.sequences, [&](int at) { return tile_base(start_of(c, at), at, group); });
     if (s < 0) return;
     const Rows rows = rows_of(c, s);
-    const int64_t row0 = (tile - tile_base(rows.row, s, group)) * kTileRows, row_end = static_cast<int64_t>(rows.count) * group;
-    if (row0 < 0 || row0 >= row_end) return;
-    const int here = static_cast<int>(min(row_end - row0, int64_t{kTileRows}));
+    // tokens * heads is below 2^31, and so are the rows of a kv head
+    const int64_t tile_at = (tile - tile_base(rows.row, s, group)) * kTileRows;
+    const int row_end = rows.count * group;
+    if (tile_at < 0 || tile_at >= row_end) return;
+    const int row0 = static_cast<int>(tile_at);
+    const int here = min(row_end - row0, kTileRows);
     // row tiles of the workgroup (1, 2 or 4), and the waves that share a tile's keys
     const int row_waves = here <= 16 ? 1 : here <= 32 ? 2 : 4, key_waves = kAttentionWaves / row_waves;
     const int row_wave = wave % row_waves, key_wave = wave / row_waves;
     const int64_t capacity = static_cast<int64_t>(c.columns) << c.page_shift;
     // keys 0 .. limit - 1 are visible to row r of the sequence
-    const auto limit_of = [&](int64_t r) {
-        const int64_t limit = rows.position + r / group + 1;
+    const auto limit_of = [&](int r) {
+        const int64_t limit = rows.position + static_cast<uint32_t>(r) / group + 1;
         return static_cast<int>(limit < 0 ? 0 : limit > capacity ? capacity : limit);
     };
     const int from = part * split.part;
@@ -320,9 +313,9 @@ __global__ __launch_bounds__(kAttentionWaves * 64, 2) void paged_attention_kerne
     if (from >= all && part > 0) return;
     const int to = part + 1 == split.count ? all : min(all, from + split.part);
     // rows past the last one stand in for it with a query of 0 and are not written
-    const int64_t tile_row = row0 + row_wave * kRowTile;
+    const int tile_row = row0 + row_wave * kRowTile;
     const bool real = row_wave * kRowTile + column < here;
-    const int64_t r = min(tile_row + column, row0 + here - 1);
+    const uint32_t r = min(tile_row + column, row0 + here - 1);
     const int limit = limit_of(r);
     const int least = limit_of(min(tile_row, row0 + here - 1));
     const int most = min(to, limit_of(min(tile_row + kRowTile - 1, row0 + here - 1)));
@@ -347,7 +340,7 @@ __global__ __launch_bounds__(kAttentionWaves * 64, 2) void paged_attention_kerne
             for (int t = 0; t < 4; ++t) {
                 int y[4], d4[4];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) y[i] = static_cast<int>(rintf(ldexpf(f[16 * u + 4 * t + i], 30 - e)));
+                for (int i = 0; i < 4; ++i) y[i] = static_cast<int>(rintf(ldexpf(f[16 * u + 4 * t + i], 30 - e))) + kDigitBias;
                 digits_of(y, d4);
 #pragma unroll
                 for (int p = 0; p < 4; ++p) digits[p][u][t] = d4[p];
@@ -356,45 +349,56 @@ __global__ __launch_bounds__(kAttentionWaves * 64, 2) void paged_attention_kerne
     }
 
     const int size = 1 << c.page_shift;
+    // Lane i of `window` holds the page of table column window_from + i, so that the table's loads are not waited for
+    // among the codes'.
     const int64_t* table = c.table + static_cast<int64_t>(s) * c.columns;
-    const auto page_at = [&](int key) {
-        const int at = key >> c.page_shift;
-        const int64_t page = table[min(at, c.columns - 1)];
-        return at < c.columns && page >= 0 && page < c.pages ? static_cast<int>(page) : -1;
+    int window = 0, window_from = -128;
+    const auto pages_of_block = [&](int key) {
+        if (((key + kKeyBlock - 1) >> c.page_shift) - window_from >= 64) {
+            window_from = key >> c.page_shift;
+            const int64_t page = table[min(window_from + lane, c.columns - 1)];
+            window = window_from + lane < c.columns && page >= 0 && page < c.pages ? static_cast<int>(page) : -1;
+        }
     };
-    // the pages of the chunk that a lane's scores belong to, and of the chunk that its piece of the keys belongs to
-    struct Pages {
-        int own, keys;
-    };
+    const auto page_at = [&](int key) { return __shfl(window, (key >> c.page_shift) - window_from); };
+
+    // A lane's piece of the keys lies in chunk column / 4, its scores and its piece of the values in chunk lane / 16. Where
+    // there is no page the first one is read, and masked.
     const int key_chunk = column / 4;
-    const auto pages_at = [&](int key) { return Pages{page_at(key + 16 * chunk), page_at(key + 16 * key_chunk)}; };
-    const auto load_values = [&](v4i (&v)[D / 16], const KeyBlock<D>& b) {
-#pragma unroll
-        for (int n = 0; n < D / 16; ++n) v[n] = *reinterpret_cast<const v4i*>(b.values + 16 * n * size);
-    };
-    const auto load = [&](KeyBlock<D>& b, int key, Pages pages) {
-        // where there is no page the first one is read, and masked
-        const int64_t own = static_cast<int64_t>(max(pages.own, 0)) * c.kv_heads + kv;
-        const int64_t other = static_cast<int64_t>(max(pages.keys, 0)) * c.kv_heads + kv;
+    v4i k[4][U], v[D / 16];
+    const int8_t* values_at;
+    float key_scale, value_scale;
+    int page;
+    const auto load_keys = [&](int key) {
+        pages_of_block(key);
+        page = page_at(key + 16 * chunk);
+        const int64_t own = static_cast<int64_t>(max(page, 0)) * c.kv_heads + kv;
+        const int64_t other = static_cast<int64_t>(max(page_at(key + 16 * key_chunk), 0)) * c.kv_heads + kv;
         const int slot = (key + 16 * key_chunk) & (size - 1), own_slot = (key + 16 * chunk) & (size - 1);
-        const int8_t* k = c.keys + (other * size + slot + lane % 4) * D + chunk * 16 * U;
-        b.values = c.values + own * size * D + column * size + own_slot;
+        const int8_t* at = c.keys + (other * size + slot + lane % 4) * D + chunk * 16 * U;
 #pragma unroll
         for (int t = 0; t < 4; ++t)
 #pragma unroll
-            for (int u = 0; u < U; ++u) b.k[t][u] = *reinterpret_cast<const v4i*>(k + 4 * t * D + 16 * u);
-        if constexpr (kValuesAhead) load_values(b.v, b);
-        b.page = pages.own;
-        b.key_scale = c.key_scales[own];
-        b.value_scale = c.value_scales[own];
+            for (int u = 0; u < U; ++u) k[t][u] = *reinterpret_cast<const v4i*>(at + 4 * t * D + 16 * u);
+        key_scale = c.key_scales[own];
+        value_scale = c.value_scales[own];
+        values_at = c.values + own * size * D + column * size + own_slot;
+    };
+    const auto load_values = [&] {
+#pragma unroll
+        for (int n = 0; n < D / 16; ++n) v[n] = *reinterpret_cast<const v4i*>(values_at + 16 * n * size);
     };
 
     float m = -INFINITY, l = 0.f;
     float o[D / 4] = {};
-    const auto work = [&](KeyBlock<D>& b, int key) {
-        if constexpr (!kValuesAhead) load_values(b.v, b);
+    const int step = key_waves * kKeyBlock;
+    int key = from + key_wave * kKeyBlock;
+    if (key < most) {
+        load_keys(key);
+        load_values();
+    }
+    for (; key < most; key += step) {
         float x[16];
-        const float factor = q_factor * b.key_scale;
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
             v4i sum[4];
@@ -403,29 +407,35 @@ __global__ __launch_bounds__(kAttentionWaves * 64, 2) void paged_attention_kerne
                 sum[p] = v4i{0, 0, 0, 0};
 #pragma unroll
                 for (int u = 0; u < U; ++u)
-                    sum[p] = __builtin_amdgcn_mfma_i32_16x16x64_i8(b.k[t][u], digits[p][u], sum[p], 0, 0, 0);
+                    sum[p] = __builtin_amdgcn_mfma_i32_16x16x64_i8(k[t][u], digits[p][u], sum[p], 0, 0, 0);
             }
 #pragma unroll
-            for (int i = 0; i < 4; ++i) x[4 * t + i] = joined(sum, i) * factor;
+            for (int i = 0; i < 4; ++i) x[4 * t + i] = joined(sum, i);
         }
         const int first = key + 16 * chunk;  // x[i] is key first + i
-        if (key + kKeyBlock > least || __any(b.page < 0)) {
-            const int seen = b.page < 0 ? 0 : limit - first;
+        const int seen = page < 0 ? 0 : limit - first;
+        const int scale_bits = seen > 0 ? __float_as_int(value_scale) & 0x7fffffff : 0;
+        const float own_scale = value_scale;
+        // never 0, so that a masked key's -inf stays what it is
+        float factor = q_factor * key_scale;
+        factor = factor == 0.f ? 0x1p-126f : factor;
+        if (key + kKeyBlock > least || __any(page < 0)) {
+            factor = seen > 0 ? factor : 1.f;  // nor NaN where the row sees none of them
 #pragma unroll
             for (int i = 0; i < 16; ++i) x[i] = i < seen ? x[i] : -INFINITY;
         }
+        load_keys(key + step < most ? key + step : key);  // the last block once more rather than a branch
         float largest = x[0];
 #pragma unroll
         for (int i = 1; i < 16; ++i) largest = fmaxf(largest, x[i]);
-        const float next = fmaxf(m, chunks_max(largest));
+        const float next = fmaxf(m, chunks_max(largest * factor));
         const float base = next == -INFINITY ? 0.f : next;  // nothing seen yet: every weight below is 0
         const float alpha = __builtin_amdgcn_exp2f(m - base);
         m = next;
         // value scales against the largest that the row sees, as bits, so that NaN is the largest of all
-        const int scale_bits = __float_as_int(b.value_scale) & 0x7fffffff;
-        const int top = over_chunks(b.page >= 0 && first < limit ? scale_bits : 0, [](int a, int b) { return max(a, b); });
+        const int top = over_chunks(scale_bits, [](int a, int b) { return max(a, b); });
         const int e = __builtin_amdgcn_frexp_expf(__int_as_float(top));
-        const float to_whole = top < 0x7f800000 ? ldexpf(b.value_scale, 30 - e) : 0.f;
+        const float to_whole = top < 0x7f800000 && seen > 0 ? ldexpf(own_scale, 30 - e) : 0.f;
         const float from_whole = top < 0x7f800000 ? ldexpf(1.f, e - 30) : NAN;
         float sum = 0.f;
         v4i weights[4];
@@ -434,9 +444,10 @@ __global__ __launch_bounds__(kAttentionWaves * 64, 2) void paged_attention_kerne
             int w[4], d4[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const float p = __builtin_amdgcn_exp2f(x[4 * t + i] - base);
+                const float p = __builtin_amdgcn_exp2f(fmaf(x[4 * t + i], factor, -base));
                 sum += p;
-                w[i] = static_cast<int>(rintf(p * to_whole));
+                // from 2^23 on an f32 is whole: the bias rounds the weight too, to half a unit or its own last bit
+                w[i] = static_cast<int>(fmaf(p, to_whole, static_cast<float>(kDigitBias)));
             }
             digits_of(w, d4);
 #pragma unroll
@@ -448,31 +459,11 @@ __global__ __launch_bounds__(kAttentionWaves * 64, 2) void paged_attention_kerne
             v4i acc[4];
 #pragma unroll
             for (int p = 0; p < 4; ++p)
-                acc[p] = __builtin_amdgcn_mfma_i32_16x16x64_i8(b.v[n], weights[p], v4i{0, 0, 0, 0}, 0, 0, 0);
+                acc[p] = __builtin_amdgcn_mfma_i32_16x16x64_i8(v[n], weights[p], v4i{0, 0, 0, 0}, 0, 0, 0);
 #pragma unroll
             for (int i = 0; i < 4; ++i) o[4 * n + i] = o[4 * n + i] * alpha + joined(acc, i) * from_whole;
         }
-    };
-
-    const int step = key_waves * kKeyBlock;
-    int key = from + key_wave * kKeyBlock;
-    if (key < most) {
-        KeyBlock<D> even, odd;
-        Pages pages = pages_at(key);
-        load(even, key, pages);
-        pages = pages_at(key + step);
-        while (true) {
-            if (key + step < most) load(odd, key + step, pages);
-            pages = pages_at(key + 2 * step);
-            work(even, key);
-            key += step;
-            if (key >= most) break;
-            if (key + step < most) load(even, key + step, pages);
-            pages = pages_at(key + 2 * step);
-            work(odd, key);
-            key += step;
-            if (key >= most) break;
-        }
+        load_values();
     }
     l = chunks_sum(l);
     if (chunk == 0) {
@@ -503,8 +494,8 @@ __global__ __launch_bounds__(kAttentionWaves * 64, 2) void paged_attention_kerne
             v.z += f * add.z;
             v.w += f * add.w;
         }
-        const int64_t row = row0 + at;
-        const int64_t to_row = (rows.row + row / group) * heads + kv * group + row % group;
+        const uint32_t row = row0 + at;
+        const int64_t to_row = (rows.row + static_cast<int64_t>(row / group)) * heads + kv * group + row % group;
         if (split.count == 1) {
             const float by = sum == 0.f ? 0.f : 1.f / sum;
             *reinterpret_cast<float4*>(out + to_row * D + d) = make_float4(v.x * by, v.y * by, v.z * by, v.w * by);
