@@ -1,5 +1,7 @@
 // kd_drafts.hip - a draft model beside its target: verification of drafted tokens against the target's probabilities,
 // and the distillation loss against the target's top logits with its gradient.
+#include <algorithm>
+
 #include "kd_internal.h"
 
 namespace kd {
@@ -12,25 +14,84 @@ __device__ __forceinline__ double wave_sum(double v) {
     return v;
 }
 
+// 16 bytes of a row whose start is aligned to its elements only.
+template <typename T> struct Piece {
+    static constexpr int kCount = 16 / sizeof(T);
+    T x[kCount];
+};
+template <typename T> __device__ __forceinline__ Piece<T> load_piece(const T* row, int64_t at, int64_t cols, T rest) {
+    Piece<T> p;
+    if (at + Piece<T>::kCount <= cols) {
+        __builtin_memcpy(&p, row + at, 16);
+    } else {
+#pragma unroll
+        for (int i = 0; i < Piece<T>::kCount; ++i) p.x[i] = at + i < cols ? row[at + i] : rest;
+    }
+    return p;
+}
+
 // ---- verification ---------------------------------------------------------------------------------
+//
+// One workgroup a sequence: it finds the first draft that is not accepted, reads that one row (the target's and the draft's)
+// and draws from it. Bound by the rows' bytes for many sequences, by the chain of dependent loads and the rate of a CU for few. The
+// draw narrows the row down in two steps, a sixteenth of it and a sixteenth of that by the waves' sums, and a wave's running
+// sums find the entry: two passes over parts that are in the L2 by then instead of running sums over the whole row.
 
 constexpr int kVerifyThreads = 1024;
 constexpr int kVerifyWaves = kVerifyThreads / 64;
 
-// The weight of entry j: p - q where that is positive, p itself without a draft row; NaN stays NaN.
+// The weights that a token is drawn from: p - q where that is positive, p itself without a draft row; NaN stays NaN.
 template <typename T> struct Weights {
     const T* p;
-    const T* q;        // NULL: no draft row
-    int64_t certain;   // q NULL: the entry whose q is 1, or -1
-    __device__ __forceinline__ double operator()(int64_t j) const {
-        double w = static_cast<double>(p[j]);
-        if (q != nullptr) w -= static_cast<double>(q[j]);
-        else if (j == certain) w -= 1.0;
-        return w < 0 ? 0.0 : w;
+    const T* q;       // NULL: no draft row
+    int64_t certain;  // q NULL: the entry whose q is 1, or -1
+    static constexpr int kCount = Piece<T>::kCount;
+
+    // the weights of the entries at .. at + kCount - 1; 0 from `to` on
+    __device__ __forceinline__ void at(int64_t at, int64_t to, double (&w)[kCount]) const {
+        const Piece<T> a = load_piece(p, at, to, T(0));
+        Piece<T> b{};
+        if (q != nullptr) b = load_piece(q, at, to, T(0));
+#pragma unroll
+        for (int i = 0; i < kCount; ++i) {
+            w[i] = static_cast<double>(a.x[i]) - (q != nullptr ? static_cast<double>(b.x[i]) : at + i == certain ? 1.0 : 0.0);
+            w[i] = w[i] < 0 || at + i >= to ? 0.0 : w[i];
+        }
+    }
+    // their sum over from .. to - 1, by a wave
+    __device__ __forceinline__ double sum(int64_t from, int64_t to) const {
+        constexpr int kPieces = 4;
+        double total = 0;
+        for (int64_t j = from + threadIdx.x % 64 * kCount; j < to; j += kPieces * 64 * kCount) {
+            double w[kPieces][kCount];
+#pragma unroll
+            for (int n = 0; n < kPieces; ++n) at(j + n * 64 * kCount, to, w[n]);
+#pragma unroll
+            for (int n = 0; n < kPieces; ++n)
+#pragma unroll
+                for (int i = 0; i < kCount; ++i) total += w[n][i];
+        }
+        return wave_sum(total);
     }
 };
 
-// One workgroup a sequence, a contiguous part of the vocabulary a wave.
+// The first part whose running sum exceeds `point`, else the last with any weight; `before` becomes the sum ahead of it.
+__device__ __forceinline__ int part_of(const double* sums, double point, double& before) {
+    int last = 0;
+    double run = before, before_last = before;
+    for (int w = 0; w < kVerifyWaves; ++w) {
+        const double after = run + sums[w];
+        if (sums[w] > 0) {
+            last = w;
+            before_last = run;
+            if (after > point) break;
+        }
+        run = after;
+    }
+    before = before_last;
+    return last;
+}
+
 template <typename T>
 __global__ __launch_bounds__(kVerifyThreads) void verify_drafts_kernel(int64_t* __restrict__ tokens, int64_t* __restrict__ accepted,
                                                                        const T* __restrict__ target, const T* __restrict__ draft,
@@ -38,49 +99,50 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_drafts_kernel(int64_t* 
                                                                        const int64_t* __restrict__ counts,
                                                                        const double* __restrict__ uniforms, int64_t drafts,
                                                                        int64_t vocab) {
-    __shared__ double sums[kVerifyWaves];
+    __shared__ double sums[2][kVerifyWaves];
+    constexpr int kCount = Weights<T>::kCount, kRound = 64 * kCount;
     const int64_t s = blockIdx.x;
     const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
-    const int64_t count = min(max(counts[s], int64_t{0}), drafts);
     const int64_t* x = drafted + s * drafts;
     const double* u = uniforms + s * (drafts + 1);
+    const int64_t given = counts[s];
+    const double last_u = u[drafts];
+    const int64_t count = given < 0 ? 0 : given > drafts ? drafts : given;
     int64_t kept = 0;
-    for (bool open = true; open && kept < count;) {
+    for (bool open = true; open && kept < drafts;) {
         const int64_t i = kept + lane;
         bool good = false;
-        if (i < count) {
+        if (i < drafts) {  // not count, whose load is under way
             const int64_t token = x[i];
+            const double draw = u[i];
             if (token >= 0 && token < vocab) {
                 const double p = static_cast<double>(target[(s * (drafts + 1) + i) * vocab + token]);
                 const double q = draft != nullptr ? static_cast<double>(draft[(s * drafts + i) * vocab + token]) : 1.0;
-                good = u[i] * q < p;
+                good = draw * q < p;
             }
         }
-        const uint64_t all = __ballot(good);
+        const uint64_t all = __ballot(good && i < count);
         const int n = all == ~uint64_t{0} ? 64 : __ffsll(static_cast<unsigned long long>(~all)) - 1;
         open = n == 64;
         kept += n;
     }
-    Weights<T> weight{target + (s * (drafts + 1) + kept) * vocab, nullptr, -1};
+    Weights<T> weights{target + (s * (drafts + 1) + kept) * vocab, nullptr, -1};
     if (kept < count) {
-        if (draft != nullptr) weight.q = draft + (s * drafts + kept) * vocab;
-        else weight.certain = x[kept];
+        if (draft != nullptr) weights.q = draft + (s * drafts + kept) * vocab;
+        else weights.certain = x[kept];
     }
-    const int64_t part = (vocab + kVerifyThreads - 1) / kVerifyThreads * 64;
-    const int64_t from = min(wave * part, vocab), to = min(from + part, vocab);
+    const int64_t part = (vocab + kVerifyWaves * kRound - 1) / (kVerifyWaves * kRound) * kRound;
     double total = 0;
-    for (int again = 0; again < 2; ++again) {
-        double sum = 0;
-        for (int64_t j = from + lane; j < to; j += 64) sum += weight(j);
-        sum = wave_sum(sum);
-        if (lane == 0) sums[wave] = sum;
+    while (true) {
+        const double sum = weights.sum(wave * part, min((wave + 1) * part, vocab));
+        if (lane == 0) sums[0][wave] = sum;
         __syncthreads();
         total = 0;
-        for (int w = 0; w < kVerifyWaves; ++w) total += sums[w];
-        if (total > 0 || (weight.q == nullptr && weight.certain < 0)) break;
+        for (int w = 0; w < kVerifyWaves; ++w) total += sums[0][w];
+        if (total > 0 || (weights.q == nullptr && weights.certain < 0)) break;
         // nothing is left of p - q (or it is NaN): the target's own probabilities
-        weight.q = nullptr;
-        weight.certain = -1;
+        weights.q = nullptr;
+        weights.certain = -1;
         __syncthreads();
     }
     int64_t* out = tokens + s * (drafts + 1);
@@ -91,165 +153,336 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_drafts_kernel(int64_t* 
         if (threadIdx.x == 0) out[kept] = -1;
         return;
     }
-    // the wave whose part holds the point: the first whose running sum exceeds it, else the last with any weight
-    const double point = u[drafts] * total;
+    const double point = last_u * total;
     double before = 0;
-    int holder = -1, last = 0;
-    double before_holder = 0, before_last = 0;
-    for (int w = 0; w < kVerifyWaves; ++w) {
-        const double after = before + sums[w];
-        if (sums[w] > 0) {
-            last = w;
-            before_last = before;
-        }
-        if (holder < 0 && after > point) {
-            holder = w;
-            before_holder = before;
-        }
-        before = after;
-    }
-    if (holder < 0) {
-        holder = last;
-        before_holder = before_last;
-    }
+    const int64_t outer = part_of(sums[0], point, before) * part, outer_end = min(outer + part, vocab);
+    const int64_t small = (part / kRound + kVerifyWaves - 1) / kVerifyWaves * kRound;
+    const double sum = weights.sum(outer + wave * small, min(outer + (wave + 1) * small, outer_end));
+    if (lane == 0) sums[1][wave] = sum;
+    __syncthreads();
+    const int holder = part_of(sums[1], point, before);
     if (wave != holder) return;
+    const int64_t from = outer + holder * small, to = min(from + small, outer_end);
     int64_t picked = -1;
-    double run = before_holder;
-    for (int64_t j0 = from; j0 < to; j0 += 64) {
-        const int64_t j = j0 + lane;
-        const double w = j < to ? weight(j) : 0.0;
-        double sum = w;
+    for (int64_t j0 = from; j0 < to; j0 += kRound) {
+        const int64_t j = j0 + lane * kCount;
+        double w[kCount], own = 0;
+        weights.at(j, to, w);
+#pragma unroll
+        for (int i = 0; i < kCount; ++i) own += w[i];
+        double run = own;
 #pragma unroll
         for (int d = 1; d < 64; d *= 2) {
-            const double other = __shfl_up(sum, d);
-            if (lane >= d) sum += other;
+            const double other = __shfl_up(run, d);
+            if (lane >= d) run += other;
         }
-        const uint64_t over = __ballot(w > 0 && run + sum > point);
-        if (over != 0) {
-            picked = j0 + __ffsll(static_cast<unsigned long long>(over)) - 1;
+        const double next = before + __shfl(run, 63);
+        // the lane's first entry over the point, and its last of any weight
+        int over = -1, any = -1;
+        run += before - own;
+#pragma unroll
+        for (int i = 0; i < kCount; ++i) {
+            run += w[i];
+            if (w[i] > 0) {
+                any = i;
+                if (over < 0 && run > point) over = i;
+            }
+        }
+        const uint64_t lanes_over = __ballot(over >= 0), lanes_any = __ballot(any >= 0);
+        if (lanes_over != 0) {
+            const int first = __ffsll(static_cast<unsigned long long>(lanes_over)) - 1;
+            picked = j0 + first * kCount + __shfl(over, first);
             break;
         }
-        const uint64_t any = __ballot(w > 0);
-        if (any != 0) picked = j0 + 63 - __clzll(static_cast<long long>(any));
-        run += __shfl(sum, 63);
+        if (lanes_any != 0) {
+            const int last = 63 - __clzll(static_cast<long long>(lanes_any));
+            picked = j0 + last * kCount + __shfl(any, last);
+        }
+        before = next;
     }
     if (lane == 0) out[kept] = picked;
 }
 
 // ---- distillation ---------------------------------------------------------------------------------
+//
+// Bound by the logits' bytes: the loss reads a row once, with each thread's running maximum and sum, the gradient reads it once
+// more and writes it once. The teacher's side (a row's kept entries) is one wave's work in f64, beside the row's.
 
 constexpr int kMaxKept = 1024;
-constexpr int kRowThreads = 256;
+constexpr int kNarrow = 256;        // columns up to which a wave holds a row
+constexpr int kNarrowRows = 4;      // rows of such a workgroup
+constexpr int kMostThreads = 1024;
 
-// The teacher's side of a row, by a whole workgroup: share[j] = pi_j (0 where the entry counts for nothing) and
-// log pi_j = (t_j - largest) / T - log_sum. Returns whether the row has any entry.
-struct Teacher {
-    double largest, log_sum;
-    bool any;
+__device__ __forceinline__ double wave_max(double v) {
+#pragma unroll
+    for (int m = 32; m > 0; m /= 2) v = max_na(v, __shfl_xor(v, m));
+    return v;
+}
+
+// exp(x / T) from x and c = kScale / T. f32: the hardware's power of two, whose argument's rounding is no worse than that of
+// the quotient itself.
+template <typename T> struct Exp;
+template <> struct Exp<float> {
+    static constexpr double kScale = 1.4426950408889634074;
+    __device__ static __forceinline__ float of(float x, float c) { return __builtin_amdgcn_exp2f(x * c); }
+};
+template <> struct Exp<double> {
+    static constexpr double kScale = 1.0;
+    __device__ static __forceinline__ double of(double x, double c) { return std::exp(x * c); }
 };
 
-__device__ __forceinline__ double group_max(double v, double* scratch) {
-    for (int m = 32; m > 0; m /= 2) v = max_na(v, __shfl_xor(v, m));
-    __syncthreads();
-    if (threadIdx.x % 64 == 0) scratch[threadIdx.x / 64] = v;
-    __syncthreads();
-    for (int w = 0; w < kRowThreads / 64; ++w) v = max_na(v, scratch[w]);
-    return v;
-}
-__device__ __forceinline__ double group_sum(double v, double* scratch) {
-    v = wave_sum(v);
-    __syncthreads();
-    if (threadIdx.x % 64 == 0) scratch[threadIdx.x / 64] = v;
-    __syncthreads();
-    v = 0;
-    for (int w = 0; w < kRowThreads / 64; ++w) v += scratch[w];
-    return v;
-}
+// A row's kept entries as one wave sees them: the largest teacher logit, the log of the sum of exponentials, and whether there
+// is any entry.
+template <typename T> struct Teacher {
+    const T* t;
+    const int64_t* index;
+    int64_t cols;
+    int kept;
+    double temperature, largest, log_sum;
+    bool any;
 
-template <typename T>
-__device__ Teacher teacher_of(const T* t, const int64_t* index, int64_t cols, int kept, double temperature, double* scratch) {
-    double largest = -INFINITY;
-    for (int j = threadIdx.x; j < kept; j += kRowThreads)
-        if (index[j] >= 0 && index[j] < cols) largest = max_na(largest, static_cast<double>(t[j]));
-    largest = group_max(largest, scratch);
-    double sum = 0;
-    if (largest != -INFINITY)
-        for (int j = threadIdx.x; j < kept; j += kRowThreads)
-            if (index[j] >= 0 && index[j] < cols) sum += exp((static_cast<double>(t[j]) - largest) / temperature);
-    sum = group_sum(sum, scratch);
-    return {largest, log(sum), largest != -INFINITY};
-}
+    __device__ __forceinline__ bool has(int j) const { return j < kept && index[j] >= 0 && index[j] < cols; }
+    __device__ __forceinline__ void sum_up() {
+        const int lane = threadIdx.x % 64;
+        largest = -INFINITY;
+        for (int j = lane; j < kept; j += 64)
+            if (has(j)) largest = max_na(largest, static_cast<double>(t[j]));
+        largest = wave_max(largest);
+        any = largest != -INFINITY;
+        double sum = 0;
+        if (any)
+            for (int j = lane; j < kept; j += 64)
+                if (has(j)) sum += exp((static_cast<double>(t[j]) - largest) / temperature);
+        log_sum = log(wave_sum(sum));
+    }
+    __device__ __forceinline__ double log_share(int j) const {
+        return (static_cast<double>(t[j]) - largest) / temperature - log_sum;
+    }
+    // T^2 sum pi (log pi - log sigma) for a row z with its maximum and log sum of exponentials
+    __device__ __forceinline__ double loss(const T* z, double row_largest, double row_log_sum) const {
+        double sum = 0;
+        if (any)
+            for (int j = threadIdx.x % 64; j < kept; j += 64) {
+                if (!has(j)) continue;
+                const double own = log_share(j), share = exp(own);
+                const double student = (static_cast<double>(z[index[j]]) - row_largest) / temperature - row_log_sum;
+                sum += share == 0 ? 0 : share * (own - student);
+            }
+        return temperature * temperature * wave_sum(sum);
+    }
+};
 
-template <typename T>
-__global__ __launch_bounds__(kRowThreads) void distill_rows_kernel(T* __restrict__ losses, T* __restrict__ stats,
-                                                                   const T* __restrict__ logits, const int64_t* __restrict__ indices,
-                                                                   const T* __restrict__ teacher, int64_t cols, int kept,
-                                                                   double temperature) {
-    __shared__ double scratch[kRowThreads / 64];
-    const int64_t row = blockIdx.x;
-    const T* z = logits + row * cols;
+template <typename T> __device__ __forceinline__ T or_zero(T largest) { return largest == -INFINITY ? T(0) : largest; }
+
+// A thread's running maximum and its sum of exp((z - largest) / T).
+template <typename T> struct Running {
     T largest = -INFINITY;
-    for (int64_t c = threadIdx.x; c < cols; c += kRowThreads) largest = max_na(largest, z[c]);
-    largest = static_cast<T>(group_max(static_cast<double>(largest), scratch));
-    const T inverse = static_cast<T>(1 / temperature);
     double sum = 0;
-    for (int64_t c = threadIdx.x; c < cols; c += kRowThreads) sum += static_cast<double>(std::exp((z[c] - largest) * inverse));
-    sum = group_sum(sum, scratch);
-    const int64_t* index = indices + row * kept;
-    const T* t = teacher + row * kept;
-    const Teacher side = teacher_of(t, index, cols, kept, temperature, scratch);
-    double loss = 0;
-    const double log_total = log(sum);
-    if (side.any)
-        for (int j = threadIdx.x; j < kept; j += kRowThreads) {
-            const int64_t i = index[j];
-            if (i < 0 || i >= cols || t[j] == -INFINITY) continue;
-            const double log_share = (static_cast<double>(t[j]) - side.largest) / temperature - side.log_sum;
-            const double log_student = (static_cast<double>(z[i]) - static_cast<double>(largest)) / temperature - log_total;
-            const double share = exp(log_share);
-            loss += share == 0 ? 0 : share * (log_share - log_student);
+    template <int N> __device__ __forceinline__ void add(const T (&x)[N], T c) {
+        T most = largest;
+#pragma unroll
+        for (int i = 0; i < N; ++i) most = fmax(most, x[i]);
+        const T base = or_zero(most);  // nothing but -inf so far: every exponential is 0
+        if (most != largest) sum *= static_cast<double>(Exp<T>::of(largest - base, c));
+        largest = most;
+#pragma unroll
+        for (int i = 0; i < N; ++i) sum += static_cast<double>(Exp<T>::of(x[i] - base, c));
+    }
+    // the same over a wave
+    __device__ __forceinline__ void over_wave(T c) {
+        T most = largest;
+#pragma unroll
+        for (int m = 32; m > 0; m /= 2) most = fmax(most, __shfl_xor(most, m));
+        sum = wave_sum(sum * static_cast<double>(Exp<T>::of(largest - or_zero(most), c)));
+        largest = most;
+    }
+};
+
+template <typename T>
+__global__ __launch_bounds__(kNarrowRows * 64) void distill_narrow_rows_kernel(T* __restrict__ losses, T* __restrict__ stats,
+                                                                               const T* __restrict__ logits,
+                                                                               const int64_t* __restrict__ indices,
+                                                                               const T* __restrict__ teacher, int64_t rows,
+                                                                               int64_t cols, int kept, double temperature) {
+    const int64_t row = static_cast<int64_t>(blockIdx.x) * kNarrowRows + threadIdx.x / 64;
+    const int lane = threadIdx.x % 64;
+    if (row >= rows) return;
+    const T* z = logits + row * cols;
+    const T c = static_cast<T>(Exp<T>::kScale / temperature);
+    T x[kNarrow / 64];
+#pragma unroll
+    for (int i = 0; i < kNarrow / 64; ++i) x[i] = lane + 64 * i < cols ? z[lane + 64 * i] : static_cast<T>(-INFINITY);
+    Teacher<T> side{teacher + row * kept, indices + row * kept, cols, kept, temperature, 0, 0, false};
+    side.sum_up();
+    Running<T> run;
+    run.add(x, c);
+    run.over_wave(c);
+    const double loss = side.loss(z, run.largest, log(run.sum));
+    if (lane == 0) {
+        losses[row] = static_cast<T>(loss);
+        stats[2 * row] = run.largest;
+        stats[2 * row + 1] = static_cast<T>(run.sum);
+    }
+}
+
+template <typename T>
+__global__ __launch_bounds__(kMostThreads) void distill_rows_kernel(T* __restrict__ losses, T* __restrict__ stats,
+                                                                    const T* __restrict__ logits, const int64_t* __restrict__ indices,
+                                                                    const T* __restrict__ teacher, int64_t cols, int kept,
+                                                                    double temperature) {
+    __shared__ T wave_largest[kMostThreads / 64];
+    __shared__ double wave_sums[kMostThreads / 64];
+    constexpr int kCount = Piece<T>::kCount, kPieces = 4;
+    const int64_t row = blockIdx.x;
+    const int waves = blockDim.x / 64, wave = threadIdx.x / 64;
+    const T* z = logits + row * cols;
+    const T c = static_cast<T>(Exp<T>::kScale / temperature);
+    Running<T> run;
+    const int64_t step = static_cast<int64_t>(blockDim.x) * kCount;
+    for (int64_t at = static_cast<int64_t>(threadIdx.x) * kCount; at < cols; at += kPieces * step) {
+        T x[kPieces * kCount];
+#pragma unroll
+        for (int i = 0; i < kPieces; ++i) {
+            const Piece<T> p = load_piece(z, at + i * step, cols, static_cast<T>(-INFINITY));
+#pragma unroll
+            for (int j = 0; j < kCount; ++j) x[i * kCount + j] = p.x[j];
         }
-    loss = group_sum(loss, scratch);
+        run.add(x, c);
+    }
+    run.over_wave(c);
+    if (threadIdx.x % 64 == 0) {
+        wave_largest[wave] = run.largest;
+        wave_sums[wave] = run.sum;
+    }
+    Teacher<T> side{teacher + row * kept, indices + row * kept, cols, kept, temperature, 0, 0, false};
+    if (wave == 0) side.sum_up();
+    __syncthreads();
+    if (wave != 0) return;
+    T largest = -INFINITY;
+    for (int w = 0; w < waves; ++w) largest = fmax(largest, wave_largest[w]);
+    double sum = 0;
+    for (int w = 0; w < waves; ++w) sum += wave_sums[w] * static_cast<double>(Exp<T>::of(wave_largest[w] - or_zero(largest), c));
+    const double loss = side.loss(z, largest, log(sum));
     if (threadIdx.x == 0) {
-        losses[row] = static_cast<T>(temperature * temperature * loss);
+        losses[row] = static_cast<T>(loss);
         stats[2 * row] = largest;
         stats[2 * row + 1] = static_cast<T>(sum);
     }
 }
 
 template <typename T>
-__global__ __launch_bounds__(kRowThreads) void distill_grad_kernel(T* out, const T* logits, const T* __restrict__ stats,
-                                                                   const int64_t* __restrict__ indices,
-                                                                   const T* __restrict__ teacher, const T* __restrict__ row_weights,
-                                                                   int64_t cols, int kept, double temperature) {
-    __shared__ double scratch[kRowThreads / 64];
-    __shared__ int places[kMaxKept];
-    __shared__ T shares[kMaxKept];
-    const int64_t row = blockIdx.x;
-    const int64_t* index = indices + row * kept;
-    const T* t = teacher + row * kept;
-    const Teacher side = teacher_of(t, index, cols, kept, temperature, scratch);
-    for (int j = threadIdx.x; j < kept; j += kRowThreads) {
-        const bool in = side.any && index[j] >= 0 && index[j] < cols;
-        places[j] = in ? static_cast<int>(index[j]) : -1;
-        shares[j] = in ? static_cast<T>(exp((static_cast<double>(t[j]) - side.largest) / temperature - side.log_sum)) : T(0);
-    }
-    const T largest = stats[2 * row], inverse = static_cast<T>(1 / temperature);
+__global__ __launch_bounds__(kNarrowRows * 64) void distill_narrow_grad_kernel(T* out, const T* logits, const T* __restrict__ stats,
+                                                                               const int64_t* __restrict__ indices,
+                                                                               const T* __restrict__ teacher,
+                                                                               const T* __restrict__ row_weights, int64_t rows,
+                                                                               int64_t cols, int kept, double temperature) {
+    const int64_t row = static_cast<int64_t>(blockIdx.x) * kNarrowRows + threadIdx.x / 64;
+    const int lane = threadIdx.x % 64;
+    if (row >= rows) return;
+    const T* z = logits + row * cols;
+    T x[kNarrow / 64], taken[kNarrow / 64] = {};
+#pragma unroll
+    for (int i = 0; i < kNarrow / 64; ++i) x[i] = lane + 64 * i < cols ? z[lane + 64 * i] : T(0);
+    Teacher<T> side{teacher + row * kept, indices + row * kept, cols, kept, temperature, 0, 0, false};
+    side.sum_up();
+    // each entry's share to the lane that holds its column, in the entries' order
+    if (side.any)
+        for (int j0 = 0; j0 < kept; j0 += 64) {
+            const int j = j0 + lane;
+            const bool in = side.has(j);
+            const int place = in ? static_cast<int>(side.index[j]) : -1;
+            const T share = in ? static_cast<T>(exp(side.log_share(j))) : T(0);
+            for (int i = 0; i < min(64, kept - j0); ++i) {
+                const int to = __shfl(place, i);
+                const T add = __shfl(share, i);
+#pragma unroll
+                for (int n = 0; n < kNarrow / 64; ++n) taken[n] += to == lane + 64 * n ? add : T(0);
+            }
+        }
+    const T c = static_cast<T>(Exp<T>::kScale / temperature);
+    const T largest = stats[2 * row], weight = static_cast<T>(static_cast<double>(row_weights[row]) * temperature);
+    const T factor = weight / stats[2 * row + 1];
+    T* g = out + row * cols;
+#pragma unroll
+    for (int n = 0; n < kNarrow / 64; ++n)
+        if (lane + 64 * n < cols) g[lane + 64 * n] = side.any ? Exp<T>::of(x[n] - largest, c) * factor - weight * taken[n] : T(0);
+}
+
+// A workgroup takes `span` columns of a row. Shared memory: the kept entries' places and shares, and a table of the places
+// (twice their number or more, a power of two) in which a place that comes twice is found out.
+template <typename T>
+__global__ __launch_bounds__(kMostThreads) void distill_grad_kernel(T* out, const T* logits, const T* __restrict__ stats,
+                                                                    const int64_t* __restrict__ indices,
+                                                                    const T* __restrict__ teacher, const T* __restrict__ row_weights,
+                                                                    int64_t cols, int kept, double temperature, int64_t span,
+                                                                    int spans, int table_size) {
+    extern __shared__ char shared[];
+    T* shares = reinterpret_cast<T*>(shared);
+    int* places = reinterpret_cast<int*>(shares + kept);
+    int* table = places + kept;
+    __shared__ int twice;
+    constexpr int kCount = Piece<T>::kCount, kPieces = 4;
+    const int64_t row = blockIdx.x / spans, from = blockIdx.x % spans * span, to = min(from + span, cols);
+    Teacher<T> side{teacher + row * kept, indices + row * kept, cols, kept, temperature, 0, 0, false};
+    bool entry = false;
+    for (int j = threadIdx.x; j < kept; j += blockDim.x) entry = entry || (side.has(j) && side.t[j] != -INFINITY);
+    const bool any = __syncthreads_or(entry);
     const T weight = static_cast<T>(static_cast<double>(row_weights[row]) * temperature);
-    const T factor = side.any ? weight / stats[2 * row + 1] : T(0);
+    if (any && threadIdx.x < 64) {
+        const int lane = threadIdx.x;
+        for (int i = lane; i < table_size; i += 64) table[i] = -1;
+        if (lane == 0) twice = 0;
+        side.sum_up();
+        for (int j = lane; j < kept; j += 64) {
+            const bool in = side.has(j) && side.index[j] >= from && side.index[j] < to;
+            const int place = in ? static_cast<int>(side.index[j]) : -1;
+            places[j] = place;
+            shares[j] = in ? static_cast<T>(exp(side.log_share(j))) : T(0);
+            if (!in) continue;
+            // half of the table at least stays empty, so the walk ends
+            for (uint32_t at = static_cast<uint32_t>(place) * 2654435761u;; ++at) {
+                const int there = atomicCAS(&table[at & (table_size - 1)], -1, place);
+                if (there == place) twice = 1;
+                if (there == place || there == -1) break;
+            }
+        }
+    }
+    const T c = static_cast<T>(Exp<T>::kScale / temperature);
+    const T largest = stats[2 * row], factor = weight / stats[2 * row + 1];
     const T* z = logits + row * cols;
     T* g = out + row * cols;
-    for (int64_t c = threadIdx.x; c < cols; c += kRowThreads) g[c] = std::exp((z[c] - largest) * inverse) * factor;
+    const int64_t step = static_cast<int64_t>(blockDim.x) * kCount;
+    for (int64_t at = from + static_cast<int64_t>(threadIdx.x) * kCount; at < to; at += kPieces * step) {
+        Piece<T> p[kPieces];
+#pragma unroll
+        for (int i = 0; i < kPieces; ++i) p[i] = load_piece(z, at + i * step, to, T(0));
+#pragma unroll
+        for (int i = 0; i < kPieces; ++i) {
+            const int64_t own = at + i * step;
+#pragma unroll
+            for (int j = 0; j < kCount; ++j) p[i].x[j] = any ? Exp<T>::of(p[i].x[j] - largest, c) * factor : T(0);
+            if (own + kCount <= to) {
+                __builtin_memcpy(g + own, &p[i], 16);
+            } else {
+#pragma unroll
+                for (int j = 0; j < kCount; ++j)
+                    if (own + j < to) g[own + j] = p[i].x[j];
+            }
+        }
+    }
+    if (!any) return;
     __syncthreads();
-    // the first entry of a place takes off the shares of all entries there
-    for (int j = threadIdx.x; j < kept; j += kRowThreads) {
+    for (int j = threadIdx.x; j < kept; j += blockDim.x) {
         const int place = places[j];
         if (place < 0) continue;
-        bool first = true;
-        for (int i = 0; i < j; ++i) first = first && places[i] != place;
-        if (!first) continue;
-        T share = 0;
-        for (int i = j; i < kept; ++i) share += places[i] == place ? shares[i] : T(0);
+        T share = shares[j];
+        if (twice) {
+            // the first entry of a place takes the shares of all entries there
+            bool first = true;
+            for (int i = 0; i < j; ++i) first = first && places[i] != place;
+            if (!first) continue;
+            for (int i = j + 1; i < kept; ++i) share += places[i] == place ? shares[i] : T(0);
+        }
         g[place] -= weight * share;
     }
 }
@@ -262,6 +495,13 @@ int check_distill(const char* what, int dtype, int64_t rows, int64_t cols, int64
     if (kept < 1 || kept > kMaxKept) return fail(KD_E_INVALID, name + ": 1 to 1024 kept entries");
     if (!(temperature > 0) || !std::isfinite(temperature)) return fail(KD_E_INVALID, name + ": temperature must be positive");
     return KD_OK;
+}
+
+// Threads of a row's workgroup: one wave for short rows, 1024 threads for long ones where there are too few to fill the card
+// with 256.
+int row_threads(int64_t rows, int64_t cols) {
+    if (cols <= 1024) return 64;
+    return rows < 2 * compute_units() && cols >= 8192 ? kMostThreads : 256;
 }
 
 } // namespace
@@ -303,9 +543,15 @@ extern "C" int kd_distill_rows(int dtype, void* losses, void* stats, const void*
     if (int rc = ensure_device()) return rc;
     const auto launch = [&](auto zero) {
         using T = decltype(zero);
-        hipLaunchKernelGGL((distill_rows_kernel<T>), dim3(static_cast<uint32_t>(rows)), dim3(kRowThreads), 0, stream(),
-                           static_cast<T*>(losses), static_cast<T*>(stats), static_cast<const T*>(logits), indices,
-                           static_cast<const T*>(teacher), cols, static_cast<int>(kept), temperature);
+        if (cols <= kNarrow)
+            hipLaunchKernelGGL((distill_narrow_rows_kernel<T>), dim3(static_cast<uint32_t>((rows + kNarrowRows - 1) / kNarrowRows)),
+                               dim3(kNarrowRows * 64), 0, stream(), static_cast<T*>(losses), static_cast<T*>(stats),
+                               static_cast<const T*>(logits), indices, static_cast<const T*>(teacher), rows, cols,
+                               static_cast<int>(kept), temperature);
+        else
+            hipLaunchKernelGGL((distill_rows_kernel<T>), dim3(static_cast<uint32_t>(rows)), dim3(row_threads(rows, cols)), 0, stream(),
+                               static_cast<T*>(losses), static_cast<T*>(stats), static_cast<const T*>(logits), indices,
+                               static_cast<const T*>(teacher), cols, static_cast<int>(kept), temperature);
     };
     if (dtype == KD_F32) launch(0.f);
     else launch(0.0);
@@ -324,10 +570,26 @@ extern "C" int kd_distill_grad(int dtype, void* out, const void* logits, const v
     if (int rc = ensure_device()) return rc;
     const auto launch = [&](auto zero) {
         using T = decltype(zero);
-        hipLaunchKernelGGL((distill_grad_kernel<T>), dim3(static_cast<uint32_t>(rows)), dim3(kRowThreads), 0, stream(),
-                           static_cast<T*>(out), static_cast<const T*>(logits), static_cast<const T*>(stats), indices,
-                           static_cast<const T*>(teacher), static_cast<const T*>(row_weights), cols, static_cast<int>(kept),
-                           temperature);
+        if (cols <= kNarrow) {
+            hipLaunchKernelGGL((distill_narrow_grad_kernel<T>), dim3(static_cast<uint32_t>((rows + kNarrowRows - 1) / kNarrowRows)),
+                               dim3(kNarrowRows * 64), 0, stream(), static_cast<T*>(out), static_cast<const T*>(logits),
+                               static_cast<const T*>(stats), indices, static_cast<const T*>(teacher),
+                               static_cast<const T*>(row_weights), rows, cols, static_cast<int>(kept), temperature);
+            return;
+        }
+        // few rows: parts of them to a workgroup, in whole rounds of it
+        const int threads = row_threads(rows, cols);
+        const int64_t round = int64_t{threads} * 4 * Piece<T>::kCount;
+        const int64_t wanted = std::max<int64_t>(1, 2 * compute_units() / rows);
+        const int64_t span = std::max<int64_t>(1, (cols + round * wanted - 1) / (round * wanted)) * round;
+        const int64_t spans = (cols + span - 1) / span;
+        int table = 2;
+        while (table < 2 * kept) table *= 2;
+        hipLaunchKernelGGL((distill_grad_kernel<T>), dim3(static_cast<uint32_t>(rows * spans)), dim3(threads),
+                           static_cast<uint32_t>(kept * (sizeof(T) + 4) + table * 4), stream(), static_cast<T*>(out),
+                           static_cast<const T*>(logits), static_cast<const T*>(stats), indices, static_cast<const T*>(teacher),
+                           static_cast<const T*>(row_weights), cols, static_cast<int>(kept), temperature, span,
+                           static_cast<int>(spans), table);
     };
     if (dtype == KD_F32) launch(0.f);
     else launch(0.0);

@@ -6,6 +6,7 @@
 // attention's products sum over. Everything that a caller's arrays can say wrongly (a table entry that is no page, a
 // start or a length out of range) is checked here against the sizes that the host passed.
 #include <algorithm>
+#include <type_traits>
 
 #include "kd_internal.h"
 
@@ -54,27 +55,85 @@ __device__ __forceinline__ int64_t page_of(const Paged& c, int s, int64_t column
     return page >= 0 && page < c.pages ? page : -1;
 }
 
-// Work is handed out by slots: sequence s owns the slots base(s) .. base(s + 1) - 1, base ascending. The sequence that slot
-// `slot` belongs to, or -1 for none, found by a whole wave (every lane of it has to call this) in one load for up to
-// 64 sequences, two for up to 4096.
-template <class Base> __device__ __forceinline__ int find_sequence(int64_t slot, int sequences, const Base& base) {
+// Work is handed out by slots: sequence s owns the slots base(start, s) .. base(next start, s + 1) - 1, base ascending. Which
+// sequence a slot belongs to (s < 0 for none) is found by a whole wave, every lane of which has to call this: in one round
+// of loads with the sequence's rows for up to 64 sequences, and 64 at a time beyond (two rounds up to 4096).
+struct Found {
+    int s;
+    int64_t base;
+    Rows rows;
+};
+
+template <class Base> __device__ __forceinline__ Found find_sequence(const Paged& c, int64_t slot, const Base& base) {
     const int lane = threadIdx.x % 64;
-    int low = 0, count = sequences;
-    bool any = false;
-    while (count > 1 || !any) {
+    if (c.sequences <= 64) {
+        const int s = min(lane, c.sequences - 1);
+        const Rows rows = rows_of(c, s);
+        const int64_t own = base(rows.row, s);
+        const int n = __popcll(__ballot(lane < c.sequences && own <= slot));
+        if (n == 0) return {-1, 0, {}};
+        return {n - 1, __shfl(own, n - 1), {__shfl(rows.row, n - 1), __shfl(rows.count, n - 1), __shfl(rows.position, n - 1)}};
+    }
+    int low = 0, count = c.sequences;
+    while (count > 1) {
         const int step = (count + 63) / 64;
-        const int at = lane * step;
-        const bool below = at < count && base(low + at) <= slot;
-        const int n = __popcll(__ballot(below));
-        if (n == 0) return -1;
-        any = true;
+        const int at = low + lane * step;
+        const int n = __popcll(__ballot(lane * step < count && base(start_of(c, at < c.sequences ? at : 0), at) <= slot));
+        if (n == 0) return {-1, 0, {}};
         low += (n - 1) * step;
         count = min(step, count - (n - 1) * step);
     }
-    return low;
+    const Rows rows = rows_of(c, low);
+    return {low, base(rows.row, low), rows};
+}
+
+// Walks on from a sequence that begins at or before `token` to the one that holds it; s is c.sequences where none does.
+__device__ __forceinline__ void walk_to(const Paged& c, int token, int& s, Rows& rows) {
+    while (s < c.sequences && token >= rows.row + rows.count) {
+        ++s;
+        if (s < c.sequences) rows = rows_of(c, s);
+    }
+}
+
+// The new tokens of one page, as the workgroup of `slot` sees them: slots held .. held + count - 1 of table column `column`.
+struct PageSlots {
+    int s;
+    int row;        // batch row of the first of them
+    int64_t first;  // its position
+    int64_t page;   // -1 for none
+    int held, count;
+    bool leads;     // the first slot of its sequence
+    Rows rows;
+};
+
+// A sequence's new tokens touch at most (count + 2 size - 2) / size pages; base(s + 1) - base(s) is at least that.
+__host__ __device__ inline int64_t page_base(int64_t start, int64_t s, int shift) {
+    return (start + s * ((int64_t{2} << shift) - 2)) >> shift;
+}
+
+__device__ __forceinline__ PageSlots page_slots(const Paged& c, int64_t slot) {
+    const Found f = find_sequence(c, slot, [&](int64_t start, int64_t s) { return page_base(start, s, c.page_shift); });
+    PageSlots p{f.s, 0, 0, -1, 0, 0, false, f.rows};
+    if (f.s < 0) return p;
+    const int64_t begin = max(f.rows.position, int64_t{0}), end = f.rows.position + f.rows.count;
+    const int64_t column = (begin >> c.page_shift) + (slot - f.base);
+    const int64_t from = max(begin, column << c.page_shift), to = min(end, (column + 1) << c.page_shift);
+    p.leads = slot == f.base;
+    if (from >= to) return p;
+    p.page = page_of(c, f.s, column);
+    p.row = f.rows.row + static_cast<int>(from - f.rows.position);
+    p.first = from;
+    p.held = static_cast<int>(from - (column << c.page_shift));
+    p.count = static_cast<int>(to - from);
+    return p;
 }
 
 // ---- append ---------------------------------------------------------------------------------------
+//
+// Bound by the bytes of q, k and v for prompts, by the chain of dependent loads (starts and lengths, table, scale, rows) for
+// single tokens. One launch: a workgroup takes one page of one kv head, its keys or its values, so that the page's scale
+// has one owner, and the workgroups behind those take the queries. Rotated and quantised in f64, where the products of two
+// f32 are exact and a rounding to the wrong side of a tie takes a value within 2^-45 of it: f64 costs less here than the bytes.
 
 struct Rotation {
     const float* cosines;
@@ -89,118 +148,262 @@ struct Strided {
     int64_t row, head;
 };
 
-// Feature d of the row x, rotated by `position`'s angle, in f64: the products of two f32 are exact there.
-__device__ __forceinline__ double rotated(const float* x, int d, int64_t position, const Rotation& r) {
-    if (d >= 2 * r.half) return x[d];
-    const int pair = r.interleaved ? d / 2 : d % r.half;
-    const bool second = r.interleaved ? d % 2 != 0 : d >= r.half;
-    const double a = x[r.interleaved ? 2 * pair : pair], b = x[r.interleaved ? 2 * pair + 1 : pair + r.half];
-    double c = NAN, s = NAN;
-    if (position < r.positions) {
-        c = r.cosines[position * r.half + pair];
-        s = r.sines[position * r.half + pair];
+constexpr int kUnit = 8;  // features of a thread: four pairs, or eight that are not rotated
+
+template <bool Vector> __device__ __forceinline__ void load4(const float* p, float (&x)[4]) {
+    if constexpr (Vector) {
+        const float4 v = *reinterpret_cast<const float4*>(p);
+        x[0] = v.x, x[1] = v.y, x[2] = v.z, x[3] = v.w;
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] = p[i];
     }
-    return second ? b * c + a * s : a * c - b * s;
+}
+
+// Where unit u of a row has its two runs of four features. Without Vector a unit is eight features that follow each other.
+template <bool Vector> __device__ __forceinline__ void unit_places(int u, const Rotation& r, int& low, int& high) {
+    low = kUnit * u;
+    high = low + 4;
+    if (Vector && !r.interleaved && low < 2 * r.half) {
+        low = 4 * u;
+        high = low + r.half;
+    }
+}
+
+// The unit of the row x, rotated by `position`'s angles, in f64. Vector: pairs never cross a unit and everything is 16-byte
+// aligned; otherwise each feature finds its partner.
+template <bool Vector>
+__device__ __forceinline__ void rotated_unit(const float* x, int low, int high, int64_t position, const Rotation& r, double (&y)[kUnit]) {
+    float a[4], b[4];
+    load4<Vector>(x + low, a);
+    load4<Vector>(x + high, b);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        y[i] = a[i];
+        y[4 + i] = b[i];
+    }
+    if (low >= 2 * r.half) return;
+    const bool known = position < r.positions;
+    if constexpr (Vector) {
+        float c[4] = {NAN, NAN, NAN, NAN}, s[4] = {NAN, NAN, NAN, NAN};
+        if (known) {
+            const int64_t at = position * r.half + (r.interleaved ? low / 2 : low);
+            load4<true>(r.cosines + at, c);
+            load4<true>(r.sines + at, s);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            // pair i of the unit: its features 2 i and 2 i + 1, or feature i of either run
+            const double p = r.interleaved ? (i < 2 ? a[2 * i % 4] : b[2 * i % 4]) : a[i];
+            const double q = r.interleaved ? (i < 2 ? a[(2 * i + 1) % 4] : b[(2 * i + 1) % 4]) : b[i];
+            const double turned = p * c[i] - q * s[i], other = q * c[i] + p * s[i];
+            if (r.interleaved) {
+                y[2 * i] = turned;
+                y[2 * i + 1] = other;
+            } else {
+                y[i] = turned;
+                y[4 + i] = other;
+            }
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < kUnit; ++i) {
+            const int d = low + i;
+            if (d >= 2 * r.half) break;
+            const int pair = r.interleaved ? d / 2 : d % r.half;
+            const bool second = r.interleaved ? d % 2 != 0 : d >= r.half;
+            const double p = x[r.interleaved ? 2 * pair : pair], q = x[r.interleaved ? 2 * pair + 1 : pair + r.half];
+            const double c = known ? r.cosines[position * r.half + pair] : NAN, s = known ? r.sines[position * r.half + pair] : NAN;
+            y[i] = second ? q * c + p * s : p * c - q * s;
+        }
+    }
+}
+
+__device__ __forceinline__ uint32_t code_of(double x, double inverse) {
+    const double r = rint(x * inverse);
+    return r != r ? 0u : static_cast<uint32_t>(static_cast<int>(fmin(fmax(r, -127.0), 127.0))) & 0xffu;
 }
 
 constexpr int kAppendThreads = 256;
 
-// A sequence's new tokens touch at most (count + 2 size - 2) / size pages; base(s + 1) - base(s) is at least that.
-__host__ __device__ inline int64_t append_base(int64_t start, int64_t s, int shift) {
-    return (start + s * ((int64_t{2} << shift) - 2)) >> shift;
-}
-
+template <bool Vector>
 __global__ __launch_bounds__(kAppendThreads) void paged_append_kernel(Paged c, Rotation rotation, Strided k, Strided v,
                                                                       Strided q, float* __restrict__ q_out, int heads,
-                                                                      int64_t cache_groups) {
-    const int group = c.kv_heads * 2;
+                                                                      int64_t cache_groups, int q_tokens) {
+    const int dim = c.head_dim, units = dim / kUnit, threads = blockDim.x;
     if (static_cast<int64_t>(blockIdx.x) >= cache_groups) {
-        // the queries, one element a thread
-        const int64_t i = (static_cast<int64_t>(blockIdx.x) - cache_groups) * kAppendThreads + threadIdx.x;
-        const int64_t per_row = static_cast<int64_t>(heads) * c.head_dim;
-        const int first = static_cast<int>((static_cast<int64_t>(blockIdx.x) - cache_groups) * kAppendThreads / per_row);
-        const int64_t row = i / per_row;
-        // a wave's elements may belong to two rows: each lane looks from the first one's sequence on
-        int s = find_sequence(first, c.sequences, [&](int at) { return int64_t{start_of(c, at)}; });
-        s = max(s, 0);
-        while (s < c.sequences && start_of(c, s + 1) <= row) ++s;
-        if (row >= c.tokens || s >= c.sequences) return;
-        const Rows rows = rows_of(c, s);
-        if (row < rows.row) return;
-        const int h = static_cast<int>(i % per_row) / c.head_dim, d = static_cast<int>(i % c.head_dim);
-        const int64_t position = rows.position + (row - rows.row);
-        const float* x = q.data + row * q.row + h * q.head;
-        q_out[i] = position < 0 ? NAN : static_cast<float>(rotated(x, d, position, rotation));
+        // the queries of q_tokens tokens
+        const int64_t token0 = (static_cast<int64_t>(blockIdx.x) - cache_groups) * q_tokens;
+        Found f = find_sequence(c, token0, [&](int64_t start, int64_t) { return start; });
+        if (f.s < 0) f = {0, 0, rows_of(c, 0)};
+        const uint32_t per_token = static_cast<uint32_t>(heads) * units;
+        for (uint32_t i = threadIdx.x; i < q_tokens * per_token; i += threads) {
+            const int64_t token = token0 + i / per_token;
+            if (token >= c.tokens) return;
+            int s = f.s;
+            Rows rows = f.rows;
+            walk_to(c, static_cast<int>(token), s, rows);
+            if (s >= c.sequences || token < rows.row) continue;
+            const uint32_t h = i % per_token / units;
+            int low, high;
+            unit_places<Vector>(i % units, rotation, low, high);
+            const int64_t position = rows.position + (token - rows.row);
+            double y[kUnit];
+            rotated_unit<Vector>(q.data + token * q.row + h * q.head, low, high, position, rotation, y);
+            float* out = q_out + (token * heads + h) * dim;
+            const auto at = [&](int j) { return position < 0 ? NAN : static_cast<float>(y[j]); };
+            *reinterpret_cast<float4*>(out + low) = make_float4(at(0), at(1), at(2), at(3));
+            *reinterpret_cast<float4*>(out + high) = make_float4(at(4), at(5), at(6), at(7));
+        }
         return;
     }
-    const int64_t slot = blockIdx.x / group;
+    const uint32_t group = c.kv_heads * 2;
     const int h = static_cast<int>(blockIdx.x % group) / 2;
     const bool keys = blockIdx.x % 2 == 0;
     const int size = 1 << c.page_shift;
-    const int s = find_sequence(slot, c.sequences, [&](int at) { return append_base(start_of(c, at), at, c.page_shift); });
-    if (s < 0) return;
-    const Rows rows = rows_of(c, s);
-    const int64_t begin = max(rows.position, int64_t{0}), end = rows.position + rows.count;
-    const int64_t column = (begin >> c.page_shift) + (slot - append_base(start_of(c, s), s, c.page_shift));
-    const int64_t from = max(begin, column << c.page_shift), to = min(end, (column + 1) << c.page_shift);
-    if (from >= to) return;
-    const int64_t page = page_of(c, s, column);
-    if (page < 0) return;
-    const int held = static_cast<int>(from - (column << c.page_shift));  // slots that the page holds already
-    const int count = static_cast<int>(to - from);
-    const int dim = c.head_dim;
-    const int64_t at = page * c.kv_heads + h;
+    const PageSlots p = page_slots(c, blockIdx.x / group);
+    if (p.page < 0) return;
+    const int64_t at = p.page * c.kv_heads + h;
     int8_t* codes = (keys ? c.keys : c.values) + at * size * dim;
     float* scales = keys ? c.key_scales : c.value_scales;
+    const float old = p.held > 0 ? scales[at] : 0.f;
     const Strided in = keys ? k : v;
-    const float* x = in.data + (rows.row + (from - rows.position)) * in.row + h * in.head;
-    const auto value = [&](int token, int d) -> double {
-        const float* row = x + token * in.row;
-        return keys ? rotated(row, d, from + token, rotation) : static_cast<double>(row[d]);
-    };
+    const float* x = in.data + static_cast<int64_t>(p.row) * in.row + h * in.head;
+    // keys: a unit of a token; values: a feature of 16 tokens that begin at a multiple of 16 slots
+    const int key_units = p.count * units;
+    const int chunk0 = p.held / 16, value_units = ((p.held + p.count + 15) / 16 - chunk0) * dim;
     double most = 0;
-    for (int i = threadIdx.x; i < count * dim; i += kAppendThreads) most = max_na(most, fabs(value(i / dim, i % dim)));
-    for (int m = 32; m > 0; m /= 2) most = max_na(most, __shfl_xor(most, m));
+    if (keys) {
+        for (int i = threadIdx.x; i < key_units; i += threads) {
+            const int token = i / units;
+            int low, high;
+            unit_places<Vector>(i % units, rotation, low, high);
+            double y[kUnit];
+            rotated_unit<Vector>(x + token * in.row, low, high, p.first + token, rotation, y);
+#pragma unroll
+            for (int j = 0; j < kUnit; ++j) most = max_na(most, fabs(y[j]));
+        }
+    } else {
+        float largest = 0;
+        for (int i = threadIdx.x; i < value_units; i += threads) {
+            const int slot0 = (chunk0 + i / dim) * 16;
+            float y[16];
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+                const int token = slot0 + j - p.held;
+                y[j] = token >= 0 && token < p.count ? x[token * in.row + i % dim] : 0.f;
+            }
+#pragma unroll
+            for (int j = 0; j < 16; ++j) largest = max_na(largest, fabsf(y[j]));
+        }
+        most = largest;
+    }
     __shared__ double wave_most[kAppendThreads / 64];
-    if (threadIdx.x % 64 == 0) wave_most[threadIdx.x / 64] = most;
-    const float old = held > 0 ? scales[at] : 0.f;
-    __syncthreads();
-    for (int w = 0; w < kAppendThreads / 64; ++w) most = max_na(most, wave_most[w]);
+#pragma unroll
+    for (int m = 32; m > 0; m /= 2) most = max_na(most, __shfl_xor(most, m));
+    if (threads > 64) {
+        if (threadIdx.x % 64 == 0) wave_most[threadIdx.x / 64] = most;
+        __syncthreads();
+        for (int w = 0; w < threads / 64; ++w) most = max_na(most, wave_most[w]);
+    }
     const float scale = most < INFINITY ? max_na(old, static_cast<float>(most / 127)) : NAN;
     if (threadIdx.x == 0) scales[at] = scale;
     const double inverse = scale > 0 ? 1.0 / scale : 0.0;  // 0 for NaN too
-    for (int i = threadIdx.x; i < count * dim; i += kAppendThreads) {
-        const int token = i / dim, d = i % dim;
-        const double r = rint(value(token, d) * inverse);
-        const int code = r != r ? 0 : static_cast<int>(fmin(fmax(r, -127.0), 127.0));
-        codes[keys ? (held + token) * dim + d : d * size + held + token] = static_cast<int8_t>(code);
+    if (keys) {
+        for (int i = threadIdx.x; i < key_units; i += threads) {
+            const int token = i / units;
+            int low, high;
+            unit_places<Vector>(i % units, rotation, low, high);
+            double y[kUnit];
+            rotated_unit<Vector>(x + token * in.row, low, high, p.first + token, rotation, y);
+            uint32_t word[2] = {};
+#pragma unroll
+            for (int j = 0; j < kUnit; ++j) word[j / 4] |= code_of(y[j], inverse) << (8 * (j % 4));
+            int8_t* to = codes + (p.held + token) * dim;
+            *reinterpret_cast<uint32_t*>(to + low) = word[0];
+            *reinterpret_cast<uint32_t*>(to + high) = word[1];
+        }
+    } else {
+        for (int i = threadIdx.x; i < value_units; i += threads) {
+            const int slot0 = (chunk0 + i / dim) * 16, d = i % dim;
+            int8_t* to = codes + d * size + slot0;
+            const int from = max(p.held - slot0, 0), end = min(p.held + p.count - slot0, 16);
+            const float* row = x + static_cast<int64_t>(slot0 - p.held) * in.row + d;
+            if (from == 0 && end == 16) {
+                float y[16];
+#pragma unroll
+                for (int j = 0; j < 16; ++j) y[j] = row[j * in.row];
+                uint4 words = make_uint4(0, 0, 0, 0);
+                uint32_t* word = &words.x;
+#pragma unroll
+                for (int j = 0; j < 16; ++j) word[j / 4] |= code_of(y[j], inverse) << (8 * (j % 4));
+                *reinterpret_cast<uint4*>(to) = words;
+            } else {
+                for (int j = from; j < end; ++j) to[j] = static_cast<int8_t>(code_of(row[j * in.row], inverse));
+            }
+        }
     }
     if (scale > old) {
         const double ratio = static_cast<double>(old) / scale;
-        for (int i = threadIdx.x; i < held * dim; i += kAppendThreads) {
-            int8_t* p = codes + (keys ? i : i / held * size + i % held);
-            *p = static_cast<int8_t>(rint(*p * ratio));
+        for (int i = threadIdx.x; i < p.held * dim; i += threads) {
+            int8_t* code = codes + (keys ? i : i / p.held * size + i % p.held);
+            *code = static_cast<int8_t>(rint(*code * ratio));
         }
     }
 }
 
 // ---- read -----------------------------------------------------------------------------------------
+//
+// The append's division into pages: four codes a thread and a 16-byte store for the keys, a feature's 16 tokens a thread for
+// the values, so that codes are read in whole pieces and rows written in whole lines.
 
 __global__ __launch_bounds__(256) void paged_read_kernel(Paged c, float* __restrict__ k, float* __restrict__ v) {
-    const int64_t row = blockIdx.x;
-    const int s = find_sequence(row, c.sequences, [&](int at) { return int64_t{start_of(c, at)}; });
-    if (s < 0) return;
-    const Rows rows = rows_of(c, s);
-    if (row >= rows.row + rows.count) return;
-    const int64_t position = rows.position + (row - rows.row);
-    const int64_t page = position < 0 ? -1 : page_of(c, s, position >> c.page_shift);
-    const int size = 1 << c.page_shift, slot = static_cast<int>(position & (size - 1));
-    for (int i = threadIdx.x; i < c.kv_heads * c.head_dim; i += 256) {
-        const int h = i / c.head_dim, d = i % c.head_dim;
-        const int64_t at = page * c.kv_heads + h, base = at * size * c.head_dim;
-        const int64_t to = row * c.kv_heads * c.head_dim + i;
-        if (k != nullptr) k[to] = page < 0 ? 0.f : static_cast<float>(c.keys[base + slot * c.head_dim + d]) * c.key_scales[at];
-        if (v != nullptr) v[to] = page < 0 ? 0.f : static_cast<float>(c.values[base + d * size + slot]) * c.value_scales[at];
+    const uint32_t group = c.kv_heads * 2;
+    const int h = static_cast<int>(blockIdx.x % group) / 2;
+    const bool keys = blockIdx.x % 2 == 0;
+    float* out = keys ? k : v;
+    if (out == nullptr) return;
+    const int dim = c.head_dim, size = 1 << c.page_shift, threads = blockDim.x;
+    const PageSlots p = page_slots(c, blockIdx.x / group);
+    if (p.s < 0) return;
+    const int64_t row_size = static_cast<int64_t>(c.kv_heads) * dim;
+    out += h * dim;
+    const auto clear = [&](int row, int count) {
+        for (int i = threadIdx.x; i < count * (dim / 4); i += threads)
+            *reinterpret_cast<float4*>(out + (row + i / (dim / 4)) * row_size + i % (dim / 4) * 4) = make_float4(0, 0, 0, 0);
+    };
+    // rows before position 0 have no page
+    if (p.leads && p.rows.position < 0) clear(p.rows.row, static_cast<int>(min(int64_t{p.rows.count}, -p.rows.position)));
+    if (p.count == 0) return;
+    if (p.page < 0) {
+        clear(p.row, p.count);
+        return;
+    }
+    const int64_t at = p.page * c.kv_heads + h;
+    out += p.row * row_size;
+    if (keys) {
+        const float scale = c.key_scales[at];
+        const int8_t* codes = c.keys + (at * size + p.held) * dim;
+        for (int i = threadIdx.x; i < p.count * (dim / 4); i += threads) {
+            const char4 x = *reinterpret_cast<const char4*>(codes + 4 * i);
+            *reinterpret_cast<float4*>(out + i / (dim / 4) * row_size + i % (dim / 4) * 4) =
+                make_float4(x.x * scale, x.y * scale, x.z * scale, x.w * scale);
+        }
+    } else {
+        const float scale = c.value_scales[at];
+        const int8_t* codes = c.values + at * size * dim;
+        const int chunk0 = p.held / 16, chunks = (p.held + p.count + 15) / 16 - chunk0;
+        for (int i = threadIdx.x; i < chunks * dim; i += threads) {
+            const int slot0 = (chunk0 + i / dim) * 16, d = i % dim;
+            const uint4 words = *reinterpret_cast<const uint4*>(codes + d * size + slot0);
+            const uint32_t* word = &words.x;
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+                const int token = slot0 + j - p.held;
+                if (token >= 0 && token < p.count)
+                    out[token * row_size + d] = static_cast<float>(static_cast<int8_t>(word[j / 4] >> (8 * (j % 4)))) * scale;
+            }
+        }
     }
 }
 
@@ -290,11 +493,12 @@ __global__ __launch_bounds__(kAttentionWaves * 64, 2) void paged_attention_kerne
     const int kv = blockIdx.x / split.count % c.kv_heads;
     // the last rows see most keys and go first
     const int64_t tile = tile_base(c.tokens, c.sequences, group) - 1 - blockIdx.x / split.count / c.kv_heads;
-    const int s = find_sequence(tile, c.sequences, [&](int at) { return tile_base(start_of(c, at), at, group); });
-    if (s < 0) return;
-    const Rows rows = rows_of(c, s);
+    const Found found = find_sequence(c, tile, [&](int64_t start, int64_t at) { return tile_base(start, at, group); });
+    if (found.s < 0) return;
+    const int s = found.s;
+    const Rows rows = found.rows;
     // tokens * heads is below 2^31, and so are the rows of a kv head
-    const int64_t tile_at = (tile - tile_base(rows.row, s, group)) * kTileRows;
+    const int64_t tile_at = (tile - found.base) * kTileRows;
     const int row_end = rows.count * group;
     if (tile_at < 0 || tile_at >= row_end) return;
     const int row0 = static_cast<int>(tile_at);
@@ -518,9 +722,9 @@ __global__ __launch_bounds__(256) void paged_join_kernel(Paged c, float* __restr
     const int lane = threadIdx.x % 64;
     if (row >= static_cast<int64_t>(c.tokens) * heads) return;
     const int token = static_cast<int>(row / heads);
-    const int s = find_sequence(token, c.sequences, [&](int at) { return int64_t{start_of(c, at)}; });
-    if (s < 0) return;
-    const Rows rows = rows_of(c, s);
+    const Found found = find_sequence(c, token, [&](int64_t start, int64_t) { return start; });
+    if (found.s < 0) return;
+    const Rows rows = found.rows;
     if (token >= rows.row + rows.count) return;
     const int64_t limit = min(rows.position + (token - rows.row) + 1, static_cast<int64_t>(c.columns) << c.page_shift);
     // the parts that begin before the row's limit were worked on, and the first one always
@@ -657,12 +861,24 @@ extern "C" int kd_paged_append(int dtype, const kd_paged_cache* cache, const kd_
     if (int rc = check_strided(what, "k", k, k_strides, c.tokens, c.kv_heads, ks)) return rc;
     if (int rc = check_strided(what, "v", v, v_strides, c.tokens, c.kv_heads, vs)) return rc;
     if (int rc = ensure_device()) return rc;
-    const int64_t cache_groups = append_base(c.tokens, c.sequences, c.page_shift) * c.kv_heads * 2;
-    const int64_t q_groups =
-        q == nullptr ? 0 : (heads * c.tokens * c.head_dim + kAppendThreads - 1) / kAppendThreads;
+    // four units a thread and pass at most, one wave where few tokens a sequence leave most of a page alone
+    int threads = static_cast<int>(std::clamp<int64_t>((int64_t{c.head_dim} << c.page_shift) / (4 * kUnit), 64, kAppendThreads));
+    if (c.tokens <= 4 * static_cast<int64_t>(c.sequences)) threads = 64;
+    const int64_t cache_groups = page_base(c.tokens, c.sequences, c.page_shift) * c.kv_heads * 2;
+    const int64_t per_token = heads * (c.head_dim / kUnit);
+    const int q_tokens = q == nullptr ? 1 : static_cast<int>(std::max<int64_t>(1, 4 * threads / per_token));
+    const int64_t q_groups = q == nullptr ? 0 : (c.tokens + q_tokens - 1) / q_tokens;
     if (int rc = check_grid(what, cache_groups + q_groups)) return rc;
-    hipLaunchKernelGGL(paged_append_kernel, dim3(static_cast<uint32_t>(cache_groups + q_groups)), dim3(kAppendThreads), 0,
-                       stream(), c, r, ks, vs, qs, static_cast<float*>(q_out), static_cast<int>(heads), cache_groups);
+    // 16-byte pieces need rows and tables that keep them aligned and pairs that come in fours
+    const auto whole = [](const Strided& x) { return aligned(x.data, 16) && x.row % 4 == 0 && x.head % 4 == 0; };
+    const bool vector = r.half % 4 == 0 && aligned(r.cosines, 16) && aligned(r.sines, 16) && whole(ks) && (q == nullptr || whole(qs));
+    const auto launch = [&](auto v_) {
+        hipLaunchKernelGGL((paged_append_kernel<decltype(v_)::value>), dim3(static_cast<uint32_t>(cache_groups + q_groups)),
+                           dim3(threads), 0, stream(), c, r, ks, vs, qs, static_cast<float*>(q_out), static_cast<int>(heads),
+                           cache_groups, q_tokens);
+    };
+    if (vector) launch(std::true_type{});
+    else launch(std::false_type{});
     KD_LAUNCH_CHECK();
     return KD_OK;
 }
@@ -673,8 +889,10 @@ extern "C" int kd_paged_read(int dtype, void* k, void* v, const kd_paged_cache* 
     if (!aligned(k, 16) || !aligned(v, 16)) return fail(KD_E_INVALID, "kd_paged_read: k and v must be 16-byte aligned");
     if (c.sequences == 0 || c.tokens == 0 || (k == nullptr && v == nullptr)) return KD_OK;
     if (int rc = ensure_device()) return rc;
-    hipLaunchKernelGGL(paged_read_kernel, dim3(static_cast<uint32_t>(c.tokens)), dim3(256), 0, stream(), c,
-                       static_cast<float*>(k), static_cast<float*>(v));
+    const int64_t groups = page_base(c.tokens, c.sequences, c.page_shift) * c.kv_heads * 2;
+    if (int rc = check_grid("kd_paged_read", groups)) return rc;
+    hipLaunchKernelGGL(paged_read_kernel, dim3(static_cast<uint32_t>(groups)), dim3(c.page_shift <= 5 ? 64 : 256), 0, stream(),
+                       c, static_cast<float*>(k), static_cast<float*>(v));
     KD_LAUNCH_CHECK();
     return KD_OK;
 }

@@ -73,6 +73,47 @@ def test_append_is_its_definition(kdb, case, interleaved):
     same_cache(run_append(kdb, again.cache, starts, lengths, tokens, x, heads, rotation)[0].read_back(), want)
 
 
+@pytest.mark.parametrize("features,interleaved,shift", [(2, False, 0), (6, True, 0), (50, False, 0), (64, False, 1), (64, True, 2),
+                                                        (8, True, 0), (64, False, 0)])
+def test_append_of_odd_views_and_rotations(kdb, features, interleaved, shift):
+    """Rows that no 16-byte piece lies aligned in, heads outside the rows, rotations of a few features."""
+    rng = np.random.default_rng(features + shift)
+    starts, lengths, tokens = batch_of([21, 1, 7], [25, 40, 7])
+    cache = paged.Cache(rng, 3, 3, 2, 16, 64)
+    wide = rng.normal(0, 1, (8, tokens, 64 + 2 * shift)).astype(np.float32)  # [q 4, k 2, v 2][token][feature]
+    q, k, v = (np.ascontiguousarray(wide[a:b, :, shift:shift + 64].transpose(1, 0, 2)) for a, b in ((0, 4), (4, 6), (6, 8)))
+    rotation = (*paged.tables(40, features), features, interleaved)
+    on = paged.Device(kdb, cache, starts, lengths, tokens)
+    dx, c, s = kdb.to_device(wide), kdb.to_device(rotation[0]), kdb.to_device(rotation[1])
+    out = kdb.to_device(np.full(q.shape, -777, np.float32))
+    row = 64 + 2 * shift
+    strides, head = kd.strides(row, tokens * row), tokens * row * 4
+    at = dx.ptr + 4 * shift
+    kdb.call("paged_append", kd.F32, on.c, on.b, kd.Rotation(c.ptr, s.ptr, 40, features, int(interleaved)), out.ptr, at, strides,
+             4, at + 4 * head, strides, at + 6 * head, strides)
+    want, want_q = paged.append(cache, starts, lengths, q, k, v, rotation)
+    np.testing.assert_array_equal(out.numpy(), want_q)
+    same_cache(on.read_back(), want)
+
+
+def test_append_over_many_sequences(kdb):
+    """More sequences than a wave has lanes, some of them without new tokens, rows before the first and behind the last."""
+    rng = np.random.default_rng(8)
+    new = [int(x) for x in rng.integers(0, 4, 200)]
+    lengths = [n + int(x) for n, x in zip(new, rng.integers(0, 30, 200))]
+    starts, lengths, tokens = batch_of(new, lengths, first=2, after=3)
+    cache = paged.Cache(rng, 200, 3, 1, 16, 64)
+    x, q, k, v = fused(rng, tokens, 2, 1, 64)
+    rotation = (*paged.tables(40, 64), 64, False)
+    on, q_out = run_append(kdb, cache, starts, lengths, tokens, x, 2, rotation)
+    want, want_q = paged.append(cache, starts, lengths, q, k, v, rotation)
+    np.testing.assert_array_equal(q_out, want_q)
+    same_cache(on.read_back(), want)
+    out, tolerance = paged.attention(want, starts, lengths, q_out, 0.125)
+    got = run_attention(kdb, on, q_out, 0.125, 40)
+    assert (np.abs(got - out) <= tolerance).all()
+
+
 def test_append_without_rotation_queries_or_pages(kdb):
     """No rotation and no queries; positions without a page, before the first or past the table, are not written; rows
     before the first and behind the last sequence are left alone."""
