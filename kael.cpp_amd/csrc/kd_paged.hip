@@ -425,11 +425,9 @@ __global__ __launch_bounds__(256) void paged_read_kernel(Paged c, float* __restr
 
 typedef int v4i __attribute__((ext_vector_type(4)));
 
-constexpr int kAttentionWaves = 4;
 constexpr int kRowTile = 16;
-constexpr int kTileRows = kAttentionWaves * kRowTile;  // rows of a workgroup
+constexpr int kTileRows = 64;  // rows of a workgroup
 constexpr int kKeyBlock = 64;
-constexpr float kLog2e = 1.44269504088896341f;
 
 // Sequence s has base(s + 1) - base(s) >= ceil(count * group / 64) tiles.
 __host__ __device__ inline int64_t tile_base(int64_t start, int64_t s, int group) { return start * group / kTileRows + s; }
@@ -471,31 +469,56 @@ __device__ __forceinline__ float joined(const v4i (&sum)[4], int r) {
     return static_cast<float>((sum[3][r] << 8) + sum[2][r]) * 65536.f + static_cast<float>((sum[1][r] << 8) + sum[0][r]);
 }
 
+// The digits of a lane's 16 U features of a query row (0 where the row is not real) and the factor that a score's whole number
+// times its key's scale takes: scale * 2^(e - 30) * log2(e), positive, the scale's sign being in the digits; NaN where the
+// row is not finite.
+template <int U> __device__ __forceinline__ float query_digits(float (&features)[16 * U], bool real, double scale, v4i (&digits)[4][U]) {
+    int bits = 0;
+#pragma unroll
+    for (int d = 0; d < 16 * U; ++d) {
+        features[d] = real ? features[d] : 0.f;
+        bits = max(bits, __float_as_int(features[d]) & 0x7fffffff);
+    }
+    bits = over_chunks(bits, [](int a, int b) { return max(a, b); });
+    const int e = __builtin_amdgcn_frexp_expf(__int_as_float(bits));  // 0 for 0; unused where not finite
+    const float sign = scale < 0 ? -1.f : 1.f;
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+            int y[4], d4[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                y[i] = static_cast<int>(rintf(ldexpf(features[16 * u + 4 * t + i] * sign, 30 - e))) + kDigitBias;
+            digits_of(y, d4);
+#pragma unroll
+            for (int p = 0; p < 4; ++p) digits[p][u][t] = d4[p];
+        }
+    return bits < 0x7f800000 ? static_cast<float>(ldexp(fabs(scale) * 1.4426950408889634074, e - 30)) : NAN;
+}
+
 struct Split {
     int count;    // parts that a row's keys are split into
     int part;     // keys of a part, a multiple of 64; the last part goes to the end
     float* sums;  // [row][count][D], then [row][count][2] of the maximum (base 2) and the sum
 };
 
-template <int D>
-__global__ __launch_bounds__(kAttentionWaves * 64, 2) void paged_attention_kernel(Paged c, float* __restrict__ out, Strided q,
-                                                                                  int heads, double scale, Split split) {
+template <int D, int Waves>
+__global__ __launch_bounds__(Waves * 64, 2) void paged_attention_kernel(Paged c, float* __restrict__ out, Strided q,
+                                                                                      int heads, FastDiv by_group, double scale,
+                                                                                      Split split) {
     constexpr int U = D / 64;
     constexpr int kLd = D + 4;
-    // two blocks of 128 features' keys and values do not fit the registers: their values are loaded when the scores begin
-    constexpr bool kValuesAhead = D == 64;
-    __shared__ float os[kAttentionWaves][kRowTile][kLd];
-    __shared__ float ms[kAttentionWaves][kRowTile], ls[kAttentionWaves][kRowTile];
-    const uint32_t group = static_cast<uint32_t>(heads) / c.kv_heads;
+    __shared__ __attribute__((aligned(16))) float os[Waves][kRowTile][kLd];
+    __shared__ float ms[Waves][kRowTile], ls[Waves][kRowTile];
+    const int group = static_cast<int>(by_group.divisor);
     const int wave = threadIdx.x / 64, lane = threadIdx.x % 64;
     const int column = lane % 16, chunk = lane / 16;
-    const int part = blockIdx.x % split.count;
-    const int kv = blockIdx.x / split.count % c.kv_heads;
+    const int part = blockIdx.y, kv = static_cast<int>(blockIdx.x % c.kv_heads);
     // the last rows see most keys and go first
-    const int64_t tile = tile_base(c.tokens, c.sequences, group) - 1 - blockIdx.x / split.count / c.kv_heads;
+    const int64_t tile = (gridDim.x - 1 - blockIdx.x) / c.kv_heads;
     const Found found = find_sequence(c, tile, [&](int64_t start, int64_t at) { return tile_base(start, at, group); });
     if (found.s < 0) return;
-    const int s = found.s;
     const Rows rows = found.rows;
     // tokens * heads is below 2^31, and so are the rows of a kv head
     const int64_t tile_at = (tile - found.base) * kTileRows;
@@ -504,58 +527,34 @@ __global__ __launch_bounds__(kAttentionWaves * 64, 2) void paged_attention_kerne
     const int row0 = static_cast<int>(tile_at);
     const int here = min(row_end - row0, kTileRows);
     // row tiles of the workgroup (1, 2 or 4), and the waves that share a tile's keys
-    const int row_waves = here <= 16 ? 1 : here <= 32 ? 2 : 4, key_waves = kAttentionWaves / row_waves;
+    const int row_waves = here <= 16 ? 1 : here <= 32 ? 2 : 4, key_waves = Waves / row_waves;
     const int row_wave = wave % row_waves, key_wave = wave / row_waves;
     const int64_t capacity = static_cast<int64_t>(c.columns) << c.page_shift;
-    // keys 0 .. limit - 1 are visible to row r of the sequence
-    const auto limit_of = [&](int r) {
-        const int64_t limit = rows.position + static_cast<uint32_t>(r) / group + 1;
+    // keys 0 .. limit - 1 are visible to the row of token `token` of the sequence
+    const auto limit_of = [&](int token) {
+        const int64_t limit = rows.position + token + 1;
         return static_cast<int>(limit < 0 ? 0 : limit > capacity ? capacity : limit);
     };
+    const auto token_of = [&](int row) { return static_cast<int>(by_group.div(row)); };
     const int from = part * split.part;
-    const int all = limit_of(row0 + here - 1);
+    const int all = limit_of(token_of(row0 + here - 1));
     if (from >= all && part > 0) return;
     const int to = part + 1 == split.count ? all : min(all, from + split.part);
     // rows past the last one stand in for it with a query of 0 and are not written
     const int tile_row = row0 + row_wave * kRowTile;
     const bool real = row_wave * kRowTile + column < here;
-    const uint32_t r = min(tile_row + column, row0 + here - 1);
-    const int limit = limit_of(r);
-    const int least = limit_of(min(tile_row, row0 + here - 1));
-    const int most = min(to, limit_of(min(tile_row + kRowTile - 1, row0 + here - 1)));
+    const int r = min(tile_row + column, row0 + here - 1);
+    const int token = token_of(r);
+    const int limit = limit_of(token);
+    const int least = __builtin_amdgcn_readfirstlane(limit);  // limits ascend with the columns
+    const int most = min(to, __builtin_amdgcn_readlane(limit, 15));
+    const int step = key_waves * kKeyBlock;
+    int key = from + key_wave * kKeyBlock;
 
-    // the row's digits: features chunk * 16 U .. + 16 U - 1 of its column's row
-    v4i digits[4][U];
-    float q_factor;
-    {
-        const float* x = q.data + (rows.row + r / group) * q.row + (kv * group + r % group) * q.head + chunk * 16 * U;
-        float f[16 * U];
-        int bits = 0;
-#pragma unroll
-        for (int d = 0; d < 16 * U; ++d) {
-            f[d] = real ? x[d] : 0.f;
-            bits = max(bits, __float_as_int(f[d]) & 0x7fffffff);
-        }
-        bits = over_chunks(bits, [](int a, int b) { return max(a, b); });
-        const int e = __builtin_amdgcn_frexp_expf(__int_as_float(bits));  // 0 for 0; unused where not finite
-#pragma unroll
-        for (int u = 0; u < U; ++u)
-#pragma unroll
-            for (int t = 0; t < 4; ++t) {
-                int y[4], d4[4];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) y[i] = static_cast<int>(rintf(ldexpf(f[16 * u + 4 * t + i], 30 - e))) + kDigitBias;
-                digits_of(y, d4);
-#pragma unroll
-                for (int p = 0; p < 4; ++p) digits[p][u][t] = d4[p];
-            }
-        q_factor = bits < 0x7f800000 ? static_cast<float>(ldexp(scale * 1.4426950408889634074, e - 30)) : NAN;
-    }
-
-    const int size = 1 << c.page_shift;
     // Lane i of `window` holds the page of table column window_from + i, so that the table's loads are not waited for
     // among the codes'.
-    const int64_t* table = c.table + static_cast<int64_t>(s) * c.columns;
+    const int size = 1 << c.page_shift;
+    const int64_t* table = c.table + static_cast<int64_t>(found.s) * c.columns;
     int window = 0, window_from = -128;
     const auto pages_of_block = [&](int key) {
         if (((key + kKeyBlock - 1) >> c.page_shift) - window_from >= 64) {
@@ -593,14 +592,20 @@ __global__ __launch_bounds__(kAttentionWaves * 64, 2) void paged_attention_kerne
         for (int n = 0; n < D / 16; ++n) v[n] = *reinterpret_cast<const v4i*>(values_at + 16 * n * size);
     };
 
-    float m = -INFINITY, l = 0.f;
-    float o[D / 4] = {};
-    const int step = key_waves * kKeyBlock;
-    int key = from + key_wave * kKeyBlock;
-    if (key < most) {
+    // the row's digits: features chunk * 16 U .. + 16 U - 1 of its column's row
+    const float* row = q.data + (rows.row + token) * q.row + (kv * group + r - token * group) * q.head + chunk * 16 * U;
+    float features[16 * U];
+#pragma unroll
+    for (int d = 0; d < 16 * U; ++d) features[d] = row[d];
+    if (key < most) {  // in flight while the digits are made
         load_keys(key);
         load_values();
     }
+    v4i digits[4][U];
+    const float q_factor = query_digits(features, real, scale, digits);
+
+    float m = -INFINITY, l = 0.f;
+    float o[D / 4] = {};
     for (; key < most; key += step) {
         float x[16];
 #pragma unroll
@@ -614,7 +619,10 @@ __global__ __launch_bounds__(kAttentionWaves * 64, 2) void paged_attention_kerne
                     sum[p] = __builtin_amdgcn_mfma_i32_16x16x64_i8(k[t][u], digits[p][u], sum[p], 0, 0, 0);
             }
 #pragma unroll
-            for (int i = 0; i < 4; ++i) x[4 * t + i] = joined(sum, i);
+            for (int i = 0; i < 4; ++i) {
+                x[4 * t + i] = joined(sum, i);
+                asm("" : "+v"(x[4 * t + i]));  // joined here, not behind the branch below with every tile's sums held
+            }
         }
         const int first = key + 16 * chunk;  // x[i] is key first + i
         const int seen = page < 0 ? 0 : limit - first;
@@ -680,7 +688,7 @@ __global__ __launch_bounds__(kAttentionWaves * 64, 2) void paged_attention_kerne
             make_float4(o[4 * n], o[4 * n + 1], o[4 * n + 2], o[4 * n + 3]);
     __syncthreads();
     // the waves that shared a row's keys joined, in their order
-    for (int i = threadIdx.x; i < here * (D / 4); i += kAttentionWaves * 64) {
+    for (int i = threadIdx.x; i < here * (D / 4); i += Waves * 64) {
         const int at = i / (D / 4), d = i % (D / 4) * 4;
         const int w0 = at / kRowTile, col = at % kRowTile;
         float top = -INFINITY;
@@ -698,8 +706,8 @@ __global__ __launch_bounds__(kAttentionWaves * 64, 2) void paged_attention_kerne
             v.z += f * add.z;
             v.w += f * add.w;
         }
-        const uint32_t row = row0 + at;
-        const int64_t to_row = (rows.row + static_cast<int64_t>(row / group)) * heads + kv * group + row % group;
+        const int of_token = token_of(row0 + at);
+        const int64_t to_row = static_cast<int64_t>(rows.row + of_token) * heads + kv * group + (row0 + at - of_token * group);
         if (split.count == 1) {
             const float by = sum == 0.f ? 0.f : 1.f / sum;
             *reinterpret_cast<float4*>(out + to_row * D + d) = make_float4(v.x * by, v.y * by, v.z * by, v.w * by);
@@ -709,6 +717,248 @@ __global__ __launch_bounds__(kAttentionWaves * 64, 2) void paged_attention_kerne
             if (d == 0) {
                 float* own = split.sums + static_cast<int64_t>(c.tokens) * heads * split.count * D + record * 2;
                 own[0] = top;
+                own[1] = sum;
+            }
+        }
+    }
+}
+
+// Many rows a sequence (prompts): the workgroup's four waves take 16 rows each and share every block of 64 keys through LDS,
+// two blocks deep, so that a wave keeps none of it in registers. What bounds it is the vector ALU, 30 operations a score in the
+// kernel above, seven of which join the digits' sums of the outputs; here the weighted sums run on the f16 matrix cores
+// into f32, which joins nothing: a code is an f16 value as it stands, converted once for the four waves, and a weight two f16
+// pieces (2^-24 of it), scaled so that the largest is 2^15 and pieces below 2^-24 are below 2^-39 of that.
+typedef _Float16 v8h __attribute__((ext_vector_type(8)));
+typedef _Float16 v2h __attribute__((ext_vector_type(2)));
+typedef float v2f __attribute__((ext_vector_type(2)));
+typedef float v4f __attribute__((ext_vector_type(4)));
+
+constexpr int kPromptWaves = 4;
+
+// 16 codes as two pieces of 8 f16: 0x6400 + b is 1024 + b for a byte b, here the code + 128.
+__device__ __forceinline__ void halves_of(const v4i& codes, v4i (&pieces)[2]) {
+    const v2h off{static_cast<_Float16>(-1152.f), static_cast<_Float16>(-1152.f)};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const uint32_t b = static_cast<uint32_t>(codes[i]) ^ 0x80808080u;
+        const uint32_t low = __builtin_amdgcn_perm(0x64646464u, b, 0x04010400u);
+        const uint32_t high = __builtin_amdgcn_perm(0x64646464u, b, 0x04030402u);
+        pieces[i / 2][2 * i % 4] = __builtin_bit_cast(int, __builtin_bit_cast(v2h, low) + off);
+        pieces[i / 2][2 * i % 4 + 1] = __builtin_bit_cast(int, __builtin_bit_cast(v2h, high) + off);
+    }
+}
+
+template <int D>
+__global__ __launch_bounds__(kPromptWaves * 64, 2) void paged_prompt_kernel(Paged c, float* __restrict__ out, Strided q,
+                                                                                  int heads, FastDiv by_group, double scale,
+                                                                                  Split split) {
+    constexpr int U = D / 64;
+    constexpr int kLd = D + 4;
+    constexpr int kKeyPieces = 4 * U, kValuePieces = 2 * D / 16;  // of 64 lanes' 16 bytes
+    union Shared {
+        v4i block[2][kKeyPieces + kValuePieces][64];
+        float os[kPromptWaves][kRowTile][kLd];
+    };
+    __shared__ __attribute__((aligned(16))) Shared shared;
+    __shared__ float ms[kPromptWaves][kRowTile], ls[kPromptWaves][kRowTile];
+    const int group = static_cast<int>(by_group.divisor);
+    const int wave = threadIdx.x / 64, lane = threadIdx.x % 64;
+    const int column = lane % 16, chunk = lane / 16;
+    const int part = blockIdx.y, kv = static_cast<int>(blockIdx.x % c.kv_heads);
+    const int64_t tile = (gridDim.x - 1 - blockIdx.x) / c.kv_heads;
+    const Found found = find_sequence(c, tile, [&](int64_t start, int64_t at) { return tile_base(start, at, group); });
+    if (found.s < 0) return;
+    const Rows rows = found.rows;
+    const int64_t tile_at = (tile - found.base) * kTileRows;
+    const int row_end = rows.count * group;
+    if (tile_at < 0 || tile_at >= row_end) return;
+    const int row0 = static_cast<int>(tile_at);
+    const int here = min(row_end - row0, kTileRows);
+    const int64_t capacity = static_cast<int64_t>(c.columns) << c.page_shift;
+    const auto limit_of = [&](int token) {
+        const int64_t limit = rows.position + token + 1;
+        return static_cast<int>(limit < 0 ? 0 : limit > capacity ? capacity : limit);
+    };
+    const auto token_of = [&](int row) { return static_cast<int>(by_group.div(row)); };
+    const int from = part * split.part;
+    const int all = limit_of(token_of(row0 + here - 1));
+    if (from >= all && part > 0) return;
+    const int to = part + 1 == split.count ? all : min(all, from + split.part);
+    const bool real = wave * kRowTile + column < here;
+    const int r = min(row0 + wave * kRowTile + column, row0 + here - 1);
+    const int token = token_of(r);
+    const int limit = limit_of(token);
+    const int least = __builtin_amdgcn_readfirstlane(limit);
+    // a wave without rows works on nothing
+    const int most = wave * kRowTile < here ? min(to, __builtin_amdgcn_readlane(limit, 15)) : 0;
+
+    const int size = 1 << c.page_shift;
+    const int64_t* table = c.table + static_cast<int64_t>(found.s) * c.columns;
+    int window = 0, window_from = -128;
+    const auto page_at = [&](int key) { return __shfl(window, (key >> c.page_shift) - window_from); };
+    const int key_chunk = column / 4;
+    // the wave's share of a block: tile `wave` of the keys, and U tiles of 16 features of the values
+    v4i k[U], v[U];
+    struct Scales {
+        float key, value;
+        int page;
+    };
+    Scales next;
+    const auto load = [&](int key) {
+        if (((key + kKeyBlock - 1) >> c.page_shift) - window_from >= 64) {
+            window_from = key >> c.page_shift;
+            const int64_t page = table[min(window_from + lane, c.columns - 1)];
+            window = window_from + lane < c.columns && page >= 0 && page < c.pages ? static_cast<int>(page) : -1;
+        }
+        next.page = page_at(key + 16 * chunk);
+        const int64_t own = static_cast<int64_t>(max(next.page, 0)) * c.kv_heads + kv;
+        const int64_t other = static_cast<int64_t>(max(page_at(key + 16 * key_chunk), 0)) * c.kv_heads + kv;
+        const int slot = (key + 16 * key_chunk) & (size - 1), own_slot = (key + 16 * chunk) & (size - 1);
+        const int8_t* at = c.keys + (other * size + slot + 4 * wave + lane % 4) * D + chunk * 16 * U;
+        const int8_t* values = c.values + own * size * D + (16 * U * wave + column) * size + own_slot;
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            k[u] = *reinterpret_cast<const v4i*>(at + 16 * u);
+            v[u] = *reinterpret_cast<const v4i*>(values + 16 * u * size);
+        }
+        next.key = c.key_scales[own];
+        next.value = c.value_scales[own];
+    };
+    const auto store = [&](int at) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            shared.block[at][wave * U + u][lane] = k[u];
+            v4i pieces[2];
+            halves_of(v[u], pieces);
+#pragma unroll
+            for (int h = 0; h < 2; ++h) shared.block[at][kKeyPieces + 2 * (wave * U + u) + h][lane] = pieces[h];
+        }
+    };
+
+    const float* row = q.data + (rows.row + token) * q.row + (kv * group + r - token * group) * q.head + chunk * 16 * U;
+    float features[16 * U];
+#pragma unroll
+    for (int d = 0; d < 16 * U; ++d) features[d] = row[d];
+    if (from < to) load(from);
+    v4i digits[4][U];
+    const float q_factor = query_digits(features, real, scale, digits);
+
+    float m = -INFINITY, l = 0.f;
+    v4f o[D / 16] = {};  // in units of 2^(exponent of `top` - 15)
+    int top = 0;         // the largest value scale that the row has seen, as bits, so that NaN is the largest of all
+    const auto work = [&](int key, const Scales& own, const v4i (*block)[64]) {
+        float x[16];
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+            v4i sum[4];
+#pragma unroll
+            for (int p = 0; p < 4; ++p) sum[p] = v4i{0, 0, 0, 0};
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const v4i piece = block[t * U + u][lane];
+#pragma unroll
+                for (int p = 0; p < 4; ++p) sum[p] = __builtin_amdgcn_mfma_i32_16x16x64_i8(piece, digits[p][u], sum[p], 0, 0, 0);
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                x[4 * t + i] = joined(sum, i);
+                asm("" : "+v"(x[4 * t + i]));  // joined here, not behind the branch below with every tile's sums held
+            }
+        }
+        const int seen = own.page < 0 ? 0 : limit - (key + 16 * chunk);
+        float factor = q_factor * own.key;
+        factor = factor == 0.f ? 0x1p-126f : factor;
+        if (key + kKeyBlock > least || __any(own.page < 0)) {
+            factor = seen > 0 ? factor : 1.f;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) x[i] = i < seen ? x[i] : -INFINITY;
+        }
+        float largest = x[0];
+#pragma unroll
+        for (int i = 1; i < 16; ++i) largest = fmaxf(largest, x[i]);
+        const float most_now = fmaxf(m, chunks_max(largest * factor));
+        const int top_now = max(top, over_chunks(seen > 0 ? __float_as_int(own.value) & 0x7fffffff : 0, [](int a, int b) { return max(a, b); }));
+        const float base = most_now == -INFINITY ? 0.f : most_now;
+        const int e = __builtin_amdgcn_frexp_expf(__int_as_float(top_now));
+        if (__any(most_now > m || top_now > top)) {
+            const float alpha = __builtin_amdgcn_exp2f(m - base);
+            const float again = ldexpf(alpha, __builtin_amdgcn_frexp_expf(__int_as_float(top)) - e);
+            l *= alpha;
+#pragma unroll
+            for (int n = 0; n < D / 16; ++n) o[n] *= again;
+            m = most_now;
+            top = top_now;
+        }
+        const float to_units = top < 0x7f800000 && seen > 0 ? ldexpf(own.value, 15 - e) : 0.f;
+        float sum = 0.f;
+        v8h high[2], low[2];
+#pragma unroll
+        for (int i = 0; i < 16; i += 2) {
+            const v2f p{__builtin_amdgcn_exp2f(fmaf(x[i], factor, -base)), __builtin_amdgcn_exp2f(fmaf(x[i + 1], factor, -base))};
+            sum += p[0];
+            sum += p[1];
+            const v2f w{p[0] * to_units, p[1] * to_units};
+            const v2h a = __builtin_convertvector(w, v2h);
+            const v2f rest{w[0] - static_cast<float>(a[0]), w[1] - static_cast<float>(a[1])};
+            const v2h b = __builtin_convertvector(rest, v2h);
+            high[i / 8][i % 8] = a[0];
+            high[i / 8][i % 8 + 1] = a[1];
+            low[i / 8][i % 8] = b[0];
+            low[i / 8][i % 8 + 1] = b[1];
+        }
+        l += sum;
+#pragma unroll
+        for (int n = 0; n < D / 16; ++n)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const v8h values = __builtin_bit_cast(v8h, block[kKeyPieces + 2 * n + h][lane]);
+                o[n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(values, low[h], o[n], 0, 0, 0);
+                o[n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(values, high[h], o[n], 0, 0, 0);
+            }
+    };
+
+    if (from < to) {
+        Scales own = next;
+        store(0);
+        if (from + kKeyBlock < to) load(from + kKeyBlock);
+        __syncthreads();
+        int buffer = 0;
+        for (int key = from; key < to; key += kKeyBlock) {
+            if (key < most) work(key, own, shared.block[buffer]);
+            buffer ^= 1;
+            if (key + kKeyBlock < to) {
+                own = next;
+                store(buffer);
+                if (key + 2 * kKeyBlock < to) load(key + 2 * kKeyBlock);
+            }
+            // the block stored is complete, and the one worked on free
+            __syncthreads();
+        }
+    }
+    l = chunks_sum(l);
+    const float unit = top < 0x7f800000 ? ldexpf(1.f, __builtin_amdgcn_frexp_expf(__int_as_float(top)) - 15) : NAN;
+    if (chunk == 0) {
+        ms[wave][column] = m;
+        ls[wave][column] = l;
+    }
+#pragma unroll
+    for (int n = 0; n < D / 16; ++n) *reinterpret_cast<v4f*>(&shared.os[wave][column][16 * n + 4 * chunk]) = o[n] * unit;
+    __syncthreads();
+    for (int i = threadIdx.x; i < here * (D / 4); i += kPromptWaves * 64) {
+        const int at = i / (D / 4), d = i % (D / 4) * 4;
+        const int w = at / kRowTile, col = at % kRowTile;
+        const v4f sums = *reinterpret_cast<const v4f*>(&shared.os[w][col][d]);
+        const float sum = ls[w][col];
+        const int of_token = token_of(row0 + at);
+        const int64_t to_row = static_cast<int64_t>(rows.row + of_token) * heads + kv * group + (row0 + at - of_token * group);
+        if (split.count == 1) {
+            *reinterpret_cast<v4f*>(out + to_row * D + d) = sums * (sum == 0.f ? 0.f : 1.f / sum);
+        } else {
+            const int64_t record = to_row * split.count + part;
+            *reinterpret_cast<v4f*>(split.sums + record * D + d) = sums;
+            if (d == 0) {
+                float* own = split.sums + static_cast<int64_t>(c.tokens) * heads * split.count * D + record * 2;
+                own[0] = ms[w][col];
                 own[1] = sum;
             }
         }
@@ -731,30 +981,72 @@ __global__ __launch_bounds__(256) void paged_join_kernel(Paged c, float* __restr
     const int parts = static_cast<int>(max(int64_t{1}, min(int64_t{split.count}, (limit + split.part - 1) / split.part)));
     const float* sums = split.sums + row * split.count * D;
     const float* ml = split.sums + static_cast<int64_t>(c.tokens) * heads * split.count * D + row * split.count * 2;
-    float top = -INFINITY;
-    for (int p = 0; p < parts; ++p) top = fmaxf(top, ml[2 * p]);
-    const float base = top == -INFINITY ? 0.f : top;
-    float sum = 0.f, v[D / 64] = {};
-    for (int p = 0; p < parts; ++p) {
-        const float f = __builtin_amdgcn_exp2f(ml[2 * p] - base);
-        sum += f * ml[2 * p + 1];
+    // a lane holds a part's maximum and sum, 64 parts at a time
+    float top = -INFINITY, sum = 0.f, v[D / 64] = {};
+    for (int p0 = 0; p0 < parts; p0 += 64) {
+        const bool in = p0 + lane < parts;
+        const float own = in ? ml[2 * (p0 + lane)] : -INFINITY;
+        const float own_sum = in ? ml[2 * (p0 + lane) + 1] : 0.f;
+        float next = own;
 #pragma unroll
-        for (int u = 0; u < D / 64; ++u) v[u] += f * sums[p * D + 64 * u + lane];
+        for (int d = 32; d > 0; d /= 2) next = fmaxf(next, __shfl_xor(next, d));
+        next = fmaxf(next, top);
+        const float base = next == -INFINITY ? 0.f : next;
+        const float again = __builtin_amdgcn_exp2f(top - base), f = __builtin_amdgcn_exp2f(own - base);
+        float add = f * own_sum;
+#pragma unroll
+        for (int d = 32; d > 0; d /= 2) add += __shfl_xor(add, d);
+        sum = sum * again + add;
+#pragma unroll
+        for (int u = 0; u < D / 64; ++u) v[u] *= again;
+        const int count = min(64, parts - p0);
+        // eight parts' loads at a time; past the last one it is read again, for nothing
+        for (int p = 0; p < count; p += 8) {
+            float x[8][D / 64];
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+#pragma unroll
+                for (int u = 0; u < D / 64; ++u) x[i][u] = sums[(p0 + min(p + i, count - 1)) * D + 64 * u + lane];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float by = p + i < count ? __shfl(f, p + i) : 0.f;
+#pragma unroll
+                for (int u = 0; u < D / 64; ++u) v[u] += by * x[i][u];
+            }
+        }
+        top = next;
     }
 #pragma unroll
     for (int u = 0; u < D / 64; ++u) out[row * D + 64 * u + lane] = sum == 0.f ? 0.f : v[u] / sum;
 }
 
-// How a call's keys are split: into as many parts as give every CU two workgroups, none of fewer than 256 keys.
+// Bytes of a part's results of `rows` rows.
 int64_t part_bytes(int64_t rows, int64_t dim) { return rows * (dim + 2) * 4; }
 
-Split split_of(int64_t heads, int64_t kv_heads, int64_t sequences, int64_t tokens, int64_t max_keys, int64_t most) {
-    const int64_t groups = std::max<int64_t>(1, tile_base(tokens, sequences, static_cast<int>(heads / kv_heads)) * kv_heads);
+// How a call runs: on the prompts' kernel or with `waves` waves that share a tile's keys, and the parts that the keys are split
+// into.
+struct Plan {
+    int64_t tiles;
+    bool prompts;
+    int waves;
+    Split split;
+};
+
+Plan plan_of(int64_t heads, int64_t kv_heads, int64_t sequences, int64_t tokens, int64_t max_keys, int64_t most) {
+    Plan plan;
+    const int64_t group = heads / kv_heads;
+    plan.tiles = tile_base(tokens, sequences, static_cast<int>(group));
+    const int64_t groups = std::max<int64_t>(1, plan.tiles * kv_heads);
     const int64_t keys = std::min<int64_t>(std::max<int64_t>(max_keys, 1), int64_t{1} << 30);
-    int64_t count = std::min({(2 * compute_units() + groups - 1) / groups, (keys + 255) / 256, most});
-    count = std::max<int64_t>(count, 1);
-    const int64_t part = ((keys + count - 1) / count + 255) / 256 * 256;
-    return {static_cast<int>((keys + part - 1) / part), static_cast<int>(part), nullptr};
+    plan.prompts = tokens * group >= kTileRows * sequences;
+    plan.waves = !plan.prompts && groups <= compute_units() && keys <= 2048 ? 8 : 4;
+    const int64_t least = 256;
+    int64_t count = (2 * compute_units() + groups - 1) / groups;
+    if (plan.waves == 8 || keys <= 1024) count = 1;
+    count = std::max<int64_t>(1, std::min({std::max(count, keys / 8192), (keys + least - 1) / least, most, int64_t{65535}}));
+    const int64_t part = ((keys + count - 1) / count + least - 1) / least * least;
+    plan.split = {static_cast<int>((keys + part - 1) / part), static_cast<int>(part), nullptr};
+    return plan;
 }
 
 // ---- checks ---------------------------------------------------------------------------------------
@@ -903,7 +1195,7 @@ extern "C" int kd_paged_attention_workspace(int64_t* bytes, int64_t heads, int64
         (head_dim != 64 && head_dim != 128) || sequences < 0 || sequences >= int64_t{1} << 24 || tokens < 0 ||
         tokens >= int64_t{1} << 31 || max_keys < 0)
         return fail(KD_E_INVALID, "kd_paged_attention_workspace: bad arguments");
-    const Split split = split_of(heads, kv_heads, sequences, tokens, max_keys, INT32_MAX);
+    const Split split = plan_of(heads, kv_heads, sequences, tokens, max_keys, INT32_MAX).split;
     *bytes = split.count > 1 ? split.count * part_bytes(tokens * heads, head_dim) : 0;
     return KD_OK;
 }
@@ -925,20 +1217,32 @@ extern "C" int kd_paged_attention(int dtype, void* out, const void* q, const int
     if (int rc = ensure_device()) return rc;
     if (c.pages == 0) c.columns = 0;  // no position has a page
     const int64_t rows = heads * c.tokens;
-    Split split = split_of(heads, c.kv_heads, c.sequences, c.tokens, max_keys, workspace_bytes / part_bytes(rows, c.head_dim));
-    split.sums = static_cast<float*>(workspace);
-    const int64_t groups = tile_base(c.tokens, c.sequences, static_cast<int>(heads / c.kv_heads)) * c.kv_heads * split.count;
-    if (int rc = check_grid(what, groups)) return rc;
-    const auto launch = [&](auto dim) {
-        constexpr int D = decltype(dim)::value;
-        hipLaunchKernelGGL((paged_attention_kernel<D>), dim3(static_cast<uint32_t>(groups)), dim3(kAttentionWaves * 64), 0,
-                           stream(), c, static_cast<float*>(out), qs, static_cast<int>(heads), scale, split);
+    Plan plan = plan_of(heads, c.kv_heads, c.sequences, c.tokens, max_keys, workspace_bytes / part_bytes(rows, c.head_dim));
+    const Split split{plan.split.count, plan.split.part, static_cast<float*>(workspace)};
+    if (int rc = check_grid(what, plan.tiles * c.kv_heads)) return rc;
+    const auto launch = [&](auto dim, auto waves) {
+        constexpr int D = decltype(dim)::value, Waves = decltype(waves)::value;
+        hipLaunchKernelGGL((paged_attention_kernel<D, Waves>), dim3(static_cast<uint32_t>(plan.tiles * c.kv_heads), split.count),
+                           dim3(Waves * 64), 0, stream(), c, static_cast<float*>(out), qs, static_cast<int>(heads),
+                           FastDiv(static_cast<uint32_t>(heads / c.kv_heads)), scale, split);
         if (split.count > 1)
             hipLaunchKernelGGL((paged_join_kernel<D>), dim3(static_cast<uint32_t>((rows + 3) / 4)), dim3(256), 0, stream(), c,
                                static_cast<float*>(out), static_cast<int>(heads), split);
     };
-    if (c.head_dim == 64) launch(std::integral_constant<int, 64>{});
-    else launch(std::integral_constant<int, 128>{});
+    const auto with_waves = [&](auto dim) {
+        constexpr int D = decltype(dim)::value;
+        if (plan.prompts) {
+            hipLaunchKernelGGL((paged_prompt_kernel<D>), dim3(static_cast<uint32_t>(plan.tiles * c.kv_heads), split.count),
+                               dim3(kPromptWaves * 64), 0, stream(), c, static_cast<float*>(out), qs, static_cast<int>(heads),
+                               FastDiv(static_cast<uint32_t>(heads / c.kv_heads)), scale, split);
+            if (split.count > 1)
+            hipLaunchKernelGGL((paged_join_kernel<D>), dim3(static_cast<uint32_t>((rows + 3) / 4)), dim3(256), 0, stream(), c,
+                               static_cast<float*>(out), static_cast<int>(heads), split);
+        } else if (plan.waves == 8) launch(dim, std::integral_constant<int, 8>{});
+        else launch(dim, std::integral_constant<int, 4>{});
+    };
+    if (c.head_dim == 64) with_waves(std::integral_constant<int, 64>{});
+    else with_waves(std::integral_constant<int, 128>{});
     KD_LAUNCH_CHECK();
     return KD_OK;
 }
