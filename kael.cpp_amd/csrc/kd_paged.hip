@@ -513,7 +513,7 @@ struct Split {
 };
 
 template <int D, int Waves>
-__global__ __launch_bounds__(Waves * 64, 2) void paged_attention_kernel(Paged c, float* __restrict__ out, Strided q,
+__global__ __launch_bounds__(Waves * 64, D == 64 ? 4 : 2) void paged_attention_kernel(Paged c, float* __restrict__ out, Strided q,
                                                                                       int heads, FastDiv by_group, double scale,
                                                                                       Split split) {
     constexpr int U = D / 64;
@@ -581,20 +581,22 @@ __global__ __launch_bounds__(Waves * 64, 2) void paged_attention_kernel(Paged c,
     const int8_t* values_at;
     float key_scale, value_scale;
     int page;
+    const uint32_t page_bytes = static_cast<uint32_t>(c.kv_heads) * size * D;  // at most 2^27
+    const int8_t* keys_base = c.keys + (kv * size + lane % 4) * D + chunk * 16 * U;
+    const int8_t* values_base = c.values + (kv * D + column) * size;
     const auto load_keys = [&](int key) {
         pages_of_block(key);
         page = page_at(key + 16 * chunk);
-        const int64_t own = static_cast<int64_t>(max(page, 0)) * c.kv_heads + kv;
-        const int64_t other = static_cast<int64_t>(max(page_at(key + 16 * key_chunk), 0)) * c.kv_heads + kv;
+        const uint32_t own = max(page, 0), other = max(page_at(key + 16 * key_chunk), 0);
         const int slot = (key + 16 * key_chunk) & (size - 1), own_slot = (key + 16 * chunk) & (size - 1);
-        const int8_t* at = c.keys + (other * size + slot + lane % 4) * D + chunk * 16 * U;
+        const int8_t* at = keys_base + uint64_t{other} * page_bytes + slot * D;
 #pragma unroll
         for (int t = 0; t < 4; ++t)
 #pragma unroll
             for (int u = 0; u < U; ++u) k[t][u] = *reinterpret_cast<const v4i*>(at + 4 * t * D + 16 * u);
-        key_scale = c.key_scales[own];
-        value_scale = c.value_scales[own];
-        values_at = c.values + own * size * D + column * size + own_slot;
+        key_scale = c.key_scales[uint64_t{own} * static_cast<uint32_t>(c.kv_heads) + kv];
+        value_scale = c.value_scales[uint64_t{own} * static_cast<uint32_t>(c.kv_heads) + kv];
+        values_at = values_base + uint64_t{own} * page_bytes + own_slot;
     };
     const auto load_values = [&] {
 #pragma unroll
@@ -791,13 +793,36 @@ __device__ __forceinline__ Found find_tile(const Paged& c, int index, int tiles,
     return found;
 }
 
+// A lane's 16 features of a query row as f16 pieces, the larger parts and the rest, of 2^(15 - e) times their value, e being
+// the exponent of the row's largest; the factor as query_digits gives it.
+__device__ __forceinline__ float query_halves(float (&features)[16], bool real, double scale, v8h (&high)[2], v8h (&low)[2]) {
+    int bits = 0;
+#pragma unroll
+    for (int d = 0; d < 16; ++d) {
+        features[d] = real ? features[d] : 0.f;
+        bits = max(bits, __float_as_int(features[d]) & 0x7fffffff);
+    }
+    bits = over_chunks(bits, [](int a, int b) { return max(a, b); });
+    const int e = __builtin_amdgcn_frexp_expf(__int_as_float(bits));
+    const float sign = scale < 0 ? -1.f : 1.f;
+#pragma unroll
+    for (int d = 0; d < 16; ++d) {
+        const float x = ldexpf(features[d] * sign, 15 - e);
+        high[d / 8][d % 8] = static_cast<_Float16>(x);
+        low[d / 8][d % 8] = static_cast<_Float16>(x - static_cast<float>(high[d / 8][d % 8]));
+    }
+    return bits < 0x7f800000 ? static_cast<float>(ldexp(fabs(scale) * 1.4426950408889634074, e - 15)) : NAN;
+}
+
 template <int D>
 __global__ __launch_bounds__(kPromptWaves * 64, 2) void paged_prompt_kernel(Paged c, float* __restrict__ out, Strided q,
                                                                                   int heads, FastDiv by_group, double scale,
                                                                                   Split split) {
     constexpr int U = D / 64;
     constexpr int kLd = D + 4;
-    constexpr int kKeyPieces = 4 * U, kValuePieces = 2 * D / 16;  // of 64 lanes' 16 bytes
+    // Heads of 64 take the keys as f16 too, which spares joining the scores' digits; at 128 LDS would hold a workgroup less.
+    constexpr bool kHalfKeys = D == 64;
+    constexpr int kKeyPieces = 8, kValuePieces = 2 * D / 16;  // of 64 lanes' 16 bytes
     union Shared {
         v4i block[2][kKeyPieces + kValuePieces][64];
         float os[kPromptWaves][kRowTile][kLd];
@@ -846,6 +871,9 @@ __global__ __launch_bounds__(kPromptWaves * 64, 2) void paged_prompt_kernel(Page
         int page;
     };
     Scales next;
+    const uint32_t page_bytes = static_cast<uint32_t>(c.kv_heads) * size * D;  // at most 2^27
+    const int8_t* keys_base = c.keys + (kv * size + 4 * wave + lane % 4) * D + chunk * 16 * U;
+    const int8_t* values_base = c.values + (kv * D + 16 * U * wave + column) * size;
     const auto load = [&](int key) {
         if (((key + kKeyBlock - 1) >> c.page_shift) - window_from >= 64) {
             window_from = key >> c.page_shift;
@@ -853,24 +881,29 @@ __global__ __launch_bounds__(kPromptWaves * 64, 2) void paged_prompt_kernel(Page
             window = window_from + lane < c.columns && page >= 0 && page < c.pages ? static_cast<int>(page) : -1;
         }
         next.page = page_at(key + 16 * chunk);
-        const int64_t own = static_cast<int64_t>(max(next.page, 0)) * c.kv_heads + kv;
-        const int64_t other = static_cast<int64_t>(max(page_at(key + 16 * key_chunk), 0)) * c.kv_heads + kv;
+        const uint32_t own = max(next.page, 0), other = max(page_at(key + 16 * key_chunk), 0);
         const int slot = (key + 16 * key_chunk) & (size - 1), own_slot = (key + 16 * chunk) & (size - 1);
-        const int8_t* at = c.keys + (other * size + slot + 4 * wave + lane % 4) * D + chunk * 16 * U;
-        const int8_t* values = c.values + own * size * D + (16 * U * wave + column) * size + own_slot;
+        const int8_t* at = keys_base + uint64_t{other} * page_bytes + slot * D;
+        const int8_t* values = values_base + uint64_t{own} * page_bytes + own_slot;
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             k[u] = *reinterpret_cast<const v4i*>(at + 16 * u);
             v[u] = *reinterpret_cast<const v4i*>(values + 16 * u * size);
         }
-        next.key = c.key_scales[own];
-        next.value = c.value_scales[own];
+        next.key = c.key_scales[uint64_t{own} * static_cast<uint32_t>(c.kv_heads) + kv];
+        next.value = c.value_scales[uint64_t{own} * static_cast<uint32_t>(c.kv_heads) + kv];
     };
     const auto store = [&](int at) {
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            shared.block[at][wave * U + u][lane] = k[u];
             v4i pieces[2];
+            if constexpr (kHalfKeys) {
+                halves_of(k[u], pieces);
+#pragma unroll
+                for (int h = 0; h < 2; ++h) shared.block[at][2 * wave + h][lane] = pieces[h];
+            } else {
+                shared.block[at][wave * U + u][lane] = k[u];
+            }
             halves_of(v[u], pieces);
 #pragma unroll
             for (int h = 0; h < 2; ++h) shared.block[at][kKeyPieces + 2 * (wave * U + u) + h][lane] = pieces[h];
@@ -883,11 +916,15 @@ __global__ __launch_bounds__(kPromptWaves * 64, 2) void paged_prompt_kernel(Page
     for (int d = 0; d < 16 * U; ++d) features[d] = row[d];
     if (from < to) load(from);
     v4i digits[4][U];
-    const float q_factor = query_digits(features, real, scale, digits);
+    v8h q_high[2], q_low[2];
+    float q_factor;
+    if constexpr (kHalfKeys) q_factor = query_halves(features, real, scale, q_high, q_low);
+    else q_factor = query_digits(features, real, scale, digits);
 
     float m = -INFINITY, l = 0.f;
-    v4f o[D / 16] = {};  // in units of 2^(exponent of `top` - 15)
-    int top = 0;         // the largest value scale that the row has seen, as bits, so that NaN is the largest of all
+    v4f o[D / 16] = {};  // in units of 2^(top_exponent - 15)
+    // the largest value scale that the row has seen, as bits, so that NaN is the largest of all, and its exponent
+    int top = 0, top_exponent = 0;
     const auto work = [&](int key, const Scales& own, const v4i (*block)[64]) {
         float x[16];
         // Heads of 64: pieces are read four at a time ahead of their use, where the scheduler would put them right before it.
@@ -902,24 +939,43 @@ __global__ __launch_bounds__(kPromptWaves * 64, 2) void paged_prompt_kernel(Page
             }
         };
         read(0);
+        if constexpr (kHalfKeys) {
 #pragma unroll
-        for (int t = 0; t < 4; ++t) {
-            v4i sum[4];
+            for (int t = 0; t < 4; t += 2) {
+                v4i held[4];
 #pragma unroll
-            for (int p = 0; p < 4; ++p) sum[p] = v4i{0, 0, 0, 0};
+                for (int i = 0; i < 4; ++i) held[i] = ahead[i];
+                read(t == 0 ? 4 : kKeyPieces);
+                v4f sum[2] = {};
 #pragma unroll
-            for (int u = 0; u < U; ++u) {
-                const v4i piece = kAhead ? ahead[t] : block[t * U + u][lane];
+                for (int i = 0; i < 4; ++i) {
+                    const int tile = i % 2, h = i / 2;
+                    const v8h keys = __builtin_bit_cast(v8h, held[2 * tile + h]);
+                    sum[tile] = __builtin_amdgcn_mfma_f32_16x16x32_f16(keys, q_low[h], sum[tile], 0, 0, 0);
+                    sum[tile] = __builtin_amdgcn_mfma_f32_16x16x32_f16(keys, q_high[h], sum[tile], 0, 0, 0);
+                }
 #pragma unroll
-                for (int p = 0; p < 4; ++p) sum[p] = __builtin_amdgcn_mfma_i32_16x16x64_i8(piece, digits[p][u], sum[p], 0, 0, 0);
+                for (int i = 0; i < 8; ++i) x[4 * t + i] = sum[i / 4][i % 4];
             }
+        } else {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                x[4 * t + i] = joined(sum, i);
-                asm("" : "+v"(x[4 * t + i]));  // joined here, not behind the branch below with every tile's sums held
+            for (int t = 0; t < 4; ++t) {
+                v4i sum[4];
+#pragma unroll
+                for (int p = 0; p < 4; ++p) sum[p] = v4i{0, 0, 0, 0};
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    const v4i piece = block[t * U + u][lane];
+#pragma unroll
+                    for (int p = 0; p < 4; ++p) sum[p] = __builtin_amdgcn_mfma_i32_16x16x64_i8(piece, digits[p][u], sum[p], 0, 0, 0);
+                }
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    x[4 * t + i] = joined(sum, i);
+                    asm("" : "+v"(x[4 * t + i]));  // joined here, not behind the branch below with every tile's sums held
+                }
             }
         }
-        read(kKeyPieces);
         const int seen = own.page < 0 ? 0 : limit - (key + 16 * chunk);
         float factor = q_factor * own.key;
         factor = factor == 0.f ? 0x1p-126f : factor;
@@ -931,28 +987,33 @@ __global__ __launch_bounds__(kPromptWaves * 64, 2) void paged_prompt_kernel(Page
         float largest = x[0];
 #pragma unroll
         for (int i = 1; i < 16; ++i) largest = fmaxf(largest, x[i]);
-        const float most_now = fmaxf(m, chunks_max(largest * factor));
-        const int top_now = max(top, over_chunks(seen > 0 ? __float_as_int(own.value) & 0x7fffffff : 0, [](int a, int b) { return max(a, b); }));
-        const float base = most_now == -INFINITY ? 0.f : most_now;
-        const int e = __builtin_amdgcn_frexp_expf(__int_as_float(top_now));
-        if (__any(most_now > m || top_now > top)) {
-            const float alpha = __builtin_amdgcn_exp2f(m - base);
-            const float again = ldexpf(alpha, __builtin_amdgcn_frexp_expf(__int_as_float(top)) - e);
+        largest *= factor;
+        const int scale_bits = seen > 0 ? __float_as_int(own.value) & 0x7fffffff : 0;
+        if (__any(largest > m || scale_bits > top)) {
+            const float next = fmaxf(m, chunks_max(largest));
+            const int next_top = max(top, over_chunks(scale_bits, [](int a, int b) { return max(a, b); }));
+            const int next_exponent = __builtin_amdgcn_frexp_expf(__int_as_float(next_top));
+            const float alpha = __builtin_amdgcn_exp2f(m - (next == -INFINITY ? 0.f : next));
+            const float again = ldexpf(alpha, top_exponent - next_exponent);
             l *= alpha;
 #pragma unroll
             for (int n = 0; n < D / 16; ++n) o[n] *= again;
-            m = most_now;
-            top = top_now;
+            m = next;
+            top = next_top;
+            top_exponent = next_exponent;
         }
-        const float to_units = top < 0x7f800000 && seen > 0 ? ldexpf(own.value, 15 - e) : 0.f;
+        const float base = m == -INFINITY ? 0.f : m;  // nothing seen yet: every weight below is 0
+        // The exponential gives the weight times its value scale at once; the chunk's scale comes off the sum of its weights. A
+        // scale of 0 stands as 2^-100 of the largest, which leaves an f16 weight of 0 and the sum.
+        const float to_units = top < 0x7f800000 && seen > 0 ? fmaxf(ldexpf(fabsf(own.value), 15 - top_exponent), 0x1p-100f) : 1.f;
+        const float log_units = __builtin_amdgcn_logf(to_units), shift = log_units - base;
         float sum = 0.f;
         v8h high[2], low[2];
 #pragma unroll
         for (int i = 0; i < 16; i += 2) {
-            const v2f p{__builtin_amdgcn_exp2f(fmaf(x[i], factor, -base)), __builtin_amdgcn_exp2f(fmaf(x[i + 1], factor, -base))};
-            sum += p[0];
-            sum += p[1];
-            const v2f w{p[0] * to_units, p[1] * to_units};
+            const v2f w{__builtin_amdgcn_exp2f(fmaf(x[i], factor, shift)), __builtin_amdgcn_exp2f(fmaf(x[i + 1], factor, shift))};
+            sum += w[0];
+            sum += w[1];
             const v2h a = __builtin_convertvector(w, v2h);
             const v2f rest{w[0] - static_cast<float>(a[0]), w[1] - static_cast<float>(a[1])};
             const v2h b = __builtin_convertvector(rest, v2h);
@@ -961,7 +1022,7 @@ __global__ __launch_bounds__(kPromptWaves * 64, 2) void paged_prompt_kernel(Page
             low[i / 8][i % 8] = b[0];
             low[i / 8][i % 8 + 1] = b[1];
         }
-        l += sum;
+        l = fmaf(sum, __builtin_amdgcn_exp2f(-log_units), l);
         // four pieces are the values of two tiles of features, each the first half of the keys and the second
 #pragma unroll
         for (int n = 0; n < D / 16; n += 2) {
@@ -998,7 +1059,7 @@ __global__ __launch_bounds__(kPromptWaves * 64, 2) void paged_prompt_kernel(Page
         }
     }
     l = chunks_sum(l);
-    const float unit = top < 0x7f800000 ? ldexpf(1.f, __builtin_amdgcn_frexp_expf(__int_as_float(top)) - 15) : NAN;
+    const float unit = top < 0x7f800000 ? ldexpf(1.f, top_exponent - 15) : NAN;
     if (chunk == 0) {
         ms[wave][column] = m;
         ls[wave][column] = l;
@@ -1094,18 +1155,19 @@ struct Plan {
     Split split;
 };
 
-Plan plan_of(int64_t heads, int64_t kv_heads, int64_t sequences, int64_t tokens, int64_t max_keys, int64_t most) {
+Plan plan_of(int64_t heads, int64_t kv_heads, int64_t dim, int64_t sequences, int64_t tokens, int64_t max_keys, int64_t most) {
     Plan plan;
     const int64_t group = heads / kv_heads;
     plan.tiles = tile_base(tokens, sequences, static_cast<int>(group));
     const int64_t groups = std::max<int64_t>(1, plan.tiles * kv_heads);
     const int64_t keys = std::min<int64_t>(std::max<int64_t>(max_keys, 1), int64_t{1} << 30);
-    plan.prompts = tokens * group >= kTileRows * sequences;
+    plan.prompts = tokens * group > 32 * sequences;
     plan.waves = !plan.prompts && groups <= compute_units() && keys <= 2048 ? 8 : 4;
     const int64_t least = 256;
-    int64_t count = (2 * compute_units() + groups - 1) / groups;
-    if (plan.waves == 8 || keys <= 1024) count = 1;
-    count = std::max<int64_t>(1, std::min({std::max(count, keys / 8192), (keys + least - 1) / least, most, int64_t{65535}}));
+    // as many workgroups as the CUs hold at once, none with fewer than 512 keys, none with more than about 8192
+    int64_t count = ((dim == 64 ? 4 : 2) * compute_units() + groups - 1) / groups;
+    if (plan.prompts ? 2 * groups > compute_units() : plan.waves == 8 || keys <= 1024) count = 1;
+    count = std::max<int64_t>(1, std::min({std::max(count, keys / 8192), keys / 512, most, int64_t{65535}}));
     const int64_t part = ((keys + count - 1) / count + least - 1) / least * least;
     plan.split = {static_cast<int>((keys + part - 1) / part), static_cast<int>(part), nullptr};
     return plan;
@@ -1257,7 +1319,7 @@ extern "C" int kd_paged_attention_workspace(int64_t* bytes, int64_t heads, int64
         (head_dim != 64 && head_dim != 128) || sequences < 0 || sequences >= int64_t{1} << 24 || tokens < 0 ||
         tokens >= int64_t{1} << 31 || max_keys < 0)
         return fail(KD_E_INVALID, "kd_paged_attention_workspace: bad arguments");
-    const Split split = plan_of(heads, kv_heads, sequences, tokens, max_keys, INT32_MAX).split;
+    const Split split = plan_of(heads, kv_heads, head_dim, sequences, tokens, max_keys, INT32_MAX).split;
     *bytes = split.count > 1 ? split.count * part_bytes(tokens * heads, head_dim) : 0;
     return KD_OK;
 }
@@ -1279,7 +1341,7 @@ extern "C" int kd_paged_attention(int dtype, void* out, const void* q, const int
     if (int rc = ensure_device()) return rc;
     if (c.pages == 0) c.columns = 0;  // no position has a page
     const int64_t rows = heads * c.tokens;
-    Plan plan = plan_of(heads, c.kv_heads, c.sequences, c.tokens, max_keys, workspace_bytes / part_bytes(rows, c.head_dim));
+    Plan plan = plan_of(heads, c.kv_heads, c.head_dim, c.sequences, c.tokens, max_keys, workspace_bytes / part_bytes(rows, c.head_dim));
     const Split split{plan.split.count, plan.split.part, static_cast<float*>(workspace)};
     if (int rc = check_grid(what, plan.tiles * c.kv_heads)) return rc;
     const auto launch = [&](auto dim, auto waves) {
