@@ -235,11 +235,12 @@ __device__ __forceinline__ uint32_t code_of(double x, double inverse) {
 
 constexpr int kAppendThreads = 256;
 
-template <bool Vector>
+template <int D, bool Vector>
 __global__ __launch_bounds__(kAppendThreads) void paged_append_kernel(Paged c, Rotation rotation, Strided k, Strided v,
                                                                       Strided q, float* __restrict__ q_out, int heads,
                                                                       int64_t cache_groups, int q_tokens) {
-    const int dim = c.head_dim, units = dim / kUnit, threads = blockDim.x;
+    constexpr int dim = D, units = D / kUnit;
+    const int threads = blockDim.x;
     if (static_cast<int64_t>(blockIdx.x) >= cache_groups) {
         // the queries of q_tokens tokens
         const int64_t token0 = (static_cast<int64_t>(blockIdx.x) - cache_groups) * q_tokens;
@@ -1288,13 +1289,17 @@ extern "C" int kd_paged_append(int dtype, const kd_paged_cache* cache, const kd_
     // 16-byte pieces need rows and tables that keep them aligned and pairs that come in fours
     const auto whole = [](const Strided& x) { return aligned(x.data, 16) && x.row % 4 == 0 && x.head % 4 == 0; };
     const bool vector = r.half % 4 == 0 && aligned(r.cosines, 16) && aligned(r.sines, 16) && whole(ks) && (q == nullptr || whole(qs));
-    const auto launch = [&](auto v_) {
-        hipLaunchKernelGGL((paged_append_kernel<decltype(v_)::value>), dim3(static_cast<uint32_t>(cache_groups + q_groups)),
+    const auto launch = [&](auto dim, auto aligned_pieces) {
+        hipLaunchKernelGGL((paged_append_kernel<decltype(dim)::value, decltype(aligned_pieces)::value>), dim3(static_cast<uint32_t>(cache_groups + q_groups)),
                            dim3(threads), 0, stream(), c, r, ks, vs, qs, static_cast<float*>(q_out), static_cast<int>(heads),
                            cache_groups, q_tokens);
     };
-    if (vector) launch(std::true_type{});
-    else launch(std::false_type{});
+    const auto with_dim = [&](auto aligned_pieces) {
+        if (c.head_dim == 64) launch(std::integral_constant<int, 64>{}, aligned_pieces);
+        else launch(std::integral_constant<int, 128>{}, aligned_pieces);
+    };
+    if (vector) with_dim(std::true_type{});
+    else with_dim(std::false_type{});
     KD_LAUNCH_CHECK();
     return KD_OK;
 }
