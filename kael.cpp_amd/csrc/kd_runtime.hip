@@ -23,12 +23,14 @@ struct DeviceState {
     int ordinal = 0;
     int cus = 0;
     std::string arch;
-    // Workspace, guarded by g_workspace_mutex: the block, its size, and the stream the last
-    // lease enqueued its kernels on (valid once `workspace_used` is set).
+    // Workspace, guarded by g_workspace_mutex: the block, its size, the stream the last lease enqueued its kernels on (valid
+    // once `workspace_used` is set), and an event recorded behind them where that is not the null stream: its owner may have
+    // destroyed the stream since, and a destroyed stream is no stream to wait for.
     void* workspace = nullptr;
     size_t workspace_bytes = 0;
     hipStream_t workspace_stream = nullptr;
     bool workspace_used = false;
+    hipEvent_t workspace_event = nullptr;
 };
 
 DeviceState& state() {
@@ -90,7 +92,15 @@ int device_ordinal() { return state().ordinal; }
 int compute_units() { return state().cus > 0 ? state().cus : 256; }
 
 Workspace::~Workspace() {
-    if (held) g_workspace_mutex.unlock();
+    if (!held) return;
+    DeviceState& s = state();
+    if (ptr != nullptr && s.workspace_stream != nullptr) {
+        // kernels that a capture takes up run when their graph does, not behind this lease
+        hipStreamCaptureStatus captured = hipStreamCaptureStatusNone;
+        if (hipStreamIsCapturing(s.workspace_stream, &captured) == hipSuccess && captured == hipStreamCaptureStatusNone)
+            (void)hipEventRecord(s.workspace_event, s.workspace_stream);
+    }
+    g_workspace_mutex.unlock();
 }
 
 int workspace(Workspace& lease, size_t bytes) {
@@ -102,7 +112,12 @@ int workspace(Workspace& lease, size_t bytes) {
     const hipStream_t current = g_stream.load();
     // The previous lease's kernels may still run on another stream: let them finish before this
     // stream reuses (or this call frees) the block.
-    if (s.workspace_used && s.workspace_stream != current) KD_HIP(hipStreamSynchronize(s.workspace_stream));
+    if (current != nullptr && s.workspace_event == nullptr)
+        KD_HIP(hipEventCreateWithFlags(&s.workspace_event, hipEventDisableTiming));
+    if (s.workspace_used && s.workspace_stream != current) {
+        if (s.workspace_stream == nullptr) KD_HIP(hipStreamSynchronize(nullptr));
+        else KD_HIP(hipEventSynchronize(s.workspace_event));
+    }
     if (s.workspace_bytes < bytes) {
         if (s.workspace != nullptr) {
             // Kernels queued by earlier leases may still read the old block: drain before freeing.
