@@ -355,7 +355,7 @@ int kd_cached_attention(int dtype, void* out, const void* q, const int64_t* q_st
  *   keys          [pages][kv_heads][page_size][head_dim]
  *   values        [pages][kv_heads][head_dim][page_size]
  *   key_scales, value_scales  [pages][kv_heads]
- * contiguous device memory; keys and values 16-byte aligned, the scales 4-byte. page_size is 16, 32,
+ * contiguous device memory; keys and values 16-byte aligned, the scales 4-byte and not negative. page_size is 16, 32,
  * 64, 128 or 256 and head_dim 64 or 128 (KD_E_UNSUPPORTED otherwise). */
 typedef struct kd_paged_cache {
     int8_t* keys;
@@ -495,7 +495,7 @@ int kd_cross_entropy_grad(int dtype, void* out, const void* logits, const int64_
  * An index outside 0 .. cols - 1 is no entry (its t is not read into the sums); a row without entries, or
  * whose t are all -inf, has loss 0. The same index twice counts twice. stats [rows][2] receives each row's max(z) and
  * sum exp((z - max) / T), which the gradient reads. dtype f32 or f64, rows contiguous, sums in double;
- * 1 <= kept <= 1024, temperature > 0. */
+ * 1 <= kept <= 1024, 1e-6 <= temperature <= 1e6. */
 int kd_distill_rows(int dtype, void* losses, void* stats, const void* logits, const int64_t* indices,
                     const void* teacher, int64_t rows, int64_t cols, int64_t kept, double temperature);
 

@@ -93,77 +93,68 @@ __device__ __forceinline__ int part_of(const double* sums, double point, double&
     return last;
 }
 
-template <typename T>
-__global__ __launch_bounds__(kVerifyThreads) void verify_drafts_kernel(int64_t* __restrict__ tokens, int64_t* __restrict__ accepted,
-                                                                       const T* __restrict__ target, const T* __restrict__ draft,
-                                                                       const int64_t* __restrict__ drafted,
-                                                                       const int64_t* __restrict__ counts,
-                                                                       const double* __restrict__ uniforms, int64_t drafts,
-                                                                       int64_t vocab) {
-    __shared__ double sums[2][kVerifyWaves];
-    constexpr int kCount = Weights<T>::kCount, kRound = 64 * kCount;
-    const int64_t s = blockIdx.x;
-    const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
-    const int64_t* x = drafted + s * drafts;
-    const double* u = uniforms + s * (drafts + 1);
-    const int64_t given = counts[s];
-    const double last_u = u[drafts];
-    const int64_t count = given < 0 ? 0 : given > drafts ? drafts : given;
-    int64_t kept = 0;
-    for (bool open = true; open && kept < drafts;) {
-        const int64_t i = kept + lane;
-        bool good = false;
-        if (i < drafts) {  // not count, whose load is under way
-            const int64_t token = x[i];
-            const double draw = u[i];
-            if (token >= 0 && token < vocab) {
-                const double p = static_cast<double>(target[(s * (drafts + 1) + i) * vocab + token]);
-                const double q = draft != nullptr ? static_cast<double>(draft[(s * drafts + i) * vocab + token]) : 1.0;
-                good = draw * q < p;
+// One sequence's operands, and how its vocabulary is divided: into 16 parts, and each part into 16 small ones, of whole rounds
+// of a wave.
+template <typename T> struct Verification {
+    const T* target;
+    const T* draft;
+    const int64_t* drafted;
+    const int64_t* counts;
+    const double* uniforms;
+    int64_t drafts, vocab;
+    static constexpr int kRound = 64 * Weights<T>::kCount;
+
+    __device__ __forceinline__ int64_t part() const {
+        return (vocab + kVerifyWaves * kRound - 1) / (kVerifyWaves * kRound) * kRound;
+    }
+    __device__ __forceinline__ int64_t small() const { return (part() / kRound + kVerifyWaves - 1) / kVerifyWaves * kRound; }
+    __device__ __forceinline__ int64_t count(int64_t s) const {
+        const int64_t given = counts[s];
+        return given < 0 ? 0 : given > drafts ? drafts : given;
+    }
+    __device__ __forceinline__ const int64_t* tokens(int64_t s) const { return drafted + s * drafts; }
+    // How many of the sequence's drafts are accepted, by a wave.
+    __device__ __forceinline__ int64_t accepted(int64_t s) const {
+        const int lane = threadIdx.x % 64;
+        const int64_t most = count(s);
+        const double* u = uniforms + s * (drafts + 1);
+        int64_t kept = 0;
+        for (bool open = true; open && kept < drafts;) {
+            const int64_t i = kept + lane;
+            bool good = false;
+            if (i < drafts) {  // not count, whose load is under way
+                const int64_t token = tokens(s)[i];
+                const double draw = u[i];
+                if (token >= 0 && token < vocab) {
+                    const double p = static_cast<double>(target[(s * (drafts + 1) + i) * vocab + token]);
+                    const double q = draft != nullptr ? static_cast<double>(draft[(s * drafts + i) * vocab + token]) : 1.0;
+                    good = draw * q < p;
+                }
             }
+            const uint64_t all = __ballot(good && i < most);
+            const int n = all == ~uint64_t{0} ? 64 : __ffsll(static_cast<unsigned long long>(~all)) - 1;
+            open = n == 64;
+            kept += n;
         }
-        const uint64_t all = __ballot(good && i < count);
-        const int n = all == ~uint64_t{0} ? 64 : __ffsll(static_cast<unsigned long long>(~all)) - 1;
-        open = n == 64;
-        kept += n;
+        return kept;
     }
-    Weights<T> weights{target + (s * (drafts + 1) + kept) * vocab, nullptr, -1};
-    if (kept < count) {
-        if (draft != nullptr) weights.q = draft + (s * drafts + kept) * vocab;
-        else weights.certain = x[kept];
+    // The weights that the token after `kept` accepted drafts is drawn from.
+    __device__ __forceinline__ Weights<T> weights(int64_t s, int64_t kept) const {
+        Weights<T> w{target + (s * (drafts + 1) + kept) * vocab, nullptr, -1};
+        if (kept < count(s)) {
+            if (draft != nullptr) w.q = draft + (s * drafts + kept) * vocab;
+            else w.certain = tokens(s)[kept];
+        }
+        return w;
     }
-    const int64_t part = (vocab + kVerifyWaves * kRound - 1) / (kVerifyWaves * kRound) * kRound;
-    double total = 0;
-    while (true) {
-        const double sum = weights.sum(wave * part, min((wave + 1) * part, vocab));
-        if (lane == 0) sums[0][wave] = sum;
-        __syncthreads();
-        total = 0;
-        for (int w = 0; w < kVerifyWaves; ++w) total += sums[0][w];
-        if (total > 0 || (weights.q == nullptr && weights.certain < 0)) break;
-        // nothing is left of p - q (or it is NaN): the target's own probabilities
-        weights.q = nullptr;
-        weights.certain = -1;
-        __syncthreads();
-    }
-    int64_t* out = tokens + s * (drafts + 1);
-    for (int64_t i = threadIdx.x; i <= drafts; i += kVerifyThreads)
-        if (i != kept) out[i] = i < kept ? x[i] : -1;
-    if (threadIdx.x == 0) accepted[s] = kept;
-    if (!(total > 0 && total < INFINITY)) {
-        if (threadIdx.x == 0) out[kept] = -1;
-        return;
-    }
-    const double point = last_u * total;
-    double before = 0;
-    const int64_t outer = part_of(sums[0], point, before) * part, outer_end = min(outer + part, vocab);
-    const int64_t small = (part / kRound + kVerifyWaves - 1) / kVerifyWaves * kRound;
-    const double sum = weights.sum(outer + wave * small, min(outer + (wave + 1) * small, outer_end));
-    if (lane == 0) sums[1][wave] = sum;
-    __syncthreads();
-    const int holder = part_of(sums[1], point, before);
-    if (wave != holder) return;
-    const int64_t from = outer + holder * small, to = min(from + small, outer_end);
+};
+
+// The entry of from .. to - 1 whose running sum, `before` ahead of it, first exceeds `point`, else the last with any weight; by
+// a wave.
+template <typename T>
+__device__ __forceinline__ int64_t entry_of(const Weights<T>& weights, int64_t from, int64_t to, double point, double before) {
+    constexpr int kCount = Weights<T>::kCount, kRound = 64 * kCount;
+    const int lane = threadIdx.x % 64;
     int64_t picked = -1;
     for (int64_t j0 = from; j0 < to; j0 += kRound) {
         const int64_t j = j0 + lane * kCount;
@@ -192,8 +183,7 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_drafts_kernel(int64_t* 
         const uint64_t lanes_over = __ballot(over >= 0), lanes_any = __ballot(any >= 0);
         if (lanes_over != 0) {
             const int first = __ffsll(static_cast<unsigned long long>(lanes_over)) - 1;
-            picked = j0 + first * kCount + __shfl(over, first);
-            break;
+            return j0 + first * kCount + __shfl(over, first);
         }
         if (lanes_any != 0) {
             const int last = 63 - __clzll(static_cast<long long>(lanes_any));
@@ -201,7 +191,125 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_drafts_kernel(int64_t* 
         }
         before = next;
     }
+    return picked;
+}
+
+template <typename T>
+__device__ __forceinline__ void write_tokens(int64_t* out, const int64_t* drafted, int64_t drafts, int64_t kept) {
+    for (int64_t i = threadIdx.x; i <= drafts; i += blockDim.x)
+        if (i != kept) out[i] = i < kept ? drafted[i] : -1;
+}
+
+template <typename T>
+__global__ __launch_bounds__(kVerifyThreads) void verify_drafts_kernel(int64_t* __restrict__ tokens, int64_t* __restrict__ accepted,
+                                                                       Verification<T> v) {
+    __shared__ double sums[2][kVerifyWaves];
+    const int64_t s = blockIdx.x;
+    const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
+    const double last_u = v.uniforms[s * (v.drafts + 1) + v.drafts];
+    const int64_t kept = v.accepted(s);
+    Weights<T> weights = v.weights(s, kept);
+    const int64_t part = v.part();
+    double total = 0;
+    while (true) {
+        const double sum = weights.sum(wave * part, min((wave + 1) * part, v.vocab));
+        if (lane == 0) sums[0][wave] = sum;
+        __syncthreads();
+        total = 0;
+        for (int w = 0; w < kVerifyWaves; ++w) total += sums[0][w];
+        if (total > 0 || (weights.q == nullptr && weights.certain < 0)) break;
+        // nothing is left of p - q (or it is NaN): the target's own probabilities
+        weights.q = nullptr;
+        weights.certain = -1;
+        __syncthreads();
+    }
+    int64_t* out = tokens + s * (v.drafts + 1);
+    write_tokens<T>(out, v.tokens(s), v.drafts, kept);
+    if (threadIdx.x == 0) accepted[s] = kept;
+    if (!(total > 0 && total < INFINITY)) {
+        if (threadIdx.x == 0) out[kept] = -1;
+        return;
+    }
+    const double point = last_u * total;
+    double before = 0;
+    const int64_t outer = part_of(sums[0], point, before) * part, outer_end = min(outer + part, v.vocab);
+    const int64_t small = v.small();
+    const double sum = weights.sum(min(outer + wave * small, outer_end), min(outer + (wave + 1) * small, outer_end));
+    if (lane == 0) sums[1][wave] = sum;
+    __syncthreads();
+    const int holder = part_of(sums[1], point, before);
+    if (wave != holder) return;
+    const int64_t from = outer + holder * small;
+    const int64_t picked = entry_of(weights, from, min(from + small, outer_end), point, before);
     if (lane == 0) out[kept] = picked;
+}
+
+// The same for few sequences in two launches: sixteen workgroups a sequence sum the small parts, of the weights and of the
+// target alone ([sequence][2][256]), and one finds the entry.
+template <typename T>
+__global__ __launch_bounds__(kVerifyThreads) void verify_sums_kernel(double* __restrict__ sums, int64_t* __restrict__ accepted,
+                                                                     Verification<T> v) {
+    const int64_t s = blockIdx.y;
+    const int lane = threadIdx.x % 64, wave = threadIdx.x / 64, outer_part = blockIdx.x;
+    const int64_t kept = v.accepted(s);
+    Weights<T> weights = v.weights(s, kept);
+    const int64_t part = v.part(), small = v.small();
+    const int64_t outer = outer_part * part, outer_end = min(outer + part, v.vocab);
+    const int64_t from = min(outer + wave * small, outer_end), to = min(outer + (wave + 1) * small, outer_end);
+    double* own = sums + s * 2 * kVerifyWaves * kVerifyWaves + outer_part * kVerifyWaves + wave;
+    const double sum = weights.sum(from, to);
+    weights.q = nullptr;
+    weights.certain = -1;
+    const double alone = weights.sum(from, to);
+    if (lane == 0) {
+        own[0] = sum;
+        own[kVerifyWaves * kVerifyWaves] = alone;
+    }
+    if (outer_part == 0 && threadIdx.x == 0) accepted[s] = kept;
+}
+
+template <typename T>
+__global__ __launch_bounds__(kVerifyWaves * kVerifyWaves) void verify_entry_kernel(int64_t* __restrict__ tokens,
+                                                                                   const int64_t* __restrict__ accepted,
+                                                                                   const double* __restrict__ sums, Verification<T> v) {
+    __shared__ double small_sums[2][kVerifyWaves * kVerifyWaves], part_sums[2][kVerifyWaves];
+    const int64_t s = blockIdx.x;
+    const int64_t kept = accepted[s];
+    const double last_u = v.uniforms[s * (v.drafts + 1) + v.drafts];
+    for (int k = 0; k < 2; ++k)
+        small_sums[k][threadIdx.x] = sums[(s * 2 + k) * kVerifyWaves * kVerifyWaves + threadIdx.x];
+    __syncthreads();
+    if (threadIdx.x < 2 * kVerifyWaves) {
+        const int k = threadIdx.x / kVerifyWaves, w = threadIdx.x % kVerifyWaves;
+        double sum = 0;
+        for (int i = 0; i < kVerifyWaves; ++i) sum += small_sums[k][w * kVerifyWaves + i];
+        part_sums[k][w] = sum;
+    }
+    __syncthreads();
+    int64_t* out = tokens + s * (v.drafts + 1);
+    write_tokens<T>(out, v.tokens(s), v.drafts, kept);
+    if (threadIdx.x >= 64) return;
+    Weights<T> weights = v.weights(s, kept);
+    int which = 0;
+    double total = 0;
+    while (true) {
+        total = 0;
+        for (int w = 0; w < kVerifyWaves; ++w) total += part_sums[which][w];
+        if (total > 0 || which == 1) break;
+        which = 1;
+        weights.q = nullptr;
+        weights.certain = -1;
+    }
+    int64_t picked = -1;
+    if (total > 0 && total < INFINITY) {
+        const double point = last_u * total;
+        double before = 0;
+        const int outer = part_of(part_sums[which], point, before);
+        const int holder = part_of(small_sums[which] + outer * kVerifyWaves, point, before);
+        const int64_t end = min((outer + 1) * v.part(), v.vocab), from = outer * v.part() + holder * v.small();
+        picked = entry_of(weights, from, min(from + v.small(), end), point, before);
+    }
+    if (threadIdx.x == 0) out[kept] = picked;
 }
 
 // ---- distillation ---------------------------------------------------------------------------------
@@ -503,7 +611,8 @@ int check_distill(const char* what, int dtype, int64_t rows, int64_t cols, int64
     if (rows < 0 || cols < 1 || rows >= (int64_t{1} << 31) || cols >= (int64_t{1} << 31))
         return fail(KD_E_INVALID, name + ": bad number of rows or columns");
     if (kept < 1 || kept > kMaxKept) return fail(KD_E_INVALID, name + ": 1 to 1024 kept entries");
-    if (!(temperature > 0) || !std::isfinite(temperature)) return fail(KD_E_INVALID, name + ": temperature must be positive");
+    if (!(temperature >= 1e-6 && temperature <= 1e6))
+        return fail(KD_E_INVALID, name + ": temperature must be between 1e-6 and 1e6");
     return KD_OK;
 }
 
@@ -532,11 +641,27 @@ extern "C" int kd_verify_drafts(int dtype, int64_t* tokens, int64_t* accepted, c
         (drafted == nullptr && drafts > 0))
         return fail(KD_E_INVALID, "kd_verify_drafts: every operand but draft must be given");
     if (int rc = ensure_device()) return rc;
+    // Few sequences: a CU streams a row at about 45 GB/s, and sixteen of them for a sequence are worth a second launch while the
+    // card has them (f32, one launch / two, us: 1 x 100000 26 / 13, 8 x 50257 18 / 12, 8 x 20000 12.5 / 10.4; 32 x 50257 19 / 19,
+    // 64 x 50257 22 / 30). Their sums go through the backend's workspace, which may grow, and that is no call to make under capture.
+    hipStreamCaptureStatus captured = hipStreamCaptureStatusNone;
+    if (stream() != nullptr) KD_HIP(hipStreamIsCapturing(stream(), &captured));
+    const bool split = vocab >= 16384 && sequences * kVerifyWaves <= compute_units() && captured == hipStreamCaptureStatusNone;
+    Workspace lease;
+    if (split)
+        if (int rc = workspace(lease, static_cast<size_t>(sequences) * 2 * kVerifyWaves * kVerifyWaves * sizeof(double))) return rc;
     const auto launch = [&](auto zero) {
         using T = decltype(zero);
-        hipLaunchKernelGGL((verify_drafts_kernel<T>), dim3(static_cast<uint32_t>(sequences)), dim3(kVerifyThreads), 0, stream(),
-                           tokens, accepted, static_cast<const T*>(target), static_cast<const T*>(draft), drafted, counts,
-                           uniforms, drafts, vocab);
+        const Verification<T> v{static_cast<const T*>(target), static_cast<const T*>(draft), drafted, counts, uniforms, drafts, vocab};
+        const uint32_t groups = static_cast<uint32_t>(sequences);
+        if (!split) {
+            hipLaunchKernelGGL((verify_drafts_kernel<T>), dim3(groups), dim3(kVerifyThreads), 0, stream(), tokens, accepted, v);
+            return;
+        }
+        double* sums = static_cast<double*>(lease.ptr);
+        hipLaunchKernelGGL((verify_sums_kernel<T>), dim3(kVerifyWaves, groups), dim3(kVerifyThreads), 0, stream(), sums, accepted, v);
+        hipLaunchKernelGGL((verify_entry_kernel<T>), dim3(groups), dim3(kVerifyWaves * kVerifyWaves), 0, stream(), tokens, accepted,
+                           sums, v);
     };
     if (dtype == KD_F32) launch(0.f);
     else launch(0.0);

@@ -135,11 +135,12 @@ def values_of(cache, sequence, head, length):
 def attention(cache, starts, lengths, q, scale):
     """out [tokens, heads, dim] in f64 (-777 in rows outside every sequence), and each row's tolerance.
 
-    A score is a sum of products of a query's fixed-point digits and the keys' codes, exact but for the digits' 2^-31 and
-    about 5 roundings of 2^-24 of it, so are the exponent's argument and its subtraction; numerator and denominator both
-    carry that, the exponential adds 2 steps, every 64 keys add about 4 roundings to the sums, and the split parts'
-    joining 8: with S the row's largest score in size, each output is within
-    2^-24 * max|v| * (2 * 6 * 1.45 * S + 4 * keys / 64 + 32)."""
+    With S a row's largest score in size and A the largest sum of its products' sizes: the query's pieces hold 2^-24 of it, and
+    heads of 64 sum two products a piece per 32 features in f32 (2 dim / 32 roundings of at most A; the whole sums of heads of
+    128 are exact); the score's factors, the exponent's argument and its base round 7 times at most S; the exponential adds 2
+    steps and its pieces 2. Numerator and denominator carry that, every 64 keys add 4 roundings to the sums, the joining of waves
+    and parts 32 altogether:
+    2^-24 * max|v| * (2 * (A * (2 + dim / 16 or 0) + 7 S + 4) + 4 * keys / 64 + 32)."""
     tokens, heads, dim = q.shape
     out, tolerance = np.full(q.shape, -777.0), np.zeros(q.shape)
     group = heads // cache.kv_heads
@@ -155,10 +156,12 @@ def attention(cache, starts, lengths, q, scale):
                     out[row, h] = 0
                     continue
                 score = k[seen] @ q[row, h].astype(np.float64) * scale
+                size = np.abs(k[seen]) @ np.abs(q[row, h].astype(np.float64)) * abs(scale)
                 p = np.exp(score - score.max())
                 out[row, h] = p @ v[seen] / p.sum()
                 tolerance[row, h] = 2.0 ** -24 * np.abs(v[seen]).max() * (
-                    17.4 * np.abs(score).max() + 4 * seen.sum() / 64 + 32)
+                    2 * (size.max() * (2 + (dim / 16 if dim == 64 else 0)) + 7 * np.abs(score).max() + 4)
+                    + 4 * seen.sum() / 64 + 32)
     return out, tolerance
 
 

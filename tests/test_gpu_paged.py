@@ -209,6 +209,8 @@ ATTENTION = [
     ([1], [2500], 1, 8, 64, 128), ([1] * 5, [1, 63, 200, 517, 1024], 2, 2, 16, 64), ([5, 3, 1], [5, 300, 77], 2, 6, 32, 64),
     ([16, 17], [16, 900], 1, 1, 16, 64), ([4, 4], [700, 4], 1, 4, 128, 128), ([5], [600], 1, 4, 64, 64),
     ([100, 1, 0, 65], [100, 500, 9, 130], 1, 2, 16, 64), ([33], [33], 2, 2, 256, 128), ([257], [300], 1, 1, 64, 64),
+    ([80], [2600], 1, 1, 16, 64), ([40], [2100], 1, 2, 64, 128), ([33, 2], [3000, 1200], 1, 2, 32, 64), ([7], [2500], 2, 2, 16, 64),
+    ([1] * 3, [5000, 20, 2100], 1, 2, 256, 128), ([1], [300], 1, 64, 16, 64), ([70, 64, 1, 128], [70, 64, 65, 200], 1, 1, 16, 128),
     ([9], [9], 1, 12, 16, 128), ([2] * 70, [2 + 7 * (s % 40) for s in range(70)], 1, 1, 16, 64),
 ]
 
@@ -229,6 +231,9 @@ def test_attention_is_its_definition(kdb, case):
         got = run_attention(kdb, on, q, dim ** -0.5, hint, room)
         off = np.abs(got - want)
         assert (off <= tolerance).all(), (hint, off.max(), (off / np.maximum(tolerance, 1e-30)).max())
+        # scores of at most about 6 whose dozen roundings of rms 2^-24 / sqrt(3) add up at random: 3.4e-8 * sqrt(12) * 6; a
+        # piece that is lost makes 2^-12
+        assert np.linalg.norm(off) <= 1e-6 * np.linalg.norm(want)
         np.testing.assert_array_equal(run_attention(kdb, on, q, dim ** -0.5, hint, room), got)
 
 
@@ -248,34 +253,39 @@ def test_attention_over_views_and_rows_of_no_sequence(kdb):
     assert (got[:2] == -777).all() and (got[-5:] == -777).all()
 
 
-def test_attention_of_positions_without_a_page(kdb):
+# `times`: as few rows a sequence as share a workgroup's keys, or as many as take the prompts' kernel
+@pytest.mark.parametrize("times", [1, 30])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_attention_of_positions_without_a_page(kdb, dim, times):
     """Evicted pages, a sequence without any page, lengths past the table, more new tokens than positions."""
     rng = np.random.default_rng(12)
-    starts, lengths, tokens = batch_of([1, 2, 3, 9], [100, 64, 500, 4])
-    cache = paged.Cache(rng, 4, 8, 2, 16, 64)
+    starts, lengths, tokens = batch_of([times * n for n in (1, 2, 3, 9)], [100, 64, 500, 4])
+    cache = paged.Cache(rng, 4, 8, 2, 16, dim)
     cache.table[0, [0, 2, 6]] = [-1, cache.pages, 1 << 40]
     cache.table[1] = -1
-    q = rng.normal(0, 1, (tokens, 4, 64)).astype(np.float32)
+    q = rng.normal(0, 1, (tokens, 4, dim)).astype(np.float32)
     on = paged.Device(kdb, cache, starts, lengths, tokens)
     want, tolerance = paged.attention(cache, starts, lengths, q, 0.125)
-    got = run_attention(kdb, on, q, 0.125, 128, workspace_for(kdb, 4, 2, 64, 4, tokens, 128))
+    got = run_attention(kdb, on, q, 0.125, 128, workspace_for(kdb, 4, 2, dim, 4, tokens, 128))
     assert (np.abs(got - want) <= tolerance).all()
-    assert (got[1:3] == 0).all() and (got[6:11] == 0).all()
+    assert (got[times:3 * times] == 0).all() and (got[6 * times:15 * times - 4] == 0).all()
 
 
-def test_attention_takes_nan_from_what_it_sees_alone(kdb):
+@pytest.mark.parametrize("heads", [1, 2])  # 20 and 40 rows a sequence: either kernel
+@pytest.mark.parametrize("dim", [64, 128])
+def test_attention_takes_nan_from_what_it_sees_alone(kdb, dim, heads):
     """A NaN scale, of a page that one row sees and another does not; a query that is not finite."""
     rng = np.random.default_rng(13)
     starts, lengths, tokens = batch_of([20, 20], [40, 40])
-    cache = paged.Cache(rng, 2, 3, 1, 16, 64)
+    cache = paged.Cache(rng, 2, 3, 1, 16, dim)
     cache.key_scales[cache.table[0, 2], 0] = np.nan     # positions 32..47: rows 12.. of the first sequence
     cache.value_scales[cache.table[1, 2], 0] = np.nan
-    q = rng.normal(0, 1, (tokens, 2, 64)).astype(np.float32)
-    q[5, 0, 3], q[6, 1, 63] = np.inf, np.nan
+    q = rng.normal(0, 1, (tokens, heads, dim)).astype(np.float32)
+    q[5, 0, 3], q[6, heads - 1, 63] = np.inf, np.nan
     on = paged.Device(kdb, cache, starts, lengths, tokens)
     with np.errstate(invalid="ignore"):
         want, tolerance = paged.attention(cache, starts, lengths, np.where(np.isfinite(q), q, 0), 0.125)
-    want[5, 0] = want[6, 1] = np.nan
+    want[5, 0] = want[6, heads - 1] = np.nan
     want[12:20] = want[32:40] = np.nan
     got = run_attention(kdb, on, q, 0.125, 40)
     np.testing.assert_array_equal(np.isnan(got), np.isnan(want))
@@ -283,23 +293,45 @@ def test_attention_takes_nan_from_what_it_sees_alone(kdb):
     assert (np.abs(got - want)[fine] <= tolerance[fine]).all()
 
 
+@pytest.mark.parametrize("new", [3, 40])
+@pytest.mark.parametrize("dim", [64, 128])
 @pytest.mark.parametrize("size", [1e-30, 1e-3, 30.0, 1e30])
-def test_attention_of_small_and_large_queries(kdb, size):
+def test_attention_of_small_and_large_queries(kdb, size, dim, new):
     """One feature a thousand times the others', queries at both ends of the range, pages of zero and tiny scales."""
     rng = np.random.default_rng(14)
-    starts, lengths, tokens = batch_of([3], [200])
-    cache = paged.Cache(rng, 1, 13, 1, 16, 64)
+    starts, lengths, tokens = batch_of([new], [200])
+    cache = paged.Cache(rng, 1, 13, 1, 16, dim)
     cache.value_scales[cache.table[0, 3]] = 0
     cache.key_scales[cache.table[0, 4]] = 0
     cache.value_scales[cache.table[0, 5]] = 1e-30
-    q = rng.normal(0, 1, (tokens, 2, 64)).astype(np.float32)
+    q = rng.normal(0, 1, (tokens, 2, dim)).astype(np.float32)
     q[:, :, 7] *= 1000
     q *= np.float32(size)
-    scale = 1 / (1000 * size)
     on = paged.Device(kdb, cache, starts, lengths, tokens)
-    want, tolerance = paged.attention(cache, starts, lengths, q, scale)
-    got = run_attention(kdb, on, q, scale, 200)
-    assert (np.abs(got - want) <= tolerance).all()
+    for scale in (1 / (1000 * size), -1 / (1000 * size), 0.0):
+        want, tolerance = paged.attention(cache, starts, lengths, q, scale)
+        got = run_attention(kdb, on, q, scale, 200)
+        assert (np.abs(got - want) <= tolerance).all(), scale
+    on.kdb.call("paged_attention", kd.F32, kdb.empty(q.shape, np.float32).ptr, kdb.to_device(q).ptr, kd.strides(2 * dim, dim), 2,
+                on.c, kd.PagedBatch(on.table.ptr, on.starts.ptr, on.lengths.ptr, 1, 0, tokens), 1.0, 200, None, 0)
+
+
+@pytest.mark.parametrize("new", [1, 40])
+def test_attention_without_any_page(kdb, new):
+    """A cache of no pages, a table of no columns: nothing is visible and every row 0."""
+    q = kdb.to_device(np.ones((new, 2, 64), np.float32))
+    starts, lengths = kdb.to_device(np.asarray([0, new])), kdb.to_device(np.asarray([new]))
+    table = kdb.to_device(np.zeros((1, 3), np.int64))
+    for cache, columns in ((kd.PagedCache(None, None, None, None, 0, 1, 16, 64), 3), (kd.PagedCache(None, None, None, None, 0, 1, 16, 64), 0)):
+        out = kdb.to_device(np.full((new, 2, 64), 7, np.float32))
+        batch = kd.PagedBatch(table.ptr, starts.ptr, lengths.ptr, 1, columns, new)
+        kdb.call("paged_attention", kd.F32, out.ptr, q.ptr, kd.strides(128, 64), 2, cache, batch, 1.0, 10, None, 0)
+        assert (out.numpy() == 0).all()
+        kdb.call("paged_append", kd.F32, cache, batch, None, None, None, None, 2, q.ptr, kd.strides(128, 64), q.ptr,
+                 kd.strides(128, 64))
+        got = kdb.to_device(np.full((new, 1, 64), 7, np.float32))
+        kdb.call("paged_read", kd.F32, got.ptr, None, cache, batch)
+        assert (got.numpy() == 0).all()
 
 
 def test_a_prompt_drafts_and_single_tokens_in_turn(kdb):

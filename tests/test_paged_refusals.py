@@ -116,7 +116,7 @@ def test_bad_distillations(lib):
     rows, grad = lib.lib.kd_distill_rows, lib.lib.kd_distill_grad
     for good, f, sizes in (([kd.F32] + [FAKE] * 5 + [2, 9, 3, 1.0], rows, 6), ([kd.F32] + [FAKE] * 6 + [2, 9, 3, 1.0], grad, 7)):
         wrong = [(0, kd.BOOL, UNSUPPORTED), (sizes, -1, INVALID), (sizes + 1, 0, INVALID), (sizes + 2, 0, INVALID),
-                 (sizes + 2, 1025, INVALID), (sizes + 3, 0.0, INVALID), (sizes + 3, float("nan"), INVALID),
+                 (sizes + 2, 1025, INVALID), (sizes + 3, 0.0, INVALID), (sizes + 3, float("nan"), INVALID), (sizes + 3, 1e-7, INVALID), (sizes + 3, 1e7, INVALID),
                  (sizes + 3, float("inf"), INVALID)] + [(at, None, INVALID) for at in range(1, sizes)]
         for at, value, status in wrong:
             args = list(good)
