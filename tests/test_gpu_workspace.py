@@ -11,15 +11,16 @@ import kd
 pytestmark = pytest.mark.gpu
 
 
+@pytest.mark.parametrize("entry", ["reduce", "reduce_noalloc"])  # the growable workspace, the static scratch
 @pytest.mark.parametrize("rounds", [1, 6])
-def test_the_workspace_outlives_its_last_stream(kdb, rounds):
+def test_the_workspace_outlives_its_last_stream(kdb, rounds, entry):
     lib = kdb.lib
     rng = np.random.default_rng(rounds)
     x = rng.integers(-1000, 1000, (3, 200000)).astype(np.int64)
     dx, out = kdb.to_device(x), kdb.empty((3,), np.int64)
 
     def total():
-        kdb.call("reduce", kd.REDUCE_SUM, kd.I64, kd.I64, out.ptr, dx.ptr, x.shape[1], 3)  # few long rows: in split sums
+        kdb.call(entry, kd.REDUCE_SUM, kd.I64, kd.I64, out.ptr, dx.ptr, x.shape[1], 3)  # few long rows: in split sums
         return out.numpy()
 
     want = x.sum(1)
