@@ -1004,17 +1004,16 @@ __global__ __launch_bounds__(kPromptWaves * 64, 2) void paged_prompt_kernel(Page
             top_exponent = next_exponent;
         }
         const float base = m == -INFINITY ? 0.f : m;  // nothing seen yet: every weight below is 0
-        // The exponential gives the weight times its value scale at once; the chunk's scale comes off the sum of its weights. A
-        // scale of 0 stands as 2^-100 of the largest, which leaves an f16 weight of 0 and the sum.
-        const float to_units = top < 0x7f800000 && seen > 0 ? fmaxf(ldexpf(fabsf(own.value), 15 - top_exponent), 0x1p-100f) : 1.f;
-        const float log_units = __builtin_amdgcn_logf(to_units), shift = log_units - base;
+        // the scale multiplies the weight rather than going into the exponent, whose rounding would differ from chunk to chunk
+        const float to_units = top < 0x7f800000 && seen > 0 ? ldexpf(own.value, 15 - top_exponent) : 0.f;
         float sum = 0.f;
         v8h high[2], low[2];
 #pragma unroll
         for (int i = 0; i < 16; i += 2) {
-            const v2f w{__builtin_amdgcn_exp2f(fmaf(x[i], factor, shift)), __builtin_amdgcn_exp2f(fmaf(x[i + 1], factor, shift))};
-            sum += w[0];
-            sum += w[1];
+            const v2f p{__builtin_amdgcn_exp2f(fmaf(x[i], factor, -base)), __builtin_amdgcn_exp2f(fmaf(x[i + 1], factor, -base))};
+            sum += p[0];
+            sum += p[1];
+            const v2f w{p[0] * to_units, p[1] * to_units};
             const v2h a = __builtin_convertvector(w, v2h);
             const v2f rest{w[0] - static_cast<float>(a[0]), w[1] - static_cast<float>(a[1])};
             const v2h b = __builtin_convertvector(rest, v2h);
@@ -1023,7 +1022,7 @@ __global__ __launch_bounds__(kPromptWaves * 64, 2) void paged_prompt_kernel(Page
             low[i / 8][i % 8] = b[0];
             low[i / 8][i % 8 + 1] = b[1];
         }
-        l = fmaf(sum, __builtin_amdgcn_exp2f(-log_units), l);
+        l += sum;
         // four pieces are the values of two tiles of features, each the first half of the keys and the second
 #pragma unroll
         for (int n = 0; n < D / 16; n += 2) {
