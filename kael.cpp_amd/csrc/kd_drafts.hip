@@ -48,29 +48,38 @@ template <typename T> struct Weights {
     int64_t certain;  // q NULL: the entry whose q is 1, or -1
     static constexpr int kCount = Piece<T>::kCount;
 
+    // the weight of entry `entry`, an entry of the pieces a and b; 0 outside from .. to - 1
+    __device__ __forceinline__ double weight(T a, T b, int64_t entry, int64_t from, int64_t to) const {
+        const double w = static_cast<double>(a) - (q != nullptr ? static_cast<double>(b) : entry == certain ? 1.0 : 0.0);
+        return w < 0 || entry < from || entry >= to ? 0.0 : w;
+    }
     // the weights of the entries at .. at + kCount - 1; 0 from `to` on
     __device__ __forceinline__ void at(int64_t at, int64_t to, double (&w)[kCount]) const {
         const Piece<T> a = load_piece(p, at, to, T(0));
         Piece<T> b{};
         if (q != nullptr) b = load_piece(q, at, to, T(0));
 #pragma unroll
-        for (int i = 0; i < kCount; ++i) {
-            w[i] = static_cast<double>(a.x[i]) - (q != nullptr ? static_cast<double>(b.x[i]) : at + i == certain ? 1.0 : 0.0);
-            w[i] = w[i] < 0 || at + i >= to ? 0.0 : w[i];
-        }
+        for (int i = 0; i < kCount; ++i) w[i] = weight(a.x[i], b.x[i], at + i, at, to);
     }
-    // their sum over from .. to - 1, by a wave
+    // Their sum over from .. to - 1, by a wave, a piece of either row at a time: more of them in flight take registers, and cost
+    // (256 x 50257: one piece 19.9 us, two 21.0, four 23.6, eight 39). A piece that would reach past `to` is read from further
+    // down, and its entries before its own first one count nothing.
     __device__ __forceinline__ double sum(int64_t from, int64_t to) const {
-        constexpr int kPieces = 4;
         double total = 0;
-        for (int64_t j = from + threadIdx.x % 64 * kCount; j < to; j += kPieces * 64 * kCount) {
-            double w[kPieces][kCount];
+        if (to < kCount) {
+            double w[kCount];
+            at(from + threadIdx.x % 64 * kCount, to, w);
 #pragma unroll
-            for (int n = 0; n < kPieces; ++n) at(j + n * 64 * kCount, to, w[n]);
+            for (int i = 0; i < kCount; ++i) total += w[i];
+            return wave_sum(total);
+        }
+        for (int64_t j = from + threadIdx.x % 64 * kCount; j < to; j += 64 * kCount) {
+            const int64_t start = min(j, to - kCount);
+            Piece<T> a, b{};
+            __builtin_memcpy(&a, p + start, 16);
+            if (q != nullptr) __builtin_memcpy(&b, q + start, 16);
 #pragma unroll
-            for (int n = 0; n < kPieces; ++n)
-#pragma unroll
-                for (int i = 0; i < kCount; ++i) total += w[n][i];
+            for (int i = 0; i < kCount; ++i) total += weight(a.x[i], b.x[i], start + i, j, to);
         }
         return wave_sum(total);
     }
@@ -641,12 +650,12 @@ extern "C" int kd_verify_drafts(int dtype, int64_t* tokens, int64_t* accepted, c
         (drafted == nullptr && drafts > 0))
         return fail(KD_E_INVALID, "kd_verify_drafts: every operand but draft must be given");
     if (int rc = ensure_device()) return rc;
-    // Few sequences: a CU streams a row at about 45 GB/s, and sixteen of them for a sequence are worth a second launch while the
-    // card has them (f32, one launch / two, us: 1 x 100000 26 / 13, 8 x 50257 18 / 12, 8 x 20000 12.5 / 10.4; 32 x 50257 19 / 19,
-    // 64 x 50257 22 / 30). Their sums go through the backend's workspace, which may grow, and that is no call to make under capture.
+    // Few sequences: one CU takes 6 to 14 us for a long row, and sixteen for each sequence are worth a second launch (one launch /
+    // two, us: 1 x 30000 9.5 / 10.4, 1 x 50257 12.9 / 10.4, 1 x 100000 21 / 10.3, 32 x 50257 14.4 / 11.1, 64 x 50257 14.7 / 15.2).
+    // Their sums go through the backend's workspace, which may grow, and that is no call to make under capture.
     hipStreamCaptureStatus captured = hipStreamCaptureStatusNone;
     if (stream() != nullptr) KD_HIP(hipStreamIsCapturing(stream(), &captured));
-    const bool split = vocab >= 16384 && sequences * kVerifyWaves <= compute_units() && captured == hipStreamCaptureStatusNone;
+    const bool split = vocab >= 40000 && sequences <= 32 && captured == hipStreamCaptureStatusNone;
     Workspace lease;
     if (split)
         if (int rc = workspace(lease, static_cast<size_t>(sequences) * 2 * kVerifyWaves * kVerifyWaves * sizeof(double))) return rc;

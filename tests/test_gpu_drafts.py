@@ -40,7 +40,7 @@ def probabilities(rng, sequences, drafts, vocab, dtype, near=0.5):
 
 @pytest.mark.parametrize("dtype", [kd.F32, kd.F64], ids=["f32", "f64"])
 @pytest.mark.parametrize("shape", [(1, 1, 1), (1, 1, 2), (3, 0, 17), (5, 4, 63), (9, 3, 64), (4, 7, 1025), (2, 70, 300),
-                                   (3, 5, 50257), (40, 2, 4099), (1, 1, 100003), (20, 2, 16400), (16, 1, 16384)], ids=lambda s: "x".join(map(str, s)))
+                                   (3, 5, 50257), (40, 2, 4099), (1, 1, 100003), (20, 2, 16400), (16, 1, 16384), (5, 2, 40000), (33, 1, 40001)], ids=lambda s: "x".join(map(str, s)))
 def test_verification_is_its_definition(kdb, shape, dtype):
     rng = np.random.default_rng(sum(shape))
     given = probabilities(rng, *shape, NUMPY[dtype], near=0.5 if shape[1] < 70 else 0.05)
@@ -53,7 +53,7 @@ def test_verification_is_its_definition(kdb, shape, dtype):
         np.testing.assert_array_equal(got[0], want[0])
 
 
-@pytest.mark.parametrize("vocab", [5000, 20011])
+@pytest.mark.parametrize("vocab", [5000, 40009])
 @pytest.mark.parametrize("dtype", [kd.F32, kd.F64], ids=["f32", "f64"])
 def test_verification_at_the_borders(kdb, dtype, vocab):
     """Draws of 0 and just below 1, weights at the ends alone, a draft equal to its target, tokens out of range, counts out

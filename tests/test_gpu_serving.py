@@ -107,7 +107,7 @@ def test_a_captured_step_follows_the_cache(kdb, start):
 def test_a_captured_verification_and_distillation(kdb):
     """Verification under capture is one launch, without the shared workspace; the loss and its gradient replay with it."""
     rng = np.random.default_rng(3)
-    sequences, drafts, vocab = 4, 3, 20011  # eager calls of these sizes take two launches
+    sequences, drafts, vocab = 4, 3, 40009  # eager calls of these sizes take two launches
     given = probabilities(rng, sequences, drafts, vocab, np.float32)
     on = [kdb.to_device(a) for a in given]
     tokens, accepted = kdb.empty((sequences, drafts + 1), np.int64), kdb.empty((sequences,), np.int64)
