@@ -1282,7 +1282,7 @@ extern "C" int kd_paged_append(int dtype, const kd_paged_cache* cache, const kd_
     if (c.tokens <= 4 * static_cast<int64_t>(c.sequences)) threads = 64;
     const int64_t cache_groups = page_base(c.tokens, c.sequences, c.page_shift) * c.kv_heads * 2;
     const int64_t per_token = heads * (c.head_dim / kUnit);
-    const int q_tokens = q == nullptr ? 1 : static_cast<int>(std::max<int64_t>(1, 4 * threads / per_token));
+    const int q_tokens = q == nullptr ? 1 : static_cast<int>(std::max<int64_t>(1, threads / per_token));
     const int64_t q_groups = q == nullptr ? 0 : (c.tokens + q_tokens - 1) / q_tokens;
     if (int rc = check_grid(what, cache_groups + q_groups)) return rc;
     // 16-byte pieces need rows and tables that keep them aligned and pairs that come in fours
