@@ -1159,14 +1159,23 @@ Plan plan_of(int64_t heads, int64_t kv_heads, int64_t dim, int64_t sequences, in
     Plan plan;
     const int64_t group = heads / kv_heads;
     plan.tiles = tile_base(tokens, sequences, static_cast<int>(group));
+    const int64_t cus = compute_units();
     const int64_t groups = std::max<int64_t>(1, plan.tiles * kv_heads);
     const int64_t keys = std::min<int64_t>(std::max<int64_t>(max_keys, 1), int64_t{1} << 30);
+    // From 33 rows a sequence on average the prompts' kernel; 32 sequences of 1000 keys, 12 heads of 64, shared keys / prompts, us:
+    // 16 rows 13 / 28, 32 rows 21 / 34, 48 rows 39 / 35, 64 rows 43 / 36. Below it a sequence's kv head is about one tile.
     plan.prompts = tokens * group > 32 * sequences;
-    plan.waves = !plan.prompts && groups <= compute_units() && keys <= 2048 ? 8 : 4;
+    const int64_t working = sequences * kv_heads;
+    // Eight waves and one launch where the CUs hold all of those workgroups at once and either the keys are few or the
+    // workgroups many; otherwise four waves, and parts to fill the CUs. Four / eight waves, us: 12 x 1000 keys of 64 8.8 / 8.2,
+    // 12 x 2000 11.0 / 11.7, 96 x 4000 15.0 / 19.4, 192 x 4000 22.1 / 21.2, 384 x 2000 23.0 / 20.6, 768 x 1000 19.0 / 20.4;
+    // of 128 64 x 2000 14.7 / 17.0, 256 x 1000 19.0 / 14.9.
+    const bool at_once = working <= (dim == 64 ? 2 : 1) * cus;
+    plan.waves = !plan.prompts && at_once && (keys <= 1024 || (keys <= 4096 && 4 * working >= 3 * cus)) ? 8 : 4;
     const int64_t least = 256;
     // as many workgroups as the CUs hold at once, none with fewer than 512 keys, none with more than about 8192
-    int64_t count = ((dim == 64 ? 4 : 2) * compute_units() + groups - 1) / groups;
-    if (plan.prompts ? 2 * groups > compute_units() : plan.waves == 8 || keys <= 1024) count = 1;
+    int64_t count = ((dim == 64 ? 4 : 2) * cus + groups - 1) / groups;
+    if (plan.prompts ? 2 * groups > cus : plan.waves == 8 || keys <= 1024) count = 1;
     count = std::max<int64_t>(1, std::min({std::max(count, keys / 8192), keys / 512, most, int64_t{65535}}));
     const int64_t part = ((keys + count - 1) / count + least - 1) / least * least;
     plan.split = {static_cast<int>((keys + part - 1) / part), static_cast<int>(part), nullptr};
