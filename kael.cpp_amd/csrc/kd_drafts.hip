@@ -20,10 +20,18 @@ template <typename T> struct Piece {
     static constexpr int kCount = 16 / sizeof(T);
     T x[kCount];
 };
-template <typename T> __device__ __forceinline__ Piece<T> load_piece(const T* row, int64_t at, int64_t cols, T rest) {
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4), aligned(4)));
+// Past: the load takes no place in the caches.
+template <bool Past = false, typename T>
+__device__ __forceinline__ Piece<T> load_piece(const T* row, int64_t at, int64_t cols, T rest) {
     Piece<T> p;
     if (at + Piece<T>::kCount <= cols) {
-        __builtin_memcpy(&p, row + at, 16);
+        if constexpr (Past) {
+            const u32x4 raw = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(row + at));
+            __builtin_memcpy(&p, &raw, 16);
+        } else {
+            __builtin_memcpy(&p, row + at, 16);
+        }
     } else {
 #pragma unroll
         for (int i = 0; i < Piece<T>::kCount; ++i) p.x[i] = at + i < cols ? row[at + i] : rest;
@@ -443,7 +451,7 @@ __global__ __launch_bounds__(kNarrowRows * 64) void distill_narrow_rows_kernel(T
     }
 }
 
-template <typename T>
+template <typename T, bool PastLoads>
 __global__ __launch_bounds__(kMostThreads) void distill_rows_kernel(T* __restrict__ losses, T* __restrict__ stats,
                                                                     const T* __restrict__ logits, const int64_t* __restrict__ indices,
                                                                     const T* __restrict__ teacher, int64_t cols, int kept,
@@ -461,7 +469,7 @@ __global__ __launch_bounds__(kMostThreads) void distill_rows_kernel(T* __restric
         T x[kPieces * kCount];
 #pragma unroll
         for (int i = 0; i < kPieces; ++i) {
-            const Piece<T> p = load_piece(z, at + i * step, cols, static_cast<T>(-INFINITY));
+            const Piece<T> p = load_piece<PastLoads>(z, at + i * step, cols, static_cast<T>(-INFINITY));
 #pragma unroll
             for (int j = 0; j < kCount; ++j) x[i * kCount + j] = p.x[j];
         }
@@ -526,7 +534,6 @@ __global__ __launch_bounds__(kNarrowRows * 64) void distill_narrow_grad_kernel(T
         if (lane + 64 * n < cols) g[lane + 64 * n] = side.any ? Exp<T>::of(x[n] - largest, c) * factor - weight * taken[n] : T(0);
 }
 
-typedef uint32_t u32x4 __attribute__((ext_vector_type(4), aligned(4)));
 template <bool Past, typename T> __device__ __forceinline__ void store_piece(T* to, const Piece<T>& p) {
     u32x4 raw;
     __builtin_memcpy(&raw, &p, 16);
@@ -534,10 +541,10 @@ template <bool Past, typename T> __device__ __forceinline__ void store_piece(T* 
     else *reinterpret_cast<u32x4*>(to) = raw;
 }
 
-// A workgroup takes `span` columns of a row. Past: the stores go past the caches, for gradients that the 256 MiB of the last
-// one cannot hold (2048 x 50257: 168 us against 195, but the loss that follows takes 87 us and not 123). Shared memory: the kept entries' places and shares, and a table of the places
-// (twice their number or more, a power of two) in which a place that comes twice is found out.
-template <typename T, bool Past>
+// A workgroup takes `span` columns of a row. Shared memory: the kept entries' places and shares, and a table of the places
+// (twice their number or more, a power of two) in which a place that comes twice is found out. Bound by the logits read and
+// the gradient written.
+template <typename T, bool PastLoads, bool PastStores>
 __global__ __launch_bounds__(kMostThreads) void distill_grad_kernel(T* out, const T* logits, const T* __restrict__ stats,
                                                                     const int64_t* __restrict__ indices,
                                                                     const T* __restrict__ teacher, const T* __restrict__ row_weights,
@@ -582,14 +589,14 @@ __global__ __launch_bounds__(kMostThreads) void distill_grad_kernel(T* out, cons
     for (int64_t at = from + static_cast<int64_t>(threadIdx.x) * kCount; at < to; at += kPieces * step) {
         Piece<T> p[kPieces];
 #pragma unroll
-        for (int i = 0; i < kPieces; ++i) p[i] = load_piece(z, at + i * step, to, T(0));
+        for (int i = 0; i < kPieces; ++i) p[i] = load_piece<PastLoads>(z, at + i * step, to, T(0));
 #pragma unroll
         for (int i = 0; i < kPieces; ++i) {
             const int64_t own = at + i * step;
 #pragma unroll
             for (int j = 0; j < kCount; ++j) p[i].x[j] = any ? Exp<T>::of(p[i].x[j] - largest, c) * factor : T(0);
             if (own + kCount <= to) {
-                store_piece<Past>(g + own, p[i]);
+                store_piece<PastStores>(g + own, p[i]);
             } else {
 #pragma unroll
                 for (int j = 0; j < kCount; ++j)
@@ -630,6 +637,20 @@ int check_distill(const char* what, int dtype, int64_t rows, int64_t cols, int64
 int row_threads(int64_t rows, int64_t cols) {
     if (cols <= 1024) return 64;
     return rows < 2 * compute_units() && cols >= 8192 ? kMostThreads : 256;
+}
+
+// What goes past the caches, by the bytes of the logits: the 256 MiB of the last one hold small logits between the loss, its
+// gradient and the gradient's reader; larger ones only drive each other out. Loss and gradient together, f32 rows of 50257,
+// logits that were not in the caches, in us: nothing past them / loads past them in both / loads and stores past them in the
+// gradient alone:
+//   80 MB 52 / 56 / 57    110 MB 82 / 76 / 74    160 MB 125 / 102 / 107    230 MB 169 / 134 / 167
+//   300 MB 216 / 183 / 171    412 MB 284 / 272 / 242    800 MB 531 / 557 / 502
+struct PastCaches {
+    bool loss_loads, grad_loads, grad_stores;
+};
+PastCaches past_caches(int64_t bytes) {
+    const bool large = bytes > int64_t{96} << 20, huge = bytes > int64_t{256} << 20;
+    return {large && !huge, large, huge};
 }
 
 } // namespace
@@ -687,15 +708,20 @@ extern "C" int kd_distill_rows(int dtype, void* losses, void* stats, const void*
     if (int rc = ensure_device()) return rc;
     const auto launch = [&](auto zero) {
         using T = decltype(zero);
+        const auto launch_wide = [&](auto kernel) {
+            hipLaunchKernelGGL(kernel, dim3(static_cast<uint32_t>(rows)), dim3(row_threads(rows, cols)), 0, stream(),
+                               static_cast<T*>(losses), static_cast<T*>(stats), static_cast<const T*>(logits), indices,
+                               static_cast<const T*>(teacher), cols, static_cast<int>(kept), temperature);
+        };
         if (cols <= kNarrow)
             hipLaunchKernelGGL((distill_narrow_rows_kernel<T>), dim3(static_cast<uint32_t>((rows + kNarrowRows - 1) / kNarrowRows)),
                                dim3(kNarrowRows * 64), 0, stream(), static_cast<T*>(losses), static_cast<T*>(stats),
                                static_cast<const T*>(logits), indices, static_cast<const T*>(teacher), rows, cols,
                                static_cast<int>(kept), temperature);
+        else if (past_caches(rows * cols * static_cast<int64_t>(sizeof(T))).loss_loads)
+            launch_wide(distill_rows_kernel<T, true>);
         else
-            hipLaunchKernelGGL((distill_rows_kernel<T>), dim3(static_cast<uint32_t>(rows)), dim3(row_threads(rows, cols)), 0, stream(),
-                               static_cast<T*>(losses), static_cast<T*>(stats), static_cast<const T*>(logits), indices,
-                               static_cast<const T*>(teacher), cols, static_cast<int>(kept), temperature);
+            launch_wide(distill_rows_kernel<T, false>);
     };
     if (dtype == KD_F32) launch(0.f);
     else launch(0.0);
@@ -729,15 +755,17 @@ extern "C" int kd_distill_grad(int dtype, void* out, const void* logits, const v
         const int64_t spans = (cols + span - 1) / span;
         int table = 2;
         while (table < 2 * kept) table *= 2;
-        const auto launch_wide = [&](auto past) {
-            hipLaunchKernelGGL((distill_grad_kernel<T, decltype(past)::value>), dim3(static_cast<uint32_t>(rows * spans)), dim3(threads),
+        const auto launch_wide = [&](auto kernel) {
+            hipLaunchKernelGGL(kernel, dim3(static_cast<uint32_t>(rows * spans)), dim3(threads),
                                static_cast<uint32_t>(kept * (sizeof(T) + 4) + table * 4), stream(), static_cast<T*>(out),
                                static_cast<const T*>(logits), static_cast<const T*>(stats), indices, static_cast<const T*>(teacher),
                                static_cast<const T*>(row_weights), cols, static_cast<int>(kept), temperature, span,
                                static_cast<int>(spans), table);
         };
-        if (rows * cols * static_cast<int64_t>(sizeof(T)) > int64_t{256} << 20) launch_wide(std::true_type{});
-        else launch_wide(std::false_type{});
+        const PastCaches past = past_caches(rows * cols * static_cast<int64_t>(sizeof(T)));
+        if (past.grad_stores) launch_wide(distill_grad_kernel<T, true, true>);
+        else if (past.grad_loads) launch_wide(distill_grad_kernel<T, true, false>);
+        else launch_wide(distill_grad_kernel<T, false, false>);
     };
     if (dtype == KD_F32) launch(0.f);
     else launch(0.0);

@@ -162,6 +162,21 @@ def test_distillation_is_its_definition(kdb, shape, dtype):
             np.testing.assert_array_equal(a, b)
 
 
+@pytest.mark.parametrize("rows", [700, 1700])
+def test_distillation_of_more_than_the_caches(kdb, rows):
+    """Logits of 107 and 259 MiB, whose loads and stores go past the caches: every row as in a call of 82 MB."""
+    rng = np.random.default_rng(rows)
+    base = rng.normal(size=(512, 40001)).astype(np.float32)
+    indices = rng.integers(0, 40001, (512, 9))
+    teacher = rng.normal(size=(512, 9)).astype(np.float32)
+    weights = rng.normal(size=512).astype(np.float32)
+    few = check_distill(kdb, base, indices, teacher, weights, 1.5)
+    which = rng.integers(0, 512, rows)
+    many = run_distill(kdb, base[which], indices[which], teacher[which], weights[which], 1.5, in_place=rows == 700)
+    for a, b in zip(few, many):
+        np.testing.assert_array_equal(a[which], b)
+
+
 @pytest.mark.parametrize("dtype", [kd.F32, kd.F64], ids=["f32", "f64"])
 @pytest.mark.parametrize("cols", [50, 3000])
 def test_distillation_of_odd_rows(kdb, cols, dtype):
