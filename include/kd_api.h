@@ -213,8 +213,8 @@ int kd_reduce_columns(int op, int out_dtype, int in_dtype, void* results, const 
  * partials would not fit fails with KD_E_INVALID (on 256 CUs they take at most 12 KiB). Every
  * call on one GPU shares that buffer. Calls from several host threads are serialised around it
  * (each call's two launches are enqueued together under a lock), and a call on another stream
- * than the previous call's first drains that stream, so calls never overlap on the buffer; work
- * that another library or a graph replay puts on the buffer's stream meanwhile is not covered. */
+ * than the previous call's waits for that call's work, so calls never overlap on the buffer; what
+ * a graph replays on it is not covered. */
 int kd_reduce_noalloc(int op, int out_dtype, int in_dtype, void* results, const void* data,
                       int64_t chunk_size, int64_t output_count);
 
@@ -376,7 +376,8 @@ typedef struct kd_paged_cache {
  * kernels run, so a captured graph follows their contents. A table entry outside 0 .. pages - 1 is no page, and
  * neither have positions below 0 or from table_columns * page_size on one: nothing is written there, and
  * attention does not see it. Rows outside every sequence are left as they were. starts is clamped to
- * 0 .. tokens. table_columns * page_size stays below 2^30, tokens * heads and the pages' number below 2^31. */
+ * 0 .. tokens. table_columns * page_size stays below 2^30, tokens * heads and the pages' number below 2^31, and
+ * tokens * heads below 2^26 with sequences * kv_heads below 2^20 always fit one launch (KD_E_INVALID where not). */
 typedef struct kd_paged_batch {
     const int64_t* table;
     const int64_t* starts;
@@ -390,7 +391,7 @@ typedef struct kd_paged_batch {
  * [positions][features / 2]), the pair (a, b) of features becomes (a c - b s, b c + a s). Pair i is
  * (i, i + features / 2), or (2 i, 2 i + 1) if interleaved; features from `features` on stay.
  * features is even, 0 .. head_dim; 0 rotates nothing. A position with no row in the tables turns
- * into NaN. */
+ * into NaN, and a query below position 0 does whatever it is rotated by. */
 typedef struct kd_rotation {
     const float* cosines;
     const float* sines;
@@ -445,7 +446,7 @@ int kd_paged_attention_workspace(int64_t* bytes, int64_t heads, int64_t kv_heads
  * 117-155). Sequence s has counts[s] (clamped to 0 .. drafts) drafted tokens x_i = drafted[s][i], drawn
  * from the draft's probabilities q_i = draft[s][i][.], and the target's p_i = target[s][i][.] for
  * i <= counts[s]. Draft i is accepted while u_i * q_i(x_i) < p_i(x_i), u_i = uniforms[s][i] in [0, 1).
- * At the first that is not, a token is drawn from max(p_i - q_i, 0) (from p_i if that is 0 everywhere);
+ * At the first that is not, a token is drawn from max(p_i - q_i, 0) (from p_i if that has no positive sum);
  * if all are accepted, from p_counts[s]. That draw uses uniforms[s][drafts]: the first entry whose
  * running sum exceeds the draw times the sum of all. draft NULL means that the drafts were certain (q_i is 1 at x_i).
  *   target [sequences][drafts + 1][vocab], draft [sequences][drafts][vocab], drafted [sequences][drafts],
@@ -454,7 +455,7 @@ int kd_paged_attention_workspace(int64_t* bytes, int64_t heads, int64_t kv_heads
  *   accepted [sequences]: how many drafts were accepted
  * dtype f32 or f64; sums and comparisons in f64. A drafted token outside 0 .. vocab - 1 is never accepted
  * (its q is 0 everywhere if certain). Where the weights have no finite positive sum the drawn token is -1. drafts may
- * be 0. */
+ * be 0; sequences stay below 2^22. */
 int kd_verify_drafts(int dtype, int64_t* tokens, int64_t* accepted, const void* target, const void* draft,
                      const int64_t* drafted, const int64_t* counts, const double* uniforms, int64_t sequences,
                      int64_t drafts, int64_t vocab);
@@ -495,7 +496,7 @@ int kd_cross_entropy_grad(int dtype, void* out, const void* logits, const int64_
  * An index outside 0 .. cols - 1 is no entry (its t is not read into the sums); a row without entries, or
  * whose t are all -inf, has loss 0. The same index twice counts twice. stats [rows][2] receives each row's max(z) and
  * sum exp((z - max) / T), which the gradient reads. dtype f32 or f64, rows contiguous, sums in double;
- * 1 <= kept <= 1024, 1e-6 <= temperature <= 1e6. */
+ * 1 <= kept <= 1024, 1e-6 <= temperature <= 1e6, rows at most 2^24 - 4 (2^26 - 4 of up to 1024 entries). */
 int kd_distill_rows(int dtype, void* losses, void* stats, const void* logits, const int64_t* indices,
                     const void* teacher, int64_t rows, int64_t cols, int64_t kept, double temperature);
 

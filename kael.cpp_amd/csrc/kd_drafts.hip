@@ -624,7 +624,7 @@ __global__ __launch_bounds__(kMostThreads) void distill_grad_kernel(T* out, cons
 int check_distill(const char* what, int dtype, int64_t rows, int64_t cols, int64_t kept, double temperature) {
     const std::string name(what);
     if (dtype != KD_F32 && dtype != KD_F64) return fail(KD_E_UNSUPPORTED, name + ": dtype must be f32 or f64");
-    if (rows < 0 || cols < 1 || rows >= (int64_t{1} << 31) || cols >= (int64_t{1} << 31))
+    if (rows < 0 || cols < 1 || !fits_grid(rows + 3, cols <= 1024 ? 64 : 256) || cols >= (int64_t{1} << 31))
         return fail(KD_E_INVALID, name + ": bad number of rows or columns");
     if (kept < 1 || kept > kMaxKept) return fail(KD_E_INVALID, name + ": 1 to 1024 kept entries");
     if (!(temperature >= 1e-6 && temperature <= 1e6))
@@ -663,7 +663,7 @@ extern "C" int kd_verify_drafts(int dtype, int64_t* tokens, int64_t* accepted, c
                                 const int64_t* drafted, const int64_t* counts, const double* uniforms, int64_t sequences,
                                 int64_t drafts, int64_t vocab) {
     if (dtype != KD_F32 && dtype != KD_F64) return fail(KD_E_UNSUPPORTED, "kd_verify_drafts: dtype must be f32 or f64");
-    if (sequences < 0 || drafts < 0 || vocab < 1 || sequences >= (int64_t{1} << 31) || drafts >= (int64_t{1} << 20) ||
+    if (sequences < 0 || drafts < 0 || vocab < 1 || !fits_grid(sequences, kVerifyThreads) || drafts >= (int64_t{1} << 20) ||
         vocab >= (int64_t{1} << 31))
         return fail(KD_E_INVALID, "kd_verify_drafts: bad number of sequences, drafts or tokens");
     if (sequences == 0) return KD_OK;

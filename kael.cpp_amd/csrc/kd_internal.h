@@ -35,13 +35,16 @@ hipStream_t stream();
 int device_ordinal();
 int compute_units();
 
+// Whether a launch of `groups` workgroups in x is one: its work items are counted in 32 bits.
+inline bool fits_grid(int64_t groups, int64_t threads) { return groups < (int64_t{1} << 32) / threads; }
+
 // A lease on the per-device workspace (scratch for split reductions and split-K partials,
 // grown on demand, never shrunk). The lease holds the workspace lock from `workspace()` until
 // it is destroyed, so a caller keeps it alive until every kernel that touches `ptr` has been
 // enqueued: calls from several host threads then use the buffer one after another in stream
 // order, and a growth (which frees the old block) never frees a block that a caller is about to
-// hand to a kernel. When the backend stream differs from the one the previous lease used, the
-// previous stream is drained first, so leases on different streams never overlap either.
+// hand to a kernel. When the backend stream differs from the one the previous lease used, it waits
+// for that lease's event first, so leases on different streams never overlap either.
 struct Workspace {
     Workspace() = default;
     Workspace(const Workspace&) = delete;

@@ -1246,9 +1246,8 @@ int check_heads(const char* what, int64_t heads, const Paged& c) {
     return KD_OK;
 }
 
-// A launch of `groups` workgroups in x has to stay within the grid's 2^31 - 1.
-int check_grid(const char* what, int64_t groups) {
-    return groups < (int64_t{1} << 31) ? KD_OK : fail(KD_E_INVALID, std::string(what) + ": shape too large");
+int check_grid(const char* what, int64_t groups, int64_t threads) {
+    return fits_grid(groups, threads) ? KD_OK : fail(KD_E_INVALID, std::string(what) + ": shape too large");
 }
 
 } // namespace
@@ -1285,7 +1284,6 @@ extern "C" int kd_paged_append(int dtype, const kd_paged_cache* cache, const kd_
     }
     if (int rc = check_strided(what, "k", k, k_strides, c.tokens, c.kv_heads, ks)) return rc;
     if (int rc = check_strided(what, "v", v, v_strides, c.tokens, c.kv_heads, vs)) return rc;
-    if (int rc = ensure_device()) return rc;
     // four units a thread and pass at most, one wave where few tokens a sequence leave most of a page alone
     int threads = static_cast<int>(std::clamp<int64_t>((int64_t{c.head_dim} << c.page_shift) / (4 * kUnit), 64, kAppendThreads));
     if (c.tokens <= 4 * static_cast<int64_t>(c.sequences)) threads = 64;
@@ -1293,7 +1291,8 @@ extern "C" int kd_paged_append(int dtype, const kd_paged_cache* cache, const kd_
     const int64_t per_token = heads * (c.head_dim / kUnit);
     const int q_tokens = q == nullptr ? 1 : static_cast<int>(std::max<int64_t>(1, threads / per_token));
     const int64_t q_groups = q == nullptr ? 0 : (c.tokens + q_tokens - 1) / q_tokens;
-    if (int rc = check_grid(what, cache_groups + q_groups)) return rc;
+    if (int rc = check_grid(what, cache_groups + q_groups, threads)) return rc;
+    if (int rc = ensure_device()) return rc;
     // 16-byte pieces need rows and tables that keep them aligned and pairs that come in fours
     const auto whole = [](const Strided& x) { return aligned(x.data, 16) && x.row % 4 == 0 && x.head % 4 == 0; };
     const bool vector = r.half % 4 == 0 && aligned(r.cosines, 16) && aligned(r.sines, 16) && whole(ks) && (q == nullptr || whole(qs));
@@ -1317,11 +1316,12 @@ extern "C" int kd_paged_read(int dtype, void* k, void* v, const kd_paged_cache* 
     if (int rc = check_paged("kd_paged_read", dtype, cache, batch, c)) return rc;
     if (!aligned(k, 16) || !aligned(v, 16)) return fail(KD_E_INVALID, "kd_paged_read: k and v must be 16-byte aligned");
     if (c.sequences == 0 || c.tokens == 0 || (k == nullptr && v == nullptr)) return KD_OK;
-    if (int rc = ensure_device()) return rc;
     const int64_t groups = page_base(c.tokens, c.sequences, c.page_shift) * c.kv_heads * 2;
-    if (int rc = check_grid("kd_paged_read", groups)) return rc;
-    hipLaunchKernelGGL(paged_read_kernel, dim3(static_cast<uint32_t>(groups)), dim3(c.page_shift <= 5 ? 64 : 256), 0, stream(),
-                       c, static_cast<float*>(k), static_cast<float*>(v));
+    const int threads = c.page_shift <= 5 ? 64 : 256;
+    if (int rc = check_grid("kd_paged_read", groups, threads)) return rc;
+    if (int rc = ensure_device()) return rc;
+    hipLaunchKernelGGL(paged_read_kernel, dim3(static_cast<uint32_t>(groups)), dim3(threads), 0, stream(), c,
+                       static_cast<float*>(k), static_cast<float*>(v));
     KD_LAUNCH_CHECK();
     return KD_OK;
 }
@@ -1351,20 +1351,19 @@ extern "C" int kd_paged_attention(int dtype, void* out, const void* q, const int
     Strided qs;
     if (int rc = check_strided(what, "q", q, q_strides, c.tokens, heads, qs)) return rc;
     if (out == nullptr || !aligned(out, 16)) return fail(KD_E_INVALID, "kd_paged_attention: out must be given, 16-byte aligned");
+    if (int rc = check_grid(what, tile_base(c.tokens, c.sequences, static_cast<int>(heads / c.kv_heads)) * c.kv_heads, 512)) return rc;
     if (int rc = ensure_device()) return rc;
     if (c.pages == 0) c.columns = 0;  // no position has a page
     const int64_t rows = heads * c.tokens;
-    Plan plan = plan_of(heads, c.kv_heads, c.head_dim, c.sequences, c.tokens, max_keys, workspace_bytes / part_bytes(rows, c.head_dim));
+    const int64_t join_groups = (rows + 3) / 4;
+    const int64_t most = fits_grid(join_groups, 256) ? workspace_bytes / part_bytes(rows, c.head_dim) : 1;
+    const Plan plan = plan_of(heads, c.kv_heads, c.head_dim, c.sequences, c.tokens, max_keys, most);
     const Split split{plan.split.count, plan.split.part, static_cast<float*>(workspace)};
-    if (int rc = check_grid(what, plan.tiles * c.kv_heads)) return rc;
     const auto launch = [&](auto dim, auto waves) {
         constexpr int D = decltype(dim)::value, Waves = decltype(waves)::value;
         hipLaunchKernelGGL((paged_attention_kernel<D, Waves>), dim3(static_cast<uint32_t>(plan.tiles * c.kv_heads), split.count),
                            dim3(Waves * 64), 0, stream(), c, static_cast<float*>(out), qs, static_cast<int>(heads),
                            FastDiv(static_cast<uint32_t>(heads / c.kv_heads)), scale, split);
-        if (split.count > 1)
-            hipLaunchKernelGGL((paged_join_kernel<D>), dim3(static_cast<uint32_t>((rows + 3) / 4)), dim3(256), 0, stream(), c,
-                               static_cast<float*>(out), static_cast<int>(heads), split);
     };
     const auto with_waves = [&](auto dim) {
         constexpr int D = decltype(dim)::value;
@@ -1372,11 +1371,11 @@ extern "C" int kd_paged_attention(int dtype, void* out, const void* q, const int
             hipLaunchKernelGGL((paged_prompt_kernel<D>), dim3(static_cast<uint32_t>(plan.tiles * c.kv_heads), split.count),
                                dim3(kPromptWaves * 64), 0, stream(), c, static_cast<float*>(out), qs, static_cast<int>(heads),
                                FastDiv(static_cast<uint32_t>(heads / c.kv_heads)), scale, split);
-            if (split.count > 1)
-            hipLaunchKernelGGL((paged_join_kernel<D>), dim3(static_cast<uint32_t>((rows + 3) / 4)), dim3(256), 0, stream(), c,
-                               static_cast<float*>(out), static_cast<int>(heads), split);
         } else if (plan.waves == 8) launch(dim, std::integral_constant<int, 8>{});
         else launch(dim, std::integral_constant<int, 4>{});
+        if (split.count > 1)
+            hipLaunchKernelGGL((paged_join_kernel<D>), dim3(static_cast<uint32_t>(join_groups)), dim3(256), 0, stream(), c,
+                               static_cast<float*>(out), static_cast<int>(heads), split);
     };
     if (c.head_dim == 64) with_waves(std::integral_constant<int, 64>{});
     else with_waves(std::integral_constant<int, 128>{});

@@ -122,3 +122,15 @@ def test_bad_distillations(lib):
             args = list(good)
             args[at] = value
             assert f(*args) == status, (at, value)
+
+
+def test_more_workgroups_than_a_launch_takes(lib):
+    """Refused before a launch whose work items would not fit 32 bits."""
+    assert lib.lib.kd_verify_drafts(kd.F32, *[FAKE] * 7, 1 << 22, 3, 10) == INVALID
+    for cols, rows in ((96, 1 << 26), (1024, 1 << 26), (1025, 1 << 24)):
+        assert lib.lib.kd_distill_rows(kd.F32, *[FAKE] * 5, rows, cols, 3, 1.0) == INVALID
+        assert lib.lib.kd_distill_grad(kd.F32, *[FAKE] * 6, rows, cols, 3, 1.0) == INVALID
+    c, b = cache(kv_heads=4096), batch(sequences=1 << 23)
+    assert lib.lib.kd_paged_append(kd.F32, c, b, None, FAKE + 64, FAKE, ROWS, 4096, FAKE, ROWS, FAKE, ROWS) == INVALID
+    assert lib.lib.kd_paged_read(kd.F32, FAKE, FAKE, c, b) == INVALID
+    assert lib.lib.kd_paged_attention(kd.F32, FAKE + 64, FAKE, ROWS, 4096, c, b, 1.0, 64, None, 0) == INVALID
