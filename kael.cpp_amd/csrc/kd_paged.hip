@@ -735,6 +735,223 @@ __global__ __launch_bounds__(Waves * 64, D == 64 ? 4 : 2) void paged_attention_k
     }
 }
 
+// One row a workgroup (single tokens whose heads share nothing). Its four digits take four of the sixteen columns, so that a tile of
+// 16 keys is one product and not four, and the sums come out one key to a lane: a weight costs a lane one exponential where the
+// kernel above computes sixteen for columns that stand in for rows that are not there.
+template <int Control> __device__ __forceinline__ int in_quad(int x) { return __builtin_amdgcn_mov_dpp(x, Control, 0xf, 0xf, true); }
+constexpr int kMostBlocks = 1024;  // that the whole sums hold: 2^10 blocks of 2^6 keys of 2^14
+constexpr int kNextLane = 0xb1, kOtherPair = 0x4e;  // lane ^ 1, lane ^ 2 (quad_perm)
+
+template <int D, int Waves>
+__global__ __launch_bounds__(Waves * 64, D == 64 ? 4 : 2) void paged_single_kernel(Paged c, float* __restrict__ out, Strided q, int heads,
+                                                                  FastDiv by_group, FastDiv by_heads, double scale, Split split) {
+    constexpr int U = D / 64;
+    __shared__ __attribute__((aligned(16))) float os[Waves][D];
+    __shared__ float ms[Waves], ls[Waves];
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = threadIdx.x % 64;
+    const int column = lane % 16, chunk = lane / 16, digit = lane % 4;
+    const int part = blockIdx.y;
+    const int token = c.tokens - 1 - static_cast<int>(by_heads.div(blockIdx.x));
+    const int head = static_cast<int>(blockIdx.x) - (c.tokens - 1 - token) * heads;
+    const int kv = static_cast<int>(by_group.div(head));
+    const Found found = find_sequence(c, token, [&](int64_t start, int64_t) { return start; });
+    if (found.s < 0) return;
+    const Rows rows = found.rows;
+    if (token >= rows.row + rows.count) return;
+    const int64_t capacity = static_cast<int64_t>(c.columns) << c.page_shift;
+    const int64_t visible = rows.position + (token - rows.row) + 1;
+    const int limit = static_cast<int>(visible < 0 ? 0 : visible > capacity ? capacity : visible);
+    const int from = part * split.part;
+    if (from >= limit && part > 0) return;
+    const int to = part + 1 == split.count ? limit : min(limit, from + split.part);
+    constexpr int step = Waves * kKeyBlock;
+    int key = from + wave * kKeyBlock;
+
+    const int size = 1 << c.page_shift;
+    const int64_t* table = c.table + static_cast<int64_t>(found.s) * c.columns;
+    int window = 0, window_from = -128;
+    const auto pages_of_block = [&](int key) {
+        if (((key + kKeyBlock - 1) >> c.page_shift) - window_from >= 64) {
+            window_from = key >> c.page_shift;
+            const int64_t page = table[min(window_from + lane, c.columns - 1)];
+            window = window_from + lane < c.columns && page >= 0 && page < c.pages ? static_cast<int>(page) : -1;
+        }
+    };
+    const auto page_at = [&](int key) { return __shfl(window, (key >> c.page_shift) - window_from); };
+    const int key_chunk = column / 4;
+    v4i k[4][U], v[D / 16];
+    const int8_t* values_at;
+    float key_scale, value_scale;
+    int page;
+    const uint32_t page_bytes = static_cast<uint32_t>(c.kv_heads) * size * D;  // at most 2^27
+    const int8_t* keys_base = c.keys + (kv * size + lane % 4) * D + chunk * 16 * U;
+    const int8_t* values_base = c.values + (kv * D + column) * size;
+    const auto load_keys = [&](int key) {
+        pages_of_block(key);
+        page = page_at(key + 16 * chunk);
+        const uint32_t own = max(page, 0), other = max(page_at(key + 16 * key_chunk), 0);
+        const int slot = (key + 16 * key_chunk) & (size - 1), own_slot = (key + 16 * chunk) & (size - 1);
+        const int8_t* at = keys_base + uint64_t{other} * page_bytes + slot * D;
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+            for (int u = 0; u < U; ++u) k[t][u] = *reinterpret_cast<const v4i*>(at + 4 * t * D + 16 * u);
+        key_scale = c.key_scales[uint64_t{own} * static_cast<uint32_t>(c.kv_heads) + kv];
+        value_scale = c.value_scales[uint64_t{own} * static_cast<uint32_t>(c.kv_heads) + kv];
+        values_at = values_base + uint64_t{own} * page_bytes + own_slot;
+    };
+    const auto load_values = [&] {
+#pragma unroll
+        for (int n = 0; n < D / 16; ++n) v[n] = *reinterpret_cast<const v4i*>(values_at + 16 * n * size);
+    };
+
+    const float* row = q.data + token * q.row + head * q.head + chunk * 16 * U;
+    float features[16 * U];
+#pragma unroll
+    for (int d = 0; d < 16 * U; ++d) features[d] = row[d];
+    if (key < to) {
+        load_keys(key);
+        load_values();
+    }
+    // a column's digit of the query: its lane's number in the quad
+    v4i digits[U];
+    float q_factor;
+    {
+        v4i all[4][U];
+        q_factor = query_digits(features, true, scale, all);
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int t = 0; t < 4; ++t) {
+                const int low = digit & 1 ? all[1][u][t] : all[0][u][t], high = digit & 1 ? all[3][u][t] : all[2][u][t];
+                digits[u][t] = digit & 2 ? high : low;
+            }
+    }
+    const int shift = 8 * (digit & 1);
+    const float pair_unit = digit & 2 ? 65536.f : 1.f;
+    const uint32_t first_bytes = digit & 1 ? 0x03070105u : 0x06020400u, second_bytes = digit & 2 ? 0x03020706u : 0x05040100u;
+
+    float m = -INFINITY, l = 0.f;  // l is the lane's own
+    float o[D / 4] = {};           // of the column's digit
+    v4i acc[D / 16] = {};          // since the last change of the unit
+    int top = 0, blocks = 0;       // the largest weight times its value scale, as bits, so that NaN is the largest of all
+    float to_whole = 0.f, from_whole = 0.f;
+    const auto flush = [&](float alpha) {
+#pragma unroll
+        for (int n = 0; n < D / 16; ++n) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) o[4 * n + i] = (o[4 * n + i] + static_cast<float>(acc[n][i]) * from_whole) * alpha;
+            acc[n] = v4i{0, 0, 0, 0};
+        }
+        blocks = 0;
+    };
+    for (; key < to; key += step) {
+        v4i sum[4];
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+            sum[t] = v4i{0, 0, 0, 0};
+#pragma unroll
+            for (int u = 0; u < U; ++u) sum[t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(k[t][u], digits[u], sum[t], 0, 0, 0);
+        }
+        // column / 4 is the tile that a lane keeps, column % 4 the row of it: key `lane` of the block
+        int pair[4];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const int low = column & 4 ? sum[1][r] : sum[0][r], high = column & 4 ? sum[3][r] : sum[2][r];
+            pair[r] = (column & 8 ? high : low) << shift;
+            pair[r] += in_quad<kNextLane>(pair[r]);
+        }
+        const int kept_low = digit & 1 ? pair[1] : pair[0], kept_high = digit & 1 ? pair[3] : pair[2];
+        const int kept = digit & 2 ? kept_high : kept_low, sent = digit & 2 ? kept_low : kept_high;
+        const float whole = static_cast<float>(kept) * pair_unit +
+                            __int_as_float(in_quad<kOtherPair>(__float_as_int(static_cast<float>(sent) * pair_unit)));
+        const bool seen = page >= 0 && key + lane < to;
+        const float own_scale = seen ? value_scale : 0.f;
+        const float x = seen ? whole * (q_factor * key_scale) : -INFINITY;
+        load_keys(key + step < to ? key + step : key);  // the last block once more rather than a branch
+        if (__any(x > m)) {
+            float next = x;
+#pragma unroll
+            for (int d = 32; d > 0; d /= 2) next = fmaxf(next, __shfl_xor(next, d));
+            next = fmaxf(next, m);
+            const float alpha = __builtin_amdgcn_exp2f(m - next);
+            flush(alpha);
+            l *= alpha;
+            top = __float_as_int(__int_as_float(top) * alpha) & 0x7fffffff;
+            m = next;
+            blocks = kMostBlocks;
+        }
+        const float p = __builtin_amdgcn_exp2f(x - (m == -INFINITY ? 0.f : m));
+        const float weight = p * own_scale;
+        l += p;
+        const int weight_bits = __float_as_int(weight) & 0x7fffffff;
+        if (blocks >= kMostBlocks || __any(weight_bits > top)) {
+            flush(1.f);
+            int next = weight_bits;
+#pragma unroll
+            for (int d = 32; d > 0; d /= 2) next = max(next, __shfl_xor(next, d));
+            top = max(top, next);
+            const int e = __builtin_amdgcn_frexp_expf(__int_as_float(top));
+            to_whole = top < 0x7f800000 ? ldexpf(1.f, 30 - e) : 0.f;
+            from_whole = top < 0x7f800000 ? ldexpf(1.f, e - 30) : NAN;
+        }
+        ++blocks;
+        // from 2^23 on an f32 is whole: the bias rounds the weight too, to half a unit or its own last bit
+        int bytes = static_cast<int>(fmaf(weight, to_whole, static_cast<float>(kDigitBias))) ^ kDigitBias;
+        bytes = static_cast<int>(__builtin_amdgcn_perm(in_quad<kNextLane>(bytes), bytes, first_bytes));
+        bytes = static_cast<int>(__builtin_amdgcn_perm(in_quad<kOtherPair>(bytes), bytes, second_bytes));
+        // the quads' digits side by side; right in the first quad's columns, which are the ones that are read
+        const v4i weights{bytes, in_quad<0x12c>(bytes), in_quad<0x128>(bytes), in_quad<0x124>(bytes)};
+#pragma unroll
+        for (int n = 0; n < D / 16; ++n) acc[n] = __builtin_amdgcn_mfma_i32_16x16x64_i8(v[n], weights, acc[n], 0, 0, 0);
+        load_values();
+    }
+    flush(1.f);
+#pragma unroll
+    for (int d = 32; d > 0; d /= 2) l += __shfl_xor(l, d);
+    if (lane == 0) {
+        ms[wave] = m;
+        ls[wave] = l;
+    }
+    const float digit_unit = pair_unit * (digit & 1 ? 256.f : 1.f);
+#pragma unroll
+    for (int i = 0; i < D / 4; ++i) {
+        float x = o[i] * digit_unit;
+        x += __int_as_float(in_quad<kNextLane>(__float_as_int(x)));
+        x += __int_as_float(in_quad<kOtherPair>(__float_as_int(x)));
+        o[i] = x;
+    }
+    if (column == 0)
+#pragma unroll
+        for (int n = 0; n < D / 16; ++n)
+            *reinterpret_cast<float4*>(&os[wave][16 * n + 4 * chunk]) = make_float4(o[4 * n], o[4 * n + 1], o[4 * n + 2], o[4 * n + 3]);
+    __syncthreads();
+    if (threadIdx.x >= D) return;
+    const int d = threadIdx.x;
+    float most = -INFINITY;
+    for (int w = 0; w < Waves; ++w) most = fmaxf(most, ms[w]);
+    const float base = most == -INFINITY ? 0.f : most;
+    float total = 0.f, value = 0.f;
+#pragma unroll
+    for (int w = 0; w < Waves; ++w) {
+        const float f = __builtin_amdgcn_exp2f(ms[w] - base);
+        total += f * ls[w];
+        value += f * os[w][d];
+    }
+    const int64_t to_row = static_cast<int64_t>(token) * heads + head;
+    if (split.count == 1) {
+        out[to_row * D + d] = total == 0.f ? 0.f : value / total;
+    } else {
+        const int64_t record = to_row * split.count + part;
+        split.sums[record * D + d] = value;
+        if (d == 0) {
+            float* own = split.sums + static_cast<int64_t>(c.tokens) * heads * split.count * D + record * 2;
+            own[0] = most;
+            own[1] = total;
+        }
+    }
+}
+
 // Many rows a sequence (prompts): the workgroup's four waves take 16 rows each and share every block of 64 keys through LDS,
 // two blocks deep, so that a wave keeps none of it in registers. What bounds it is the vector ALU, 30 operations a score in the
 // kernel above, seven of which join the digits' sums of the outputs; here the weighted sums run on the f16 matrix cores
@@ -1150,7 +1367,7 @@ int64_t part_bytes(int64_t rows, int64_t dim) { return rows * (dim + 2) * 4; }
 // into.
 struct Plan {
     int64_t tiles;
-    bool prompts;
+    bool prompts, single;
     int waves;
     Split split;
 };
@@ -1165,19 +1382,36 @@ Plan plan_of(int64_t heads, int64_t kv_heads, int64_t dim, int64_t sequences, in
     // From 33 rows a sequence on average the prompts' kernel; 32 sequences of 1000 keys, 12 heads of 64, shared keys / prompts, us:
     // 16 rows 13 / 28, 32 rows 21 / 34, 48 rows 39 / 35, 64 rows 43 / 36. Below it a sequence's kv head is about one tile.
     plan.prompts = tokens * group > 32 * sequences;
-    const int64_t working = sequences * kv_heads;
+    // One row a tile: 64 x 1024 keys of 64, 12 heads, 18.6 -> 16.4 us, 16 x 4000 21.5 -> 16.5, 1 x 1000 8.6 -> 8.2 (7 without the
+    // call's 8 on the host); of 128, 16 heads, 32 x 2000 37.8 -> 36.1.
+    plan.single = tokens * group <= sequences;
     // Eight waves and one launch where the CUs hold all of those workgroups at once and either the keys are few or the
     // workgroups many; otherwise four waves, and parts to fill the CUs. Four / eight waves, us: 12 x 1000 keys of 64 8.8 / 8.2,
     // 12 x 2000 11.0 / 11.7, 96 x 4000 15.0 / 19.4, 192 x 4000 22.1 / 21.2, 384 x 2000 23.0 / 20.6, 768 x 1000 19.0 / 20.4;
     // of 128 64 x 2000 14.7 / 17.0, 256 x 1000 19.0 / 14.9.
-    const bool at_once = working <= (dim == 64 ? 2 : 1) * cus;
-    plan.waves = !plan.prompts && at_once && (keys <= 1024 || (keys <= 4096 && 4 * working >= 3 * cus)) ? 8 : 4;
-    const int64_t least = 256;
-    // as many workgroups as the CUs hold at once, none with fewer than 512 keys, none with more than about 8192
-    int64_t count = ((dim == 64 ? 4 : 2) * cus + groups - 1) / groups;
-    if (plan.prompts ? 2 * groups > cus : plan.waves == 8 || keys <= 1024) count = 1;
-    count = std::max<int64_t>(1, std::min({std::max(count, keys / 8192), keys / 512, most, int64_t{65535}}));
-    const int64_t part = ((keys + count - 1) / count + least - 1) / least * least;
+    const bool narrow = dim == 64;
+    const int64_t working = plan.single ? std::max<int64_t>(1, tokens * heads) : sequences * kv_heads;
+    int64_t count, least = 512;  // parts, and the keys that one is worth
+    if (plan.single) {
+        // Parts where there are few rows of many keys. One launch / parts, us: 12 rows of 64 x 2000 8.5 / 10.4, x 4000 11.2 / 10.8,
+        // x 8000 17.2 / 10.9, 96 x 4000 13.1 / 13.3, 192 x 8000 27.7 / 30.9; of 128 16 x 1000 10.8 / 10.6, x 2000 16.1 / 10.6,
+        // 128 x 4000 27.3 / 24.6, 256 x 4000 37.1 / 41.1. A CU takes about 50 GB/s, whatever its waves: eight of them are worth
+        // it for the latency of keys of 64 (192 x 4000: four 18.0, eight 16.4), while the CUs hold them (384 x 2000 16.7 / 17.3).
+        const bool whole = keys <= (narrow ? 4096 : 1024) || 4 * working >= 3 * cus;
+        count = whole ? 1 : ((narrow ? 2 : 1) * cus + working - 1) / working;
+        if (!narrow) least = 256;
+    } else {
+        const bool at_once = working <= (narrow ? 2 : 1) * cus;
+        plan.waves = !plan.prompts && at_once && (keys <= 1024 || (keys <= 4096 && 4 * working >= 3 * cus)) ? 8 : 4;
+        // as many workgroups as the CUs hold at once
+        count = ((narrow ? 4 : 2) * cus + groups - 1) / groups;
+        if (plan.prompts ? 2 * groups > cus : plan.waves == 8 || keys <= 1024) count = 1;
+    }
+    // no part longer than about 8192 keys
+    count = std::max<int64_t>(1, std::min({std::max(count, keys / 8192), keys / least, most, int64_t{65535}}));
+    if (plan.single) plan.waves = narrow && count == 1 && working <= cus ? 8 : 4;
+    constexpr int64_t unit = 256;
+    const int64_t part = ((keys + count - 1) / count + unit - 1) / unit * unit;
     plan.split = {static_cast<int>((keys + part - 1) / part), static_cast<int>(part), nullptr};
     return plan;
 }
@@ -1371,6 +1605,16 @@ extern "C" int kd_paged_attention(int dtype, void* out, const void* q, const int
             hipLaunchKernelGGL((paged_prompt_kernel<D>), dim3(static_cast<uint32_t>(plan.tiles * c.kv_heads), split.count),
                                dim3(kPromptWaves * 64), 0, stream(), c, static_cast<float*>(out), qs, static_cast<int>(heads),
                                FastDiv(static_cast<uint32_t>(heads / c.kv_heads)), scale, split);
+        } else if (plan.single) {
+            const auto launch_single = [&](auto waves) {
+                constexpr int Waves = decltype(waves)::value;
+                hipLaunchKernelGGL((paged_single_kernel<D, Waves>), dim3(static_cast<uint32_t>(rows), split.count), dim3(Waves * 64), 0,
+                                   stream(), c, static_cast<float*>(out), qs, static_cast<int>(heads),
+                                   FastDiv(static_cast<uint32_t>(heads / c.kv_heads)), FastDiv(static_cast<uint32_t>(heads)), scale, split);
+            };
+            if constexpr (D == 64)
+                if (plan.waves == 8) launch_single(std::integral_constant<int, 8>{});
+            if (plan.waves == 4) launch_single(std::integral_constant<int, 4>{});
         } else if (plan.waves == 8) launch(dim, std::integral_constant<int, 8>{});
         else launch(dim, std::integral_constant<int, 4>{});
         if (split.count > 1)

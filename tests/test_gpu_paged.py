@@ -316,6 +316,25 @@ def test_attention_of_small_and_large_queries(kdb, size, dim, new):
                 on.c, kd.PagedBatch(on.table.ptr, on.starts.ptr, on.lengths.ptr, 1, 0, tokens), 1.0, 200, None, 0)
 
 
+def test_attention_of_more_keys_than_whole_sums_hold(kdb):
+    """1.2 million keys of weight 1 to one row, whose lowest digits are all -128: some 2340 blocks of 64 to each of eight waves
+    add up to more than 2^31. The weights and their sum are exact; a digit's sums round at most three times as they are turned
+    into f32 and joined, the digits twice, the waves eight times, the quotient once, all within 2^-24 of the result."""
+    pages, page, dim = 4688, 256, 64
+    keys = pages * page
+    scale = np.float32((2 ** 29 + 2 ** 23 + 2 ** 15 + 2 ** 7) / 2 ** 29)
+    on = {n: kdb.to_device(a) for n, a in (
+        ("keys", np.zeros((pages, 1, page, dim), np.int8)), ("values", np.full((pages, 1, dim, page), 127, np.int8)),
+        ("key_scales", np.ones((pages, 1), np.float32)), ("value_scales", np.full((pages, 1), scale, np.float32)),
+        ("table", np.arange(pages)[None]), ("starts", np.asarray([0, 1])), ("lengths", np.asarray([keys])),
+        ("q", np.ones((1, 1, dim), np.float32)), ("out", np.zeros((1, 1, dim), np.float32)))}
+    cache = kd.PagedCache(*(on[n].ptr for n in ("keys", "values", "key_scales", "value_scales")), pages, 1, page, dim)
+    batch = kd.PagedBatch(on["table"].ptr, on["starts"].ptr, on["lengths"].ptr, 1, pages, 1)
+    kdb.call("paged_attention", kd.F32, on["out"].ptr, on["q"].ptr, kd.strides(dim, dim), 1, cache, batch, 1.0, keys, None, 0)
+    want = 127 * np.float64(scale)
+    assert (np.abs(on["out"].numpy() - want) <= 14 * 2.0 ** -24 * want).all()
+
+
 @pytest.mark.parametrize("new", [1, 40])
 def test_attention_without_any_page(kdb, new):
     """A cache of no pages, a table of no columns: nothing is visible and every row 0."""
