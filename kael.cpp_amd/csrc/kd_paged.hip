@@ -656,9 +656,12 @@ __global__ __launch_bounds__(Waves * 64, D == 64 ? 4 : 2) void paged_attention_k
         const float base = next == -INFINITY ? 0.f : next;  // nothing seen yet: every weight below is 0
         const float alpha = __builtin_amdgcn_exp2f(m - base);
         m = next;
-        // value scales against the largest that the row sees, as bits, so that NaN is the largest of all
-        const int top = over_chunks(scale_bits, [](int a, int b) { return max(a, b); });
-        const int e = __builtin_amdgcn_frexp_expf(__int_as_float(top));
+        // The unit of the weights times their value scales: the largest of them that the row has here, as bits, so that NaN is the
+        // largest of all, but not below 2^-40 of the largest scale, so that the scale in units stays finite.
+        const float weight = __builtin_amdgcn_exp2f(fmaf(largest, factor, -base)) * own_scale;
+        const int weight_bits = seen > 0 ? __float_as_int(weight) & 0x7fffffff : 0;
+        const int top = over_chunks(max(weight_bits, scale_bits - (40 << 23)), [](int a, int b) { return max(a, b); });
+        const int e = __builtin_amdgcn_frexp_expf(__int_as_float(max(top, 0)));
         const float to_whole = top < 0x7f800000 && seen > 0 ? ldexpf(own_scale, 30 - e) : 0.f;
         const float from_whole = top < 0x7f800000 ? ldexpf(1.f, e - 30) : NAN;
         float sum = 0.f;

@@ -316,6 +316,33 @@ def test_attention_of_small_and_large_queries(kdb, size, dim, new):
                 on.c, kd.PagedBatch(on.table.ptr, on.starts.ptr, on.lengths.ptr, 1, 0, tokens), 1.0, 200, None, 0)
 
 
+@pytest.mark.parametrize("new", [1, 3, 40])  # one kernel each
+@pytest.mark.parametrize("dim", [64, 128])
+def test_attention_beside_pages_of_far_larger_values(kdb, dim, new):
+    """A page whose values are 10^5 times the others' and whose keys get weights of about 10^-9: the error follows what the rows
+    sum up, and not the largest value that they see. The definition's tolerance, with the weighted mean of |v| in place of
+    its largest."""
+    rng = np.random.default_rng(17)
+    starts, lengths, tokens = batch_of([new], [500])
+    cache = paged.Cache(rng, 1, 32, 1, 16, dim)
+    far = cache.table[0, 3]
+    cache.keys[far] = -127
+    cache.key_scales[far] = 21 / (127 * dim ** 0.5)
+    cache.value_scales[far] = 1500
+    q = (1 + 0.1 * rng.normal(0, 1, (tokens, 1, dim))).astype(np.float32)
+    on = paged.Device(kdb, cache, starts, lengths, tokens)
+    want, tolerance = paged.attention(cache, starts, lengths, q, dim ** -0.5)
+    k, v, _ = paged.values_of(cache, 0, 0, 500)
+    for i in range(tokens):
+        seen = 500 - new + i + 1
+        score = k[:seen] @ q[i, 0].astype(np.float64) * dim ** -0.5
+        p = np.exp(score - score.max())
+        tolerance[i] *= (p @ np.abs(v[:seen]) / p.sum()).max() / np.abs(v[:seen]).max()
+    got = run_attention(kdb, on, q, dim ** -0.5, 500)
+    off = np.abs(got - want)
+    assert (off <= tolerance).all(), (off / tolerance).max()
+
+
 def test_attention_of_more_keys_than_whole_sums_hold(kdb):
     """1.2 million keys of weight 1 to one row, whose lowest digits are all -128: some 2340 blocks of 64 to each of eight waves
     add up to more than 2^31. The weights and their sum are exact; a digit's sums round at most three times as they are turned
