@@ -422,7 +422,7 @@ __global__ __launch_bounds__(256) void paged_read_kernel(Paged c, float* __restr
 // Scores and weighted sums run on the signed 8-bit matrix cores, whose sums are exact: the cached codes go in as they
 // are, and the other operand as four signed digits of base 256. A query row is q = 2^(e - 30) * x with x whole, e the
 // exponent of its largest feature (x is exact for features of at least 2^-6 of that one, and off by 2^-31 of it at
-// most otherwise); a weight exp(score - max) times its value scale likewise, against the block's largest scale. Four products a
+// most otherwise); a weight exp(score - max) times its value scale likewise, against the largest of a row's block. Four products a
 // tile and twice bf16's rate are as many cycles as two bf16 products, where three would be needed for f32's bits, and the
 // codes need no conversion.
 //
@@ -432,6 +432,13 @@ __global__ __launch_bounds__(256) void paged_read_kernel(Paged c, float* __restr
 //   weights: their digits are the B operand of the second product as they stand, no lane exchanges anything;
 //   sums: O^T += V^T . P^T, the values' pages holding a feature's 16 tokens side by side.
 // The next block's codes are loaded while the present one is worked on, and the table entries of the one after it.
+//
+// Where there are fewer rows, a row takes S = 2 or 4 columns, each of them 4 / S of its digits: a tile is S times fewer products,
+// and the columns that join a score's digits share its row's keys out between them, so that a lane computes 16 / S
+// weights; their digits go back to the columns that multiply with them by exchanges within four lanes.
+//
+// Bound by the codes' bytes for many sequences (4 x 40000 keys of 128, 32 heads over 8: 46 us, 5.5 TB/s; 64 x 4000 of 64, one row,
+// 52 us, 5.7 TB/s), by the vector ALU for 9 to 32 rows, by the chain of loads (starts, table, codes) and 50 GB/s a CU for few.
 
 typedef int v4i __attribute__((ext_vector_type(4)));
 
@@ -440,7 +447,10 @@ constexpr int kTileRows = 64;  // rows of a workgroup
 constexpr int kKeyBlock = 64;
 
 // Sequence s has base(s + 1) - base(s) >= ceil(count * group / 64) tiles.
-__host__ __device__ inline int64_t tile_base(int64_t start, int64_t s, int group) { return start * group / kTileRows + s; }
+__host__ __device__ inline int64_t tile_base(int64_t start, int64_t s, int group, int rows = kTileRows) { return start * group / rows + s; }
+
+template <int Control> __device__ __forceinline__ int in_quad(int x) { return __builtin_amdgcn_mov_dpp(x, Control, 0xf, 0xf, true); }
+constexpr int kNextLane = 0xb1, kOtherPair = 0x4e;  // lane ^ 1, lane ^ 2 (quad_perm)
 
 // x of the lanes l, l ^ 16, l ^ 32 and l ^ 48 put together, in every one of them.
 template <class Op> __device__ __forceinline__ int over_chunks(int x, const Op& op) {
@@ -513,21 +523,44 @@ struct Split {
     float* sums;  // [row][count][D], then [row][count][2] of the maximum (base 2) and the sum
 };
 
-template <int D, int Waves>
+// The one of S values that column `sub` of a row's S takes.
+template <int S> __device__ __forceinline__ int taken(int sub, int a, int b, int c, int d) {
+    if constexpr (S == 2) return sub == 0 ? a : b;
+    else return sub & 2 ? (sub & 1 ? d : c) : sub & 1 ? b : a;
+}
+// x of a row's S columns put together, in each of them.
+template <int S, class T, class Op> __device__ __forceinline__ T over_row(T x, const Op& op) {
+    if constexpr (S > 1) x = op(x, __builtin_bit_cast(T, in_quad<kNextLane>(__builtin_bit_cast(int, x))));
+    if constexpr (S > 2) x = op(x, __builtin_bit_cast(T, in_quad<kOtherPair>(__builtin_bit_cast(int, x))));
+    return x;
+}
+struct MostOf {
+    __device__ __forceinline__ int operator()(int a, int b) const { return max(a, b); }
+    __device__ __forceinline__ float operator()(float a, float b) const { return fmaxf(a, b); }
+};
+struct SumOf {
+    __device__ __forceinline__ float operator()(float a, float b) const { return a + b; }
+};
+constexpr MostOf most_of;
+constexpr SumOf sum_of;
+
+template <int D, int Waves, int S>
 __global__ __launch_bounds__(Waves * 64, D == 64 ? 4 : 2) void paged_attention_kernel(Paged c, float* __restrict__ out, Strided q,
                                                                                       int heads, FastDiv by_group, double scale,
                                                                                       Split split) {
-    constexpr int U = D / 64;
+    constexpr int U = D / 64, J = 4 / S;
+    constexpr int kRowTile = 16 / S, kTileRows = 4 * kRowTile;
     constexpr int kLd = D + 4;
     __shared__ __attribute__((aligned(16))) float os[Waves][kRowTile][kLd];
     __shared__ float ms[Waves][kRowTile], ls[Waves][kRowTile];
     const int group = static_cast<int>(by_group.divisor);
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = threadIdx.x % 64;
     const int column = lane % 16, chunk = lane / 16;
+    const int sub = column % S;
     const int part = blockIdx.y, kv = static_cast<int>(blockIdx.x % c.kv_heads);
     // the last rows see most keys and go first
     const int64_t tile = (gridDim.x - 1 - blockIdx.x) / c.kv_heads;
-    const Found found = find_sequence(c, tile, [&](int64_t start, int64_t at) { return tile_base(start, at, group); });
+    const Found found = find_sequence(c, tile, [&](int64_t start, int64_t at) { return tile_base(start, at, group, kTileRows); });
     if (found.s < 0) return;
     const Rows rows = found.rows;
     // tokens * heads is below 2^31, and so are the rows of a kv head
@@ -537,7 +570,7 @@ __global__ __launch_bounds__(Waves * 64, D == 64 ? 4 : 2) void paged_attention_k
     const int row0 = static_cast<int>(tile_at);
     const int here = min(row_end - row0, kTileRows);
     // row tiles of the workgroup (1, 2 or 4), and the waves that share a tile's keys
-    const int row_waves = here <= 16 ? 1 : here <= 32 ? 2 : 4, key_waves = Waves / row_waves;
+    const int row_waves = here <= kRowTile ? 1 : here <= 2 * kRowTile ? 2 : 4, key_waves = Waves / row_waves;
     const int row_wave = wave % row_waves, key_wave = wave / row_waves;
     const int64_t capacity = static_cast<int64_t>(c.columns) << c.page_shift;
     // keys 0 .. limit - 1 are visible to the row of token `token` of the sequence
@@ -552,8 +585,8 @@ __global__ __launch_bounds__(Waves * 64, D == 64 ? 4 : 2) void paged_attention_k
     const int to = part + 1 == split.count ? all : min(all, from + split.part);
     // rows past the last one stand in for it with a query of 0 and are not written
     const int tile_row = row0 + row_wave * kRowTile;
-    const bool real = row_wave * kRowTile + column < here;
-    const int r = min(tile_row + column, row0 + here - 1);
+    const bool real = row_wave * kRowTile + column / S < here;
+    const int r = min(tile_row + column / S, row0 + here - 1);
     const int token = token_of(r);
     const int limit = limit_of(token);
     const int least = __builtin_amdgcn_readfirstlane(limit);  // limits ascend with the columns
@@ -613,18 +646,36 @@ __global__ __launch_bounds__(Waves * 64, D == 64 ? 4 : 2) void paged_attention_k
         load_keys(key);
         load_values();
     }
-    v4i digits[4][U];
-    const float q_factor = query_digits(features, real, scale, digits);
+    v4i digits[J][U];
+    float q_factor;
+    if constexpr (S == 1) {
+        q_factor = query_digits(features, real, scale, digits);
+    } else {
+        v4i all[4][U];
+        q_factor = query_digits(features, real, scale, all);
+#pragma unroll
+        for (int j = 0; j < J; ++j)
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+#pragma unroll
+                for (int t = 0; t < 4; ++t) digits[j][u][t] = taken<S>(sub, all[j][u][t], all[J + j][u][t], all[(2 * J + j) % 4][u][t], all[(3 * J + j) % 4][u][t]);
+    }
+    // of the digits that a column holds, and of those of lane ^ 1 or lane ^ 2 (S == 4) that hold the other half
+    const bool upper = sub >= S / 2 && S > 1, odd = sub % 2 != 0;
+    const float half_unit = upper ? 65536.f : 1.f, other_unit = upper ? 1.f : 65536.f;
+    const float sub_unit = S == 4 && odd ? 256.f * half_unit : half_unit;
+    const int shift = odd ? 8 : 0;
 
     float m = -INFINITY, l = 0.f;
     float o[D / 4] = {};
     for (; key < most; key += step) {
-        float x[16];
+        float x[4 * J];  // of the tiles J sub .. J sub + J - 1
+        int half[4][4];
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
-            v4i sum[4];
+            v4i sum[J];
 #pragma unroll
-            for (int p = 0; p < 4; ++p) {
+            for (int p = 0; p < J; ++p) {
                 sum[p] = v4i{0, 0, 0, 0};
 #pragma unroll
                 for (int u = 0; u < U; ++u)
@@ -632,11 +683,36 @@ __global__ __launch_bounds__(Waves * 64, D == 64 ? 4 : 2) void paged_attention_k
             }
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                x[4 * t + i] = joined(sum, i);
-                asm("" : "+v"(x[4 * t + i]));  // joined here, not behind the branch below with every tile's sums held
+                if constexpr (S == 1) {
+                    x[4 * t + i] = joined(sum, i);
+                    asm("" : "+v"(x[4 * t + i]));  // joined here, not behind the branch below with every tile's sums held
+                } else if constexpr (S == 2) {
+                    half[t][i] = (sum[1][i] << 8) + sum[0][i];
+                } else {
+                    half[t][i] = sum[0][i] << shift;
+                }
             }
         }
-        const int first = key + 16 * chunk;  // x[i] is key first + i
+        if constexpr (S == 4) {  // the halves of the tiles of the lane's parity, in half[0] and half[2]
+#pragma unroll
+            for (int t = 0; t < 4; t += 2)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int kept = odd ? half[t + 1][i] : half[t][i], sent = odd ? half[t][i] : half[t + 1][i];
+                    half[t][i] = kept + in_quad<kNextLane>(sent);
+                }
+        }
+        if constexpr (S > 1)
+#pragma unroll
+            for (int t = 0; t < J; ++t)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int kept = upper ? half[2 + t][i] : half[t][i], sent = upper ? half[t][i] : half[2 + t][i];
+                    x[4 * t + i] = static_cast<float>(kept) * half_unit +
+                                   static_cast<float>(in_quad<S == 4 ? kOtherPair : kNextLane>(sent)) * other_unit;
+                    asm("" : "+v"(x[4 * t + i]));
+                }
+        const int first = key + 16 * chunk + 4 * J * sub;  // x[i] is key first + i
         const int seen = page < 0 ? 0 : limit - first;
         const int scale_bits = seen > 0 ? __float_as_int(value_scale) & 0x7fffffff : 0;
         const float own_scale = value_scale;
@@ -646,13 +722,13 @@ __global__ __launch_bounds__(Waves * 64, D == 64 ? 4 : 2) void paged_attention_k
         if (key + kKeyBlock > least || __any(page < 0)) {
             factor = seen > 0 ? factor : 1.f;  // nor NaN where the row sees none of them
 #pragma unroll
-            for (int i = 0; i < 16; ++i) x[i] = i < seen ? x[i] : -INFINITY;
+            for (int i = 0; i < 4 * J; ++i) x[i] = i < seen ? x[i] : -INFINITY;
         }
         load_keys(key + step < most ? key + step : key);  // the last block once more rather than a branch
         float largest = x[0];
 #pragma unroll
-        for (int i = 1; i < 16; ++i) largest = fmaxf(largest, x[i]);
-        const float next = fmaxf(m, chunks_max(largest * factor));
+        for (int i = 1; i < 4 * J; ++i) largest = fmaxf(largest, x[i]);
+        const float next = fmaxf(m, chunks_max(over_row<S>(largest * factor, most_of)));
         const float base = next == -INFINITY ? 0.f : next;  // nothing seen yet: every weight below is 0
         const float alpha = __builtin_amdgcn_exp2f(m - base);
         m = next;
@@ -660,14 +736,14 @@ __global__ __launch_bounds__(Waves * 64, D == 64 ? 4 : 2) void paged_attention_k
         // largest of all, but not below 2^-40 of the largest scale, so that the scale in units stays finite.
         const float weight = __builtin_amdgcn_exp2f(fmaf(largest, factor, -base)) * own_scale;
         const int weight_bits = seen > 0 ? __float_as_int(weight) & 0x7fffffff : 0;
-        const int top = over_chunks(max(weight_bits, scale_bits - (40 << 23)), [](int a, int b) { return max(a, b); });
+        const int top = over_chunks(over_row<S>(max(weight_bits, scale_bits - (40 << 23)), most_of), most_of);
         const int e = __builtin_amdgcn_frexp_expf(__int_as_float(max(top, 0)));
         const float to_whole = top < 0x7f800000 && seen > 0 ? ldexpf(own_scale, 30 - e) : 0.f;
         const float from_whole = top < 0x7f800000 ? ldexpf(1.f, e - 30) : NAN;
         float sum = 0.f;
-        v4i weights[4];
+        v4i weights[J];
 #pragma unroll
-        for (int t = 0; t < 4; ++t) {
+        for (int t = 0; t < J; ++t) {
             int w[4], d4[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
@@ -678,29 +754,62 @@ __global__ __launch_bounds__(Waves * 64, D == 64 ? 4 : 2) void paged_attention_k
             }
             digits_of(w, d4);
 #pragma unroll
-            for (int p = 0; p < 4; ++p) weights[p][t] = d4[p];
+            for (int p = 0; p < J; ++p) {
+                if constexpr (S == 1) {
+                    weights[p][t] = d4[p];
+                } else if constexpr (S == 2) {
+                    const int own = sub == 0 ? d4[p] : d4[J + p];
+                    const int other = in_quad<kNextLane>(sub == 0 ? d4[J + p] : d4[p]);
+                    weights[p][t] = sub == 0 ? own : other;
+                    weights[p][J + t] = sub == 0 ? other : own;
+                }
+            }
+            if constexpr (S == 4) {
+                // the quad's digits the other way round: d4[p] of tile t from lane t to lane p, as weights[0][t]
+#pragma unroll
+                for (int p = 0; p < 4; p += 2) {
+                    const int other = in_quad<kNextLane>(odd ? d4[p] : d4[p + 1]);
+                    d4[p] = odd ? other : d4[p];
+                    d4[p + 1] = odd ? d4[p + 1] : other;
+                }
+#pragma unroll
+                for (int p = 0; p < 2; ++p) {
+                    const int other = in_quad<kOtherPair>(upper ? d4[p] : d4[p + 2]);
+                    weights[0][p] = upper ? other : d4[p];
+                    weights[0][p + 2] = upper ? d4[p + 2] : other;
+                }
+            }
         }
         l = l * alpha + sum;
 #pragma unroll
         for (int n = 0; n < D / 16; ++n) {
-            v4i acc[4];
+            v4i acc[J];
 #pragma unroll
-            for (int p = 0; p < 4; ++p)
+            for (int p = 0; p < J; ++p)
                 acc[p] = __builtin_amdgcn_mfma_i32_16x16x64_i8(v[n], weights[p], v4i{0, 0, 0, 0}, 0, 0, 0);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) o[4 * n + i] = o[4 * n + i] * alpha + joined(acc, i) * from_whole;
+            for (int i = 0; i < 4; ++i) {
+                float part;
+                if constexpr (S == 1) part = joined(acc, i);
+                else if constexpr (S == 2) part = static_cast<float>((acc[1][i] << 8) + acc[0][i]);
+                else part = static_cast<float>(acc[0][i]);
+                o[4 * n + i] = o[4 * n + i] * alpha + part * from_whole;
+            }
         }
         load_values();
     }
-    l = chunks_sum(l);
-    if (chunk == 0) {
-        ms[wave][column] = m;
-        ls[wave][column] = l;
+    l = chunks_sum(over_row<S>(l, sum_of));
+    if (chunk == 0 && sub == 0) {
+        ms[wave][column / S] = m;
+        ls[wave][column / S] = l;
     }
 #pragma unroll
-    for (int n = 0; n < D / 16; ++n)
-        *reinterpret_cast<float4*>(&os[wave][column][16 * n + 4 * chunk]) =
-            make_float4(o[4 * n], o[4 * n + 1], o[4 * n + 2], o[4 * n + 3]);
+    for (int d = 0; d < D / 4; ++d) o[d] = over_row<S>(o[d] * sub_unit, sum_of);
+    if (sub == 0)
+#pragma unroll
+        for (int n = 0; n < D / 16; ++n)
+            *reinterpret_cast<float4*>(&os[wave][column / S][16 * n + 4 * chunk]) =
+                make_float4(o[4 * n], o[4 * n + 1], o[4 * n + 2], o[4 * n + 3]);
     __syncthreads();
     // the waves that shared a row's keys joined, in their order
     for (int i = threadIdx.x; i < here * (D / 4); i += Waves * 64) {
@@ -738,12 +847,10 @@ __global__ __launch_bounds__(Waves * 64, D == 64 ? 4 : 2) void paged_attention_k
     }
 }
 
-// One row a workgroup (single tokens whose heads share nothing). Its four digits take four of the sixteen columns, so that a tile of
-// 16 keys is one product and not four, and the sums come out one key to a lane: a weight costs a lane one exponential where the
-// kernel above computes sixteen for columns that stand in for rows that are not there.
-template <int Control> __device__ __forceinline__ int in_quad(int x) { return __builtin_amdgcn_mov_dpp(x, Control, 0xf, 0xf, true); }
+// One row a workgroup (single tokens whose heads share nothing). Its four digits take four columns, and all sixteen columns share the
+// keys out, one to a lane: a weight costs a lane one exponential where the kernel above computes four. The sums of the outputs stay
+// whole over the blocks, and are turned into f32 when the largest weight or weighted scale changes or they could pass 2^31.
 constexpr int kMostBlocks = 1024;  // that the whole sums hold: 2^10 blocks of 2^6 keys of 2^14
-constexpr int kNextLane = 0xb1, kOtherPair = 0x4e;  // lane ^ 1, lane ^ 2 (quad_perm)
 
 template <int D, int Waves>
 __global__ __launch_bounds__(Waves * 64, D == 64 ? 4 : 2) void paged_single_kernel(Paged c, float* __restrict__ out, Strided q, int heads,
@@ -1366,53 +1473,54 @@ __global__ __launch_bounds__(256) void paged_join_kernel(Paged c, float* __restr
 // Bytes of a part's results of `rows` rows.
 int64_t part_bytes(int64_t rows, int64_t dim) { return rows * (dim + 2) * 4; }
 
-// How a call runs: on the prompts' kernel or with `waves` waves that share a tile's keys, and the parts that the keys are split
-// into.
+// How a call runs: on which kernel, with how many waves that share a tile's keys, and in how many parts of the keys.
 struct Plan {
-    int64_t tiles;
     bool prompts, single;
-    int waves;
+    int waves, columns;  // columns of the matrix instruction for a row (paged_attention_kernel)
+    int64_t tiles;
     Split split;
 };
 
 Plan plan_of(int64_t heads, int64_t kv_heads, int64_t dim, int64_t sequences, int64_t tokens, int64_t max_keys, int64_t most) {
     Plan plan;
-    const int64_t group = heads / kv_heads;
-    plan.tiles = tile_base(tokens, sequences, static_cast<int>(group));
-    const int64_t cus = compute_units();
-    const int64_t groups = std::max<int64_t>(1, plan.tiles * kv_heads);
-    const int64_t keys = std::min<int64_t>(std::max<int64_t>(max_keys, 1), int64_t{1} << 30);
-    // From 33 rows a sequence on average the prompts' kernel; 32 sequences of 1000 keys, 12 heads of 64, shared keys / prompts, us:
-    // 16 rows 13 / 28, 32 rows 21 / 34, 48 rows 39 / 35, 64 rows 43 / 36. Below it a sequence's kv head is about one tile.
-    plan.prompts = tokens * group > 32 * sequences;
-    // One row a tile: 64 x 1024 keys of 64, 12 heads, 18.6 -> 16.4 us, 16 x 4000 21.5 -> 16.5, 1 x 1000 8.6 -> 8.2 (7 without the
-    // call's 8 on the host); of 128, 16 heads, 32 x 2000 37.8 -> 36.1.
-    plan.single = tokens * group <= sequences;
-    // Eight waves and one launch where the CUs hold all of those workgroups at once and either the keys are few or the
-    // workgroups many; otherwise four waves, and parts to fill the CUs. Four / eight waves, us: 12 x 1000 keys of 64 8.8 / 8.2,
-    // 12 x 2000 11.0 / 11.7, 96 x 4000 15.0 / 19.4, 192 x 4000 22.1 / 21.2, 384 x 2000 23.0 / 20.6, 768 x 1000 19.0 / 20.4;
-    // of 128 64 x 2000 14.7 / 17.0, 256 x 1000 19.0 / 14.9.
+    const int64_t group = heads / kv_heads, rows = tokens * group, cus = compute_units();
     const bool narrow = dim == 64;
-    const int64_t working = plan.single ? std::max<int64_t>(1, tokens * heads) : sequences * kv_heads;
+    const int64_t keys = std::min<int64_t>(std::max<int64_t>(max_keys, 1), int64_t{1} << 30);
+    // By the rows of a sequence's kv head on average. From 33 on the prompts' kernel; 32 sequences of 1000 keys, 12 heads of 64,
+    // 16 rows a tile / prompts, us: 16 rows 13 / 28, 32 rows 21 / 34, 48 rows 39 / 35, 64 rows 43 / 36.
+    plan.prompts = rows > 32 * sequences;
+    // One row: 64 x 1024 keys of 64, 12 heads, 16 rows a tile / single 18.6 / 16.4 us, 16 x 4000 21.5 / 16.5; of 128, 16 heads,
+    // 32 x 2000 37.8 / 36.1.
+    plan.single = rows <= sequences;
+    // Up to 8 and up to 4 rows, 16 / 8 / 4 rows a tile: 5 rows, 32 x 2000, 12 heads of 64 21.0 / 18.2 / 21.3 us, 4 rows, 64 x 4000,
+    // 4 kv heads 31.7 / 26.2 / 23.8; of 128 4 rows, 16 x 2000, 8 kv heads 20.4 / 19.8 / 19.7, and 64 x 500, 4 kv heads
+    // 10.2 / 10.3 / 14.3, whose tiles of 4 rows leave more workgroups empty than a round of the CUs has room for.
+    plan.columns = narrow && rows <= 4 * sequences ? 4 : rows <= 8 * sequences ? 2 : 1;
+    const int64_t tile_rows = kTileRows / plan.columns;
+    plan.tiles = tile_base(tokens, sequences, static_cast<int>(group), static_cast<int>(tile_rows));
+    // the workgroups with work, if the sequences are alike
+    const int64_t working = std::max<int64_t>(1, plan.single ? tokens * heads
+                                                             : std::max(sequences, (rows + tile_rows - 1) / tile_rows) * kv_heads);
     int64_t count, least = 512;  // parts, and the keys that one is worth
-    if (plan.single) {
-        // Parts where there are few rows of many keys. One launch / parts, us: 12 rows of 64 x 2000 8.5 / 10.4, x 4000 11.2 / 10.8,
-        // x 8000 17.2 / 10.9, 96 x 4000 13.1 / 13.3, 192 x 8000 27.7 / 30.9; of 128 16 x 1000 10.8 / 10.6, x 2000 16.1 / 10.6,
-        // 128 x 4000 27.3 / 24.6, 256 x 4000 37.1 / 41.1. A CU takes about 50 GB/s, whatever its waves: eight of them are worth
-        // it for the latency of keys of 64 (192 x 4000: four 18.0, eight 16.4), while the CUs hold them (384 x 2000 16.7 / 17.3).
-        const bool whole = keys <= (narrow ? 4096 : 1024) || 4 * working >= 3 * cus;
+    if (plan.prompts) {
+        count = 2 * working > cus ? 1 : ((narrow ? 4 : 2) * cus + working - 1) / working;
+    } else {
+        // Parts where there are few workgroups of many keys. One launch / parts, us: of 64, one row, 12 x 2000 keys 8.5 / 10.4,
+        // x 4000 11.2 / 10.8, x 8000 17.2 / 10.9, 96 x 4000 13.1 / 13.3, 192 x 8000 27.7 / 30.9; four rows, 32 x 2000 8.8 / 11.4,
+        // x 4000 12.9 / 11.0, 128 x 2000 9.1 / 11.7; five, 96 x 4000 16.3 / 15.0; of 128, one row, 16 x 1000 10.8 / 10.6,
+        // x 2000 16.1 / 10.6, 128 x 2000 17.1 / 17.0, x 4000 27.3 / 24.6, 256 x 4000 37.1 / 41.1; four rows, 8 x 4000 26.8 / 11.4,
+        // 128 x 2000 17.9 / 19.1, and 32 x 40000 in 4 / 8 / 16 parts 66.6 / 46.5 / 49.4.
+        const int64_t few = narrow ? (plan.single ? 4096 : 2048) : 2 * working >= cus ? 2048 : 1024;
+        const bool whole = keys <= few || 4 * working >= 3 * cus;
         count = whole ? 1 : ((narrow ? 2 : 1) * cus + working - 1) / working;
         if (!narrow) least = 256;
-    } else {
-        const bool at_once = working <= (narrow ? 2 : 1) * cus;
-        plan.waves = !plan.prompts && at_once && (keys <= 1024 || (keys <= 4096 && 4 * working >= 3 * cus)) ? 8 : 4;
-        // as many workgroups as the CUs hold at once
-        count = ((narrow ? 4 : 2) * cus + groups - 1) / groups;
-        if (plan.prompts ? 2 * groups > cus : plan.waves == 8 || keys <= 1024) count = 1;
     }
     // no part longer than about 8192 keys
     count = std::max<int64_t>(1, std::min({std::max(count, keys / 8192), keys / least, most, int64_t{65535}}));
-    if (plan.single) plan.waves = narrow && count == 1 && working <= cus ? 8 : 4;
+    // Eight waves for the latency of a CU's only workgroup. Four / eight, us: of 64, one row, 12 x 2000 9.5 / 8.5, 192 x 4000
+    // 18.0 / 16.4, 384 x 2000 16.7 / 17.3; four rows, 128 x 2000 10.0 / 9.1, 256 x 1000 9.0 / 9.6. Keys of 128 keep a CU at the
+    // 50 GB/s that it takes with four: 16 x 1000 10.8 / 11.3, 256 x 500 11.6 / 10.2, 384 x 1000 19.3 / 25.1.
+    plan.waves = count == 1 && (narrow ? working < cus : 4 * working >= 3 * cus && working <= cus) ? 8 : 4;
     constexpr int64_t unit = 256;
     const int64_t part = ((keys + count - 1) / count + unit - 1) / unit * unit;
     plan.split = {static_cast<int>((keys + part - 1) / part), static_cast<int>(part), nullptr};
@@ -1588,7 +1696,9 @@ extern "C" int kd_paged_attention(int dtype, void* out, const void* q, const int
     Strided qs;
     if (int rc = check_strided(what, "q", q, q_strides, c.tokens, heads, qs)) return rc;
     if (out == nullptr || !aligned(out, 16)) return fail(KD_E_INVALID, "kd_paged_attention: out must be given, 16-byte aligned");
-    if (int rc = check_grid(what, tile_base(c.tokens, c.sequences, static_cast<int>(heads / c.kv_heads)) * c.kv_heads, 512)) return rc;
+    // the most workgroups that a plan has, of at most 512 threads
+    if (int rc = check_grid(what, tile_base(c.tokens, c.sequences, static_cast<int>(heads / c.kv_heads), kTileRows / 4) * c.kv_heads, 512))
+        return rc;
     if (int rc = ensure_device()) return rc;
     if (c.pages == 0) c.columns = 0;  // no position has a page
     const int64_t rows = heads * c.tokens;
@@ -1596,9 +1706,9 @@ extern "C" int kd_paged_attention(int dtype, void* out, const void* q, const int
     const int64_t most = fits_grid(join_groups, 256) ? workspace_bytes / part_bytes(rows, c.head_dim) : 1;
     const Plan plan = plan_of(heads, c.kv_heads, c.head_dim, c.sequences, c.tokens, max_keys, most);
     const Split split{plan.split.count, plan.split.part, static_cast<float*>(workspace)};
-    const auto launch = [&](auto dim, auto waves) {
-        constexpr int D = decltype(dim)::value, Waves = decltype(waves)::value;
-        hipLaunchKernelGGL((paged_attention_kernel<D, Waves>), dim3(static_cast<uint32_t>(plan.tiles * c.kv_heads), split.count),
+    const auto launch = [&](auto dim, auto waves, auto columns) {
+        constexpr int D = decltype(dim)::value, Waves = decltype(waves)::value, S = decltype(columns)::value;
+        hipLaunchKernelGGL((paged_attention_kernel<D, Waves, S>), dim3(static_cast<uint32_t>(plan.tiles * c.kv_heads), split.count),
                            dim3(Waves * 64), 0, stream(), c, static_cast<float*>(out), qs, static_cast<int>(heads),
                            FastDiv(static_cast<uint32_t>(heads / c.kv_heads)), scale, split);
     };
@@ -1615,11 +1725,18 @@ extern "C" int kd_paged_attention(int dtype, void* out, const void* q, const int
                                    stream(), c, static_cast<float*>(out), qs, static_cast<int>(heads),
                                    FastDiv(static_cast<uint32_t>(heads / c.kv_heads)), FastDiv(static_cast<uint32_t>(heads)), scale, split);
             };
+            if (plan.waves == 8) launch_single(std::integral_constant<int, 8>{});
+            else launch_single(std::integral_constant<int, 4>{});
+        } else {
+            const auto with_columns = [&](auto columns) {
+                if (plan.waves == 8) launch(dim, std::integral_constant<int, 8>{}, columns);
+                else launch(dim, std::integral_constant<int, 4>{}, columns);
+            };
             if constexpr (D == 64)
-                if (plan.waves == 8) launch_single(std::integral_constant<int, 8>{});
-            if (plan.waves == 4) launch_single(std::integral_constant<int, 4>{});
-        } else if (plan.waves == 8) launch(dim, std::integral_constant<int, 8>{});
-        else launch(dim, std::integral_constant<int, 4>{});
+                if (plan.columns == 4) with_columns(std::integral_constant<int, 4>{});
+            if (plan.columns == 2) with_columns(std::integral_constant<int, 2>{});
+            if (plan.columns == 1) with_columns(std::integral_constant<int, 1>{});
+        }
         if (split.count > 1)
             hipLaunchKernelGGL((paged_join_kernel<D>), dim3(static_cast<uint32_t>(join_groups)), dim3(256), 0, stream(), c,
                                static_cast<float*>(out), static_cast<int>(heads), split);

@@ -293,6 +293,53 @@ def test_attention_takes_nan_from_what_it_sees_alone(kdb, dim, heads):
     assert (np.abs(got - want)[fine] <= tolerance[fine]).all()
 
 
+# new tokens, lengths, kv heads, heads: one, up to 4 and up to 8 rows a sequence on average, and some of them far more
+FEW = [([1, 1, 0, 1, 0, 2], [300, 1, 9, 700, 5, 66], 2, 2), ([5, 0, 0, 0, 0], [333, 4, 4, 4, 4], 1, 1), ([1] * 9, [40 * s + 1 for s in range(9)], 1, 3),
+       ([9, 1, 1, 0, 2], [300, 70, 1, 5, 900], 1, 1), ([20, 1, 1, 1, 1, 1], [400, 20, 64, 65, 63, 1], 2, 2), ([3], [1500], 2, 4),
+       ([40, 1, 1, 1, 1, 1, 1, 1], [600, 9, 9, 9, 200, 9, 9, 1], 1, 1), ([4, 4, 1], [64, 1024, 3], 2, 4), ([1, 1], [5000, 2600], 1, 7)]
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("case", FEW, ids=[f"{len(a[0])}s{sum(a[0])}t{max(a[1])}k{a[2]}of{a[3]}" for a in FEW])
+def test_attention_of_few_rows_is_its_definition(kdb, case, dim):
+    new, lengths, kv, heads = case
+    rng = np.random.default_rng(dim + sum(lengths))
+    starts, lengths, tokens = batch_of(new, lengths)
+    cache = paged.Cache(rng, len(new), -(-max(lengths) // 16), kv, 16, dim)
+    cache.table[0, -(-int(lengths[0]) // 32)] = -1  # a page in the middle
+    cache.value_scales[::3] *= 100
+    q = rng.normal(0, 1, (tokens, heads, dim)).astype(np.float32)
+    on = paged.Device(kdb, cache, starts, lengths, tokens)
+    want, tolerance = paged.attention(cache, starts, lengths, q, dim ** -0.5)
+    space = workspace_for(kdb, heads, kv, dim, len(new), tokens, max(lengths))
+    for hint, room in ((max(lengths), space), (1, None)):
+        got = run_attention(kdb, on, q, dim ** -0.5, hint, room)
+        assert (np.abs(got - want) <= tolerance).all(), (np.abs(got - want) / np.maximum(tolerance, 1e-30)).max()
+        np.testing.assert_array_equal(run_attention(kdb, on, q, dim ** -0.5, hint, room), got)
+
+
+@pytest.mark.parametrize("heads", [1, 3, 6])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_few_rows_take_nan_from_what_they_see_alone(kdb, dim, heads):
+    """A sequence with a NaN key scale, one with a NaN value scale, one with queries that are not finite, one with neither."""
+    rng = np.random.default_rng(18)
+    starts, lengths, tokens = batch_of([1] * 5, [40, 200, 130, 300, 32])
+    cache = paged.Cache(rng, 5, 20, 1, 16, dim)
+    cache.key_scales[cache.table[0, 2], 0] = np.nan
+    cache.value_scales[cache.table[1, 5], 0] = np.nan
+    cache.key_scales[cache.table[4, 2], 0] = cache.value_scales[cache.table[4, 2], 0] = np.nan  # from position 32 on: not seen
+    q = rng.normal(0, 1, (tokens, heads, dim)).astype(np.float32)
+    q[2, 0, 3], q[3, heads - 1, 63] = np.inf, np.nan
+    on = paged.Device(kdb, cache, starts, lengths, tokens)
+    with np.errstate(invalid="ignore"):
+        want, tolerance = paged.attention(cache, starts, lengths, np.where(np.isfinite(q), q, 0), 0.125)
+    want[:2] = want[2, 0] = want[3, heads - 1] = np.nan
+    got = run_attention(kdb, on, q, 0.125, 300, workspace_for(kdb, heads, 1, dim, 5, tokens, 300))
+    np.testing.assert_array_equal(np.isnan(got), np.isnan(want))
+    fine = ~np.isnan(want)
+    assert (np.abs(got - want)[fine] <= tolerance[fine]).all()
+
+
 @pytest.mark.parametrize("new", [3, 40])
 @pytest.mark.parametrize("dim", [64, 128])
 @pytest.mark.parametrize("size", [1e-30, 1e-3, 30.0, 1e30])
