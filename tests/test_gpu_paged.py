@@ -318,6 +318,40 @@ def test_attention_of_few_rows_is_its_definition(kdb, case, dim):
         np.testing.assert_array_equal(run_attention(kdb, on, q, dim ** -0.5, hint, room), got)
 
 
+# single rows and few rows of more keys than one launch takes, split over the workspace that the call asks for
+@pytest.mark.parametrize("heads", [2, 4, 10])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_few_rows_of_many_keys_are_split(kdb, dim, heads):
+    rng = np.random.default_rng(dim + heads)
+    starts, lengths, tokens = batch_of([1, 0, 1], [5000, 7, 2222])
+    cache = paged.Cache(rng, 3, 40, 2, 128, dim)
+    cache.table[0, 20] = -1
+    q = rng.normal(0, 1, (tokens, heads, dim)).astype(np.float32)
+    on = paged.Device(kdb, cache, starts, lengths, tokens)
+    want, tolerance = paged.attention(cache, starts, lengths, q, dim ** -0.5)
+    space = workspace_for(kdb, heads, 2, dim, 3, tokens, 5000)
+    assert space.nbytes >= 2 * tokens * heads * (dim + 2) * 4
+    for hint, room in ((5000, space), (1 << 20, space), (5000, kdb.empty((space.nbytes // 2 // 16 * 16,), np.uint8)), (1 << 25, None)):
+        got = run_attention(kdb, on, q, dim ** -0.5, hint, room)
+        assert (np.abs(got - want) <= tolerance).all(), (np.abs(got - want) / np.maximum(tolerance, 1e-30)).max()
+        np.testing.assert_array_equal(run_attention(kdb, on, q, dim ** -0.5, hint, room), got)
+
+
+# as many workgroups as take eight waves at either width, and more: one, two and ten rows to a kv head, or five
+@pytest.mark.parametrize("heads", [2, 4, 20])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("sequences,new", [(110, 1), (150, 1), (110, 5)])
+def test_attention_of_many_short_sequences(kdb, sequences, new, dim, heads):
+    rng = np.random.default_rng(sequences + heads)
+    starts, lengths, tokens = batch_of([new] * sequences, rng.integers(new, 40, sequences))
+    cache = paged.Cache(rng, sequences, 3, 2, 16, dim)
+    q = rng.normal(0, 1, (tokens, heads, dim)).astype(np.float32)
+    on = paged.Device(kdb, cache, starts, lengths, tokens)
+    want, tolerance = paged.attention(cache, starts, lengths, q, dim ** -0.5)
+    got = run_attention(kdb, on, q, dim ** -0.5, 39)
+    assert (np.abs(got - want) <= tolerance).all(), (np.abs(got - want) / np.maximum(tolerance, 1e-30)).max()
+
+
 @pytest.mark.parametrize("heads", [1, 3, 6])
 @pytest.mark.parametrize("dim", [64, 128])
 def test_few_rows_take_nan_from_what_they_see_alone(kdb, dim, heads):
