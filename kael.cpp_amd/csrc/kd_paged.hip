@@ -1070,12 +1070,14 @@ __global__ __launch_bounds__(Waves * 64, D == 64 ? 4 : 2) void paged_single_kern
 }
 
 // Many rows a sequence (prompts): the workgroup's four waves take 16 rows each and share every block of 64 keys through LDS,
-// two blocks deep, so that a wave keeps none of it in registers. What bounds it is the vector ALU, 30 operations a score in the
-// kernel above, seven of which join the digits' sums of the outputs; here the weighted sums run on the f16 matrix cores
-// into f32, which joins nothing: a code is an f16 value as it stands, converted once for the four waves, and a weight two f16
-// pieces (2^-24 of it), scaled so that the largest is 2^15 and pieces below 2^-24 are below 2^-39 of that. 2 prompts of up to 4096,
-// 32 heads over 8 of 128: 422 us, 480 TFLOP/s of the formula's products, VALU busy 0.74 and matrix cores 0.43 of the cycles;
-// 8 of up to 1000, 12 heads of 64: 31 us; 4 x 4096 of 64: VALU busy 0.95.
+// two blocks deep, so that a wave keeps none of it in registers. Few workgroups have two such teams (G = 2) that take every
+// other block: a wave alone on its SIMD takes 1.05 us for a block of 64 features, two of them 1.5 for both.
+// What bounds it is the vector ALU, 30 operations a score in the kernel above, seven of which join the digits' sums of the
+// outputs; here the weighted sums run on the f16 matrix cores into f32, which joins nothing: a code is an f16 value as it stands,
+// converted once for the four waves, and a weight two f16 pieces (2^-24 of it), scaled so that the largest is 2^15 and pieces
+// below 2^-24 are below 2^-39 of that. 2 prompts of up to 4096, 32 heads over 8 of 128: 422 us, 480 TFLOP/s of the formula's
+// products, VALU busy 0.74 and matrix cores 0.43 of the cycles; 8 of up to 1000, 12 heads of 64: 31 us; 4 x 4096 of 64: VALU busy
+// 0.95.
 typedef _Float16 v8h __attribute__((ext_vector_type(8)));
 typedef _Float16 v2h __attribute__((ext_vector_type(2)));
 typedef float v2f __attribute__((ext_vector_type(2)));
@@ -1151,8 +1153,8 @@ __device__ __forceinline__ float query_halves(float (&features)[16], bool real, 
     return bits < 0x7f800000 ? static_cast<float>(ldexp(fabs(scale) * 1.4426950408889634074, e - 15)) : NAN;
 }
 
-template <int D>
-__global__ __launch_bounds__(kPromptWaves * 64, 2) void paged_prompt_kernel(Paged c, float* __restrict__ out, Strided q,
+template <int D, int G>
+__global__ __launch_bounds__(G * kPromptWaves * 64, 2) void paged_prompt_kernel(Paged c, float* __restrict__ out, Strided q,
                                                                                   int heads, FastDiv by_group, double scale,
                                                                                   Split split) {
     constexpr int U = D / 64;
@@ -1161,13 +1163,14 @@ __global__ __launch_bounds__(kPromptWaves * 64, 2) void paged_prompt_kernel(Page
     constexpr bool kHalfKeys = D == 64;
     constexpr int kKeyPieces = 8, kValuePieces = 2 * D / 16;  // of 64 lanes' 16 bytes
     union Shared {
-        v4i block[2][kKeyPieces + kValuePieces][64];
-        float os[kPromptWaves][kRowTile][kLd];
+        v4i block[G][2][kKeyPieces + kValuePieces][64];
+        float os[G * kPromptWaves][kRowTile][kLd];
     };
     __shared__ __attribute__((aligned(16))) Shared shared;
-    __shared__ float ms[kPromptWaves][kRowTile], ls[kPromptWaves][kRowTile];
+    __shared__ float ms[G * kPromptWaves][kRowTile], ls[G * kPromptWaves][kRowTile];
     const int group = static_cast<int>(by_group.divisor);
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = threadIdx.x % 64;
+    const int any_wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = threadIdx.x % 64;
+    const int wave = any_wave % kPromptWaves, team = any_wave / kPromptWaves;
     const int column = lane % 16, chunk = lane / 16;
     const int part = blockIdx.y, kv = static_cast<int>(blockIdx.x % c.kv_heads);
     const Found found = find_tile(c, static_cast<int>(blockIdx.x) / c.kv_heads, static_cast<int>(gridDim.x) / c.kv_heads, group);
@@ -1237,13 +1240,13 @@ __global__ __launch_bounds__(kPromptWaves * 64, 2) void paged_prompt_kernel(Page
             if constexpr (kHalfKeys) {
                 halves_of(k[u], pieces);
 #pragma unroll
-                for (int h = 0; h < 2; ++h) shared.block[at][2 * wave + h][lane] = pieces[h];
+                for (int h = 0; h < 2; ++h) shared.block[team][at][2 * wave + h][lane] = pieces[h];
             } else {
-                shared.block[at][wave * U + u][lane] = k[u];
+                shared.block[team][at][wave * U + u][lane] = k[u];
             }
             halves_of(v[u], pieces);
 #pragma unroll
-            for (int h = 0; h < 2; ++h) shared.block[at][kKeyPieces + 2 * (wave * U + u) + h][lane] = pieces[h];
+            for (int h = 0; h < 2; ++h) shared.block[team][at][kKeyPieces + 2 * (wave * U + u) + h][lane] = pieces[h];
         }
     };
 
@@ -1251,7 +1254,9 @@ __global__ __launch_bounds__(kPromptWaves * 64, 2) void paged_prompt_kernel(Page
     float features[16 * U];
 #pragma unroll
     for (int d = 0; d < 16 * U; ++d) features[d] = row[d];
-    if (from < to) load(from);
+    const int first = from + team * kKeyBlock;
+    constexpr int step = G * kKeyBlock;
+    if (first < to) load(first);
     v4i digits[4][U];
     v8h q_high[2], q_low[2];
     float q_factor;
@@ -1378,17 +1383,17 @@ __global__ __launch_bounds__(kPromptWaves * 64, 2) void paged_prompt_kernel(Page
 
     if (from < to) {
         Scales own = next;
-        store(0);
-        if (from + kKeyBlock < to) load(from + kKeyBlock);
+        if (first < to) store(0);
+        if (first + step < to) load(first + step);
         __syncthreads();
         int buffer = 0;
-        for (int key = from; key < to; key += kKeyBlock) {
-            if (key < most) work(key, own, shared.block[buffer]);
+        for (int key = first; key - team * kKeyBlock < to; key += step) {
+            if (key < most) work(key, own, shared.block[team][buffer]);
             buffer ^= 1;
-            if (key + kKeyBlock < to) {
+            if (key + step < to) {
                 own = next;
                 store(buffer);
-                if (key + 2 * kKeyBlock < to) load(key + 2 * kKeyBlock);
+                if (key + 2 * step < to) load(key + 2 * step);
             }
             // the block stored is complete, and the one worked on free
             __syncthreads();
@@ -1397,17 +1402,26 @@ __global__ __launch_bounds__(kPromptWaves * 64, 2) void paged_prompt_kernel(Page
     l = chunks_sum(l);
     const float unit = top < 0x7f800000 ? ldexpf(1.f, top_exponent - 15) : NAN;
     if (chunk == 0) {
-        ms[wave][column] = m;
-        ls[wave][column] = l;
+        ms[any_wave][column] = m;
+        ls[any_wave][column] = l;
     }
 #pragma unroll
-    for (int n = 0; n < D / 16; ++n) *reinterpret_cast<v4f*>(&shared.os[wave][column][16 * n + 4 * chunk]) = o[n] * unit;
+    for (int n = 0; n < D / 16; ++n) *reinterpret_cast<v4f*>(&shared.os[any_wave][column][16 * n + 4 * chunk]) = o[n] * unit;
     __syncthreads();
-    for (int i = threadIdx.x; i < here * (D / 4); i += kPromptWaves * 64) {
+    for (int i = threadIdx.x; i < here * (D / 4); i += G * kPromptWaves * 64) {
         const int at = i / (D / 4), d = i % (D / 4) * 4;
         const int w = at / kRowTile, col = at % kRowTile;
-        const v4f sums = *reinterpret_cast<const v4f*>(&shared.os[w][col][d]);
-        const float sum = ls[w][col];
+        // the teams joined, in their order
+        float largest = ms[w][col], sum = ls[w][col];
+        v4f sums = *reinterpret_cast<const v4f*>(&shared.os[w][col][d]);
+        if constexpr (G == 2) {
+            const int other = w + kPromptWaves;
+            const float top = fmaxf(largest, ms[other][col]), base = top == -INFINITY ? 0.f : top;
+            const float f = __builtin_amdgcn_exp2f(largest - base), g = __builtin_amdgcn_exp2f(ms[other][col] - base);
+            sum = f * sum + g * ls[other][col];
+            sums = sums * f + *reinterpret_cast<const v4f*>(&shared.os[other][col][d]) * g;
+            largest = top;
+        }
         const int of_token = token_of(row0 + at);
         const int64_t to_row = static_cast<int64_t>(rows.row + of_token) * heads + kv * group + (row0 + at - of_token * group);
         if (split.count == 1) {
@@ -1417,7 +1431,7 @@ __global__ __launch_bounds__(kPromptWaves * 64, 2) void paged_prompt_kernel(Page
             *reinterpret_cast<v4f*>(split.sums + record * D + d) = sums;
             if (d == 0) {
                 float* own = split.sums + static_cast<int64_t>(c.tokens) * heads * split.count * D + record * 2;
-                own[0] = ms[w][col];
+                own[0] = largest;
                 own[1] = sum;
             }
         }
@@ -1485,7 +1499,8 @@ int64_t part_bytes(int64_t rows, int64_t dim) { return rows * (dim + 2) * 4; }
 // How a call runs: on which kernel, with how many waves that share a tile's keys, and in how many parts of the keys.
 struct Plan {
     bool prompts, single;
-    int waves, columns;  // columns of the matrix instruction for a row (paged_attention_kernel)
+    int waves;    // of a workgroup; prompts: two teams of four, or one
+    int columns;  // of the matrix instruction for a row (paged_attention_kernel)
     int64_t tiles;
     Split split;
 };
@@ -1530,6 +1545,10 @@ Plan plan_of(int64_t heads, int64_t kv_heads, int64_t dim, int64_t sequences, in
     // 18.0 / 16.4, 384 x 2000 16.7 / 17.3; four rows, 128 x 2000 10.0 / 9.1, 256 x 1000 9.0 / 9.6. Keys of 128 keep a CU at the
     // 50 GB/s that it takes with four: 16 x 1000 10.8 / 11.3, 256 x 500 11.6 / 10.2, 384 x 1000 19.3 / 25.1.
     plan.waves = count == 1 && (narrow ? working < cus : 4 * working >= 3 * cus && working <= cus) ? 8 : 4;
+    // Prompts: two teams where the workgroups are few. One / two, us: 12 heads of 64, 1 x 500 13.3 / 11.4, 1 x 1000 22.2 / 18.1,
+    // 1 x 3000 58.5 / 52.8, 4 x 1000 25.8 / 24.1, 8 x 1000 35.5 / 41.5; 32 heads over 8 of 128, 1 x 500 21.5 / 17.8, 1 x 600
+    // 24.9 / 24.8, 1 x 1000 38.7 / 39.5, 4 x 1000 73 / 114; in parts 100 new ones over 8000 of 64 25.4 / 23.4, of 128 51 / 55.
+    if (plan.prompts) plan.waves = working * count <= (narrow ? 3 : 1) * cus ? 8 : 4;
     constexpr int64_t unit = 256;
     const int64_t part = ((keys + count - 1) / count + unit - 1) / unit * unit;
     plan.split = {static_cast<int>((keys + part - 1) / part), static_cast<int>(part), nullptr};
@@ -1724,9 +1743,14 @@ extern "C" int kd_paged_attention(int dtype, void* out, const void* q, const int
     const auto with_waves = [&](auto dim) {
         constexpr int D = decltype(dim)::value;
         if (plan.prompts) {
-            hipLaunchKernelGGL((paged_prompt_kernel<D>), dim3(static_cast<uint32_t>(plan.tiles * c.kv_heads), split.count),
-                               dim3(kPromptWaves * 64), 0, stream(), c, static_cast<float*>(out), qs, static_cast<int>(heads),
+            const auto launch_prompts = [&](auto teams) {
+                constexpr int G = decltype(teams)::value;
+                hipLaunchKernelGGL((paged_prompt_kernel<D, G>), dim3(static_cast<uint32_t>(plan.tiles * c.kv_heads), split.count),
+                               dim3(G * kPromptWaves * 64), 0, stream(), c, static_cast<float*>(out), qs, static_cast<int>(heads),
                                FastDiv(static_cast<uint32_t>(heads / c.kv_heads)), scale, split);
+            };
+            if (plan.waves == 8) launch_prompts(std::integral_constant<int, 2>{});
+            else launch_prompts(std::integral_constant<int, 1>{});
         } else if (plan.single) {
             const auto launch_single = [&](auto waves) {
                 constexpr int Waves = decltype(waves)::value;

@@ -318,6 +318,26 @@ def test_attention_of_few_rows_is_its_definition(kdb, case, dim):
         np.testing.assert_array_equal(run_attention(kdb, on, q, dim ** -0.5, hint, room), got)
 
 
+# prompts of few workgroups, whose teams of waves share a tile's keys, and of many; either in parts
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("new,lengths,kv,heads", [([40], [40], 1, 1), ([150, 34], [170, 34], 2, 4), ([100], [3000], 1, 3), ([70], [64], 1, 1),
+                                                  ([40] * 60, [40 + 3 * i for i in range(60)], 7, 14)],
+                         ids=lambda x: str(len(x)) if isinstance(x, list) else str(x))
+def test_attention_of_prompts_by_one_team_or_two(kdb, new, lengths, kv, heads, dim):
+    rng = np.random.default_rng(dim + sum(lengths))
+    starts, lengths, tokens = batch_of(new, lengths)
+    cache = paged.Cache(rng, len(new), -(-max(lengths) // 32), kv, 32, dim)
+    cache.table[0, -1] = -1
+    cache.value_scales[::3] *= 100
+    q = rng.normal(0, 1, (tokens, heads, dim)).astype(np.float32)
+    on = paged.Device(kdb, cache, starts, lengths, tokens)
+    want, tolerance = paged.attention(cache, starts, lengths, q, dim ** -0.5)
+    for room in (workspace_for(kdb, heads, kv, dim, len(new), tokens, max(lengths)), None):
+        got = run_attention(kdb, on, q, dim ** -0.5, max(lengths), room)
+        assert (np.abs(got - want) <= tolerance).all(), (np.abs(got - want) / np.maximum(tolerance, 1e-30)).max()
+        np.testing.assert_array_equal(run_attention(kdb, on, q, dim ** -0.5, max(lengths), room), got)
+
+
 # single rows and few rows of more keys than one launch takes, split over the workspace that the call asks for
 @pytest.mark.parametrize("heads", [2, 4, 10])
 @pytest.mark.parametrize("dim", [64, 128])
