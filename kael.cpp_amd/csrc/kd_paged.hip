@@ -1388,13 +1388,14 @@ __global__ __launch_bounds__(G * kPromptWaves * 64, 2) void paged_prompt_kernel(
         __syncthreads();
         int buffer = 0;
         for (int key = first; key - team * kKeyBlock < to; key += step) {
-            if (key < most) work(key, own, shared.block[team][buffer]);
-            buffer ^= 1;
+            const Scales following = next;
             if (key + step < to) {
-                own = next;
-                store(buffer);
+                store(buffer ^ 1);
                 if (key + 2 * step < to) load(key + 2 * step);
             }
+            if (key < most) work(key, own, shared.block[team][buffer]);
+            own = following;
+            buffer ^= 1;
             // the block stored is complete, and the one worked on free
             __syncthreads();
         }
