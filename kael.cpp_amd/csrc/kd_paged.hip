@@ -162,8 +162,17 @@ struct Strided {
 
 constexpr int kUnit = 8;  // features of a thread: four pairs, or eight that are not rotated
 
-template <bool Vector> __device__ __forceinline__ void load4(const float* p, float (&x)[4]) {
-    if constexpr (Vector) {
+// Past: the access takes no place in the caches.
+typedef float v4f __attribute__((ext_vector_type(4)));
+template <bool Past> __device__ __forceinline__ void store4(float* p, const v4f& x) {
+    if constexpr (Past) __builtin_nontemporal_store(x, reinterpret_cast<v4f*>(p));
+    else *reinterpret_cast<v4f*>(p) = x;
+}
+template <bool Vector, bool Past = false> __device__ __forceinline__ void load4(const float* p, float (&x)[4]) {
+    if constexpr (Vector && Past) {
+        const v4f v = __builtin_nontemporal_load(reinterpret_cast<const v4f*>(p));
+        x[0] = v[0], x[1] = v[1], x[2] = v[2], x[3] = v[3];
+    } else if constexpr (Vector) {
         const float4 v = *reinterpret_cast<const float4*>(p);
         x[0] = v.x, x[1] = v.y, x[2] = v.z, x[3] = v.w;
     } else {
@@ -184,11 +193,11 @@ template <bool Vector> __device__ __forceinline__ void unit_places(int u, const 
 
 // The unit of the row x, rotated by `position`'s angles, in f64. Vector: pairs never cross a unit and everything is 16-byte
 // aligned; otherwise each feature finds its partner.
-template <bool Vector>
+template <bool Vector, bool Past = false>
 __device__ __forceinline__ void rotated_unit(const float* x, int low, int high, int64_t position, const Rotation& r, double (&y)[kUnit]) {
     float a[4], b[4];
-    load4<Vector>(x + low, a);
-    load4<Vector>(x + high, b);
+    load4<Vector, Past>(x + low, a);
+    load4<Vector, Past>(x + high, b);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         y[i] = a[i];
@@ -237,8 +246,9 @@ __device__ __forceinline__ uint32_t code_of(double x, double inverse) {
 }
 
 constexpr int kAppendThreads = 256;
+constexpr int64_t kPastBytes = int64_t{32} << 20;  // of rows, from which on they go past the caches
 
-template <int D, bool Vector>
+template <int D, bool Vector, bool Past>
 __global__ __launch_bounds__(kAppendThreads) void paged_append_kernel(Paged c, Rotation rotation, Strided k, Strided v,
                                                                       Strided q, float* __restrict__ q_out, int heads,
                                                                       int64_t cache_groups, int q_tokens) {
@@ -262,11 +272,11 @@ __global__ __launch_bounds__(kAppendThreads) void paged_append_kernel(Paged c, R
             unit_places<Vector>(i % units, rotation, low, high);
             const int64_t position = rows.position + (token - rows.row);
             double y[kUnit];
-            rotated_unit<Vector>(q.data + token * q.row + h * q.head, low, high, position, rotation, y);
+            rotated_unit<Vector, Past>(q.data + token * q.row + h * q.head, low, high, position, rotation, y);
             float* out = q_out + (token * heads + h) * dim;
             const auto at = [&](int j) { return position < 0 ? NAN : static_cast<float>(y[j]); };
-            *reinterpret_cast<float4*>(out + low) = make_float4(at(0), at(1), at(2), at(3));
-            *reinterpret_cast<float4*>(out + high) = make_float4(at(4), at(5), at(6), at(7));
+            store4<Past>(out + low, v4f{at(0), at(1), at(2), at(3)});
+            store4<Past>(out + high, v4f{at(4), at(5), at(6), at(7)});
         }
         return;
     }
@@ -328,7 +338,7 @@ __global__ __launch_bounds__(kAppendThreads) void paged_append_kernel(Paged c, R
             int low, high;
             unit_places<Vector>(i % units, rotation, low, high);
             double y[kUnit];
-            rotated_unit<Vector>(x + token * in.row, low, high, p.first + token, rotation, y);
+            rotated_unit<Vector, Past>(x + token * in.row, low, high, p.first + token, rotation, y);
             uint32_t word[2] = {};
 #pragma unroll
             for (int j = 0; j < kUnit; ++j) word[j / 4] |= code_of(y[j], inverse) << (8 * (j % 4));
@@ -371,6 +381,7 @@ __global__ __launch_bounds__(kAppendThreads) void paged_append_kernel(Paged c, R
 // the values, so that codes are read in whole pieces and rows written in whole lines. Bound by the bytes, the rows' above all:
 // 67 MB in 17.0 us.
 
+template <bool Past>
 __global__ __launch_bounds__(256) void paged_read_kernel(Paged c, float* __restrict__ k, float* __restrict__ v) {
     const uint32_t group = c.kv_heads * 2;
     const int h = static_cast<int>(blockIdx.x % group) / 2;
@@ -400,8 +411,7 @@ __global__ __launch_bounds__(256) void paged_read_kernel(Paged c, float* __restr
         const int8_t* codes = c.keys + (at * size + p.held) * dim;
         for (int i = threadIdx.x; i < p.count * (dim / 4); i += threads) {
             const char4 x = *reinterpret_cast<const char4*>(codes + 4 * i);
-            *reinterpret_cast<float4*>(out + i / (dim / 4) * row_size + i % (dim / 4) * 4) =
-                make_float4(x.x * scale, x.y * scale, x.z * scale, x.w * scale);
+            store4<Past>(out + i / (dim / 4) * row_size + i % (dim / 4) * 4, v4f{x.x * scale, x.y * scale, x.z * scale, x.w * scale});
         }
     } else {
         const float scale = c.value_scales[at];
@@ -414,8 +424,12 @@ __global__ __launch_bounds__(256) void paged_read_kernel(Paged c, float* __restr
 #pragma unroll
             for (int j = 0; j < 16; ++j) {
                 const int token = slot0 + j - p.held;
-                if (token >= 0 && token < p.count)
-                    out[token * row_size + d] = static_cast<float>(static_cast<int8_t>(word[j / 4] >> (8 * (j % 4)))) * scale;
+                const float x = static_cast<float>(static_cast<int8_t>(word[j / 4] >> (8 * (j % 4)))) * scale;
+                float* to = out + token * row_size + d;
+                if (token >= 0 && token < p.count) {
+                    if constexpr (Past) __builtin_nontemporal_store(x, to);
+                    else *to = x;
+                }
             }
         }
     }
@@ -1081,7 +1095,6 @@ __global__ __launch_bounds__(Waves * 64, D == 64 ? 4 : 2) void paged_single_kern
 typedef _Float16 v8h __attribute__((ext_vector_type(8)));
 typedef _Float16 v2h __attribute__((ext_vector_type(2)));
 typedef float v2f __attribute__((ext_vector_type(2)));
-typedef float v4f __attribute__((ext_vector_type(4)));
 
 constexpr int kPromptWaves = 4;
 
@@ -1670,17 +1683,23 @@ extern "C" int kd_paged_append(int dtype, const kd_paged_cache* cache, const kd_
     // 16-byte pieces need rows and tables that keep them aligned and pairs that come in fours
     const auto whole = [](const Strided& x) { return aligned(x.data, 16) && x.row % 4 == 0 && x.head % 4 == 0; };
     const bool vector = r.half % 4 == 0 && aligned(r.cosines, 16) && aligned(r.sines, 16) && whole(ks) && (q == nullptr || whole(qs));
-    const auto launch = [&](auto dim, auto aligned_pieces) {
-        hipLaunchKernelGGL((paged_append_kernel<decltype(dim)::value, decltype(aligned_pieces)::value>), dim3(static_cast<uint32_t>(cache_groups + q_groups)),
-                           dim3(threads), 0, stream(), c, r, ks, vs, qs, static_cast<float*>(q_out), static_cast<int>(heads),
-                           cache_groups, q_tokens);
+    // Large queries go past the caches both ways, and so do the keys the second time: what they leave there is the second reading
+    // of the keys and values. With the pages read back, us, all through the caches / past them, by the bytes of q: 13 MB
+    // 24.2 / 24.9, 25 MB 27.5 / 29.1, 38 MB 36.1 / 35.4, 50 MB 46.5 / 41.4, 100 MB 90.2 / 75.9, 200 MB 169 / 152.
+    const bool past = q != nullptr && vector && int64_t{c.tokens} * heads * c.head_dim * 4 > kPastBytes;
+    const auto launch = [&](auto dim, auto aligned_pieces, auto past_caches) {
+        constexpr int D = decltype(dim)::value;
+        hipLaunchKernelGGL((paged_append_kernel<D, decltype(aligned_pieces)::value, decltype(past_caches)::value>),
+                           dim3(static_cast<uint32_t>(cache_groups + q_groups)), dim3(threads), 0, stream(), c, r, ks, vs, qs,
+                           static_cast<float*>(q_out), static_cast<int>(heads), cache_groups, q_tokens);
     };
-    const auto with_dim = [&](auto aligned_pieces) {
-        if (c.head_dim == 64) launch(std::integral_constant<int, 64>{}, aligned_pieces);
-        else launch(std::integral_constant<int, 128>{}, aligned_pieces);
+    const auto with_dim = [&](auto aligned_pieces, auto past_caches) {
+        if (c.head_dim == 64) launch(std::integral_constant<int, 64>{}, aligned_pieces, past_caches);
+        else launch(std::integral_constant<int, 128>{}, aligned_pieces, past_caches);
     };
-    if (vector) with_dim(std::true_type{});
-    else with_dim(std::false_type{});
+    if (past) with_dim(std::true_type{}, std::true_type{});
+    else if (vector) with_dim(std::true_type{}, std::false_type{});
+    else with_dim(std::false_type{}, std::false_type{});
     KD_LAUNCH_CHECK();
     return KD_OK;
 }
@@ -1694,8 +1713,14 @@ extern "C" int kd_paged_read(int dtype, void* k, void* v, const kd_paged_cache* 
     const int threads = c.page_shift <= 5 ? 64 : 256;
     if (int rc = check_grid("kd_paged_read", groups, threads)) return rc;
     if (int rc = ensure_device()) return rc;
-    hipLaunchKernelGGL(paged_read_kernel, dim3(static_cast<uint32_t>(groups)), dim3(threads), 0, stream(), c,
-                       static_cast<float*>(k), static_cast<float*>(v));
+    // past the caches, 50 MB of rows 17.3 / 15.4 us, 100 MB 33 / 27
+    const auto launch = [&](auto kernel) {
+        hipLaunchKernelGGL(kernel, dim3(static_cast<uint32_t>(groups)), dim3(threads), 0, stream(), c, static_cast<float*>(k),
+                           static_cast<float*>(v));
+    };
+    const int64_t rows = int64_t{c.tokens} * c.kv_heads * ((k != nullptr) + (v != nullptr));
+    if (rows * c.head_dim * 4 > kPastBytes) launch(paged_read_kernel<true>);
+    else launch(paged_read_kernel<false>);
     KD_LAUNCH_CHECK();
     return KD_OK;
 }

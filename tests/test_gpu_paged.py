@@ -184,6 +184,35 @@ def test_read_gives_the_values(kdb, page, dim):
             np.testing.assert_array_equal(got[n].numpy(), np.full_like(want[n], -777) if n == skipped else want[n])
 
 
+@pytest.mark.parametrize("dim,page", [(64, 16), (128, 64)])
+def test_large_appends_and_reads_are_those_of_their_parts(kdb, dim, page):
+    """Rows of more than 32 MiB, which go past the caches: the same bits as sequence by sequence."""
+    rng = np.random.default_rng(dim)
+    kv, heads, columns = 8, 16, 2400 // page + 1
+    starts, lengths, tokens = batch_of([1900, 2300, 700 * 64 // dim, 2100, 2000 * 64 // dim], [1900, 2390, 1400, 2100, 2000])
+    whole = paged.Cache(rng, 5, columns, kv, page, dim)
+    rotation = (*paged.tables(2400, dim), dim, False)
+    x, q, k, v = fused(rng, tokens, heads, kv, dim)
+    on, q_out = run_append(kdb, whole, starts, lengths, tokens, x, heads, rotation)
+    got = on.read_back()
+    rows = [kdb.empty((tokens, kv, dim), np.float32) for _ in range(2)]
+    kdb.call("paged_read", kd.F32, rows[0].ptr, rows[1].ptr, on.c, on.b)
+    for s in range(5):
+        part = slice(starts[s], starts[s + 1])
+        count = starts[s + 1] - starts[s]
+        cache = whole.copy()
+        cache.table = whole.table[s:s + 1]
+        alone, q_part = run_append(kdb, cache, [0, count], lengths[s:s + 1], count, np.ascontiguousarray(x[part]), heads, rotation)
+        np.testing.assert_array_equal(q_out[part], q_part)
+        own, used = alone.read_back(), whole.table[s][:-(-lengths[s] // page)]
+        for name in paged.Cache.NAMES:
+            np.testing.assert_array_equal(getattr(got, name)[used], getattr(own, name)[used])
+        apart = [kdb.empty((count, kv, dim), np.float32) for _ in range(2)]
+        for i in range(2):
+            kdb.call("paged_read", kd.F32, *(a.ptr if j == i else None for j, a in enumerate(apart)), alone.c, alone.b)
+            np.testing.assert_array_equal(rows[i].numpy()[part], apart[i].numpy())
+
+
 # ---- attention ------------------------------------------------------------------------------------
 
 
