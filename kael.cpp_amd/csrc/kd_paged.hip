@@ -144,8 +144,8 @@ __device__ __forceinline__ PageSlots page_slots(const Paged& c, int64_t slot) {
 // has one owner, and the workgroups behind those take the queries. Rotated and quantised in f64, where the products of two
 // f32 are exact and a rounding to the wrong side of a tie takes a value within 2^-45 of it: f64 costs less here than the bytes.
 // Keys and values are read twice, for the scale and for the codes, the second time mostly from the L2: a page held in registers
-// or LDS in between left fewer workgroups on a CU and took longer. 6347 tokens of 32 + 2 x 8 heads of 128: 67.5 us, 274 MB at
-// 4.1 TB/s; 64 single tokens of 12 heads of 64: 6.9 us.
+// or LDS in between left fewer workgroups on a CU and took longer. 6347 tokens of 32 + 2 x 8 heads of 128: 71 us, 274 MB at
+// 3.9 TB/s; 64 single tokens of 12 heads of 64: 6.9 us.
 
 struct Rotation {
     const float* cosines;
@@ -379,7 +379,7 @@ __global__ __launch_bounds__(kAppendThreads) void paged_append_kernel(Paged c, R
 //
 // The append's division into pages: four codes a thread and a 16-byte store for the keys, a feature's 16 tokens a thread for
 // the values, so that codes are read in whole pieces and rows written in whole lines. Bound by the bytes, the rows' above all:
-// 67 MB in 17.0 us.
+// 67 MB in 13.5 us, past the caches.
 
 template <bool Past>
 __global__ __launch_bounds__(256) void paged_read_kernel(Paged c, float* __restrict__ k, float* __restrict__ v) {
