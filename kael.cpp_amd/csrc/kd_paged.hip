@@ -1547,10 +1547,18 @@ Plan plan_of(int64_t heads, int64_t kv_heads, int64_t dim, int64_t sequences, in
         // x 4000 11.2 / 10.8, x 8000 17.2 / 10.9, 96 x 4000 13.1 / 13.3, 192 x 8000 27.7 / 30.9; four rows, 32 x 2000 8.8 / 11.4,
         // x 4000 12.9 / 11.0, 128 x 2000 9.1 / 11.7; five, 96 x 4000 16.3 / 15.0; of 128, one row, 16 x 1000 10.8 / 10.6,
         // x 2000 16.1 / 10.6, 128 x 2000 17.1 / 17.0, x 4000 27.3 / 24.6, 256 x 4000 37.1 / 41.1; four rows, 8 x 4000 26.8 / 11.4,
-        // 128 x 2000 17.9 / 19.1, and 32 x 40000 in 4 / 8 / 16 parts 66.6 / 46.5 / 49.4.
+        // 128 x 2000 17.9 / 19.1.
         const int64_t few = narrow ? (plan.single ? 4096 : 2048) : 2 * working >= cus ? 2048 : 1024;
         const bool whole = keys <= few || 4 * working >= 3 * cus;
-        count = whole ? 1 : ((narrow ? 2 : 1) * cus + working - 1) / working;
+        // Of 64, two workgroups a CU, four for 9 rows and more (68 x 20000, 24 rows, in 4 / 8 / 16 parts 83 / 64 / 48 us; 4 rows
+        // 31.4 / 31.1 / 29.0). Of 128, one or else two: a CU with one more than the others is what the call waits for (96 x 8000 in
+        // 2 / 3 / 5 parts 33.7 / 41.8 / 36.0, 32 x 40000 in 4 / 8 / 16 66.6 / 46.5 / 49.4), two from 17 rows on (68 x 10000, 24
+        // rows, in 3 / 7 / 8 67 / 47 / 43).
+        const int64_t grid = plan.single ? working : std::max<int64_t>(1, plan.tiles * kv_heads);
+        if (narrow) count = ((plan.columns == 1 ? 4 : 2) * cus + working - 1) / working;
+        else if (rows > 16 * sequences) count = 2 * cus / working;
+        else count = cus / grid > 1 ? cus / grid : 2 * cus / grid;
+        if (whole) count = 1;
         if (!narrow) least = 256;
     }
     // no part longer than about 8192 keys
