@@ -464,7 +464,7 @@ constexpr int kRowTile = 16;
 constexpr int kTileRows = 64;  // rows of a workgroup
 constexpr int kKeyBlock = 64;
 
-// Sequence s has base(s + 1) - base(s) >= ceil(count * group / 64) tiles.
+// Sequence s has base(s + 1) - base(s) >= ceil(count * group / rows) tiles of `rows` rows.
 __host__ __device__ inline int64_t tile_base(int64_t start, int64_t s, int group, int rows = kTileRows) { return start * group / rows + s; }
 
 template <int Control> __device__ __forceinline__ int in_quad(int x) { return __builtin_amdgcn_mov_dpp(x, Control, 0xf, 0xf, true); }
@@ -1541,7 +1541,10 @@ Plan plan_of(int64_t heads, int64_t kv_heads, int64_t dim, int64_t sequences, in
                                                              : std::max(sequences, (rows + tile_rows - 1) / tile_rows) * kv_heads);
     int64_t count, least = 512;  // parts, and the keys that one is worth
     if (plan.prompts) {
-        count = 2 * working > cus ? 1 : ((narrow ? 4 : 2) * cus + working - 1) / working;
+        // up to half of the CUs in one launch take parts, and up to all of them for long keys: one launch / parts, us: 300 new ones
+        // over 8000 of 128, 152 workgroups, 152 / 123, 1000 over 16000 of 64, 188, 183 / 152, 300 over 3000, 240, 39.8 / 40.0
+        const bool whole = working > cus || (2 * working > cus && keys <= 4096);
+        count = whole ? 1 : ((narrow ? 4 : 2) * cus + working - 1) / working;
     } else {
         // Parts where there are few workgroups of many keys. One launch / parts, us: of 64, one row, 12 x 2000 keys 8.5 / 10.4,
         // x 4000 11.2 / 10.8, x 8000 17.2 / 10.9, 96 x 4000 13.1 / 13.3, 192 x 8000 27.7 / 30.9; four rows, 32 x 2000 8.8 / 11.4,
