@@ -1740,7 +1740,7 @@ extern "C" int kd_paged_attention_workspace(int64_t* bytes, int64_t heads, int64
                                             int64_t sequences, int64_t tokens, int64_t max_keys) {
     if (bytes == nullptr || heads < 1 || kv_heads < 1 || heads % kv_heads != 0 || heads > 4096 ||
         (head_dim != 64 && head_dim != 128) || sequences < 0 || sequences >= int64_t{1} << 24 || tokens < 0 ||
-        tokens >= int64_t{1} << 31 || max_keys < 0)
+        tokens >= int64_t{1} << 31 || heads * tokens >= int64_t{1} << 31 || max_keys < 0)
         return fail(KD_E_INVALID, "kd_paged_attention_workspace: bad arguments");
     const Split split = plan_of(heads, kv_heads, head_dim, sequences, tokens, max_keys, INT32_MAX).split;
     *bytes = split.count > 1 ? split.count * part_bytes(tokens * heads, head_dim) : 0;

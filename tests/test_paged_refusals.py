@@ -134,3 +134,14 @@ def test_more_workgroups_than_a_launch_takes(lib):
     assert lib.lib.kd_paged_append(kd.F32, c, b, None, FAKE + 64, FAKE, ROWS, 4096, FAKE, ROWS, FAKE, ROWS) == INVALID
     assert lib.lib.kd_paged_read(kd.F32, FAKE, FAKE, c, b) == INVALID
     assert lib.lib.kd_paged_attention(kd.F32, FAKE + 64, FAKE, ROWS, 4096, c, b, 1.0, 64, None, 0) == INVALID
+
+
+def test_workspaces_of_the_largest_calls(lib):
+    """As many rows as a call takes have a size that is one, more have none; the part sizes follow the split's own rule."""
+    n, g = ctypes.c_int64(), lib.lib.kd_paged_attention_workspace
+    assert g(ctypes.byref(n), 4096, 4096, 128, 1, 1 << 19, 64) == INVALID
+    assert g(ctypes.byref(n), 4096, 1, 128, 1, (1 << 19) - 1, 1 << 62) == 0 and n.value > 0
+    rows = ((1 << 19) - 1) * 4096
+    assert n.value % (rows * (128 + 2) * 4) == 0
+    for sequences, tokens in ((0, 0), (5, 0), (1 << 23, 1)):
+        assert g(ctypes.byref(n), 8, 2, 64, sequences, tokens, 1 << 20) == 0 and n.value >= 0
