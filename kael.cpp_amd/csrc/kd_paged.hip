@@ -1539,6 +1539,7 @@ Plan plan_of(int64_t heads, int64_t kv_heads, int64_t dim, int64_t sequences, in
     // the workgroups with work, if the sequences are alike
     const int64_t working = std::max<int64_t>(1, plan.single ? tokens * heads
                                                              : std::max(sequences, (rows + tile_rows - 1) / tile_rows) * kv_heads);
+    const int64_t grid = plan.single ? working : std::max<int64_t>(1, plan.tiles * kv_heads);  // with those that find none
     int64_t count, least = 512;  // parts, and the keys that one is worth
     if (plan.prompts) {
         // up to half of the CUs in one launch take parts, and up to all of them for long keys: one launch / parts, us: 300 new ones
@@ -1557,7 +1558,6 @@ Plan plan_of(int64_t heads, int64_t kv_heads, int64_t dim, int64_t sequences, in
         // 31.4 / 31.1 / 29.0). Of 128, one or else two: a CU with one more than the others is what the call waits for (96 x 8000 in
         // 2 / 3 / 5 parts 33.7 / 41.8 / 36.0, 32 x 40000 in 4 / 8 / 16 66.6 / 46.5 / 49.4), two from 17 rows on (68 x 10000, 24
         // rows, in 3 / 7 / 8 67 / 47 / 43).
-        const int64_t grid = plan.single ? working : std::max<int64_t>(1, plan.tiles * kv_heads);
         if (narrow) count = ((plan.columns == 1 ? 4 : 2) * cus + working - 1) / working;
         else if (rows > 16 * sequences) count = 2 * cus / working;
         else count = cus / grid > 1 ? cus / grid : 2 * cus / grid;
@@ -1568,8 +1568,9 @@ Plan plan_of(int64_t heads, int64_t kv_heads, int64_t dim, int64_t sequences, in
     count = std::max<int64_t>(1, std::min({std::max(count, keys / 8192), keys / least, most, int64_t{65535}}));
     // Eight waves for the latency of a CU's only workgroup. Four / eight, us: of 64, one row, 12 x 2000 9.5 / 8.5, 192 x 4000
     // 18.0 / 16.4, 384 x 2000 16.7 / 17.3; four rows, 128 x 2000 10.0 / 9.1, 256 x 1000 9.0 / 9.6. Keys of 128 keep a CU at the
-    // 50 GB/s that it takes with four: 16 x 1000 10.8 / 11.3, 256 x 500 11.6 / 10.2, 384 x 1000 19.3 / 25.1.
-    plan.waves = count == 1 && (narrow ? working < cus : 4 * working >= 3 * cus && working <= cus) ? 8 : 4;
+    // 50 GB/s that it takes with four: 16 x 1000 10.8 / 11.3, 256 x 500 (288 workgroups) 11.6 / 10.2, 237 x 574 of 8 rows (294) 14.1 /
+    // 19.4, 220 x 500 of 12 rows 14.1 / 20.0, 384 x 1000 19.3 / 25.1.
+    plan.waves = count == 1 && (narrow ? working < cus : plan.columns > 1 && 4 * working >= 3 * cus && 8 * grid <= 9 * cus) ? 8 : 4;
     // Prompts: two teams where the workgroups are few. One / two, us: 12 heads of 64, 1 x 500 13.3 / 11.4, 1 x 1000 22.2 / 18.1,
     // 1 x 3000 58.5 / 52.8, 4 x 1000 25.8 / 24.1, 8 x 1000 35.5 / 41.5; 32 heads over 8 of 128, 1 x 500 21.5 / 17.8, 1 x 600
     // 24.9 / 24.8, 1 x 1000 38.7 / 39.5, 4 x 1000 73 / 114; in parts 100 new ones over 8000 of 64 25.4 / 23.4, of 128 51 / 55.
@@ -1799,8 +1800,9 @@ extern "C" int kd_paged_attention(int dtype, void* out, const void* q, const int
             else launch_single(std::integral_constant<int, 4>{});
         } else {
             const auto with_columns = [&](auto columns) {
-                if (plan.waves == 8) launch(dim, std::integral_constant<int, 8>{}, columns);
-                else launch(dim, std::integral_constant<int, 4>{}, columns);
+                if constexpr (D == 64 || decltype(columns)::value > 1)
+                    if (plan.waves == 8) launch(dim, std::integral_constant<int, 8>{}, columns);
+                if (plan.waves == 4) launch(dim, std::integral_constant<int, 4>{}, columns);
             };
             if constexpr (D == 64)
                 if (plan.columns == 4) with_columns(std::integral_constant<int, 4>{});
