@@ -11,7 +11,6 @@ its whole range.
 """
 from __future__ import annotations
 
-import functools
 import math
 import sys
 from pathlib import Path
@@ -378,9 +377,10 @@ PLAIN = {"append": plain_append, "attention": plain_attention, "verify": plain_v
 # ---- the framework's calls ------------------------------------------------------------------------
 
 
-@functools.cache
 def backend():
-    sys.path.insert(0, str(Path(__file__).resolve().parents[1] / "kael.cpp_amd"))
+    package = str(Path(__file__).resolve().parents[1] / "kael.cpp_amd")
+    if package not in sys.path:
+        sys.path.insert(0, package)
     import kd
     return kd, kd.load()
 
