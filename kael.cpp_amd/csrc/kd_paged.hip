@@ -204,7 +204,7 @@ __device__ __forceinline__ void rotated_unit(const float* x, int low, int high, 
         y[4 + i] = b[i];
     }
     if (low >= 2 * r.half) return;
-    const bool known = position < r.positions;
+    const bool known = position >= 0 && position < r.positions;  // queries may stand below position 0
     if constexpr (Vector) {
         float c[4] = {NAN, NAN, NAN, NAN}, s[4] = {NAN, NAN, NAN, NAN};
         if (known) {

@@ -160,6 +160,33 @@ def test_a_position_past_the_rotation_tables_turns_into_nan(kdb):
     assert np.isnan(q_out[4:, :, :32]).all() and np.isfinite(q_out[:4]).all()
 
 
+@pytest.mark.parametrize("interleaved", [False, True], ids=["halves", "pairs"])
+@pytest.mark.parametrize("shift", [0, 1])  # rows that 16-byte pieces lie aligned in, and rows that they do not
+@pytest.mark.parametrize("positions", [0, 70])  # no tables, and tables
+def test_append_of_rotated_rows_below_position_zero(kdb, interleaved, shift, positions):
+    """More new rows than positions, with a rotation: there is no table row for them, the queries there are NaN, and the
+    other rows and the cache are as ever."""
+    rng = np.random.default_rng(19 + shift)
+    starts, lengths, tokens = batch_of([40, 90, 7, 3], [11, 0, -5, 60], first=1, after=2)
+    cache = paged.Cache(rng, 4, 4, 2, 16, 64)
+    wide = rng.normal(0, 1, (tokens, 8, 64 + shift)).astype(np.float32)  # [token][q 4, k 2, v 2][feature]
+    q, k, v = (np.ascontiguousarray(wide[:, a:b, shift:]) for a, b in ((0, 4), (4, 6), (6, 8)))
+    cosines, sines = (t[:positions] for t in paged.tables(70, 48))
+    on = paged.Device(kdb, cache, starts, lengths, tokens)
+    dx, c, s = kdb.to_device(wide), kdb.to_device(cosines), kdb.to_device(sines)
+    turn = kd.Rotation(c.ptr if positions else None, s.ptr if positions else None, positions, 48, int(interleaved))
+    out = kdb.to_device(np.full(q.shape, -777, np.float32))
+    strides, head = kd.strides(8 * (64 + shift), 64 + shift), 4 * (64 + shift)
+    at = dx.ptr + 4 * shift
+    kdb.call("paged_append", kd.F32, on.c, on.b, turn, out.ptr, at, strides, 4, at + 4 * head, strides, at + 6 * head, strides)
+    lengths = [max(n, 0) for n in lengths]  # a length below 0 counts as 0
+    want, want_q = paged.append(cache, starts, lengths, q, k, v, (cosines, sines, 48, interleaved))
+    got = out.numpy()
+    np.testing.assert_array_equal(got, want_q)
+    assert np.isnan(got[1:30]).all() and np.isnan(got[41:138]).all() and np.isfinite(got[138:141, :, 48:]).all()
+    same_cache(on.read_back(), want)
+
+
 @pytest.mark.parametrize("page,dim", [(16, 64), (64, 128), (256, 64)])
 def test_read_gives_the_values(kdb, page, dim):
     rng = np.random.default_rng(page)
