@@ -966,7 +966,8 @@ __global__ __launch_bounds__(Waves * 64, D == 64 ? 4 : 2) void paged_single_kern
     float o[D / 4] = {};           // of the column's digit
     v4i acc[D / 16] = {};          // since the last change of the unit
     int top = 0, blocks = 0;       // the largest weight times its value scale, as bits, so that NaN is the largest of all
-    float to_whole = 0.f, from_whole = 0.f;
+    int to_whole = 0;              // the exponent that a weight takes to its units
+    float from_whole = 0.f;
     const auto flush = [&](float alpha) {
 #pragma unroll
         for (int n = 0; n < D / 16; ++n) {
@@ -1023,12 +1024,13 @@ __global__ __launch_bounds__(Waves * 64, D == 64 ? 4 : 2) void paged_single_kern
             for (int d = 32; d > 0; d /= 2) next = max(next, __shfl_xor(next, d));
             top = max(top, next);
             const int e = __builtin_amdgcn_frexp_expf(__int_as_float(top));
-            to_whole = top < 0x7f800000 ? ldexpf(1.f, 30 - e) : 0.f;
+            to_whole = 30 - e;  // to 178: as a factor it would be infinite for weighted scales below 2^-98
             from_whole = top < 0x7f800000 ? ldexpf(1.f, e - 30) : NAN;
         }
         ++blocks;
         // from 2^23 on an f32 is whole: the bias rounds the weight too, to half a unit or its own last bit
-        int bytes = static_cast<int>(fmaf(weight, to_whole, static_cast<float>(kDigitBias))) ^ kDigitBias;
+        const float units = top < 0x7f800000 ? ldexpf(weight, to_whole) : 0.f;
+        int bytes = static_cast<int>(units + static_cast<float>(kDigitBias)) ^ kDigitBias;
         bytes = static_cast<int>(__builtin_amdgcn_perm(in_quad<kNextLane>(bytes), bytes, first_bytes));
         bytes = static_cast<int>(__builtin_amdgcn_perm(in_quad<kOtherPair>(bytes), bytes, second_bytes));
         // the quads' digits side by side; right in the first quad's columns, which are the ones that are read
