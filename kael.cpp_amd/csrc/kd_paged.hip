@@ -535,6 +535,13 @@ template <int U> __device__ __forceinline__ float query_digits(float (&features)
     return bits < 0x7f800000 ? static_cast<float>(ldexp(fabs(scale) * 1.4426950408889634074, e - 30)) : NAN;
 }
 
+// The exponent e of the largest of a row's weighted value scales, whose bits are `top`, at least `least`: 2^(e - 30) is the unit of
+// whole weights and 2^(e - 15) that of f16 ones, and neither may fall below f32's least number.
+constexpr int kLeastWhole = 30 - 149, kLeastHalf = 15 - 149;
+__device__ __forceinline__ int unit_exponent(int top, int least) {
+    return max(__builtin_amdgcn_frexp_expf(__int_as_float(top)), least);
+}
+
 struct Split {
     int count;    // parts that a row's keys are split into
     int part;     // keys of a part, a multiple of 64; the last part goes to the end
@@ -757,9 +764,10 @@ __global__ __launch_bounds__(Waves * 64, D == 64 ? 4 : 2) void paged_attention_k
         const float weight = __builtin_amdgcn_exp2f(fmaf(largest, factor, -base)) * own_scale;
         const int weight_bits = seen > 0 ? __float_as_int(weight) & 0x7fffffff : 0;
         const int top = over_chunks(over_row<S>(max(weight_bits, scale_bits - (40 << 23)), most_of), most_of);
-        const int e = __builtin_amdgcn_frexp_expf(__int_as_float(max(top, 0)));
+        const int e = unit_exponent(max(top, 0), kLeastWhole);
         const float to_whole = top < 0x7f800000 && seen > 0 ? ldexpf(own_scale, 30 - e) : 0.f;
-        const float from_whole = top < 0x7f800000 ? ldexpf(1.f, e - 30) : NAN;
+        // with the unit of the column's digits, so that the sums are never smaller than what they stand for
+        const float from_whole = top < 0x7f800000 ? ldexpf(sub_unit, e - 30) : NAN;
         float sum = 0.f;
         v4i weights[J];
 #pragma unroll
@@ -824,7 +832,7 @@ __global__ __launch_bounds__(Waves * 64, D == 64 ? 4 : 2) void paged_attention_k
         ls[wave][column / S] = l;
     }
 #pragma unroll
-    for (int d = 0; d < D / 4; ++d) o[d] = over_row<S>(o[d] * sub_unit, sum_of);
+    for (int d = 0; d < D / 4; ++d) o[d] = over_row<S>(o[d], sum_of);
     if (sub == 0)
 #pragma unroll
         for (int n = 0; n < D / 16; ++n)
@@ -959,11 +967,11 @@ __global__ __launch_bounds__(Waves * 64, D == 64 ? 4 : 2) void paged_single_kern
             }
     }
     const int shift = 8 * (digit & 1);
-    const float pair_unit = digit & 2 ? 65536.f : 1.f;
+    const float pair_unit = digit & 2 ? 65536.f : 1.f, digit_unit = pair_unit * (digit & 1 ? 256.f : 1.f);
     const uint32_t first_bytes = digit & 1 ? 0x03070105u : 0x06020400u, second_bytes = digit & 2 ? 0x03020706u : 0x05040100u;
 
     float m = -INFINITY, l = 0.f;  // l is the lane's own
-    float o[D / 4] = {};           // of the column's digit
+    float o[D / 4] = {};           // what the column's digit adds
     v4i acc[D / 16] = {};          // since the last change of the unit
     int top = 0, blocks = 0;       // the largest weight times its value scale, as bits, so that NaN is the largest of all
     int to_whole = 0;              // the exponent that a weight takes to its units
@@ -1023,9 +1031,9 @@ __global__ __launch_bounds__(Waves * 64, D == 64 ? 4 : 2) void paged_single_kern
 #pragma unroll
             for (int d = 32; d > 0; d /= 2) next = max(next, __shfl_xor(next, d));
             top = max(top, next);
-            const int e = __builtin_amdgcn_frexp_expf(__int_as_float(top));
-            to_whole = 30 - e;  // to 178: as a factor it would be infinite for weighted scales below 2^-98
-            from_whole = top < 0x7f800000 ? ldexpf(1.f, e - 30) : NAN;
+            const int e = unit_exponent(top, kLeastWhole);
+            to_whole = 30 - e;  // to 149: as a factor it would be infinite for weighted scales below 2^-98
+            from_whole = top < 0x7f800000 ? ldexpf(digit_unit, e - 30) : NAN;
         }
         ++blocks;
         // from 2^23 on an f32 is whole: the bias rounds the weight too, to half a unit or its own last bit
@@ -1046,10 +1054,9 @@ __global__ __launch_bounds__(Waves * 64, D == 64 ? 4 : 2) void paged_single_kern
         ms[wave] = m;
         ls[wave] = l;
     }
-    const float digit_unit = pair_unit * (digit & 1 ? 256.f : 1.f);
 #pragma unroll
     for (int i = 0; i < D / 4; ++i) {
-        float x = o[i] * digit_unit;
+        float x = o[i];
         x += __int_as_float(in_quad<kNextLane>(__float_as_int(x)));
         x += __int_as_float(in_quad<kOtherPair>(__float_as_int(x)));
         o[i] = x;
@@ -1349,7 +1356,7 @@ __global__ __launch_bounds__(G * kPromptWaves * 64, 2) void paged_prompt_kernel(
         if (__any(largest > m || scale_bits > top)) {
             const float next = fmaxf(m, chunks_max(largest));
             const int next_top = max(top, over_chunks(scale_bits, [](int a, int b) { return max(a, b); }));
-            const int next_exponent = __builtin_amdgcn_frexp_expf(__int_as_float(next_top));
+            const int next_exponent = unit_exponent(next_top, kLeastHalf);
             const float alpha = __builtin_amdgcn_exp2f(m - (next == -INFINITY ? 0.f : next));
             const float again = ldexpf(alpha, top_exponent - next_exponent);
             l *= alpha;

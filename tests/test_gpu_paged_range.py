@@ -13,6 +13,21 @@ pytestmark = pytest.mark.gpu
 ROWS = [1, 3, 40]  # new tokens of a sequence, one kernel each
 
 
+def sums_of_weights(cache, starts, lengths, q, scale):
+    """Each row's sum of weights, in units of the largest, [tokens, heads, 1]."""
+    total = np.ones((*q.shape[:2], 1))
+    group = q.shape[1] // cache.kv_heads
+    for s, length in enumerate(lengths):
+        n = starts[s + 1] - starts[s]
+        for h in range(q.shape[1]):
+            k, _, there = paged.values_of(cache, s, h // group, length)
+            for i in range(n):
+                seen = there & (np.arange(length) <= length - n + i)
+                score = k[seen] @ q[starts[s] + i, h].astype(np.float64) * scale
+                total[starts[s] + i, h] = np.exp(score - score.max()).sum()
+    return total
+
+
 @pytest.mark.parametrize("split", [False, True], ids=["whole", "parts"])
 @pytest.mark.parametrize("new", ROWS)
 @pytest.mark.parametrize("dim", [64, 128])
@@ -32,3 +47,25 @@ def test_attention_of_tiny_values(kdb, size, dim, new, split):
     got = run_attention(kdb, on, q, dim ** -0.5, keys, workspace_for(kdb, q.shape[1], 1, dim, 1, tokens, 1 << 20))
     off = np.abs(got - want)
     assert (off <= tolerance).all(), (off / tolerance).max()
+
+
+@pytest.mark.parametrize("keys", [300, 3000])  # in one launch and in parts
+@pytest.mark.parametrize("new", ROWS)
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("size", [1e-33, 1e-35, 1e-37, 1e-39])
+def test_attention_of_values_near_the_least(kdb, size, dim, new, keys):
+    """Value scales around 2^-117, 2^-123, 2^-130 and 2^-137, the last two below the least normal number. A weight in
+    units of 2^-149 is off by half a unit, so the sums of n keys by n * 127 * 2^-150, divided by the weights' sum, beside the
+    definition's tolerance and 16 roundings to multiples of 2^-149."""
+    rng = np.random.default_rng(22)
+    starts, lengths, tokens = batch_of([new], [keys])
+    cache = paged.Cache(rng, 1, -(-keys // 64), 1, 64, dim)
+    cache.value_scales = (cache.value_scales * np.float64(size)).astype(np.float32)
+    q = rng.normal(0, 1, (tokens, 1, dim)).astype(np.float32)
+    on = paged.Device(kdb, cache, starts, lengths, tokens)
+    want, tolerance = paged.attention(cache, starts, lengths, q, dim ** -0.5)
+    tolerance = tolerance + keys * 127 * 2.0 ** -150 / sums_of_weights(cache, starts, lengths, q, dim ** -0.5) + 16 * 2.0 ** -150
+    got = run_attention(kdb, on, q, dim ** -0.5, keys, workspace_for(kdb, 1, 1, dim, 1, tokens, 1 << 20))
+    off = np.abs(got - want)
+    assert (off <= tolerance).all(), (off / tolerance).max()
+    assert (tolerance < 0.1 * np.abs(want).max()).all()  # a sum that is lost is seen
