@@ -538,6 +538,8 @@ template <int U> __device__ __forceinline__ float query_digits(float (&features)
 // The exponent e of the largest of a row's weighted value scales, whose bits are `top`, at least `least`: 2^(e - 30) is the unit of
 // whole weights and 2^(e - 15) that of f16 ones, and neither may fall below f32's least number.
 constexpr int kLeastWhole = 30 - 149, kLeastHalf = 15 - 149;
+// The unit is not below that of 2^-96 of the largest value scale, so that the scale in units stays finite.
+constexpr int kFarBelow = 96 << 23;
 __device__ __forceinline__ int unit_exponent(int top, int least) {
     return max(__builtin_amdgcn_frexp_expf(__int_as_float(top)), least);
 }
@@ -759,11 +761,11 @@ __global__ __launch_bounds__(Waves * 64, D == 64 ? 4 : 2) void paged_attention_k
         const float base = next == -INFINITY ? 0.f : next;  // nothing seen yet: every weight below is 0
         const float alpha = __builtin_amdgcn_exp2f(m - base);
         m = next;
-        // The unit of the weights times their value scales: the largest of them that the row has here, as bits, so that NaN is the
-        // largest of all, but not below 2^-40 of the largest scale, so that the scale in units stays finite.
+        // the unit of the weights times their value scales: the largest of them that the row has here, as bits, so that NaN is the
+        // largest of all
         const float weight = __builtin_amdgcn_exp2f(fmaf(largest, factor, -base)) * own_scale;
         const int weight_bits = seen > 0 ? __float_as_int(weight) & 0x7fffffff : 0;
-        const int top = over_chunks(over_row<S>(max(weight_bits, scale_bits - (40 << 23)), most_of), most_of);
+        const int top = over_chunks(over_row<S>(max(weight_bits, scale_bits - kFarBelow), most_of), most_of);
         const int e = unit_exponent(max(top, 0), kLeastWhole);
         const float to_whole = top < 0x7f800000 && seen > 0 ? ldexpf(own_scale, 30 - e) : 0.f;
         // with the unit of the column's digits, so that the sums are never smaller than what they stand for
@@ -1097,8 +1099,8 @@ __global__ __launch_bounds__(Waves * 64, D == 64 ? 4 : 2) void paged_single_kern
 // other block: a wave alone on its SIMD takes 1.05 us for a block of 64 features, two of them 1.5 for both.
 // What bounds it is the vector ALU, 30 operations a score in the kernel above, seven of which join the digits' sums of the
 // outputs; here the weighted sums run on the f16 matrix cores into f32, which joins nothing: a code is an f16 value as it stands,
-// converted once for the four waves, and a weight two f16 pieces (2^-24 of it), scaled so that the largest is 2^15 and pieces
-// below 2^-24 are below 2^-39 of that. 2 prompts of up to 4096, 32 heads over 8 of 128: 422 us, 480 TFLOP/s of the formula's
+// converted once for the four waves, and a weight times its value scale two f16 pieces (2^-23 of it), scaled so that the
+// largest that the row has is 2^15 and pieces below 2^-24 are below 2^-39 of that. 2 prompts of up to 4096, 32 heads over 8 of 128: 422 us, 480 TFLOP/s of the formula's
 // products, VALU busy 0.74 and matrix cores 0.43 of the cycles; 8 of up to 1000, 12 heads of 64: 31 us; 4 x 4096 of 64: VALU busy
 // 0.95.
 typedef _Float16 v8h __attribute__((ext_vector_type(8)));
@@ -1287,7 +1289,8 @@ __global__ __launch_bounds__(G * kPromptWaves * 64, 2) void paged_prompt_kernel(
 
     float m = -INFINITY, l = 0.f;
     v4f o[D / 16] = {};  // in units of 2^(top_exponent - 15)
-    // the largest value scale that the row has seen, as bits, so that NaN is the largest of all, and its exponent
+    // the largest weight times its value scale that the row has seen, in units of its maximum, as bits, so that NaN is the
+    // largest of all, and its exponent
     int top = 0, top_exponent = 0;
     const auto work = [&](int key, const Scales& own, const v4i (*block)[64]) {
         float x[16];
@@ -1353,20 +1356,26 @@ __global__ __launch_bounds__(G * kPromptWaves * 64, 2) void paged_prompt_kernel(
         for (int i = 1; i < 16; ++i) largest = fmaxf(largest, x[i]);
         largest *= factor;
         const int scale_bits = seen > 0 ? __float_as_int(own.value) & 0x7fffffff : 0;
-        if (__any(largest > m || scale_bits > top)) {
+        const bool higher = __any(largest > m);
+        float alpha = 1.f;
+        if (higher) {
             const float next = fmaxf(m, chunks_max(largest));
-            const int next_top = max(top, over_chunks(scale_bits, [](int a, int b) { return max(a, b); }));
-            const int next_exponent = unit_exponent(next_top, kLeastHalf);
-            const float alpha = __builtin_amdgcn_exp2f(m - (next == -INFINITY ? 0.f : next));
-            const float again = ldexpf(alpha, top_exponent - next_exponent);
+            alpha = __builtin_amdgcn_exp2f(m - (next == -INFINITY ? 0.f : next));
             l *= alpha;
-#pragma unroll
-            for (int n = 0; n < D / 16; ++n) o[n] *= again;
             m = next;
-            top = next_top;
-            top_exponent = next_exponent;
+            top = __float_as_int(__int_as_float(top) * alpha) & 0x7fffffff;
         }
         const float base = m == -INFINITY ? 0.f : m;  // nothing seen yet: every weight below is 0
+        const float weight = __builtin_amdgcn_exp2f(largest - base) * own.value;
+        const int weight_bits = seen > 0 ? max(__float_as_int(weight) & 0x7fffffff, scale_bits - kFarBelow) : 0;
+        if (higher || __any(weight_bits > top)) {
+            top = max(top, over_chunks(weight_bits, [](int a, int b) { return max(a, b); }));
+            const int next_exponent = unit_exponent(top, kLeastHalf);
+            const float again = ldexpf(alpha, top_exponent - next_exponent);
+#pragma unroll
+            for (int n = 0; n < D / 16; ++n) o[n] *= again;
+            top_exponent = next_exponent;
+        }
         // the scale multiplies the weight rather than going into the exponent, whose rounding would differ from chunk to chunk
         const float to_units = top < 0x7f800000 && seen > 0 ? ldexpf(own.value, 15 - top_exponent) : 0.f;
         float sum = 0.f;

@@ -1,5 +1,5 @@
-"""kd_paged_attention at the ends of f32's range: values of tiny size. Against the definition in 64 bits
-(tests/paged.py).
+"""kd_paged_attention at the ends of f32's range: values of tiny size, pages whose values are far larger than the others'.
+Against the definition in 64 bits (tests/paged.py).
 """
 import numpy as np
 import pytest
@@ -69,3 +69,32 @@ def test_attention_of_values_near_the_least(kdb, size, dim, new, keys):
     off = np.abs(got - want)
     assert (off <= tolerance).all(), (off / tolerance).max()
     assert (tolerance < 0.1 * np.abs(want).max()).all()  # a sum that is lost is seen
+
+
+@pytest.mark.parametrize("new", ROWS)
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("ratio", [24, 40, 60, 90])
+def test_attention_beside_values_of_any_size(kdb, dim, new, ratio):
+    """One page's values are 2^ratio times the others', its keys' weights 2^-ratio / 8000: the error follows what the rows sum
+    up. The definition's tolerance, with the weighted mean of |v| in place of its largest. The page comes first, in the middle
+    and last."""
+    rng = np.random.default_rng(23)
+    starts, lengths, tokens = batch_of([new], [500])
+    for column in (0, 12, 29):
+        cache = paged.Cache(rng, 1, 32, 1, 16, dim)
+        far = cache.table[0, column]
+        cache.keys[far] = -127
+        cache.key_scales[far] = (np.log(2.0) * ratio + 9) / (127 * dim ** 0.5)
+        cache.value_scales[far] = 0.0175 * 2.0 ** ratio
+        q = (1 + 0.1 * rng.normal(0, 1, (tokens, 1, dim))).astype(np.float32)
+        on = paged.Device(kdb, cache, starts, lengths, tokens)
+        want, tolerance = paged.attention(cache, starts, lengths, q, dim ** -0.5)
+        k, v, _ = paged.values_of(cache, 0, 0, 500)
+        for i in range(tokens):
+            seen = 500 - new + i + 1
+            score = k[:seen] @ q[i, 0].astype(np.float64) * dim ** -0.5
+            p = np.exp(score - score.max())
+            tolerance[i] *= (p @ np.abs(v[:seen]) / p.sum()).max() / np.abs(v[:seen]).max()
+        got = run_attention(kdb, on, q, dim ** -0.5, 500)
+        off = np.abs(got - want)
+        assert (off <= tolerance).all(), (column, (off / tolerance).max())
