@@ -544,6 +544,11 @@ __device__ __forceinline__ int unit_exponent(int top, int least) {
     return max(__builtin_amdgcn_frexp_expf(__int_as_float(top)), least);
 }
 
+// A row's maximum is a rounded product, and a weight's exponent the fused product less that maximum: the largest weight is
+// 2^(that rounding), 2^(1/16) at most for maxima below this. From here on the products are rounded ahead of the subtraction, so
+// that it is 1 again and none is larger.
+constexpr float kFarScore = 0x1p20f;
+
 struct Split {
     int count;    // parts that a row's keys are split into
     int part;     // keys of a part, a multiple of 64; the last part goes to the end
@@ -761,6 +766,12 @@ __global__ __launch_bounds__(Waves * 64, D == 64 ? 4 : 2) void paged_attention_k
         const float base = next == -INFINITY ? 0.f : next;  // nothing seen yet: every weight below is 0
         const float alpha = __builtin_amdgcn_exp2f(m - base);
         m = next;
+        if (__any(fabsf(base) >= kFarScore)) {
+#pragma unroll
+            for (int i = 0; i < 4 * J; ++i) x[i] *= factor;
+            largest *= factor;
+            factor = 1.f;
+        }
         // the unit of the weights times their value scales: the largest of them that the row has here, as bits, so that NaN is the
         // largest of all
         const float weight = __builtin_amdgcn_exp2f(fmaf(largest, factor, -base)) * own_scale;
@@ -1375,6 +1386,11 @@ __global__ __launch_bounds__(G * kPromptWaves * 64, 2) void paged_prompt_kernel(
 #pragma unroll
             for (int n = 0; n < D / 16; ++n) o[n] *= again;
             top_exponent = next_exponent;
+        }
+        if (__any(fabsf(base) >= kFarScore)) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) x[i] *= factor;
+            factor = 1.f;
         }
         // the scale multiplies the weight rather than going into the exponent, whose rounding would differ from chunk to chunk
         const float to_units = top < 0x7f800000 && seen > 0 ? ldexpf(own.value, 15 - top_exponent) : 0.f;

@@ -1,5 +1,5 @@
-"""kd_paged_attention at the ends of f32's range: values of tiny size, pages whose values are far larger than the others'.
-Against the definition in 64 bits (tests/paged.py).
+"""kd_paged_attention at the ends of f32's range: values of tiny size, pages whose values are far larger than the others',
+scores that f32 holds to no better than many units. Against the definition in 64 bits (tests/paged.py).
 """
 import numpy as np
 import pytest
@@ -98,3 +98,32 @@ def test_attention_beside_values_of_any_size(kdb, dim, new, ratio):
         got = run_attention(kdb, on, q, dim ** -0.5, 500)
         off = np.abs(got - want)
         assert (off <= tolerance).all(), (column, (off / tolerance).max())
+
+
+@pytest.mark.parametrize("new", ROWS)
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("size", [2.0 ** 21, 2.0 ** 25, 2.0 ** 33, -2.0 ** 33, 2.0 ** 60, 2.0 ** 110])
+def test_attention_of_scores_far_from_zero(kdb, size, dim, new):
+    """Scores of 2^21 to 2^110 in size: the largest has the whole weight, and the row is its key's values. Their weighted sum is exact
+    but for the unit's pieces (2^-22) and the quotient, the joins of waves multiply by 1: 2^-20 of the value."""
+    rng = np.random.default_rng(24)
+    keys = 700
+    starts, lengths, tokens = batch_of([new], [keys])
+    cache = paged.Cache(rng, 1, 44, 1, 16, dim)
+    q = rng.normal(0, 1, (tokens, 1, dim)).astype(np.float32)
+    k, v, _ = paged.values_of(cache, 0, 0, keys)
+    unit = np.abs(k @ q[:, 0].T.astype(np.float64)).max(0)  # scores of about 1 by it
+    q = (q / unit[:, None, None] * np.sqrt(abs(size))).astype(np.float32)
+    scale = float(np.sign(size) * np.sqrt(abs(size)))
+    on = paged.Device(kdb, cache, starts, lengths, tokens)
+    got = run_attention(kdb, on, q, scale, keys)
+    compared = 0
+    for i in range(tokens):
+        score = k[:keys - new + i + 1] @ q[i, 0].astype(np.float64) * scale
+        order = np.argsort(score)
+        if score[order[-1]] - score[order[-2]] < max(2.0 ** -16 * np.abs(score).max(), 40):
+            continue  # the roundings of the scores decide between the two
+        compared += 1
+        want = v[order[-1]]
+        assert (np.abs(got[i, 0] - want) <= 2.0 ** -20 * np.abs(want)).all(), (i, score[order[-1]])
+    assert compared >= 0.8 * tokens
