@@ -549,6 +549,13 @@ __device__ __forceinline__ int unit_exponent(int top, int least) {
 // that it is 1 again and none is larger.
 constexpr float kFarScore = 0x1p20f;
 
+// What a row's factor and a key's scale make of a score's whole number. Infinity is NaN: times a number below 0 it would be
+// -infinity, a weight of nothing.
+__device__ __forceinline__ float score_factor(float query, float key_scale) {
+    const float factor = query * key_scale;
+    return factor < INFINITY ? factor : NAN;
+}
+
 struct Split {
     int count;    // parts that a row's keys are split into
     int part;     // keys of a part, a multiple of 64; the last part goes to the end
@@ -751,7 +758,7 @@ __global__ __launch_bounds__(Waves * 64, D == 64 ? 4 : 2) void paged_attention_k
         const int scale_bits = seen > 0 ? __float_as_int(value_scale) & 0x7fffffff : 0;
         const float own_scale = value_scale;
         // never 0, so that a masked key's -inf stays what it is
-        float factor = q_factor * key_scale;
+        float factor = score_factor(q_factor, key_scale);
         factor = factor == 0.f ? 0x1p-126f : factor;
         if (key + kKeyBlock > least || __any(page < 0)) {
             factor = seen > 0 ? factor : 1.f;  // nor NaN where the row sees none of them
@@ -1020,7 +1027,7 @@ __global__ __launch_bounds__(Waves * 64, D == 64 ? 4 : 2) void paged_single_kern
                             __int_as_float(in_quad<kOtherPair>(__float_as_int(static_cast<float>(sent) * pair_unit)));
         const bool seen = page >= 0 && key + lane < to;
         const float own_scale = seen ? value_scale : 0.f;
-        const float x = seen ? whole * (q_factor * key_scale) : -INFINITY;
+        const float x = seen ? whole * score_factor(q_factor, key_scale) : -INFINITY;
         load_keys(key + step < to ? key + step : key);  // the last block once more rather than a branch
         if (__any(x > m)) {
             float next = x;
@@ -1355,7 +1362,7 @@ __global__ __launch_bounds__(G * kPromptWaves * 64, 2) void paged_prompt_kernel(
             }
         }
         const int seen = own.page < 0 ? 0 : limit - (key + 16 * chunk);
-        float factor = q_factor * own.key;
+        float factor = score_factor(q_factor, own.key);
         factor = factor == 0.f ? 0x1p-126f : factor;
         if (key + kKeyBlock > least || __any(own.page < 0)) {
             factor = seen > 0 ? factor : 1.f;

@@ -1,5 +1,6 @@
 """kd_paged_attention at the ends of f32's range: values of tiny size, pages whose values are far larger than the others',
-scores that f32 holds to no better than many units. Against the definition in 64 bits (tests/paged.py).
+scores that f32 holds to no better than many units, key scales that are not finite. Against the definition in 64 bits
+(tests/paged.py).
 """
 import numpy as np
 import pytest
@@ -127,3 +128,24 @@ def test_attention_of_scores_far_from_zero(kdb, size, dim, new):
         want = v[order[-1]]
         assert (np.abs(got[i, 0] - want) <= 2.0 ** -20 * np.abs(want)).all(), (i, score[order[-1]])
     assert compared >= 0.8 * tokens
+
+
+@pytest.mark.parametrize("new", ROWS)
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("which", [np.inf, np.nan])
+def test_a_key_scale_that_is_not_finite_gives_nan(kdb, which, dim, new):
+    """Also where the page's scores would all be -inf, whose weights are nothing."""
+    rng = np.random.default_rng(25)
+    starts, lengths, tokens = batch_of([new, new], [300, 300])
+    cache = paged.Cache(rng, 2, 19, 1, 16, dim)
+    cache.keys[cache.table[0, 4]] = -1
+    cache.key_scales[cache.table[0, 4]] = which
+    cache.key_scales[cache.table[1, 18]] = which
+    lengths = [300, 280]  # the second sequence's page is not seen
+    q = np.abs(rng.normal(0, 1, (tokens, 1, dim))).astype(np.float32)
+    on = paged.Device(kdb, cache, starts, lengths, tokens)
+    got = run_attention(kdb, on, q, dim ** -0.5, 300)
+    assert np.isnan(got[:new]).all()
+    with np.errstate(invalid="ignore"):
+        want, tolerance = paged.attention(cache, starts, lengths, np.where(np.arange(tokens)[:, None, None] < new, 0, q), dim ** -0.5)
+    assert (np.abs(got - want) <= tolerance)[new:].all()
