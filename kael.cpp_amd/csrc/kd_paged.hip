@@ -536,8 +536,8 @@ template <int U> __device__ __forceinline__ float query_digits(float (&features)
 }
 
 // The exponent e of the largest of a row's weighted value scales, whose bits are `top`, at least `least`: 2^(e - 30) is the unit of
-// whole weights and 2^(e - 15) that of f16 ones, and neither may fall below f32's least number.
-constexpr int kLeastWhole = 30 - 149, kLeastHalf = 15 - 149;
+// whole weights and 2^(e - 13) that of f16 ones, and neither may fall below f32's least number.
+constexpr int kLeastWhole = 30 - 149, kLeastHalf = 13 - 149;
 // The unit is not below that of 2^-96 of the largest value scale, so that the scale in units stays finite.
 constexpr int kFarBelow = 96 << 23;
 __device__ __forceinline__ int unit_exponent(int top, int least) {
@@ -548,6 +548,10 @@ __device__ __forceinline__ int unit_exponent(int top, int least) {
 // 2^(that rounding), 2^(1/16) at most for maxima below this. From here on the products are rounded ahead of the subtraction, so
 // that it is 1 again and none is larger.
 constexpr float kFarScore = 0x1p20f;
+__device__ __forceinline__ float rounded_product(float a, float b) {
+#pragma clang fp contract(off)
+    return a * b;
+}
 
 // What a row's factor and a key's scale make of a score's whole number. Infinity is NaN: times a number below 0 it would be
 // -infinity, a weight of nothing.
@@ -773,10 +777,12 @@ __global__ __launch_bounds__(Waves * 64, D == 64 ? 4 : 2) void paged_attention_k
         const float base = next == -INFINITY ? 0.f : next;  // nothing seen yet: every weight below is 0
         const float alpha = __builtin_amdgcn_exp2f(m - base);
         m = next;
-        if (__any(fabsf(base) >= kFarScore)) {
+        // Heads of 64 with several columns a row: always, where the branch would spill four registers (32 x 5 x 2000 keys 19.0 us, with
+        // the branch 20.6; of 128, 4 x 40000 of 4 rows 48.6 / 47.0).
+        if ((D == 64 && S > 1) || __any(fabsf(base) >= kFarScore)) {
 #pragma unroll
-            for (int i = 0; i < 4 * J; ++i) x[i] *= factor;
-            largest *= factor;
+            for (int i = 0; i < 4 * J; ++i) x[i] = rounded_product(x[i], factor);
+            largest = rounded_product(largest, factor);
             factor = 1.f;
         }
         // the unit of the weights times their value scales: the largest of them that the row has here, as bits, so that NaN is the
@@ -1027,7 +1033,7 @@ __global__ __launch_bounds__(Waves * 64, D == 64 ? 4 : 2) void paged_single_kern
                             __int_as_float(in_quad<kOtherPair>(__float_as_int(static_cast<float>(sent) * pair_unit)));
         const bool seen = page >= 0 && key + lane < to;
         const float own_scale = seen ? value_scale : 0.f;
-        const float x = seen ? whole * score_factor(q_factor, key_scale) : -INFINITY;
+        const float x = seen ? rounded_product(whole, score_factor(q_factor, key_scale)) : -INFINITY;
         load_keys(key + step < to ? key + step : key);  // the last block once more rather than a branch
         if (__any(x > m)) {
             float next = x;
@@ -1118,7 +1124,7 @@ __global__ __launch_bounds__(Waves * 64, D == 64 ? 4 : 2) void paged_single_kern
 // What bounds it is the vector ALU, 30 operations a score in the kernel above, seven of which join the digits' sums of the
 // outputs; here the weighted sums run on the f16 matrix cores into f32, which joins nothing: a code is an f16 value as it stands,
 // converted once for the four waves, and a weight times its value scale two f16 pieces (2^-23 of it), scaled so that the
-// largest that the row has is 2^15 and pieces below 2^-24 are below 2^-39 of that. 2 prompts of up to 4096, 32 heads over 8 of 128: 422 us, 480 TFLOP/s of the formula's
+// largest that the row has is 2^13 and pieces below 2^-24 are below 2^-36 of that. 2 prompts of up to 4096, 32 heads over 8 of 128: 422 us, 480 TFLOP/s of the formula's
 // products, VALU busy 0.74 and matrix cores 0.43 of the cycles; 8 of up to 1000, 12 heads of 64: 31 us; 4 x 4096 of 64: VALU busy
 // 0.95.
 typedef _Float16 v8h __attribute__((ext_vector_type(8)));
@@ -1306,10 +1312,10 @@ __global__ __launch_bounds__(G * kPromptWaves * 64, 2) void paged_prompt_kernel(
     else q_factor = query_digits(features, real, scale, digits);
 
     float m = -INFINITY, l = 0.f;
-    v4f o[D / 16] = {};  // in units of 2^(top_exponent - 15)
+    v4f o[D / 16] = {};  // in units of 2^(top_exponent - 13)
     // the largest weight times its value scale that the row has seen, in units of its maximum, as bits, so that NaN is the
     // largest of all, and its exponent
-    int top = 0, top_exponent = 0;
+    int top = 0, top_exponent = 0, scale_limit = 0;
     const auto work = [&](int key, const Scales& own, const v4i (*block)[64]) {
         float x[16];
         // Heads of 64: pieces are read four at a time ahead of their use, where the scheduler would put them right before it.
@@ -1374,33 +1380,31 @@ __global__ __launch_bounds__(G * kPromptWaves * 64, 2) void paged_prompt_kernel(
         for (int i = 1; i < 16; ++i) largest = fmaxf(largest, x[i]);
         largest *= factor;
         const int scale_bits = seen > 0 ? __float_as_int(own.value) & 0x7fffffff : 0;
-        const bool higher = __any(largest > m);
-        float alpha = 1.f;
-        if (higher) {
-            const float next = fmaxf(m, chunks_max(largest));
-            alpha = __builtin_amdgcn_exp2f(m - (next == -INFINITY ? 0.f : next));
+        // A scale of up to four units' largest weight fits whatever its weight; a larger one only if its weight makes it so, and where
+        // that is looked at the unit goes by the weights: one page of far larger values takes no bits from the others.
+        if (__any(largest > m || scale_bits > scale_limit)) {
+            const float next = fmaxf(m, chunks_max(largest)), to = next == -INFINITY ? 0.f : next;
+            const float alpha = __builtin_amdgcn_exp2f(m - to);
             l *= alpha;
             m = next;
-            top = __float_as_int(__int_as_float(top) * alpha) & 0x7fffffff;
-        }
-        const float base = m == -INFINITY ? 0.f : m;  // nothing seen yet: every weight below is 0
-        const float weight = __builtin_amdgcn_exp2f(largest - base) * own.value;
-        const int weight_bits = seen > 0 ? max(__float_as_int(weight) & 0x7fffffff, scale_bits - kFarBelow) : 0;
-        if (higher || __any(weight_bits > top)) {
-            top = max(top, over_chunks(weight_bits, [](int a, int b) { return max(a, b); }));
+            const int weight_bits = __float_as_int(__builtin_amdgcn_exp2f(largest - to) * own.value) & 0x7fffffff;
+            top = max(__float_as_int(__int_as_float(top) * alpha) & 0x7fffffff,
+                      over_chunks(seen > 0 ? max(weight_bits, scale_bits - kFarBelow) : 0, [](int a, int b) { return max(a, b); }));
             const int next_exponent = unit_exponent(top, kLeastHalf);
             const float again = ldexpf(alpha, top_exponent - next_exponent);
 #pragma unroll
             for (int n = 0; n < D / 16; ++n) o[n] *= again;
             top_exponent = next_exponent;
+            scale_limit = __float_as_int(ldexpf(4.f, top_exponent));
         }
+        const float base = m == -INFINITY ? 0.f : m;  // nothing seen yet: every weight below is 0
         if (__any(fabsf(base) >= kFarScore)) {
 #pragma unroll
-            for (int i = 0; i < 16; ++i) x[i] *= factor;
+            for (int i = 0; i < 16; ++i) x[i] = rounded_product(x[i], factor);
             factor = 1.f;
         }
         // the scale multiplies the weight rather than going into the exponent, whose rounding would differ from chunk to chunk
-        const float to_units = top < 0x7f800000 && seen > 0 ? ldexpf(own.value, 15 - top_exponent) : 0.f;
+        const float to_units = top < 0x7f800000 && seen > 0 ? ldexpf(own.value, 13 - top_exponent) : 0.f;
         float sum = 0.f;
         v8h high[2], low[2];
 #pragma unroll
@@ -1455,7 +1459,7 @@ __global__ __launch_bounds__(G * kPromptWaves * 64, 2) void paged_prompt_kernel(
         }
     }
     l = chunks_sum(l);
-    const float unit = top < 0x7f800000 ? ldexpf(1.f, top_exponent - 15) : NAN;
+    const float unit = top < 0x7f800000 ? ldexpf(1.f, top_exponent - 13) : NAN;
     if (chunk == 0) {
         ms[any_wave][column] = m;
         ls[any_wave][column] = l;
