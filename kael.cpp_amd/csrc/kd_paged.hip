@@ -393,9 +393,10 @@ __global__ __launch_bounds__(256) void paged_read_kernel(Paged c, float* __restr
     if (p.s < 0) return;
     const int64_t row_size = static_cast<int64_t>(c.kv_heads) * dim;
     out += h * dim;
-    const auto clear = [&](int row, int count) {
-        for (int i = threadIdx.x; i < count * (dim / 4); i += threads)
-            *reinterpret_cast<float4*>(out + (row + i / (dim / 4)) * row_size + i % (dim / 4) * 4) = make_float4(0, 0, 0, 0);
+    const auto clear = [&](int row, int count) {  // of any number of rows: 2^27 have 2^31 pieces
+        const int shift = dim == 64 ? 4 : 5;
+        for (int64_t i = threadIdx.x; i < int64_t{count} << shift; i += threads)
+            *reinterpret_cast<float4*>(out + (row + (i >> shift)) * row_size + (i & ((1 << shift) - 1)) * 4) = make_float4(0, 0, 0, 0);
     };
     // rows before position 0 have no page
     if (p.leads && p.rows.position < 0) clear(p.rows.row, static_cast<int>(min(int64_t{p.rows.count}, -p.rows.position)));

@@ -211,6 +211,27 @@ def test_read_gives_the_values(kdb, page, dim):
             np.testing.assert_array_equal(got[n].numpy(), np.full_like(want[n], -777) if n == skipped else want[n])
 
 
+def test_read_of_more_rows_below_position_zero_than_31_bits_count(kdb):
+    """2^27 rows without a position, 2^31 pieces of 16 bytes of keys (34 GB): all of them 0, and the rows behind them the values."""
+    rng = np.random.default_rng(20)
+    below, held = (1 << 27) + 3, 20
+    cache = paged.Cache(rng, 1, 1, 1, 256, 64)
+    on = paged.Device(kdb, cache, [0, below + held], [held], below + held)
+    out = kdb.empty((below + held, 64), np.float32)
+    kdb.call("fill", kd.F32, out.ptr, out.shape[0] * 64, ctypes.byref(ctypes.c_float(-777)))
+    kdb.call("paged_read", kd.F32, out.ptr, None, on.c, on.b)
+    for op in (kd.REDUCE_MIN, kd.REDUCE_MAX):  # of 1024 rows each, and of the last three
+        ends = kdb.empty((1 << 17,), np.float32)
+        kdb.call("reduce", op, kd.F32, kd.F32, ends.ptr, out.ptr, 64 << 10, 1 << 17)
+        assert (ends.numpy() == 0).all()
+        kdb.call("reduce", op, kd.F32, kd.F32, ends.ptr, out.ptr + (256 << 27), 3 * 64, 1)
+        assert ends.numpy()[0] == 0
+    rest = np.empty((held, 64), np.float32)
+    kdb.check(kdb.lib.kd_copy_d2h(rest.ctypes.data_as(ctypes.c_void_p), ctypes.c_void_p(out.ptr + below * 256), rest.nbytes), "kd_copy_d2h")
+    at = cache.table[0, 0]
+    np.testing.assert_array_equal(rest, cache.keys[at, 0, :held] * cache.key_scales[at, 0])
+
+
 @pytest.mark.parametrize("dim,page", [(64, 16), (128, 64)])
 def test_large_appends_and_reads_are_those_of_their_parts(kdb, dim, page):
     """Rows of more than 32 MiB, which go past the caches: the same bits as sequence by sequence."""
