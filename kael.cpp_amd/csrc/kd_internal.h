@@ -38,13 +38,26 @@ int compute_units();
 // Whether a launch of `groups` workgroups in x is one: its work items are counted in 32 bits.
 inline bool fits_grid(int64_t groups, int64_t threads) { return groups < (int64_t{1} << 32) / threads; }
 
+// Who used a buffer last that calls on any stream share; its owner's lock is held around both. `wait` goes ahead of a use and
+// `record` behind it: a use on another stream than the one before waits for that use's event, and not for its stream, which
+// may be gone by then. A stream that kd_set_stream was given since may be another one at the same address, so it waits
+// too. Kernels that a capture takes up run when their graph does, and nothing waits for those.
+struct LastUse {
+    int wait(hipStream_t current);
+    void record(hipStream_t current);
+    int drain();  // of the host, for what the buffer was last used for on a stream of the caller's
+    hipStream_t stream = nullptr;
+    uint64_t turn = 0;  // kd_set_stream calls ahead of that use
+    hipEvent_t done = nullptr;
+    bool used = false;
+};
+
 // A lease on the per-device workspace (scratch for split reductions and split-K partials,
 // grown on demand, never shrunk). The lease holds the workspace lock from `workspace()` until
 // it is destroyed, so a caller keeps it alive until every kernel that touches `ptr` has been
 // enqueued: calls from several host threads then use the buffer one after another in stream
 // order, and a growth (which frees the old block) never frees a block that a caller is about to
-// hand to a kernel. When the backend stream differs from the one the previous lease used, it waits
-// for that lease's event first, so leases on different streams never overlap either.
+// hand to a kernel. Leases on different streams wait for each other (LastUse), so they never overlap either.
 struct Workspace {
     Workspace() = default;
     Workspace(const Workspace&) = delete;

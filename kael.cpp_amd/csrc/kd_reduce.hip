@@ -820,14 +820,10 @@ void* g_scratch_ptr[kMaxDevices] = {};
 
 // Who used a device's scratch last. A call holds its device's lock from before its split kernel
 // until its combine kernel is enqueued, so calls from several host threads on one stream enqueue
-// their launch pairs whole, one pair after another; when the stream differs from the previous
-// call's, that call's work is waited for first, so calls on different streams never overlap either: by an event recorded
-// behind it, since its stream may be destroyed by then, where it was not the null stream's.
+// their launch pairs whole, one pair after another; calls on different streams wait for each other.
 struct ScratchUse {
     std::mutex mutex;
-    hipStream_t last = nullptr;
-    hipEvent_t done = nullptr;
-    bool used = false;
+    LastUse last;
 };
 ScratchUse g_scratch_use[kMaxDevices];
 
@@ -877,21 +873,10 @@ extern "C" int kd_reduce_noalloc(int op, int out_dtype, int in_dtype, void* resu
         ScratchUse& use = g_scratch_use[dev];
         std::lock_guard<std::mutex> lock(use.mutex);
         hipStream_t current = stream();
-        if (use.used && use.last != current) {
-            if (use.last == nullptr) KD_HIP(hipStreamSynchronize(nullptr));
-            else KD_HIP(hipEventSynchronize(use.done));
-        }
-        if (current != nullptr && use.done == nullptr) KD_HIP(hipEventCreateWithFlags(&use.done, hipEventDisableTiming));
+        if (int rc = use.last.wait(current)) return rc;
         const int rc = reduce_entry("kd_reduce_noalloc", op, in_dtype, results, data, chunk_size, output_count, ptr,
                                     kStaticScratchBytes);
-        if (current != nullptr) {
-            // what a capture takes up runs when its graph does
-            hipStreamCaptureStatus captured = hipStreamCaptureStatusNone;
-            KD_HIP(hipStreamIsCapturing(current, &captured));
-            if (captured == hipStreamCaptureStatusNone) KD_HIP(hipEventRecord(use.done, current));
-        }
-        use.last = current;
-        use.used = true;
+        use.last.record(current);
         return rc;
     }
     return reduce_entry("kd_reduce_noalloc", op, in_dtype, results, data, chunk_size, output_count, nullptr,

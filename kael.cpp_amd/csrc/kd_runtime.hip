@@ -17,20 +17,17 @@ namespace {
 
 thread_local std::string g_error;
 std::atomic<hipStream_t> g_stream{nullptr};
+std::atomic<uint64_t> g_stream_turn{0};
 
 struct DeviceState {
     std::atomic<int> checked{0};  // 0 = not probed, 1 = usable, -1 = unusable
     int ordinal = 0;
     int cus = 0;
     std::string arch;
-    // Workspace, guarded by g_workspace_mutex: the block, its size, the stream the last lease enqueued its kernels on (valid
-    // once `workspace_used` is set), and an event recorded behind them where that is not the null stream: its owner may have
-    // destroyed the stream since, and a destroyed stream is no stream to wait for.
+    // Workspace, guarded by g_workspace_mutex.
     void* workspace = nullptr;
     size_t workspace_bytes = 0;
-    hipStream_t workspace_stream = nullptr;
-    bool workspace_used = false;
-    hipEvent_t workspace_event = nullptr;
+    LastUse workspace_use;
 };
 
 DeviceState& state() {
@@ -91,15 +88,40 @@ hipStream_t stream() { return g_stream.load(); }
 int device_ordinal() { return state().ordinal; }
 int compute_units() { return state().cus > 0 ? state().cus : 256; }
 
+int LastUse::wait(hipStream_t current) {
+    if (current != nullptr && done == nullptr) KD_HIP(hipEventCreateWithFlags(&done, hipEventDisableTiming));
+    const uint64_t now = g_stream_turn.load();
+    if (used && stream != current) {
+        if (stream == nullptr) KD_HIP(hipStreamSynchronize(nullptr));
+        else KD_HIP(hipEventSynchronize(done));
+    } else if (used && current != nullptr && turn != now) {
+        hipStreamCaptureStatus captured = hipStreamCaptureStatusNone;
+        KD_HIP(hipStreamIsCapturing(current, &captured));
+        if (captured == hipStreamCaptureStatusNone) KD_HIP(hipStreamWaitEvent(current, done, 0));
+    }
+    used = true;
+    stream = current;
+    turn = now;
+    return KD_OK;
+}
+
+void LastUse::record(hipStream_t current) {
+    if (current == nullptr) return;
+    hipStreamCaptureStatus captured = hipStreamCaptureStatusNone;
+    if (hipStreamIsCapturing(current, &captured) == hipSuccess && captured != hipStreamCaptureStatusNone) return;
+    // without an event behind this use nothing could wait for it later, so it is waited for now
+    if (hipEventRecord(done, current) != hipSuccess && hipStreamSynchronize(current) != hipSuccess) (void)hipDeviceSynchronize();
+}
+
+int LastUse::drain() {
+    if (done != nullptr) KD_HIP(hipEventSynchronize(done));
+    return KD_OK;
+}
+
 Workspace::~Workspace() {
     if (!held) return;
-    DeviceState& s = state();
-    if (ptr != nullptr && s.workspace_stream != nullptr) {
-        // kernels that a capture takes up run when their graph does, not behind this lease
-        hipStreamCaptureStatus captured = hipStreamCaptureStatusNone;
-        if (hipStreamIsCapturing(s.workspace_stream, &captured) == hipSuccess && captured == hipStreamCaptureStatusNone)
-            (void)hipEventRecord(s.workspace_event, s.workspace_stream);
-    }
+    LastUse& use = state().workspace_use;
+    if (ptr != nullptr) use.record(use.stream);
     g_workspace_mutex.unlock();
 }
 
@@ -112,15 +134,11 @@ int workspace(Workspace& lease, size_t bytes) {
     const hipStream_t current = g_stream.load();
     // The previous lease's kernels may still run on another stream: let them finish before this
     // stream reuses (or this call frees) the block.
-    if (current != nullptr && s.workspace_event == nullptr)
-        KD_HIP(hipEventCreateWithFlags(&s.workspace_event, hipEventDisableTiming));
-    if (s.workspace_used && s.workspace_stream != current) {
-        if (s.workspace_stream == nullptr) KD_HIP(hipStreamSynchronize(nullptr));
-        else KD_HIP(hipEventSynchronize(s.workspace_event));
-    }
+    if (int rc = s.workspace_use.wait(current)) return rc;
     if (s.workspace_bytes < bytes) {
         if (s.workspace != nullptr) {
             // Kernels queued by earlier leases may still read the old block: drain before freeing.
+            if (int rc = s.workspace_use.drain()) return rc;
             KD_HIP(hipStreamSynchronize(current));
             KD_HIP(hipFree(s.workspace));
             s.workspace = nullptr;
@@ -131,8 +149,6 @@ int workspace(Workspace& lease, size_t bytes) {
         KD_HIP(hipMalloc(&s.workspace, size));
         s.workspace_bytes = size;
     }
-    s.workspace_stream = current;
-    s.workspace_used = true;
     lease.ptr = s.workspace;
     return KD_OK;
 }
@@ -154,6 +170,7 @@ int kd_synchronize(void) {
 }
 
 int kd_set_stream(void* s) {
+    ++g_stream_turn;
     g_stream.store(static_cast<hipStream_t>(s));
     return KD_OK;
 }

@@ -38,3 +38,31 @@ def test_the_workspace_outlives_its_last_stream(kdb, rounds, entry):
         held = [kdb.empty((1 << 16,), np.float32) for _ in range(8)]  # host and device memory taken up meanwhile
         np.testing.assert_array_equal(total(), want)
         del held
+
+
+@pytest.mark.parametrize("entry", ["reduce", "reduce_noalloc"])
+def test_a_stream_that_goes_with_work_in_flight(kdb, entry):
+    """Streams that are destroyed behind calls of theirs that still run, each followed by a new one, which may have the same
+    address: every call's sums are its own."""
+    lib = kdb.lib
+    rng = np.random.default_rng(7)
+    long, short = (rng.integers(-1000, 1000, (3, n)).astype(np.int64) for n in (4000000, 60000))
+    dl, ds = kdb.to_device(long), kdb.to_device(short)
+    want = long.sum(1), short.sum(1)
+    before = ctypes.c_void_p(lib.kd_get_stream())
+    outs = [kdb.to_device(np.full(3, -777, np.int64)) for _ in range(40)]
+    kdb.synchronize()
+    for i in range(0, 40, 5):
+        stream = ctypes.c_void_p()
+        assert lib.hipStreamCreate(ctypes.byref(stream)) == 0
+        try:
+            lib.kd_set_stream(stream)
+            for j in range(i, i + 5):  # the short one first: it is what follows the other stream's long ones
+                data, n = (dl, 4000000) if j > i else (ds, 60000)
+                kdb.call(entry, kd.REDUCE_SUM, kd.I64, kd.I64, outs[j].ptr, data.ptr, n, 3)
+        finally:
+            lib.kd_set_stream(before)
+            assert lib.hipStreamDestroy(stream) == 0
+    assert lib.hipDeviceSynchronize() == 0
+    for j, out in enumerate(outs):
+        np.testing.assert_array_equal(out.numpy(), want[0 if j % 5 else 1], err_msg=f"call {j}")
