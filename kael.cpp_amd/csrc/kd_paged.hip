@@ -162,12 +162,9 @@ struct Strided {
 
 constexpr int kUnit = 8;  // features of a thread: four pairs, or eight that are not rotated
 
-// Past: the access takes no place in the caches.
+// Past: the load takes no place in the caches.
 typedef float v4f __attribute__((ext_vector_type(4)));
-template <bool Past> __device__ __forceinline__ void store4(float* p, const v4f& x) {
-    if constexpr (Past) __builtin_nontemporal_store(x, reinterpret_cast<v4f*>(p));
-    else *reinterpret_cast<v4f*>(p) = x;
-}
+__device__ __forceinline__ void store4(float* p, const v4f& x) { *reinterpret_cast<v4f*>(p) = x; }
 template <bool Vector, bool Past = false> __device__ __forceinline__ void load4(const float* p, float (&x)[4]) {
     if constexpr (Vector && Past) {
         const v4f v = __builtin_nontemporal_load(reinterpret_cast<const v4f*>(p));
@@ -246,7 +243,7 @@ __device__ __forceinline__ uint32_t code_of(double x, double inverse) {
 }
 
 constexpr int kAppendThreads = 256;
-constexpr int64_t kPastBytes = int64_t{32} << 20;  // of rows, from which on they go past the caches
+constexpr int64_t kPastBytes = int64_t{32} << 20;  // of queries, from which on they are loaded past the caches
 
 template <int D, bool Vector, bool Past>
 __global__ __launch_bounds__(kAppendThreads) void paged_append_kernel(Paged c, Rotation rotation, Strided k, Strided v,
@@ -275,8 +272,8 @@ __global__ __launch_bounds__(kAppendThreads) void paged_append_kernel(Paged c, R
             rotated_unit<Vector, Past>(q.data + token * q.row + h * q.head, low, high, position, rotation, y);
             float* out = q_out + (token * heads + h) * dim;
             const auto at = [&](int j) { return position < 0 ? NAN : static_cast<float>(y[j]); };
-            store4<Past>(out + low, v4f{at(0), at(1), at(2), at(3)});
-            store4<Past>(out + high, v4f{at(4), at(5), at(6), at(7)});
+            store4(out + low, v4f{at(0), at(1), at(2), at(3)});
+            store4(out + high, v4f{at(4), at(5), at(6), at(7)});
         }
         return;
     }
@@ -379,9 +376,9 @@ __global__ __launch_bounds__(kAppendThreads) void paged_append_kernel(Paged c, R
 //
 // The append's division into pages: four codes a thread and a 16-byte store for the keys, a feature's 16 tokens a thread for
 // the values, so that codes are read in whole pieces and rows written in whole lines. Bound by the bytes, the rows' above all:
-// 67 MB in 13.5 us, past the caches.
+// 67 MB in 14 us. Rows stored past the caches take less time alone (79 MB of them 17 us instead of 27) and cost their reader more than that
+// (with a sum of keys and values behind it 49.3 / 47.3, 102 MB 61.1 / 59.3, 52 MB 31.5 / 31.5), so they are not.
 
-template <bool Past>
 __global__ __launch_bounds__(256) void paged_read_kernel(Paged c, float* __restrict__ k, float* __restrict__ v) {
     const uint32_t group = c.kv_heads * 2;
     const int h = static_cast<int>(blockIdx.x % group) / 2;
@@ -412,7 +409,7 @@ __global__ __launch_bounds__(256) void paged_read_kernel(Paged c, float* __restr
         const int8_t* codes = c.keys + (at * size + p.held) * dim;
         for (int i = threadIdx.x; i < p.count * (dim / 4); i += threads) {
             const char4 x = *reinterpret_cast<const char4*>(codes + 4 * i);
-            store4<Past>(out + i / (dim / 4) * row_size + i % (dim / 4) * 4, v4f{x.x * scale, x.y * scale, x.z * scale, x.w * scale});
+            store4(out + i / (dim / 4) * row_size + i % (dim / 4) * 4, v4f{x.x * scale, x.y * scale, x.z * scale, x.w * scale});
         }
     } else {
         const float scale = c.value_scales[at];
@@ -427,10 +424,7 @@ __global__ __launch_bounds__(256) void paged_read_kernel(Paged c, float* __restr
                 const int token = slot0 + j - p.held;
                 const float x = static_cast<float>(static_cast<int8_t>(word[j / 4] >> (8 * (j % 4)))) * scale;
                 float* to = out + token * row_size + d;
-                if (token >= 0 && token < p.count) {
-                    if constexpr (Past) __builtin_nontemporal_store(x, to);
-                    else *to = x;
-                }
+                if (token >= 0 && token < p.count) *to = x;
             }
         }
     }
@@ -1741,9 +1735,11 @@ extern "C" int kd_paged_append(int dtype, const kd_paged_cache* cache, const kd_
     // 16-byte pieces need rows and tables that keep them aligned and pairs that come in fours
     const auto whole = [](const Strided& x) { return aligned(x.data, 16) && x.row % 4 == 0 && x.head % 4 == 0; };
     const bool vector = r.half % 4 == 0 && aligned(r.cosines, 16) && aligned(r.sines, 16) && whole(ks) && (q == nullptr || whole(qs));
-    // Large queries go past the caches both ways, and so do the keys the second time: what they leave there is the second reading
-    // of the keys and values. With the pages read back, us, all through the caches / past them, by the bytes of q: 13 MB
-    // 24.2 / 24.9, 25 MB 27.5 / 29.1, 38 MB 36.1 / 35.4, 50 MB 46.5 / 41.4, 100 MB 90.2 / 75.9, 200 MB 169 / 152.
+    // Large queries are loaded past the caches, and the keys the second time: what they leave there is the second reading of the keys
+    // and values. They are stored through them, for the attention reads them next. Append and attention, us, all through the caches /
+    // loads past them / stores too, by the bytes of q: 40 MB 227.3 / 226.8 / 228.1, 67 MB 321.7 / 321.8 / 322.5, 104 MB 187.8 / 186.5 / 191.0
+    // and 270.2 / 267.2 / 273.9, 113 MB 483.1 / 482.6 / 486.5, 203 MB 361.5 / 358.1 / 358.6; the append and a reading of its pages alone
+    // take 85 / 82 / 72 at 104 MB.
     const bool past = q != nullptr && vector && int64_t{c.tokens} * heads * c.head_dim * 4 > kPastBytes;
     const auto launch = [&](auto dim, auto aligned_pieces, auto past_caches) {
         constexpr int D = decltype(dim)::value;
@@ -1771,14 +1767,8 @@ extern "C" int kd_paged_read(int dtype, void* k, void* v, const kd_paged_cache* 
     const int threads = c.page_shift <= 5 ? 64 : 256;
     if (int rc = check_grid("kd_paged_read", groups, threads)) return rc;
     if (int rc = ensure_device()) return rc;
-    // past the caches, 50 MB of rows 17.3 / 15.4 us, 100 MB 33 / 27
-    const auto launch = [&](auto kernel) {
-        hipLaunchKernelGGL(kernel, dim3(static_cast<uint32_t>(groups)), dim3(threads), 0, stream(), c, static_cast<float*>(k),
-                           static_cast<float*>(v));
-    };
-    const int64_t rows = int64_t{c.tokens} * c.kv_heads * ((k != nullptr) + (v != nullptr));
-    if (rows * c.head_dim * 4 > kPastBytes) launch(paged_read_kernel<true>);
-    else launch(paged_read_kernel<false>);
+    hipLaunchKernelGGL(paged_read_kernel, dim3(static_cast<uint32_t>(groups)), dim3(threads), 0, stream(), c, static_cast<float*>(k),
+                       static_cast<float*>(v));
     KD_LAUNCH_CHECK();
     return KD_OK;
 }
