@@ -177,6 +177,31 @@ def test_distillation_of_more_than_the_caches(kdb, rows):
         np.testing.assert_array_equal(a[which], b)
 
 
+@pytest.mark.parametrize("rows,dtype", [(1700, np.float32), (900, np.float64)])
+def test_large_distillation_in_place(kdb, rows, dtype):
+    """Gradients stored past the caches over the logits that they come from, f32 and f64: every row as in a call of 512,
+    which sums a row by as many threads."""
+    rng = np.random.default_rng(rows)
+    base = rng.normal(size=(512, 40001)).astype(dtype)
+    indices = rng.integers(0, 40001, (512, 9))
+    teacher, weights = rng.normal(size=(512, 9)).astype(dtype), rng.normal(size=512).astype(dtype)
+    few = run_distill(kdb, base, indices, teacher, weights, 1.5)
+    # As check_distill, but log sigma is of size X + log(cols), which is not below X by far here, and the definition in f64 rounds
+    # as often as f64 losses do: twice T^2 (X + log(cols) + 4) eps + eps |loss|, and twice (X + log(cols) + 11) eps of sigma and pi.
+    eps, z = np.finfo(dtype).eps, base.astype(np.float64)
+    want, grad = definition.distill(base, indices, teacher, 1.5)
+    size = (z.max(1) - z.min(1)) / 1.5 + np.log(40001)
+    assert (np.abs(few[0] - want) <= 2 * eps * (1.5 ** 2 * (size + 4) + np.abs(want))).all()
+    hit = np.zeros(z.shape)
+    np.put_along_axis(hit, indices, 1, 1)  # the shares of a row add up to 1
+    bound = 2 * eps * (size + 11)[:, None] * np.abs(weights.astype(np.float64))[:, None] * 1.5 * (softmax(z / 1.5) + hit)
+    assert (np.abs(few[2] - weights.astype(np.float64)[:, None] * grad) <= bound + np.finfo(dtype).tiny).all()
+    which = rng.integers(0, 512, rows)
+    many = run_distill(kdb, base[which], indices[which], teacher[which], weights[which], 1.5, in_place=True)
+    for a, b in zip(few, many):
+        np.testing.assert_array_equal(a[which], b)
+
+
 @pytest.mark.parametrize("dtype", [kd.F32, kd.F64], ids=["f32", "f64"])
 @pytest.mark.parametrize("cols", [50, 3000])
 def test_distillation_of_odd_rows(kdb, cols, dtype):

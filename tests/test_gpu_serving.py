@@ -235,3 +235,47 @@ def test_a_distilled_draft_is_accepted(kdb):
     tokens, accepted = kdb.empty((rows, 2), np.int64), kdb.empty((rows,), np.int64)
     kdb.call("verify_drafts", kd.F64, tokens.ptr, accepted.ptr, *(a.ptr for a in on), rows, 1, vocab)
     assert (accepted.numpy() == 1).all() and (tokens.numpy()[:, 0] == drafted[:, 0]).all()
+
+
+def test_a_draft_that_distillation_trains_is_taken_more_often(kdb):
+    """A draft's logits follow the loss's gradient towards the target's largest ones; the tokens that the trained and the untrained draft
+    draw are verified against the target, each as the definition does."""
+    rng = np.random.default_rng(8)
+    rows, vocab, kept, drafts = 300, 60, 30, 2
+    target_logits = 2 * rng.normal(size=(rows, vocab))
+    index = np.argsort(-target_logits, 1)[:, :kept].astype(np.int64)
+    teacher = np.take_along_axis(target_logits, index, 1)
+    values = np.zeros((rows, vocab))
+    z, di, dt, w = (kdb.to_device(a) for a in (values, index, teacher, np.ones(rows)))
+    losses, stats, grad = (kdb.empty(s, np.float64) for s in ((rows,), (rows, 2), (rows, vocab)))
+
+    def softmax(x):
+        e = np.exp(x - x.max(-1, keepdims=True))
+        return e / e.sum(-1, keepdims=True)
+
+    def taken():
+        """The share of the draft's own tokens that the target takes."""
+        p = softmax(target_logits)[:, None].repeat(drafts + 1, 1)
+        q = softmax(values)[:, None].repeat(drafts, 1)
+        over = np.cumsum(q, 2) > rng.random((rows, drafts))[..., None]
+        drafted = np.where(over.any(2), over.argmax(2), vocab - 1).astype(np.int64)
+        given = p, q, drafted, np.full(rows, drafts), rng.random((rows, drafts + 1))
+        on = [kdb.to_device(a) for a in given]
+        tokens, accepted = kdb.empty((rows, drafts + 1), np.int64), kdb.empty((rows,), np.int64)
+        kdb.call("verify_drafts", kd.F64, tokens.ptr, accepted.ptr, *(a.ptr for a in on), rows, drafts, vocab)
+        want = draft_definition.verify(*given)
+        np.testing.assert_array_equal(tokens.numpy(), want[0])
+        np.testing.assert_array_equal(accepted.numpy(), want[1])
+        return want[1].sum() / (rows * drafts)
+
+    untrained = taken()
+    for _ in range(60):
+        z.upload(values)
+        kdb.call("distill_rows", kd.F64, losses.ptr, stats.ptr, z.ptr, di.ptr, dt.ptr, rows, vocab, kept, 1.0)
+        kdb.call("distill_grad", kd.F64, grad.ptr, z.ptr, stats.ptr, di.ptr, dt.ptr, w.ptr, rows, vocab, kept, 1.0)
+        want_losses, want_grad = draft_definition.distill(values, index, teacher, 1.0)
+        assert (np.abs(grad.numpy() - want_grad) <= 40 * 2.0 ** -52).all()
+        assert (np.abs(losses.numpy() - want_losses) <= 40 * 2.0 ** -52 * (1 + np.abs(want_losses))).all()
+        values = values - 2 * grad.numpy()
+    # of 600 tokens each a share of at most 1: deviations below 0.03
+    assert taken() > untrained + 6 * 0.03
