@@ -1390,7 +1390,7 @@ __global__ __launch_bounds__(G * kPromptWaves * 64, 2) void paged_prompt_kernel(
 #pragma unroll
             for (int n = 0; n < D / 16; ++n) o[n] *= again;
             top_exponent = next_exponent;
-            scale_limit = __float_as_int(ldexpf(4.f, top_exponent));
+            scale_limit = min(__float_as_int(ldexpf(4.f, top_exponent)), 0x7f7fffff);  // infinity and NaN are always looked at
         }
         const float base = m == -INFINITY ? 0.f : m;  // nothing seen yet: every weight below is 0
         if (__any(fabsf(base) >= kFarScore)) {

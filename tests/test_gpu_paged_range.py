@@ -149,3 +149,20 @@ def test_a_key_scale_that_is_not_finite_gives_nan(kdb, which, dim, new):
     with np.errstate(invalid="ignore"):
         want, tolerance = paged.attention(cache, starts, lengths, np.where(np.arange(tokens)[:, None, None] < new, 0, q), dim ** -0.5)
     assert (np.abs(got - want) <= tolerance)[new:].all()
+
+
+@pytest.mark.parametrize("new", ROWS)
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("which", [np.inf, np.nan])
+def test_a_value_scale_that_is_not_finite_gives_nan(kdb, which, dim, new):
+    """Beside values near f32's largest, and of keys whose weight is next to nothing."""
+    rng = np.random.default_rng(26)
+    starts, lengths, tokens = batch_of([new], [300])
+    cache = paged.Cache(rng, 1, 19, 1, 16, dim)
+    cache.value_scales[:] = 2.0 ** 120
+    far = cache.table[0, 9]
+    cache.keys[far], cache.key_scales[far] = -1, 8 / dim ** 0.5  # scores of about -8 with queries of 1
+    cache.value_scales[far] = which
+    q = np.ones((tokens, 1, dim), np.float32)
+    got = run_attention(kdb, paged.Device(kdb, cache, starts, lengths, tokens), q, dim ** -0.5, 300)
+    assert np.isnan(got).all()
