@@ -64,6 +64,7 @@ struct Workspace {
     Workspace& operator=(const Workspace&) = delete;
     ~Workspace();
     void* ptr = nullptr;
+    hipStream_t stream = nullptr;
     bool held = false;
 };
 int workspace(Workspace& lease, size_t bytes);

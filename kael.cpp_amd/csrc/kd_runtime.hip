@@ -95,13 +95,14 @@ int LastUse::wait(hipStream_t current) {
     if (current != nullptr && done == nullptr)
         KD_HIP(hipEventCreateWithFlags(&done, hipEventDisableTiming | hipEventDisableSystemFence));
     const uint64_t now = g_stream_turn.load();
-    if (used && stream != current) {
-        if (stream == nullptr) KD_HIP(hipStreamSynchronize(nullptr));
-        else KD_HIP(hipEventSynchronize(done));
-    } else if (used && current != nullptr && turn != now) {
+    if (used && (stream != current || turn != now)) {
         hipStreamCaptureStatus captured = hipStreamCaptureStatusNone;
-        KD_HIP(hipStreamIsCapturing(current, &captured));
-        if (captured == hipStreamCaptureStatusNone) KD_HIP(hipStreamWaitEvent(current, done, 0));
+        if (current != nullptr) KD_HIP(hipStreamIsCapturing(current, &captured));
+        if (stream != current && stream == nullptr) KD_HIP(hipStreamSynchronize(nullptr));
+        // no call to make under capture, whose kernels run later: the last use stays the one to wait for
+        else if (captured != hipStreamCaptureStatusNone) return KD_OK;
+        else if (stream != current) KD_HIP(hipEventSynchronize(done));
+        else if (current != nullptr) KD_HIP(hipStreamWaitEvent(current, done, 0));
     }
     used = true;
     stream = current;
@@ -124,8 +125,7 @@ int LastUse::drain() {
 
 Workspace::~Workspace() {
     if (!held) return;
-    LastUse& use = state().workspace_use;
-    if (ptr != nullptr) use.record(use.stream);
+    if (ptr != nullptr) state().workspace_use.record(stream);
     g_workspace_mutex.unlock();
 }
 
@@ -154,6 +154,7 @@ int workspace(Workspace& lease, size_t bytes) {
         s.workspace_bytes = size;
     }
     lease.ptr = s.workspace;
+    lease.stream = current;
     return KD_OK;
 }
 

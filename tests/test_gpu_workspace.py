@@ -66,3 +66,47 @@ def test_a_stream_that_goes_with_work_in_flight(kdb, entry):
     assert lib.hipDeviceSynchronize() == 0
     for j, out in enumerate(outs):
         np.testing.assert_array_equal(out.numpy(), want[0 if j % 5 else 1], err_msg=f"call {j}")
+
+
+@pytest.mark.parametrize("entry", ["reduce", "reduce_noalloc"])
+def test_a_captured_call_after_another_streams(kdb, entry):
+    """A call on one stream, then the same captured on a second: replays with eager calls between give the eager sums."""
+    lib = kdb.lib
+    rng = np.random.default_rng(9)
+    x = rng.integers(-1000, 1000, (3, 200000)).astype(np.int64)
+    dx, out, captured = kdb.to_device(x), kdb.empty((3,), np.int64), kdb.empty((3,), np.int64)
+
+    def call(to):
+        kdb.call(entry, kd.REDUCE_SUM, kd.I64, kd.I64, to.ptr, dx.ptr, x.shape[1], 3)
+
+    before = ctypes.c_void_p(lib.kd_get_stream())
+    first, second = ctypes.c_void_p(), ctypes.c_void_p()
+    for stream in (first, second):
+        assert lib.hipStreamCreate(ctypes.byref(stream)) == 0
+    graph, run = ctypes.c_void_p(), ctypes.c_void_p()
+    try:
+        lib.kd_set_stream(first)
+        call(out)
+        lib.kd_set_stream(second)
+        assert lib.hipStreamBeginCapture(second, 1) == 0  # thread-local
+        call(captured)
+        assert lib.hipStreamEndCapture(second, ctypes.byref(graph)) == 0
+        assert lib.hipGraphInstantiate(ctypes.byref(run), graph, None, None, 0) == 0
+        for stream in (second, first, second):
+            x = rng.integers(-1000, 1000, x.shape).astype(np.int64)
+            dx.upload(x)
+            lib.kd_set_stream(stream)
+            call(out)
+            assert lib.hipStreamSynchronize(stream) == 0
+            assert lib.hipGraphLaunch(run, second) == 0
+            assert lib.hipStreamSynchronize(second) == 0
+            np.testing.assert_array_equal(out.numpy(), x.sum(1))
+            np.testing.assert_array_equal(captured.numpy(), x.sum(1))
+    finally:
+        lib.kd_set_stream(before)
+        if run:
+            lib.hipGraphExecDestroy(run)
+        if graph:
+            lib.hipGraphDestroy(graph)
+        for stream in (first, second):
+            lib.hipStreamDestroy(stream)
