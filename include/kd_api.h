@@ -154,7 +154,9 @@ int kd_available(void);
 /* reference device_kernels.h:97 `void synchronize()`: drains the backend stream. */
 int kd_synchronize(void);
 /* Selects the stream every later call issues on (hipStream_t; NULL = null stream).
- * No reference counterpart: the reference always uses the default stream. */
+ * No reference counterpart: the reference always uses the default stream. Calls that share a buffer of
+ * the backend's wait for each other across streams, also where the earlier stream has been destroyed since. A
+ * new stream is selected by a call of its own, also where it has an earlier one's address. */
 int kd_set_stream(void* stream);
 void* kd_get_stream(void);
 
@@ -214,7 +216,7 @@ int kd_reduce_columns(int op, int out_dtype, int in_dtype, void* results, const 
  * call on one GPU shares that buffer. Calls from several host threads are serialised around it
  * (each call's two launches are enqueued together under a lock), and a call on another stream
  * than the previous call's waits for that call's work, so calls never overlap on the buffer; what
- * a graph replays on it is not covered. */
+ * a graph replays on it is not covered, and a call under capture waits for nothing. */
 int kd_reduce_noalloc(int op, int out_dtype, int in_dtype, void* results, const void* data,
                       int64_t chunk_size, int64_t output_count);
 
@@ -426,8 +428,11 @@ int kd_paged_read(int dtype, void* k, void* v, const kd_paged_cache* cache, cons
  * over the positions j up to the row's own that have a page; kv head h * kv_heads / heads serves head
  * h (heads a multiple of kv_heads). A row that sees nothing is 0. q is f32 with element strides (row,
  * head) in q_strides, features contiguous; out [tokens][heads][head_dim] contiguous, 16-byte aligned,
- * not overlapping q. Sums and products are exact to about f32's rounding; a non-finite query or scale
- * gives NaN where it is seen.
+ * not overlapping q. Sums and products are exact to about f32's rounding of their terms; a query's feature
+ * is held to 2^-23 of itself or 2^-30 of its row's largest, a weight times its value scale to 2^-23 of itself or
+ * 2^-30 of the row's largest such product, which counts as 2^-96 of its largest value scale at least. A
+ * non-finite query or scale gives NaN where it is seen. Scores beyond f32's range in size are NaN or, below 0,
+ * no weight.
  * max_keys is the largest of `lengths` as far as the host knows it, and only decides how the work is
  * split; results are right whatever it says. Long caches are split over workgroups whose partial
  * results pass through `workspace` (device, 16-byte aligned; kd_paged_attention_workspace says how many

@@ -143,8 +143,8 @@ __device__ __forceinline__ PageSlots page_slots(const Paged& c, int64_t slot) {
 // single tokens. One launch: a workgroup takes one page of one kv head, its keys or its values, so that the page's scale
 // has one owner, and the workgroups behind those take the queries. Rotated and quantised in f64, where the products of two
 // f32 are exact and a rounding to the wrong side of a tie takes a value within 2^-45 of it: f64 costs less here than the bytes.
-// Keys and values are read twice, for the scale and for the codes, the second time mostly from the L2: a page held in registers
-// or LDS in between left fewer workgroups on a CU and took longer. 6347 tokens of 32 + 2 x 8 heads of 128: 71 us, 274 MB at
+// Keys and values are read twice, for the scale and for the codes, the second time mostly from behind the L2 (42 of 52 MB in the
+// case below): a page held in registers or LDS in between left fewer workgroups on a CU and took longer. 6347 tokens of 32 + 2 x 8 heads of 128: 71 us, 274 MB at
 // 3.9 TB/s; 64 single tokens of 12 heads of 64: 6.9 us.
 
 struct Rotation {
@@ -434,7 +434,7 @@ __global__ __launch_bounds__(256) void paged_read_kernel(Paged c, float* __restr
 //
 // Scores and weighted sums run on the signed 8-bit matrix cores, whose sums are exact: the cached codes go in as they
 // are, and the other operand as four signed digits of base 256. A query row is q = 2^(e - 30) * x with x whole, e the
-// exponent of its largest feature (x is exact for features of at least 2^-6 of that one, and off by 2^-31 of it at
+// exponent of its largest feature (x is exact for features of at least 2^-6 of that one, and off by 2^-30 of it at
 // most otherwise); a weight exp(score - max) times its value scale likewise, against the largest of a row's block. Four products a
 // tile and twice bf16's rate are as many cycles as two bf16 products, where three would be needed for f32's bits, and the
 // codes need no conversion.
@@ -450,8 +450,9 @@ __global__ __launch_bounds__(256) void paged_read_kernel(Paged c, float* __restr
 // and the columns that join a score's digits share its row's keys out between them, so that a lane computes 16 / S
 // weights; their digits go back to the columns that multiply with them by exchanges within four lanes.
 //
-// Bound by the codes' bytes for many sequences (4 x 40000 keys of 128, 32 heads over 8: 46 us, 5.5 TB/s; 64 x 4000 of 64, one row,
-// 52 us, 5.7 TB/s), by the vector ALU for 9 to 32 rows, by the chain of loads (starts, table, codes) and 50 GB/s a CU for few.
+// Bound by the codes' bytes for many sequences (4 x 40000 keys of 128, 32 heads over 8: 47 us, 5.5 TB/s; 64 x 4000 of 64, one row,
+// 52 us, 5.7 TB/s), by the loads' latency for 9 to 32 rows (17 x 20000 of 64, 24 rows: vector ALU
+// busy 0.42 of the cycles, matrix cores 0.10, waves waiting 0.31), by the chain of loads (starts, table, codes) and 50 GB/s a CU for few.
 
 typedef int v4i __attribute__((ext_vector_type(4)));
 
@@ -899,7 +900,7 @@ __global__ __launch_bounds__(Waves * 64, D == 64 ? 4 : 2) void paged_attention_k
 // One row a workgroup (single tokens whose heads share nothing). Its four digits take four columns, and all sixteen columns
 // share the keys out, one to a lane: a weight costs a lane one exponential where the kernel above computes four. The sums of the
 // outputs stay whole over the blocks, and are turned into f32 when the largest weight or weighted scale changes or they could
-// pass 2^31. 64 x 1024 keys of 64, 12 heads: 16.0 us, 76 MB at 4.8 TB/s; 1 x 1000: 6.8 us, the launch and the chain of loads.
+// pass 2^31. 64 x 1024 keys of 64, 12 heads: 16.5 us, 76 MB at 4.6 TB/s; 1 x 1000: 6.8 us, the launch and the chain of loads.
 constexpr int kMostBlocks = 1024;  // that the whole sums hold: 2^10 blocks of 2^6 keys of 2^14
 
 template <int D, int Waves>
@@ -1116,12 +1117,13 @@ __global__ __launch_bounds__(Waves * 64, D == 64 ? 4 : 2) void paged_single_kern
 // Many rows a sequence (prompts): the workgroup's four waves take 16 rows each and share every block of 64 keys through LDS,
 // two blocks deep, so that a wave keeps none of it in registers. Few workgroups have two such teams (G = 2) that take every
 // other block: a wave alone on its SIMD takes 1.05 us for a block of 64 features, two of them 1.5 for both.
-// What bounds it is the vector ALU, 30 operations a score in the kernel above, seven of which join the digits' sums of the
-// outputs; here the weighted sums run on the f16 matrix cores into f32, which joins nothing: a code is an f16 value as it stands,
+// What bounds it where workgroups are many is the vector ALU, 30 operations a score in the kernel above, seven of which join
+// the digits' sums of the outputs; here the weighted sums run on the f16 matrix cores into f32, which joins nothing: a code is an f16 value as it stands,
 // converted once for the four waves, and a weight times its value scale two f16 pieces (2^-23 of it), scaled so that the
-// largest that the row has is 2^13 and pieces below 2^-24 are below 2^-36 of that. 2 prompts of up to 4096, 32 heads over 8 of 128: 422 us, 480 TFLOP/s of the formula's
-// products, VALU busy 0.74 and matrix cores 0.43 of the cycles; 8 of up to 1000, 12 heads of 64: 31 us; 4 x 4096 of 64: VALU busy
-// 0.95.
+// largest that the row has is 2^13 and pieces below 2^-24 are below 2^-36 of that. 2 prompts of up to 4096, 32 heads over 8 of 128:
+// 428 us, 474 TFLOP/s of the formula's products, VALU busy 0.76 and matrix cores 0.42 of the cycles; 4 x 4096 of 64: 191 us, VALU
+// busy 0.83. 8 of up to 1000, 12 heads of 64: 32.5 us, VALU busy 0.54: about four workgroups a CU of unlike lengths, the longest alone
+// at the end.
 typedef _Float16 v8h __attribute__((ext_vector_type(8)));
 typedef _Float16 v2h __attribute__((ext_vector_type(2)));
 typedef float v2f __attribute__((ext_vector_type(2)));
