@@ -550,6 +550,153 @@ int kd_layer_norm_rows_backward(int dtype, void* grad_in, void* grad_weight, voi
                                 const void* standardized, const void* grad, const void* weight, int64_t rows,
                                 int64_t cols, double eps);
 
+/* ---- training on sampled answers and on pairs of them (no reference counterpart) -------------- */
+
+/* Where a counter-based mask's words come from. Element (r, c) of a tensor's rows takes the 32-bit word c % 4 of
+ * Philox4x32-10 (Salmon, Moraes, Dror and Shaw, "Parallel random numbers: as easy as 1, 2, 3", SC 2011) of the counter
+ * (c / 4, row + r, stream, step') under the key `seed` (low word first), step' = step + *more_steps modulo 2^32. The
+ * element is kept where its word is below keep * 2^32, rounded to the nearest whole number. So the mask needs no memory: the
+ * same counter gives it again in the backward pass, and in parts of the tensor's rows, in any order. A program gives each
+ * of a step's dropouts a stream of its own. more_steps (device, may be NULL for 0) is read when the kernels run, so a
+ * captured step draws a new mask at every replay whose program counts it up, ahead of the step or behind it. */
+typedef struct kd_counter {
+    uint64_t seed;
+    uint32_t stream;
+    uint32_t step;
+    int64_t row;
+    const int64_t* more_steps;
+} kd_counter;
+
+/* Dropout with such a mask, beside kd_dropout's from kael's own stream: out = in * T(1 / keep) where an element is
+ * kept and 0 where it is not, whatever `in` holds there. The backward pass is the same call on the gradient. f32 or f64
+ * in `rows` contiguous rows of `cols`; out may be in, and must not overlap it otherwise. keep is 2^-32 .. 1; 1 copies.
+ * 0 <= counter->row and row + rows <= 2^32; cols <= 2^34. */
+int kd_counter_dropout(int dtype, void* out, const void* in, int64_t rows, int64_t cols, double keep,
+                       const kd_counter* counter);
+
+/* A norm over a row v of n values: (v - m) / sqrt(mean((v - m)^2) + eps) * weight + bias, with m the mean
+ * (KD_NORM_LAYER) or 0 (KD_NORM_RMS). weight and bias [n]; NULL for 1 and 0. eps is finite and not negative.
+ * KD_NORM_NONE leaves v as it is; weight, bias and eps are not read then. */
+#define KD_NORM_NONE 0
+#define KD_NORM_LAYER 1
+#define KD_NORM_RMS 2
+typedef struct kd_norm {
+    const void* weight;
+    const void* bias;
+    double eps;
+    int32_t kind;
+} kd_norm;
+
+/* The end of a transformer's block with the start of the next one, for `rows` contiguous rows of `cols`:
+ *   a = dropout(after(x))            x the block's output; dropout as kd_counter_dropout, none for keep = 1
+ *   h = residual_scale * residual + block_scale * gate * a
+ *   y = before(h)
+ * gate is NULL (1), one row of [cols] (gate_rows = 1) or a row for each row (gate_rows = rows); gate_rows is 0 without a
+ * gate. residual may be NULL: h = block_scale * gate * a. With all but x left out it is an embedding's dropout and the
+ * first norm; with one row a decoding step's. kael composes the same from dropout, add and LayerNorm (reference
+ * src/nn/transformer.cpp:149-165). */
+typedef struct kd_block {
+    const void* x;
+    const void* residual;
+    const void* gate;
+    int64_t rows;
+    int64_t cols;
+    int64_t gate_rows;
+    double residual_scale;
+    double block_scale;
+    double keep;
+    kd_norm after;
+    kd_norm before;
+    kd_counter counter;
+} kd_block;
+
+/* Writes h, y and stats, each of which may be NULL where it is not wanted: h [rows][cols]; y [rows][cols], NULL if
+ * before.kind is KD_NORM_NONE; stats [rows][4] f64, which the backward pass reads: mean and 1 / sqrt(mean square + eps) of
+ * `after`, then of `before` (0 and 1 for KD_NORM_NONE). y is the norm of h as it is stored (rounded to dtype). A row is
+ * computed in 64 bits and rounded once. h may be x or residual, y may be x or residual; no output overlaps an input or another
+ * output otherwise. f32 or f64. */
+int kd_block_rows(int dtype, void* h, void* y, double* stats, const kd_block* block);
+
+/* The gradients of kd_block_rows's inputs; each may be NULL (not computed). x and residual [rows][cols], gate
+ * [gate_rows][cols], the norms' weights and biases [cols]. */
+typedef struct kd_block_grads {
+    void* x;
+    void* residual;
+    void* gate;
+    void* after_weight;
+    void* after_bias;
+    void* before_weight;
+    void* before_bias;
+} kd_block_grads;
+
+/* Backward of kd_block_rows for the gradients grad_h of h (NULL: 0) and grad_y of y (NULL: 0; NULL if before.kind is
+ * KD_NORM_NONE), from the block as the forward call had it (residual is not read, x only where after.kind is not
+ * KD_NORM_NONE or the gate's gradient is wanted), its h (read with grad_y only) and its stats:
+ *   G = grad_h + the gradient through before; residual: residual_scale * G; gate: block_scale * a * G (summed over the
+ *   rows for one row of gate); x: the gradient of block_scale * gate * G through dropout and after
+ * A row is computed in 64 bits and rounded once. Sums over rows are f64 over parts of at most 32 rows, which are summed in dtype
+ * at least. No rows: the
+ * summed gradients are 0. grads->residual may be grad_h or grad_y, grads->x may be x, grad_h or grad_y; no output overlaps
+ * an input or another output otherwise.
+ * Summed gradients pass through `workspace` (device, 16-byte aligned, as many bytes as kd_block_rows_workspace says; not
+ * needed where none of them is wanted). Calls that may run at the same time (streams, graphs) need workspaces of their own.
+ * The same arguments and contents give the same bits. */
+int kd_block_rows_backward(int dtype, const kd_block_grads* grads, const kd_block* block, const void* h,
+                           const double* stats, const void* grad_h, const void* grad_y, void* workspace,
+                           int64_t workspace_bytes);
+int kd_block_rows_workspace(int64_t* bytes, int dtype, int64_t rows, int64_t cols);
+
+/* The log-probability of each row's target, logps[r] = z_t - log(sum exp z) with z = logits[r] / temperature and
+ * t = targets[r], and stats [rows][2]: the row's max(logits) and sum exp((logits - max) / temperature), which
+ * kd_token_logps_grad reads. A target outside 0 .. cols - 1 is none (a prompt's token, padding): its row of logits is not
+ * read, logps is 0 and stats are 0 and 1. logps are f64, since sums over long answers cancel against the reference's;
+ * the exponentials are dtype's, their sum f64. A logit of -inf has no part; a row of nothing else, of NaN or of +inf is NaN.
+ * dtype f32 or f64, rows contiguous; 1e-6 <= temperature <= 1e6, rows at most 2^22 - 4, cols below 2^31. */
+int kd_token_logps(int dtype, double* logps, void* stats, const void* logits, const int64_t* targets, int64_t rows,
+                   int64_t cols, double temperature);
+
+/* Its gradient: out = slopes[r] / temperature * ((c == target) - softmax(logits[r] / temperature)_c) for the loss's
+ * derivatives `slopes` (dtype, [rows]) with respect to logps; 0 in a row without a target, or of slope 0, whatever its
+ * logits. stats from kd_token_logps on the same logits; out may be logits. */
+int kd_token_logps_grad(int dtype, void* out, const void* logits, const void* stats, const int64_t* targets,
+                        const void* slopes, int64_t rows, int64_t cols, double temperature);
+
+/* The preference loss of `pairs` of answers. Sequence 2 p is pair p's chosen answer, 2 p + 1 the rejected one; sequence s has
+ * the rows starts[s] .. starts[s + 1] - 1 (starts [2 * pairs + 1] ascending, read when the kernel runs, clamped to
+ * 0 .. rows). With logps from kd_token_logps and `reference` the reference model's (f64, [rows]; NULL for 0), over the rows
+ * with a target in 0 .. cols - 1:
+ *   rewards[p] = beta * sum of (logps - reference), of the chosen and of the rejected answer;  m = their difference
+ *   losses[p] = -(1 - smoothing) * log sigma(m) - smoothing * log sigma(-m)
+ *   slopes[r] = weights[p] * the derivative of losses[p] with respect to logps[r], for kd_token_logps_grad; 0 for
+ *   rows without a target and for rows outside every sequence
+ * losses [pairs], rewards [pairs][2], slopes [rows] and weights [pairs] are dtype's, sums f64. 0 <= smoothing < 0.5,
+ * 0 < beta <= 1e6, pairs below 2^22. rewards may be NULL. No pairs: slopes are 0. */
+int kd_preference_pairs(int dtype, void* losses, void* rewards, void* slopes, const double* logps,
+                        const double* reference, const int64_t* targets, const int64_t* starts, const void* weights,
+                        int64_t pairs, int64_t rows, int64_t cols, double beta, double smoothing);
+
+/* The clipped policy loss of sampled tokens, row by row, with its gradient in the same pass. With lp the row's
+ * log-probability (as kd_token_logps defines it), w = exp(lp - old_logps[r]), A = advantages[r] and d = reference_logps[r] - lp:
+ *   losses[r] = -min(w A, clamp(w, 1 - clip_low, 1 + clip_high) A) + kl_weight * (exp(d) - d - 1)
+ *   grad[r]   = row_weights[r] * dlosses[r] / dlogits[r]
+ * The first term's derivative with respect to lp is -w A where w A is the smaller one or equal, else 0; an A of 0
+ * has neither term nor derivative, whatever w is. A row without a target (as there) has loss, lp and gradient 0.
+ * old_logps and reference_logps f64 [rows] (old_logps NULL: lp itself, w = 1, for answers that this very model sampled;
+ * reference_logps NULL or kl_weight 0: no second term); advantages and row_weights dtype [rows]. logps (f64 [rows], may be NULL) receives
+ * lp. grad may be NULL (then row_weights is not read) and may be logits. clip_low is 0 .. 1, clip_high and kl_weight
+ * are 0 .. 1e6; sizes and temperature as in kd_token_logps. */
+typedef struct kd_policy {
+    const double* old_logps;
+    const double* reference_logps;
+    const void* advantages;
+    double temperature;
+    double clip_low;
+    double clip_high;
+    double kl_weight;
+} kd_policy;
+int kd_policy_rows(int dtype, void* losses, double* logps, void* grad, const void* logits, const int64_t* targets,
+                   const kd_policy* policy, const void* row_weights, int64_t rows, int64_t cols);
+
 /* ---- optimizer steps (extensions replacing composed device paths) ------ */
 
 /* One Adam / AdamW step of a contiguous parameter tensor in place, with its first and second

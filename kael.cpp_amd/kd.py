@@ -9,7 +9,8 @@ from __future__ import annotations
 
 import ctypes
 import os
-from ctypes import POINTER, Structure, c_char_p, c_double, c_float, c_int, c_int32, c_int64, c_void_p
+from ctypes import (POINTER, Structure, c_char_p, c_double, c_float, c_int, c_int32, c_int64, c_uint32, c_uint64,
+                    c_void_p)
 from pathlib import Path
 
 import numpy as np
@@ -106,6 +107,33 @@ class Rotation(Structure):
                 ("interleaved", c_int32)]
 
 
+NORM_NONE, NORM_LAYER, NORM_RMS = 0, 1, 2
+
+
+class Counter(Structure):
+    _fields_ = [("seed", c_uint64), ("stream", c_uint32), ("step", c_uint32), ("row", c_int64), ("more_steps", c_void_p)]
+
+
+class Norm(Structure):
+    _fields_ = [("weight", c_void_p), ("bias", c_void_p), ("eps", c_double), ("kind", c_int32)]
+
+
+class Block(Structure):
+    _fields_ = [("x", c_void_p), ("residual", c_void_p), ("gate", c_void_p), ("rows", c_int64), ("cols", c_int64),
+                ("gate_rows", c_int64), ("residual_scale", c_double), ("block_scale", c_double), ("keep", c_double),
+                ("after", Norm), ("before", Norm), ("counter", Counter)]
+
+
+class BlockGrads(Structure):
+    _fields_ = [("x", c_void_p), ("residual", c_void_p), ("gate", c_void_p), ("after_weight", c_void_p),
+                ("after_bias", c_void_p), ("before_weight", c_void_p), ("before_bias", c_void_p)]
+
+
+class Policy(Structure):
+    _fields_ = [("old_logps", c_void_p), ("reference_logps", c_void_p), ("advantages", c_void_p),
+                ("temperature", c_double), ("clip_low", c_double), ("clip_high", c_double), ("kl_weight", c_double)]
+
+
 class GptConfig(Structure):
     _fields_ = [("vocab_size", c_int64), ("max_positions", c_int64), ("layers", c_int64), ("heads", c_int64),
                 ("dimension", c_int64), ("tanh_gelu", c_int32), ("flags", c_int32)]
@@ -195,6 +223,17 @@ BACKEND_ONLY = {
                              c_double]),
     "distill_grad": (c_int, [c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int64,
                              c_int64, c_double]),
+    "counter_dropout": (c_int, [c_int, c_void_p, c_void_p, c_int64, c_int64, c_double, POINTER(Counter)]),
+    "block_rows": (c_int, [c_int, c_void_p, c_void_p, c_void_p, POINTER(Block)]),
+    "block_rows_backward": (c_int, [c_int, POINTER(BlockGrads), POINTER(Block), c_void_p, c_void_p, c_void_p, c_void_p,
+                                    c_void_p, c_int64]),
+    "block_rows_workspace": (c_int, [POINTER(c_int64), c_int, c_int64, c_int64]),
+    "token_logps": (c_int, [c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_double]),
+    "token_logps_grad": (c_int, [c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_double]),
+    "preference_pairs": (c_int, [c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
+                                 c_int64, c_int64, c_int64, c_double, c_double]),
+    "policy_rows": (c_int, [c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, POINTER(Policy), c_void_p, c_int64,
+                            c_int64]),
     "event_create": (c_int, [POINTER(c_void_p)]),
     "event_destroy": (c_int, [c_void_p]),
     "event_record": (c_int, [c_void_p]),
