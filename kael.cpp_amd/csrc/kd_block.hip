@@ -110,14 +110,41 @@ struct MomentSums {
         s2 += d * d;
     }
     __device__ __forceinline__ Moments moments() const {
-        return n > 0 ? Moments{n, p + s1 / n, s2 - s1 * (s1 / n)} : Moments{0, 0, 0};
+        const double squares = s2 - s1 * (s1 / n);
+        return n > 0 ? Moments{n, p + s1 / n, squares < 0 ? 0.0 : squares} : Moments{0, 0, 0};
     }
 };
 
-__device__ __forceinline__ double wave_sum(double v) {
-#pragma unroll
-    for (int m = 32; m > 0; m /= 2) v += __shfl_xor(v, m);
+// v + the value of the lane that `Control` names, 0 where there is none.
+template <int Control, int Rows = 0xf> __device__ __forceinline__ double dpp_add(double v) {
+    int2 in, from;
+    __builtin_memcpy(&in, &v, 8);
+    from.x = __builtin_amdgcn_update_dpp(0, in.x, Control, Rows, 0xf, false);
+    from.y = __builtin_amdgcn_update_dpp(0, in.y, Control, Rows, 0xf, false);
+    double other;
+    __builtin_memcpy(&other, &from, 8);
+    return v + other;
+}
+__device__ __forceinline__ double from_lane(double v, int lane) {
+    int2 in;
+    __builtin_memcpy(&in, &v, 8);
+    in.x = __builtin_amdgcn_readlane(in.x, lane);
+    in.y = __builtin_amdgcn_readlane(in.y, lane);
+    __builtin_memcpy(&v, &in, 8);
     return v;
+}
+// Running sums in each row of 16 lanes, then the rows' last ones handed on: the whole stays in the vector registers.
+__device__ __forceinline__ double sum_of_16(double v) {
+    v = dpp_add<0x111>(v);  // row_shr by 1, 2, 4, 8
+    v = dpp_add<0x112>(v);
+    v = dpp_add<0x114>(v);
+    return dpp_add<0x118>(v);
+}
+__device__ __forceinline__ double wave_sum(double v) {
+    v = sum_of_16(v);
+    v = dpp_add<0x142, 0xa>(v);  // row_bcast:15 into rows 1 and 3
+    v = dpp_add<0x143, 0xc>(v);  // row_bcast:31 into rows 2 and 3
+    return from_lane(v, 63);
 }
 
 // Sums over the workgroup, the waves' in order; `room` holds a value a wave.
@@ -215,6 +242,161 @@ __global__ __launch_bounds__(kThreads) void block_rows_wide_kernel(T* h, T* y, d
             stats[4 * row + 2] = before.mean;
             stats[4 * row + 3] = before.rate;
         }
+    }
+}
+
+// A team of `Threads` threads has a row: each thread the columns 4 * (thread + i * Threads) .. + 3 for i < Quads.
+struct Pair {
+    double a, b;
+};
+constexpr int kMostWaves = 16;
+
+template <int Threads, int Quads> struct Team {
+    static constexpr int kWaves = Threads / 64;
+    int team, wave, lane;  // wave: its place in the team
+    __device__ __forceinline__ Team() {
+        const int wave_at = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) / 64);
+        team = wave_at / kWaves;
+        wave = wave_at % kWaves;
+        lane = threadIdx.x % 64;
+    }
+    __device__ __forceinline__ int column(int i) const { return 4 * (wave * 64 + lane + i * Threads); }
+    // How many of a row's values the team's wave w holds.
+    __device__ __forceinline__ static int held(int w, int cols) {
+        int n = 0;
+#pragma unroll
+        for (int i = 0; i < Quads; ++i) n += min(max(cols - 4 * (w * 64 + i * Threads), 0), 256);
+        return n;
+    }
+    // Lane w < kWaves gets wave w's pair; one barrier, so a team's next exchange takes another room.
+    __device__ __forceinline__ Pair exchange(Pair own, Pair* room) const {
+        if (lane == 0) room[team * kWaves + wave] = own;
+        __syncthreads();
+        const int w = lane % kMostWaves;
+        return w < kWaves ? room[team * kWaves + w] : Pair{0, 0};
+    }
+    __device__ __forceinline__ Pair sums(double a, double b, Pair* room) const {
+        a = wave_sum(a);
+        b = wave_sum(b);
+        if constexpr (kWaves == 1) return {a, b};
+        const Pair p = exchange({a, b}, room);
+        return {from_lane(sum_of_16(p.a), 15), from_lane(sum_of_16(p.b), 15)};
+    }
+    // A row's statistics. A wave's sums are taken about its first value, and the waves' means about wave 0's: see Moments.
+    template <typename T>
+    __device__ __forceinline__ RowStats stats(int kind, double eps, int cols, const Quad<T> (&v)[Quads], Pair* room) const {
+        if (kind == KD_NORM_NONE) return {0.0, 1.0};
+        const double pivot = kind == KD_NORM_LAYER ? from_lane(static_cast<double>(v[0].v[0]), 0) : 0.0;
+        double s1 = 0, s2 = 0;
+#pragma unroll
+        for (int i = 0; i < Quads; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const double d = column(i) + e < cols ? static_cast<double>(v[i].v[e]) - pivot : 0.0;
+                s1 += d;
+                s2 += d * d;
+            }
+        const double all = static_cast<double>(cols);
+        if (kind == KD_NORM_RMS) {
+            const Pair p = sums(s2, 0.0, room);
+            return {0.0, 1.0 / sqrt(p.a / all + eps)};
+        }
+        s1 = wave_sum(s1);
+        s2 = wave_sum(s2);
+        const double n = static_cast<double>(held(wave, cols)), by = n > 0 ? s1 / n : 0.0;
+        double mean = pivot + by, squares = s2 - s1 * by;
+        if constexpr (kWaves > 1) {
+            const Pair p = exchange({mean, squares}, room);
+            const int w = lane % kMostWaves;
+            const double base = from_lane(p.a, 0), count = w < kWaves ? static_cast<double>(held(w, cols)) : 0.0;
+            const double d = count > 0 ? p.a - base : 0.0;
+            s1 = from_lane(sum_of_16(count * d), 15);
+            s2 = from_lane(sum_of_16((count > 0 ? p.b : 0.0) + count * d * d), 15);
+            mean = base + s1 / all;
+            squares = s2 - s1 * (s1 / all);
+        }
+        return {mean, 1.0 / sqrt((squares < 0 ? 0.0 : squares) / all + eps)};
+    }
+};
+
+// Whether a thread's values are kept, a bit each.
+template <typename T, int Threads, int Quads>
+__device__ __forceinline__ uint32_t kept_bits(const BlockArgs<T>& a, const Team<Threads, Quads>& at, int64_t row, uint32_t step) {
+    uint32_t bits = ~0u;
+    if (a.masked) {
+        bits = 0;
+#pragma unroll
+        for (int i = 0; i < Quads; ++i) {
+            bool k[4];
+            a.mask.kept(k, static_cast<uint32_t>(row), static_cast<uint32_t>(at.column(i) / 4), step);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) bits |= (k[e] ? 1u : 0u) << (4 * i + e);
+        }
+    }
+    return bits;
+}
+
+template <typename T> __device__ __forceinline__ Quad<T> quad_or(const T* p, int64_t c, int64_t cols, T otherwise) {
+    Quad<T> q{otherwise, otherwise, otherwise, otherwise};
+    if (p != nullptr) q = load_quad(p, c, cols);
+    return q;
+}
+
+constexpr int group_of(int threads) { return threads < 256 ? 256 : threads; }
+
+// A row is read once, held in registers and written once.
+template <typename T, int Threads, int Quads>
+__global__ __launch_bounds__(group_of(Threads)) void block_rows_kernel(T* h, T* y, double* stats, BlockArgs<T> a) {
+    __shared__ Pair room[2][kMostWaves];
+    const Team<Threads, Quads> at;
+    constexpr int kTeams = group_of(Threads) / Threads;
+    static_assert(kTeams == 1 || Threads == 64, "teams that leave early may not meet at barriers");
+    const int64_t row = static_cast<int64_t>(blockIdx.x) * kTeams + at.team;
+    if (row >= a.rows) return;
+    const int cols = static_cast<int>(a.cols);
+    const int64_t base = row * a.cols;
+    Quad<T> v[Quads], r[Quads];
+#pragma unroll
+    for (int i = 0; i < Quads; ++i) {
+        v[i] = load_quad(a.x + base, at.column(i), cols);
+        r[i] = quad_or(a.residual != nullptr ? a.residual + base : nullptr, at.column(i), cols, T(0));
+    }
+    const uint32_t bits = kept_bits(a, at, row, a.mask.step_now());
+    const RowStats after = at.stats(a.after.kind, a.after.eps, cols, v, room[0]);
+#pragma unroll
+    for (int i = 0; i < Quads; ++i) {
+        const int c = at.column(i);
+        const Quad<T> gate = quad_or(a.gate != nullptr ? a.gate + row * a.gate_step : nullptr, c, cols, T(1));
+        const Quad<T> w = quad_or(a.after.weight, c, cols, T(1)), b = quad_or(a.after.bias, c, cols, T(0));
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            double n = static_cast<double>(v[i].v[e]);
+            if (a.after.kind != KD_NORM_NONE) n = after.unit(n) * static_cast<double>(w.v[e]) + static_cast<double>(b.v[e]);
+            n = bits >> (4 * i + e) & 1 ? n * a.mask.scale : 0.0;
+            v[i].v[e] = static_cast<T>(a.block_scale * static_cast<double>(gate.v[e]) * n + a.residual_scale * static_cast<double>(r[i].v[e]));
+        }
+        if (h != nullptr) store_quad(h + base, c, cols, v[i]);
+    }
+    RowStats before{0.0, 1.0};
+    if (a.before.kind != KD_NORM_NONE && (y != nullptr || stats != nullptr)) {
+        before = at.stats(a.before.kind, a.before.eps, cols, v, room[1]);
+        if (y != nullptr)
+#pragma unroll
+            for (int i = 0; i < Quads; ++i) {
+                const int c = at.column(i);
+                const Quad<T> w = quad_or(a.before.weight, c, cols, T(1)), b = quad_or(a.before.bias, c, cols, T(0));
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    v[i].v[e] = static_cast<T>(before.unit(static_cast<double>(v[i].v[e])) * static_cast<double>(w.v[e]) +
+                                               static_cast<double>(b.v[e]));
+                store_quad(y + base, c, cols, v[i]);
+            }
+    }
+    if (stats != nullptr && at.wave == 0 && at.lane == 0) {
+        stats[4 * row] = after.mean;
+        stats[4 * row + 1] = after.rate;
+        stats[4 * row + 2] = before.mean;
+        stats[4 * row + 3] = before.rate;
     }
 }
 
@@ -325,7 +507,7 @@ template <typename T> __global__ __launch_bounds__(kThreads) void block_means_ke
 
 // The sums over a segment of rows: [segment][sum][cols]. A workgroup takes 64 columns, its waves share the rows.
 template <typename T>
-__global__ __launch_bounds__(kThreads) void block_columns_kernel(double* parts, const double* means, BackArgs<T> a,
+__global__ __launch_bounds__(kThreads) void block_columns_kernel(T* parts, const double* means, BackArgs<T> a,
                                                                  int64_t rows_per_segment) {
     __shared__ double room[kThreads / 64][kSums][64];
     const uint32_t step = a.b.mask.step_now();
@@ -358,14 +540,222 @@ __global__ __launch_bounds__(kThreads) void block_columns_kernel(double* parts, 
         for (int k = 0; k < kSums; ++k) {
             double total = room[0][k][lane];
             for (int w = 1; w < kThreads / 64; ++w) total += room[w][k][lane];
-            parts[(blockIdx.y * kSums + k) * cols + c] = total;
+            parts[(blockIdx.y * kSums + k) * cols + c] = static_cast<T>(total);
         }
+}
+
+// A team's rows one after another, each read once: the rows' gradients and the sums over the team's rows. Those lie in LDS,
+// [team][wanted sum][cols up to a quad], where each thread adds to the places of its own columns: in registers they took 20 a
+// quad (40 in f64), and the row spilled. Ahead: a row is loaded while the one before it is worked on.
+// Held: the norms' weights and the gate stay in registers.
+template <typename T> constexpr int kBackThreads = std::is_same_v<T, float> ? 1024 : 512;
+
+struct SumPlaces {
+    int at[kSums];  // a sum's place in LDS, -1 if it is not wanted
+    int wanted;
+};
+template <typename T> __device__ __forceinline__ void add_quad(T* place, const Quad<T>& q) {
+    Quad<T> own;
+    T* p = static_cast<T*>(__builtin_assume_aligned(place, 16));
+    __builtin_memcpy(&own, p, sizeof own);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) own.v[e] += q.v[e];
+    __builtin_memcpy(p, &own, sizeof own);
+}
+
+template <typename T, int Quads> struct BackRow {
+    Quad<T> x[Quads], h[Quads], grad_h[Quads], grad_y[Quads];
+    RowStats after, before;
+    template <int Threads> __device__ __forceinline__ void load(const BackArgs<T>& a, const Team<Threads, Quads>& at, int64_t row, bool x_read) {
+        const int64_t base = row * a.b.cols;
+#pragma unroll
+        for (int i = 0; i < Quads; ++i) {
+            const int c = at.column(i);
+            if (x_read) x[i] = load_quad(a.b.x + base, c, a.b.cols);
+            if (a.grad_y != nullptr) {
+                h[i] = load_quad(a.h + base, c, a.b.cols);
+                grad_y[i] = load_quad(a.grad_y + base, c, a.b.cols);
+            }
+            grad_h[i] = quad_or(a.grad_h != nullptr ? a.grad_h + base : nullptr, c, a.b.cols, T(0));
+        }
+        after = a.after(row);
+        before = a.before(row);
+    }
+    // The statistics, the same for a wave's lanes, to scalar registers.
+    __device__ __forceinline__ void arrived() {
+        after = {from_lane(after.mean, 0), from_lane(after.rate, 0)};
+        before = {from_lane(before.mean, 0), from_lane(before.rate, 0)};
+    }
+};
+
+// Keeps the compiler from holding the f64 forms of a loop's f32 constants, twice the registers, all through the loop.
+__device__ __forceinline__ void converted_late(Quad<float>& q) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) asm volatile("" : "+v"(q.v[e]));
+}
+__device__ __forceinline__ void converted_late(Quad<double>&) {}
+
+template <typename T, int Threads, int Quads, bool Ahead, bool Held>
+__global__ __launch_bounds__(kBackThreads<T>) void block_back_kernel(T* parts, BackArgs<T> a, int64_t rows_per_team, SumPlaces places) {
+    constexpr int kTeams = kBackThreads<T> / Threads;
+    extern __shared__ __attribute__((aligned(16))) char shared[];
+    __shared__ Pair room[2][kMostWaves];
+    const Team<Threads, Quads> at;
+    const int64_t first = (static_cast<int64_t>(blockIdx.x) * kTeams + at.team) * rows_per_team, end = min(a.b.rows, first + rows_per_team);
+    const int cols = static_cast<int>(a.b.cols);
+    const uint32_t step = a.b.mask.step_now();
+    const bool normed = a.b.after.kind != KD_NORM_NONE, gate_sum = a.sums[kGate] != nullptr;
+    const bool branch = gate_sum || a.gate != nullptr, x_read = normed || branch;
+    Quad<T> before_w[Quads], after_w[Quads], after_b[Quads], gate[Quads];
+    const auto load_weights = [&](int i, int64_t row) {
+        const int c = at.column(i);
+        before_w[i] = quad_or(a.b.before.weight, c, cols, T(1));
+        after_w[i] = quad_or(a.b.after.weight, c, cols, T(1));
+        after_b[i] = quad_or(branch ? a.b.after.bias : nullptr, c, cols, T(0));
+        gate[i] = quad_or(a.b.gate != nullptr ? a.b.gate + row * a.b.gate_step : nullptr, c, cols, T(1));
+    };
+    if constexpr (Held)
+#pragma unroll
+        for (int i = 0; i < Quads; ++i) load_weights(i, 0);
+    const int padded = (cols + 3) & ~3;
+    T* sums = reinterpret_cast<T*>(shared) + at.team * places.wanted * padded;
+    const auto sum_place = [&](Sum k, int c) { return sums + places.at[k] * padded + c; };
+    for (int k = 0; k < places.wanted; ++k)
+#pragma unroll
+        for (int i = 0; i < Quads; ++i)
+            if (at.column(i) < cols) __builtin_memset(sums + k * padded + at.column(i), 0, 4 * sizeof(T));
+    BackRow<T, Quads> now, next;
+    if (Ahead && first < end) next.load(a, at, first, x_read);
+    for (int64_t n = 0; n < rows_per_team; ++n) {
+        const int64_t row = first + n, base = row * a.b.cols;
+        const bool here = row < end;  // the same for all threads of a team; the teams meet at the barriers
+        if constexpr (Ahead) {
+            now = next;
+            if (row + 1 < end) next.load(a, at, row + 1, x_read);
+        } else if (here) {
+            now.load(a, at, row, x_read);
+        }
+        if (here) now.arrived();
+        if constexpr (Held) {
+#pragma unroll
+            for (int i = 0; i < Quads; ++i) {
+                converted_late(before_w[i]);
+                converted_late(after_w[i]);
+                converted_late(after_b[i]);
+                converted_late(gate[i]);
+            }
+        }
+        double p_sum = 0, pv_sum = 0;
+        uint32_t bits = 0;
+        if (here) {
+            bits = kept_bits(a.b, at, row, step);
+            if (a.grad_y != nullptr) {
+#pragma unroll
+                for (int i = 0; i < Quads; ++i) {
+                    Quad<T> by_weight;
+                    if constexpr (!Held) before_w[i] = quad_or(a.b.before.weight, at.column(i), cols, T(1));
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const double g = static_cast<double>(now.grad_y[i].v[e]), p = g * static_cast<double>(before_w[i].v[e]);
+                        const double v = now.before.unit(static_cast<double>(now.h[i].v[e]));
+                        p_sum += p;
+                        pv_sum += p * v;
+                        by_weight.v[e] = static_cast<T>(g * v);
+                    }
+                    if (at.column(i) < cols) {
+                        if (places.at[kBeforeWeight] >= 0) add_quad(sum_place(kBeforeWeight, at.column(i)), by_weight);
+                        if (places.at[kBeforeBias] >= 0) add_quad(sum_place(kBeforeBias, at.column(i)), now.grad_y[i]);
+                    }
+                }
+            }
+        }
+        double mean = 0, along = 0;
+        if (a.grad_y != nullptr) {
+            const Pair s = at.sums(p_sum, pv_sum, room[0]);
+            mean = a.b.before.kind == KD_NORM_LAYER ? s.a / cols : 0.0;
+            along = s.b / cols;
+        }
+        double q_sum = 0, qu_sum = 0, d[Quads][4];
+        if (here) {
+#pragma unroll
+            for (int i = 0; i < Quads; ++i) {
+                const int c = at.column(i);
+                if constexpr (!Held) load_weights(i, row);
+                else if (a.b.gate_step != 0) gate[i] = load_quad(a.b.gate + row * a.b.gate_step, c, cols);
+                Quad<T> to_residual, to_gate, by_weight, by_bias;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    double g = static_cast<double>(now.grad_h[i].v[e]);
+                    if (a.grad_y != nullptr)
+                        g += now.before.rate * (static_cast<double>(now.grad_y[i].v[e]) * static_cast<double>(before_w[i].v[e]) - mean -
+                                                now.before.unit(static_cast<double>(now.h[i].v[e])) * along);
+                    to_residual.v[e] = static_cast<T>(a.b.residual_scale * g);
+                    const bool kept = bits >> (4 * i + e) & 1;
+                    d[i][e] = kept ? a.b.block_scale * static_cast<double>(gate[i].v[e]) * g * a.b.mask.scale : 0.0;
+                    double u = 0;
+                    if (x_read) u = now.after.unit(static_cast<double>(now.x[i].v[e]));
+                    if (branch) {
+                        const double b = normed ? u * static_cast<double>(after_w[i].v[e]) + static_cast<double>(after_b[i].v[e]) : u;
+                        const double own = kept ? a.b.block_scale * (b * a.b.mask.scale) * g : 0.0;
+                        to_gate.v[e] = static_cast<T>(own);
+                    }
+                    if (normed && c + e < cols) {
+                        by_weight.v[e] = static_cast<T>(d[i][e] * u);
+                        by_bias.v[e] = static_cast<T>(d[i][e]);
+                        const double q = d[i][e] * static_cast<double>(after_w[i].v[e]);
+                        q_sum += q;
+                        qu_sum += q * u;
+                    }
+                }
+                if (c < cols) {
+                    if (places.at[kAfterWeight] >= 0) add_quad(sum_place(kAfterWeight, c), by_weight);
+                    if (places.at[kAfterBias] >= 0) add_quad(sum_place(kAfterBias, c), by_bias);
+                    if (gate_sum) add_quad(sum_place(kGate, c), to_gate);
+                }
+                if (a.residual != nullptr) store_quad(a.residual + base, c, cols, to_residual);
+                if (a.gate != nullptr) store_quad(a.gate + base, c, cols, to_gate);
+            }
+        }
+        if (normed) {
+            const Pair s = at.sums(q_sum, qu_sum, room[1]);
+            mean = a.b.after.kind == KD_NORM_LAYER ? s.a / cols : 0.0;
+            along = s.b / cols;
+        }
+        if (here && a.x != nullptr) {
+#pragma unroll
+            for (int i = 0; i < Quads; ++i) {
+                Quad<T> to;
+                if constexpr (!Held) after_w[i] = quad_or(a.b.after.weight, at.column(i), cols, T(1));
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    double g = d[i][e];
+                    if (normed)
+                        g = now.after.rate * (g * static_cast<double>(after_w[i].v[e]) - mean -
+                                              now.after.unit(static_cast<double>(now.x[i].v[e])) * along);
+                    to.v[e] = static_cast<T>(g);
+                }
+                store_quad(a.x + base, at.column(i), cols, to);
+            }
+        }
+    }
+    // the teams' sums in order
+    __syncthreads();
+    for (int k = 0; k < kSums; ++k) {
+        if (places.at[k] < 0) continue;
+        T* out = parts + (static_cast<int64_t>(blockIdx.x) * kSums + k) * cols;
+        const T* own = reinterpret_cast<const T*>(shared) + places.at[k] * padded;
+        for (int c = threadIdx.x; c < cols; c += kBackThreads<T>) {
+            double total = static_cast<double>(own[c]);
+            for (int t = 1; t < kTeams; ++t) total += static_cast<double>(own[t * places.wanted * padded + c]);
+            out[c] = static_cast<T>(total);
+        }
+    }
 }
 
 // The segments' sums in order: a workgroup takes 64 columns of one sum, its 16 waves a run of segments each.
 constexpr int kJoinWaves = 16;
 template <typename T>
-__global__ __launch_bounds__(kJoinWaves * 64) void block_join_kernel(BackArgs<T> a, const double* parts, int64_t segments) {
+__global__ __launch_bounds__(kJoinWaves * 64) void block_join_kernel(BackArgs<T> a, const T* parts, int64_t segments) {
     __shared__ double room[kJoinWaves][64];
     const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
     T* out = a.sums[blockIdx.y];
@@ -374,7 +764,7 @@ __global__ __launch_bounds__(kJoinWaves * 64) void block_join_kernel(BackArgs<T>
     const int64_t run = (segments + kJoinWaves - 1) / kJoinWaves;
     double sum = 0;
     if (c < cols)
-        for (int64_t s = wave * run; s < min(segments, (wave + 1) * run); ++s) sum += parts[(s * kSums + blockIdx.y) * cols + c];
+        for (int64_t s = wave * run; s < min(segments, (wave + 1) * run); ++s) sum += static_cast<double>(parts[(s * kSums + blockIdx.y) * cols + c]);
     room[wave][lane] = sum;
     __syncthreads();
     if (wave != 0 || c >= cols) return;
@@ -384,12 +774,44 @@ __global__ __launch_bounds__(kJoinWaves * 64) void block_join_kernel(BackArgs<T>
 
 // ---- plans and checks -----------------------------------------------------------------------------
 
-// Segments of rows whose sums are kept apart: enough to fill the card, at most 64 MiB of them.
-int64_t segments_of(int64_t rows, int64_t cols) {
-    const int64_t most = std::max<int64_t>(1, (int64_t{64} << 20) / (cols * kSums * 8));
-    return std::max<int64_t>(1, std::min({(rows + 15) / 16, int64_t{1024}, most}));
+// How a backward pass is divided. threads: a row's team, 0 for rows that registers do not hold; segments: parts of the rows
+// whose sums are kept apart.
+struct BackPlan {
+    int threads, quads;
+    int64_t rows_per_team, segments;
+};
+int group_threads(int dtype) { return dtype == KD_F32 ? kBackThreads<float> : kBackThreads<double>; }
+// Bytes of LDS that `wanted` sums take for teams of `threads`.
+int64_t sums_bytes(int dtype, int64_t cols, int threads, int wanted) {
+    return group_threads(dtype) / threads * wanted * ((cols + 3) / 4 * 4) * dtype_size(dtype);
 }
-int64_t means_bytes(int64_t rows) { return rows * 16; }
+BackPlan wide_plan(int64_t rows, int64_t cols) {
+    // enough segments to fill the card, at most 64 MiB of them
+    const int64_t most = std::max<int64_t>(1, (int64_t{64} << 20) / (cols * kSums * 8));
+    const int64_t segments = std::max<int64_t>(1, std::min({(rows + 15) / 16, int64_t{1024}, most}));
+    const int64_t each = (rows + segments - 1) / segments;
+    return {0, 0, each, (rows + each - 1) / each};
+}
+BackPlan back_plan(int dtype, int64_t rows, int64_t cols, int wanted) {
+    if (cols > (dtype == KD_F32 ? 8192 : 4096)) return wide_plan(rows, cols);
+    const int group = group_threads(dtype);
+    int threads = 64;
+    while (threads < group && threads * 4 < cols) threads *= 2;
+    if (sums_bytes(dtype, cols, threads, wanted) > 159 * 1024) return wide_plan(rows, cols);
+    const int64_t teams = group / threads;
+    const int64_t each = std::clamp<int64_t>((rows + teams * compute_units() - 1) / (teams * compute_units()), 1, 32);
+    return {threads, threads * 4 < cols ? 2 : 1, each, (rows + teams * each - 1) / (teams * each)};
+}
+// What the passes of any number of sums need at most.
+int64_t room_of(int dtype, int64_t rows, int64_t cols) {
+    if (rows == 0 || cols == 0) return 0;
+    int64_t most = 0;
+    for (int wanted = 1; wanted <= kSums; ++wanted) {
+        const BackPlan plan = back_plan(dtype, rows, cols, wanted);
+        most = std::max(most, (plan.threads == 0 ? rows * 16 : 0) + plan.segments * kSums * cols * dtype_size(dtype));
+    }
+    return most;
+}
 
 bool fits(int64_t rows, int64_t cols) { return rows <= (int64_t{1} << 40) && cols <= (int64_t{1} << 40) && (cols == 0 || rows <= (int64_t{1} << 46) / cols); }
 
@@ -492,9 +914,19 @@ extern "C" int kd_block_rows(int dtype, void* h, void* y, double* stats, const k
     const auto launch = [&](auto zero) {
         using T = decltype(zero);
         const BlockArgs<T> a = args_of<T>(b, mask);
-        const uint32_t groups = static_cast<uint32_t>(std::min<int64_t>(b.rows, int64_t{compute_units()} * 32));
-        hipLaunchKernelGGL((block_rows_wide_kernel<T>), dim3(groups), dim3(kThreads), 0, stream(), static_cast<T*>(h),
-                           static_cast<T*>(y), stats, a);
+        const auto one = [&](auto kernel, int threads, int64_t groups) {
+            hipLaunchKernelGGL(kernel, dim3(static_cast<uint32_t>(groups)), dim3(threads), 0, stream(), static_cast<T*>(h),
+                               static_cast<T*>(y), stats, a);
+        };
+        if (b.rows >= int64_t{1} << 22 || b.cols > 16384)
+            one(block_rows_wide_kernel<T>, kThreads, std::min<int64_t>(b.rows, int64_t{compute_units()} * 32));
+        else if (b.cols <= 256) one(block_rows_kernel<T, 64, 1>, 256, (b.rows + 3) / 4);
+        else if (b.cols <= 512) one(block_rows_kernel<T, 64, 2>, 256, (b.rows + 3) / 4);
+        else if (b.cols <= 1024) one(block_rows_kernel<T, 256, 1>, 256, b.rows);
+        else if (b.cols <= 2048) one(block_rows_kernel<T, 256, 2>, 256, b.rows);
+        else if (b.cols <= 4096) one(block_rows_kernel<T, 512, 2>, 512, b.rows);
+        else if (b.cols <= 8192) one(block_rows_kernel<T, 1024, 2>, 1024, b.rows);
+        else one(block_rows_kernel<T, 1024, 4>, 1024, b.rows);
     };
     if (dtype == KD_F32) launch(0.f);
     else launch(0.0);
@@ -506,7 +938,7 @@ extern "C" int kd_block_rows_workspace(int64_t* bytes, int dtype, int64_t rows, 
     const std::string name("kd_block_rows_workspace");
     if (dtype != KD_F32 && dtype != KD_F64) return fail(KD_E_UNSUPPORTED, name + ": dtype must be f32 or f64");
     if (bytes == nullptr || rows < 0 || cols < 0 || !fits(rows, cols)) return fail(KD_E_INVALID, name + ": bad arguments");
-    *bytes = rows == 0 || cols == 0 ? 0 : means_bytes(rows) + segments_of(rows, cols) * kSums * cols * 8;
+    *bytes = room_of(dtype, rows, cols);
     return KD_OK;
 }
 
@@ -541,7 +973,7 @@ extern "C" int kd_block_rows_backward(int dtype, const kd_block_grads* grads, co
             const void* at;
             int64_t bytes;
         };
-        needed = means_bytes(b.rows) + segments_of(b.rows, b.cols) * kSums * b.cols * 8;
+        needed = room_of(dtype, b.rows, b.cols);
         const bool x_read = b.after.kind != KD_NORM_NONE || grads->gate != nullptr;
         const Memory outs[] = {{grads->x, bytes}, {grads->residual, bytes}, {grads->gate, b.gate_rows * row_bytes},
                                {grads->after_weight, row_bytes}, {grads->after_bias, row_bytes},
@@ -571,25 +1003,40 @@ extern "C" int kd_block_rows_backward(int dtype, const kd_block_grads* grads, co
                       static_cast<const T*>(grad_y), static_cast<T*>(grads->x), static_cast<T*>(grads->residual),
                       shared_gate ? nullptr : static_cast<T*>(grads->gate), {}};
         for (int k = 0; k < kSums; ++k) a.sums[k] = static_cast<T*>(sums[k]);
+        SumPlaces places;
+        places.wanted = 0;
+        for (int k = 0; k < kSums; ++k) places.at[k] = sums[k] != nullptr ? places.wanted++ : -1;
+        const BackPlan plan = b.rows > 0 ? back_plan(dtype, b.rows, b.cols, places.wanted) : BackPlan{0, 0, 0, 0};
+        const int64_t column_groups = (b.cols + 63) / 64;
+        if (!fits_grid(column_groups, kJoinWaves * 64) || !fits_grid(plan.segments, kBackThreads<float>))
+            return fail(KD_E_INVALID, name + ": too many rows or columns");
         const uint32_t groups = static_cast<uint32_t>(std::min<int64_t>(b.rows, int64_t{compute_units()} * 32));
-        if (summed) {
-            const int64_t column_groups = (b.cols + 63) / 64;
-            if (!fits_grid(column_groups, kJoinWaves * 64)) return fail(KD_E_INVALID, name + ": too many columns");
-            double* means = static_cast<double*>(workspace);
-            double* parts = means + 2 * b.rows;
-            int64_t segments = 0;
-            if (b.rows > 0) {
-                segments = segments_of(b.rows, b.cols);
-                const int64_t per_segment = (b.rows + segments - 1) / segments;
-                segments = (b.rows + per_segment - 1) / per_segment;
-                hipLaunchKernelGGL((block_means_kernel<T>), dim3(groups), dim3(kThreads), 0, stream(), means, a);
-                hipLaunchKernelGGL((block_columns_kernel<T>), dim3(static_cast<uint32_t>(column_groups), static_cast<uint32_t>(segments)),
-                                   dim3(kThreads), 0, stream(), parts, means, a, per_segment);
-            }
-            hipLaunchKernelGGL((block_join_kernel<T>), dim3(static_cast<uint32_t>(column_groups), kSums), dim3(kJoinWaves * 64), 0,
-                               stream(), a, parts, segments);
+        double* means = static_cast<double*>(workspace);
+        T* parts = summed ? reinterpret_cast<T*>(means + (plan.threads == 0 ? 2 * b.rows : 0)) : nullptr;
+        if (b.rows > 0 && plan.threads == 0 && summed) {
+            hipLaunchKernelGGL((block_means_kernel<T>), dim3(groups), dim3(kThreads), 0, stream(), means, a);
+            hipLaunchKernelGGL((block_columns_kernel<T>), dim3(static_cast<uint32_t>(column_groups), static_cast<uint32_t>(plan.segments)),
+                               dim3(kThreads), 0, stream(), parts, means, a, plan.rows_per_team);
         }
-        if (by_row && b.rows > 0) hipLaunchKernelGGL((block_back_wide_kernel<T>), dim3(groups), dim3(kThreads), 0, stream(), a);
+        if (b.rows > 0 && plan.threads == 0 && by_row)
+            hipLaunchKernelGGL((block_back_wide_kernel<T>), dim3(groups), dim3(kThreads), 0, stream(), a);
+        if (plan.threads != 0) {
+            const auto one = [&](auto kernel) {
+                hipLaunchKernelGGL(kernel, dim3(static_cast<uint32_t>(plan.segments)), dim3(kBackThreads<T>),
+                                   static_cast<uint32_t>(sums_bytes(dtype, b.cols, plan.threads, places.wanted)), stream(), parts, a,
+                                   plan.rows_per_team, places);
+            };
+            constexpr int kMost = kBackThreads<T>;
+            if (plan.quads == 2) one(block_back_kernel<T, kMost, 2, false, false>);
+            else if (plan.threads == kMost) one(block_back_kernel<T, kMost, 1, true, true>);
+            else if (plan.threads == 64) one(block_back_kernel<T, 64, 1, true, true>);
+            else if (plan.threads == 128) one(block_back_kernel<T, 128, 1, true, true>);
+            else if (plan.threads == 256) one(block_back_kernel<T, 256, 1, true, true>);
+            else one(block_back_kernel<T, 512, 1, true, true>);
+        }
+        if (summed)
+            hipLaunchKernelGGL((block_join_kernel<T>), dim3(static_cast<uint32_t>(column_groups), kSums), dim3(kJoinWaves * 64), 0,
+                               stream(), a, parts, plan.segments);
         KD_LAUNCH_CHECK();
         return KD_OK;
     };
