@@ -5,6 +5,7 @@
 #include "kd_counter.h"
 #include "kd_internal.h"
 #include "kd_logits.h"
+#include "kd_waves.h"
 
 namespace kd {
 
@@ -30,90 +31,7 @@ template <> struct Tempered<double> {
     __device__ __forceinline__ double exp(double d) const { return std::exp(d * inverse); }
 };
 
-// A row's largest logit and its sum of exp((z - largest) / temperature), by a workgroup or by its first wave; `room` holds two
-// values a wave.
-template <typename T> struct RowSum {
-    T largest;
-    double sum;
-};
-template <typename T>
-__device__ __forceinline__ RowSum<T> join_rows(RowSum<T> own, const Tempered<T>& t, int lanes) {
-    for (int m = lanes / 2; m > 0; m /= 2) {
-        const T other = __shfl_xor(own.largest, m);
-        const double sum = __shfl_xor(own.sum, m);
-        const T most = max_na(own.largest, other);
-        const T base = or_zero(most);
-        own.sum = own.sum * static_cast<double>(t.exp(own.largest - base)) + sum * static_cast<double>(t.exp(other - base));
-        own.largest = most;
-    }
-    return own;
-}
-template <typename T> __device__ __forceinline__ RowSum<T> row_sum(const T* z, int64_t cols, const Tempered<T>& t, RowSum<T>* room) {
-    RowSum<T> own{static_cast<T>(-INFINITY), 0.0};
-    for (int64_t c = threadIdx.x; c < cols; c += blockDim.x) {
-        const T v = z[c], most = max_na(own.largest, v), base = or_zero(most);
-        own.sum = own.sum * static_cast<double>(t.exp(own.largest - base)) + static_cast<double>(t.exp(v - base));
-        own.largest = most;
-    }
-    own = join_rows(own, t, 64);
-    __syncthreads();
-    if (threadIdx.x % 64 == 0) room[threadIdx.x / 64] = own;
-    __syncthreads();
-    own = room[0];
-    for (int w = 1; w < static_cast<int>(blockDim.x) / 64; ++w) {
-        const RowSum<T> o = room[w];
-        const T most = max_na(own.largest, o.largest), base = or_zero(most);
-        own.sum = own.sum * static_cast<double>(t.exp(own.largest - base)) + o.sum * static_cast<double>(t.exp(o.largest - base));
-        own.largest = most;
-    }
-    return own;
-}
-
-template <typename T>
-__device__ __forceinline__ double logp_of(T at, const RowSum<T>& s, double temperature) {
-    return (static_cast<double>(at) - static_cast<double>(s.largest)) / temperature - log(s.sum);
-}
-
 __device__ __forceinline__ bool is_target(int64_t t, int64_t cols) { return t >= 0 && t < cols; }
-
-template <typename T>
-__global__ __launch_bounds__(256) void token_logps_kernel(double* logps, T* stats, const T* logits, const int64_t* targets, int64_t cols,
-                                                          double temperature, Tempered<T> t) {
-    __shared__ RowSum<T> room[4];
-    const int64_t row = blockIdx.x, target = targets[row];
-    if (!is_target(target, cols)) {
-        if (threadIdx.x == 0) {
-            logps[row] = 0;
-            stats[2 * row] = 0;
-            stats[2 * row + 1] = 1;
-        }
-        return;
-    }
-    const T* z = logits + row * cols;
-    const RowSum<T> s = row_sum(z, cols, t, room);
-    if (threadIdx.x == 0) {
-        logps[row] = logp_of(z[target], s, temperature);
-        stats[2 * row] = s.largest;
-        stats[2 * row + 1] = static_cast<T>(s.sum);
-    }
-}
-
-// slope / temperature ((c == target) - softmax_c) for a row; 0 for a slope of 0.
-template <typename T>
-__device__ __forceinline__ void write_grad(T* g, const T* z, int64_t cols, int64_t target, T largest, T sum, double slope,
-                                           double temperature, const Tempered<T>& t) {
-    const T by = static_cast<T>(slope / temperature), factor = static_cast<T>(slope / temperature / static_cast<double>(sum));
-    for (int64_t c = threadIdx.x; c < cols; c += blockDim.x)
-        g[c] = slope == 0 ? T(0) : (c == target ? by : T(0)) - t.exp(z[c] - largest) * factor;
-}
-
-template <typename T>
-__global__ __launch_bounds__(256) void token_logps_grad_kernel(T* out, const T* logits, const T* stats, const int64_t* targets,
-                                                               const T* slopes, int64_t cols, double temperature, Tempered<T> t) {
-    const int64_t row = blockIdx.x, target = targets[row];
-    const double slope = is_target(target, cols) ? static_cast<double>(slopes[row]) : 0.0;
-    write_grad(out + row * cols, logits + row * cols, cols, target, stats[2 * row], stats[2 * row + 1], slope, temperature, t);
-}
 
 // ---- pairs ----------------------------------------------------------------------------------------
 
@@ -143,7 +61,7 @@ template <typename T> __global__ __launch_bounds__(256) void preference_pairs_ke
     for (int i = 0; i < 2; ++i) {
         for (int64_t r = at[i] + threadIdx.x; r < at[i + 1]; r += blockDim.x)
             if (is_target(a.targets[r], a.cols)) sums[i] += a.logps[r] - (a.reference != nullptr ? a.reference[r] : 0.0);
-        sums[i] = wave_sum(sums[i]);
+        sums[i] = wave_total(sums[i]);
         if (threadIdx.x % 64 == 0) room[i][threadIdx.x / 64] = sums[i];
     }
     __syncthreads();
@@ -178,7 +96,7 @@ template <typename T> struct Policy {
     const double* reference_logps;
     const T* advantages;
     const T* row_weights;
-    double temperature, low, high, kl_weight;
+    double low, high, kl_weight;
 };
 
 // A row's loss and its derivative with respect to the log-probability.
@@ -201,26 +119,185 @@ template <typename T> __device__ __forceinline__ void policy_terms(const Policy<
     }
 }
 
-template <typename T>
-__global__ __launch_bounds__(256) void policy_rows_kernel(T* losses, double* logps, T* grad, const T* logits, const int64_t* targets,
-                                                          int64_t cols, Policy<T> a, Tempered<T> t) {
-    __shared__ RowSum<T> room[4];
-    const int64_t row = blockIdx.x, target = targets[row];
+// ---- rows -----------------------------------------------------------------------------------------
+//
+// The log-probability of a row's target, and with `policy` the row's loss and gradient. A row is read once and held in the
+// registers of its team (a wave, or a workgroup): its largest logit, then the exponentials in the logits' places and their sum,
+// then the gradient from them. What a team's registers do not hold of a long row is read again, from the caches for the most part.
+// Bound by the logits read and the gradient written.
+
+template <typename T> struct AnswerRows {
+    T* losses;
+    T* grad;
+    T* stats;
+    double* logps;
+    const T* logits;
+    const int64_t* targets;
+    int64_t rows, cols;
+    double temperature;
+    Tempered<T> t;
+    bool with_policy;
+    Policy<T> policy;
+};
+
+// What a team writes a row's gradient from: -e * factor, and by more at the target.
+template <typename T> struct Slope {
+    T factor, by;
+};
+template <typename T> __device__ __forceinline__ Slope<T> slope_of(double slope, double sum, double temperature) {
+    const double by = slope / temperature;
+    if (slope == 0) return {0, 0};  // whatever the row holds
+    return {static_cast<T>(by / sum), static_cast<T>(by)};
+}
+
+// The gradient of a piece whose exponentials are given.
+template <bool Past, typename T>
+__device__ __forceinline__ void store_grad(T* g, int64_t at, int64_t cols, Piece<T> p, int64_t target, const Slope<T>& s) {
+    constexpr int kCount = Piece<T>::kCount;
+#pragma unroll
+    for (int j = 0; j < kCount; ++j) p.x[j] = s.factor == 0 && s.by == 0 ? T(0) : (at + j == target ? s.by : T(0)) - p.x[j] * s.factor;
+    if (at + kCount <= cols) {
+        store_piece<Past>(g + at, p);
+    } else {
+#pragma unroll
+        for (int j = 0; j < kCount; ++j)
+            if (at + j < cols) g[at + j] = p.x[j];
+    }
+}
+
+constexpr int group_of(int threads) { return threads < 256 ? 256 : threads; }
+
+template <typename T, int Threads, int Pieces, bool Past>
+__global__ __launch_bounds__(group_of(Threads)) void answer_rows_kernel(AnswerRows<T> a) {
+    constexpr int kWaves = Threads / 64, kTeams = group_of(Threads) / Threads, kCount = Piece<T>::kCount;
+    static_assert(kTeams == 1 || kWaves == 1, "teams that leave early may not meet at barriers");
+    __shared__ T room_most[16];
+    __shared__ double room_sum[16];
+    __shared__ Slope<T> room_slope;
+    const int wave_at = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) / 64), lane = threadIdx.x % 64;
+    const int wave = wave_at % kWaves;
+    const int64_t row = static_cast<int64_t>(blockIdx.x) * kTeams + wave_at / kWaves;
+    if (row >= a.rows) return;
+    const int64_t target = from_lane(a.targets[row], 0), own = static_cast<int64_t>(wave * 64 + lane) * kCount;
+    constexpr int64_t kStep = Threads * kCount, kHeld = kStep * Pieces;
+    T* g = a.grad != nullptr ? a.grad + row * a.cols : nullptr;
+    if (!is_target(target, a.cols)) {
+        if (g != nullptr)
+            for (int64_t at = own; at < a.cols; at += kStep) store_grad<Past>(g, at, a.cols, Piece<T>{}, -1, Slope<T>{0, 0});
+        if (wave == 0 && lane == 0) {
+            if (a.losses != nullptr) a.losses[row] = 0;
+            if (a.logps != nullptr) a.logps[row] = 0;
+            if (a.stats != nullptr) {
+                a.stats[2 * row] = 0;
+                a.stats[2 * row + 1] = 1;
+            }
+        }
+        return;
+    }
+    const T* z = a.logits + row * a.cols;
+    const T lowest = static_cast<T>(-INFINITY);
+    Piece<T> v[Pieces];
+#pragma unroll
+    for (int i = 0; i < Pieces; ++i) v[i] = load_piece<Past>(z, own + i * kStep, a.cols, lowest);
+    const T there = z[target];
+    T most = lowest;  // a NaN is passed over here and comes through its exponential
+#pragma unroll
+    for (int i = 0; i < Pieces; ++i)
+#pragma unroll
+        for (int j = 0; j < kCount; ++j) most = fmax(most, v[i].x[j]);
+    for (int64_t at = own + kHeld; at < a.cols; at += kStep) {
+        const Piece<T> p = load_piece(z, at, a.cols, lowest);
+#pragma unroll
+        for (int j = 0; j < kCount; ++j) most = fmax(most, p.x[j]);
+    }
+    most = wave_most(most);
+    if constexpr (kWaves > 1) {
+        if (lane == 0) room_most[wave] = most;
+        __syncthreads();
+        most = from_lane(most_of_16(room_most[lane % 16 < kWaves ? lane % 16 : 0]), 15);
+    }
+    const T base = or_zero(most);
+    double sum = 0;
+#pragma unroll
+    for (int i = 0; i < Pieces; ++i)
+#pragma unroll
+        for (int j = 0; j < kCount; ++j) {
+            v[i].x[j] = a.t.exp(v[i].x[j] - base);
+            sum += static_cast<double>(v[i].x[j]);
+        }
+    for (int64_t at = own + kHeld; at < a.cols; at += kStep) {
+        const Piece<T> p = load_piece(z, at, a.cols, lowest);
+#pragma unroll
+        for (int j = 0; j < kCount; ++j) sum += static_cast<double>(a.t.exp(p.x[j] - base));
+    }
+    sum = wave_total(sum);
+    if constexpr (kWaves > 1) {
+        if (lane == 0) room_sum[wave] = sum;
+        __syncthreads();
+        sum = from_lane(sum_of_16(lane % 16 < kWaves ? room_sum[lane % 16] : 0.0), 15);
+    }
+    Slope<T> slope{0, 0};
+    if (wave == 0) {
+        const double lp = (static_cast<double>(there) - static_cast<double>(most)) / a.temperature - log(sum);
+        double loss = 0, derivative = 0;
+        if (a.with_policy) {
+            policy_terms(a.policy, row, lp, loss, derivative);
+            if (g != nullptr) slope = slope_of<T>(derivative * static_cast<double>(a.policy.row_weights[row]), sum, a.temperature);
+        }
+        if (lane == 0) {
+            if (a.losses != nullptr) a.losses[row] = static_cast<T>(loss);
+            if (a.logps != nullptr) a.logps[row] = lp;
+            if (a.stats != nullptr) {
+                a.stats[2 * row] = most;
+                a.stats[2 * row + 1] = static_cast<T>(sum);
+            }
+            if (kWaves > 1) room_slope = slope;
+        }
+    }
+    if (g == nullptr) return;
+    if constexpr (kWaves > 1) {
+        __syncthreads();
+        slope = room_slope;
+    }
+#pragma unroll
+    for (int i = 0; i < Pieces; ++i)
+        if (own + i * kStep < a.cols) store_grad<Past>(g, own + i * kStep, a.cols, v[i], target, slope);
+    for (int64_t at = own + kHeld; at < a.cols; at += kStep) {
+        Piece<T> p = load_piece(z, at, a.cols, lowest);
+#pragma unroll
+        for (int j = 0; j < kCount; ++j) p.x[j] = a.t.exp(p.x[j] - base);
+        store_grad<Past>(g, at, a.cols, p, target, slope);
+    }
+}
+
+// The gradient from a row's statistics: a workgroup takes `span` columns of a row, the last rows first, whose logits the caches
+// may still hold from kd_token_logps.
+template <typename T, bool PastLoads, bool PastStores>
+__global__ __launch_bounds__(256) void token_logps_grad_kernel(T* out, const T* logits, const T* stats, const int64_t* targets,
+                                                               const T* slopes, int64_t rows, int64_t cols, double temperature,
+                                                               Tempered<T> t, int64_t span, int spans) {
+    constexpr int kCount = Piece<T>::kCount, kPieces = 4;
+    const int64_t row = rows - 1 - blockIdx.x / spans, from = blockIdx.x % spans * span, to = min(from + span, cols);
+    const int64_t target = targets[row];
+    const double own = is_target(target, cols) ? static_cast<double>(slopes[row]) : 0.0;
+    const Slope<T> slope = slope_of<T>(own, static_cast<double>(stats[2 * row + 1]), temperature);
+    const T base = or_zero(stats[2 * row]);
     const T* z = logits + row * cols;
-    RowSum<T> s{T(0), 1.0};
-    double lp = 0, loss = 0, slope = 0;
-    if (is_target(target, cols)) {
-        s = row_sum(z, cols, t, room);
-        lp = logp_of(z[target], s, a.temperature);
-        policy_terms(a, row, lp, loss, slope);
-        if (grad != nullptr) slope *= static_cast<double>(a.row_weights[row]);
+    T* g = out + row * cols;
+    constexpr int64_t kStep = 256 * kCount;
+    for (int64_t at = from + static_cast<int64_t>(threadIdx.x) * kCount; at < to; at += kPieces * kStep) {
+        Piece<T> p[kPieces] = {};
+        if (own != 0)
+#pragma unroll
+            for (int i = 0; i < kPieces; ++i) p[i] = load_piece<PastLoads>(z, at + i * kStep, to, base);
+#pragma unroll
+        for (int i = 0; i < kPieces; ++i) {
+            if (at + i * kStep >= to) continue;
+#pragma unroll
+            for (int j = 0; j < kCount; ++j) p[i].x[j] = t.exp(p[i].x[j] - base);
+            store_grad<PastStores>(g, at + i * kStep, to, p[i], target, slope);
+        }
     }
-    __syncthreads();  // the target's logit is read before its place is written
-    if (threadIdx.x == 0) {
-        losses[row] = static_cast<T>(loss);
-        if (logps != nullptr) logps[row] = lp;
-    }
-    if (grad != nullptr) write_grad(grad + row * cols, z, cols, target, s.largest, static_cast<T>(s.sum), slope, a.temperature, t);
 }
 
 // ---- checks ---------------------------------------------------------------------------------------
@@ -232,6 +309,30 @@ int check_rows(const std::string& name, int dtype, int64_t rows, int64_t cols, d
     if (!(temperature >= 1e-6 && temperature <= 1e6))
         return fail(KD_E_INVALID, name + ": temperature must be between 1e-6 and 1e6");
     return KD_OK;
+}
+
+// A team's threads and the 16-byte pieces that each of them holds, by the row's pieces.
+template <typename T> void launch_rows(const AnswerRows<T>& a) {
+    const int64_t pieces = (a.cols + Piece<T>::kCount - 1) / Piece<T>::kCount;
+    const bool past = a.rows * a.cols * static_cast<int64_t>(sizeof(T)) > int64_t{96} << 20;
+    const auto one = [&](auto kernel, int threads) {
+        const int teams = group_of(threads) / threads;
+        hipLaunchKernelGGL(kernel, dim3(static_cast<uint32_t>((a.rows + teams - 1) / teams)), dim3(group_of(threads)), 0, stream(), a);
+    };
+    const auto both = [&](auto threads, auto held) {
+        constexpr int kThreads = decltype(threads)::value, kPieces = decltype(held)::value;
+        if (past) one(answer_rows_kernel<T, kThreads, kPieces, true>, kThreads);
+        else one(answer_rows_kernel<T, kThreads, kPieces, false>, kThreads);
+    };
+    using std::integral_constant;
+    if (pieces <= 64) both(integral_constant<int, 64>{}, integral_constant<int, 1>{});
+    else if (pieces <= 256) both(integral_constant<int, 64>{}, integral_constant<int, 4>{});
+    else if (pieces <= 1024) both(integral_constant<int, 256>{}, integral_constant<int, 4>{});
+    else if (pieces <= 2048) both(integral_constant<int, 512>{}, integral_constant<int, 4>{});
+    else if (pieces <= 4096) both(integral_constant<int, 1024>{}, integral_constant<int, 4>{});
+    else if (pieces <= 8192) both(integral_constant<int, 1024>{}, integral_constant<int, 8>{});
+    else if (pieces <= 13 * 1024) both(integral_constant<int, 1024>{}, integral_constant<int, 13>{});
+    else both(integral_constant<int, 1024>{}, integral_constant<int, 20>{});
 }
 
 // Whether `out` is neither apart from the logits nor the logits themselves.
@@ -256,8 +357,9 @@ extern "C" int kd_token_logps(int dtype, double* logps, void* stats, const void*
     if (int rc = ensure_device()) return rc;
     const auto launch = [&](auto zero) {
         using T = decltype(zero);
-        hipLaunchKernelGGL((token_logps_kernel<T>), dim3(static_cast<uint32_t>(rows)), dim3(256), 0, stream(), logps,
-                           static_cast<T*>(stats), static_cast<const T*>(logits), targets, cols, temperature, Tempered<T>(temperature));
+        AnswerRows<T> a{nullptr, nullptr, static_cast<T*>(stats), logps, static_cast<const T*>(logits), targets, rows, cols, temperature,
+                        Tempered<T>(temperature), false, {}};
+        launch_rows(a);
     };
     if (dtype == KD_F32) launch(0.f);
     else launch(0.0);
@@ -274,16 +376,26 @@ extern "C" int kd_token_logps_grad(int dtype, void* out, const void* logits, con
         return fail(KD_E_INVALID, name + ": every operand must be given");
     if (crosses(out, logits, dtype, rows, cols)) return fail(KD_E_INVALID, name + ": out overlaps the logits");
     if (int rc = ensure_device()) return rc;
-    const auto launch = [&](auto zero) {
+    const auto launch = [&](auto zero) -> int {
         using T = decltype(zero);
-        hipLaunchKernelGGL((token_logps_grad_kernel<T>), dim3(static_cast<uint32_t>(rows)), dim3(256), 0, stream(),
-                           static_cast<T*>(out), static_cast<const T*>(logits), static_cast<const T*>(stats), targets,
-                           static_cast<const T*>(slopes), cols, temperature, Tempered<T>(temperature));
+        // parts of a row to a workgroup, in whole rounds of it
+        const int64_t round = int64_t{256} * 4 * Piece<T>::kCount;
+        const int64_t span = round * std::max<int64_t>(1, std::min<int64_t>((cols + round - 1) / round, 4));
+        const int64_t spans = (cols + span - 1) / span;
+        if (!fits_grid(rows * spans, 256)) return fail(KD_E_INVALID, name + ": too many rows and columns");
+        const auto one = [&](auto kernel) {
+            hipLaunchKernelGGL(kernel, dim3(static_cast<uint32_t>(rows * spans)), dim3(256), 0, stream(), static_cast<T*>(out),
+                               static_cast<const T*>(logits), static_cast<const T*>(stats), targets, static_cast<const T*>(slopes),
+                               rows, cols, temperature, Tempered<T>(temperature), span, static_cast<int>(spans));
+        };
+        const PastCaches past = past_caches(rows * cols * static_cast<int64_t>(sizeof(T)));
+        if (past.grad_stores) one(token_logps_grad_kernel<T, true, true>);
+        else if (past.grad_loads) one(token_logps_grad_kernel<T, true, false>);
+        else one(token_logps_grad_kernel<T, false, false>);
+        KD_LAUNCH_CHECK();
+        return KD_OK;
     };
-    if (dtype == KD_F32) launch(0.f);
-    else launch(0.0);
-    KD_LAUNCH_CHECK();
-    return KD_OK;
+    return dtype == KD_F32 ? launch(0.f) : launch(0.0);
 }
 
 extern "C" int kd_preference_pairs(int dtype, void* losses, void* rewards, void* slopes, const double* logps,
@@ -332,12 +444,11 @@ extern "C" int kd_policy_rows(int dtype, void* losses, double* logps, void* grad
     if (int rc = ensure_device()) return rc;
     const auto launch = [&](auto zero) {
         using T = decltype(zero);
-        const Policy<T> a{policy->old_logps, policy->reference_logps, static_cast<const T*>(policy->advantages),
-                          static_cast<const T*>(row_weights), policy->temperature, policy->clip_low, policy->clip_high,
-                          policy->kl_weight};
-        hipLaunchKernelGGL((policy_rows_kernel<T>), dim3(static_cast<uint32_t>(rows)), dim3(256), 0, stream(),
-                           static_cast<T*>(losses), logps, static_cast<T*>(grad), static_cast<const T*>(logits), targets, cols, a,
-                           Tempered<T>(policy->temperature));
+        AnswerRows<T> a{static_cast<T*>(losses), static_cast<T*>(grad), nullptr, logps, static_cast<const T*>(logits), targets, rows,
+                        cols, policy->temperature, Tempered<T>(policy->temperature), true,
+                        {policy->old_logps, policy->reference_logps, static_cast<const T*>(policy->advantages),
+                         static_cast<const T*>(row_weights), policy->clip_low, policy->clip_high, policy->kl_weight}};
+        launch_rows(a);
     };
     if (dtype == KD_F32) launch(0.f);
     else launch(0.0);

@@ -4,6 +4,7 @@
 
 #include "kd_counter.h"
 #include "kd_internal.h"
+#include "kd_waves.h"
 
 namespace kd {
 
@@ -115,42 +116,10 @@ struct MomentSums {
     }
 };
 
-// v + the value of the lane that `Control` names, 0 where there is none.
-template <int Control, int Rows = 0xf> __device__ __forceinline__ double dpp_add(double v) {
-    int2 in, from;
-    __builtin_memcpy(&in, &v, 8);
-    from.x = __builtin_amdgcn_update_dpp(0, in.x, Control, Rows, 0xf, false);
-    from.y = __builtin_amdgcn_update_dpp(0, in.y, Control, Rows, 0xf, false);
-    double other;
-    __builtin_memcpy(&other, &from, 8);
-    return v + other;
-}
-__device__ __forceinline__ double from_lane(double v, int lane) {
-    int2 in;
-    __builtin_memcpy(&in, &v, 8);
-    in.x = __builtin_amdgcn_readlane(in.x, lane);
-    in.y = __builtin_amdgcn_readlane(in.y, lane);
-    __builtin_memcpy(&v, &in, 8);
-    return v;
-}
-// Running sums in each row of 16 lanes, then the rows' last ones handed on: the whole stays in the vector registers.
-__device__ __forceinline__ double sum_of_16(double v) {
-    v = dpp_add<0x111>(v);  // row_shr by 1, 2, 4, 8
-    v = dpp_add<0x112>(v);
-    v = dpp_add<0x114>(v);
-    return dpp_add<0x118>(v);
-}
-__device__ __forceinline__ double wave_sum(double v) {
-    v = sum_of_16(v);
-    v = dpp_add<0x142, 0xa>(v);  // row_bcast:15 into rows 1 and 3
-    v = dpp_add<0x143, 0xc>(v);  // row_bcast:31 into rows 2 and 3
-    return from_lane(v, 63);
-}
-
 // Sums over the workgroup, the waves' in order; `room` holds a value a wave.
 __device__ __forceinline__ double group_sum(double v, double* room) {
     const int waves = blockDim.x / 64;
-    v = wave_sum(v);
+    v = wave_total(v);
     __syncthreads();
     if (threadIdx.x % 64 == 0) room[threadIdx.x / 64] = v;
     __syncthreads();
@@ -276,8 +245,8 @@ template <int Threads, int Quads> struct Team {
         return w < kWaves ? room[team * kWaves + w] : Pair{0, 0};
     }
     __device__ __forceinline__ Pair sums(double a, double b, Pair* room) const {
-        a = wave_sum(a);
-        b = wave_sum(b);
+        a = wave_total(a);
+        b = wave_total(b);
         if constexpr (kWaves == 1) return {a, b};
         const Pair p = exchange({a, b}, room);
         return {from_lane(sum_of_16(p.a), 15), from_lane(sum_of_16(p.b), 15)};
@@ -301,8 +270,8 @@ template <int Threads, int Quads> struct Team {
             const Pair p = sums(s2, 0.0, room);
             return {0.0, 1.0 / sqrt(p.a / all + eps)};
         }
-        s1 = wave_sum(s1);
-        s2 = wave_sum(s2);
+        s1 = wave_total(s1);
+        s2 = wave_total(s2);
         const double n = static_cast<double>(held(wave, cols)), by = n > 0 ? s1 / n : 0.0;
         double mean = pivot + by, squares = s2 - s1 * by;
         if constexpr (kWaves > 1) {
