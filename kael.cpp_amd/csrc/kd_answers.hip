@@ -99,12 +99,17 @@ template <typename T> struct Policy {
     double low, high, kl_weight;
 };
 
-// A row's loss and its derivative with respect to the log-probability.
-template <typename T> __device__ __forceinline__ void policy_terms(const Policy<T>& a, int64_t row, double lp, double& loss, double& slope) {
+// A row's loss and its derivative with respect to the log-probability, in lane l and, the same, in lane l + 32 of a wave: its
+// two exponentials are one, of the lower and the upper half.
+template <typename T>
+__device__ __forceinline__ void policy_terms(const Policy<T>& a, int64_t row, double lp, double& loss, double& slope) {
     const double advantage = static_cast<double>(a.advantages[row]);
+    const bool held_near = a.reference_logps != nullptr && a.kl_weight != 0;
+    const double moved = a.old_logps != nullptr ? lp - a.old_logps[row] : lp == lp ? 0.0 : lp, d = held_near ? a.reference_logps[row] - lp : 0.0;
+    const int lane = threadIdx.x % 64;
+    const double both = exp(lane < 32 ? moved : d), ratio = __shfl(both, lane % 32), away = __shfl(both, lane % 32 + 32);
     loss = slope = 0;
     if (advantage != 0) {
-        const double ratio = a.old_logps != nullptr ? exp(lp - a.old_logps[row]) : lp == lp ? 1.0 : lp;
         const double free = ratio * advantage, held = fmin(fmax(ratio, 1 - a.low), 1 + a.high) * advantage;
         if (held < free) {
             loss = -held;
@@ -112,10 +117,9 @@ template <typename T> __device__ __forceinline__ void policy_terms(const Policy<
             loss = slope = -free;
         }
     }
-    if (a.reference_logps != nullptr && a.kl_weight != 0) {
-        const double d = a.reference_logps[row] - lp, e = expm1(d);
-        loss += a.kl_weight * (e - d);
-        slope -= a.kl_weight * e;
+    if (held_near) {
+        loss += a.kl_weight * (away - d - 1);
+        slope += a.kl_weight * (1 - away);
     }
 }
 
@@ -134,20 +138,51 @@ template <typename T> struct AnswerRows {
     const T* logits;
     const int64_t* targets;
     int64_t rows, cols;
-    double temperature;
+    double inverse;  // 1 / temperature
     Tempered<T> t;
     bool with_policy;
     Policy<T> policy;
 };
 
-// What a team writes a row's gradient from: -e * factor, and by more at the target.
+// The gradient's factors of a row: -e * factor, and by more at the target.
 template <typename T> struct Slope {
     T factor, by;
 };
-template <typename T> __device__ __forceinline__ Slope<T> slope_of(double slope, double sum, double temperature) {
-    const double by = slope / temperature;
+template <typename T> __device__ __forceinline__ Slope<T> slope_of(double slope, double sum, double inverse) {
+    const double by = slope * inverse;
     if (slope == 0) return {0, 0};  // whatever the row holds
     return {static_cast<T>(by / sum), static_cast<T>(by)};
+}
+// What is written of a row beside its gradient, from its largest logit and the sum of exponentials; the gradient's factors. A lane
+// and the one 32 above it have the same row; `lead` says which lanes write. A wave's f64 functions take as long as some hundred
+// logits a lane, so they are few, and as far as rows share a wave they are theirs together.
+template <typename T>
+__device__ __forceinline__ Slope<T> finish_row(const AnswerRows<T>& a, int64_t row, T there, T most, double sum, bool lead) {
+    const double lp = (static_cast<double>(there) - static_cast<double>(most)) * a.inverse - log(sum);
+    double loss = 0, derivative = 0;
+    Slope<T> slope{0, 0};
+    if (a.with_policy) {
+        policy_terms(a.policy, row, lp, loss, derivative);
+        if (a.grad != nullptr) slope = slope_of<T>(derivative * static_cast<double>(a.policy.row_weights[row]), sum, a.inverse);
+    }
+    if (lead) {
+        if (a.losses != nullptr) a.losses[row] = static_cast<T>(loss);
+        if (a.logps != nullptr) a.logps[row] = lp;
+        if (a.stats != nullptr) {
+            a.stats[2 * row] = most;
+            a.stats[2 * row + 1] = static_cast<T>(sum);
+        }
+    }
+    return slope;
+}
+// The same for a row without a target.
+template <typename T> __device__ __forceinline__ void empty_row(const AnswerRows<T>& a, int64_t row) {
+    if (a.losses != nullptr) a.losses[row] = 0;
+    if (a.logps != nullptr) a.logps[row] = 0;
+    if (a.stats != nullptr) {
+        a.stats[2 * row] = 0;
+        a.stats[2 * row + 1] = 1;
+    }
 }
 
 // The gradient of a piece whose exponentials are given.
@@ -165,57 +200,122 @@ __device__ __forceinline__ void store_grad(T* g, int64_t at, int64_t cols, Piece
     }
 }
 
-constexpr int group_of(int threads) { return threads < 256 ? 256 : threads; }
+// Short rows: a wave has `Rows` of them, `Pieces` a lane each.
+constexpr int kShortThreads = 256;
 
-template <typename T, int Threads, int Pieces, bool Past>
-__global__ __launch_bounds__(group_of(Threads)) void answer_rows_kernel(AnswerRows<T> a) {
-    constexpr int kWaves = Threads / 64, kTeams = group_of(Threads) / Threads, kCount = Piece<T>::kCount;
-    static_assert(kTeams == 1 || kWaves == 1, "teams that leave early may not meet at barriers");
+template <typename T, int Pieces, int Rows, bool PastLoads, bool PastStores>
+__global__ __launch_bounds__(kShortThreads) void answer_short_kernel(AnswerRows<T> a) {
+    constexpr int kCount = Piece<T>::kCount, kStep = 64 * kCount;
+    const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) / 64), lane = threadIdx.x % 64;
+    const int64_t first = (static_cast<int64_t>(blockIdx.x) * (kShortThreads / 64) + wave) * Rows;
+    if (first >= a.rows) return;
+    const T lowest = static_cast<T>(-INFINITY);
+    const int own = lane * kCount;
+    // lane r and lane 32 + r: row r's
+    const int64_t lane_row = min(first + lane % 32 % Rows, a.rows - 1), lane_target = a.targets[lane_row];
+    int64_t target[Rows];
+    Piece<T> v[Rows][Pieces];
+#pragma unroll
+    for (int r = 0; r < Rows; ++r) {
+        target[r] = from_lane(lane_target, r);
+        if (first + r >= a.rows || !is_target(target[r], a.cols)) target[r] = -1;
+        const T* z = a.logits + (first + r) * a.cols;
+#pragma unroll
+        for (int i = 0; i < Pieces; ++i)
+            if (target[r] >= 0) v[r][i] = load_piece<PastLoads>(z, own + i * kStep, a.cols, lowest);
+    }
+    const bool counted = is_target(lane_target, a.cols);
+    const T there = counted ? a.logits[lane_row * a.cols + lane_target] : T(0);
+    T lane_most = 0;
+    double lane_sum = 1;
+#pragma unroll
+    for (int r = 0; r < Rows; ++r) {
+        if (target[r] < 0) continue;
+        T most = lowest;  // a NaN is passed over here and comes through its exponential
+#pragma unroll
+        for (int i = 0; i < Pieces; ++i)
+#pragma unroll
+            for (int j = 0; j < kCount; ++j) most = fmax(most, v[r][i].x[j]);
+        most = wave_most(most);
+        const T base = or_zero(most);
+        double sum = 0;
+#pragma unroll
+        for (int i = 0; i < Pieces; ++i)
+#pragma unroll
+            for (int j = 0; j < kCount; ++j) {
+                v[r][i].x[j] = a.t.exp(v[r][i].x[j] - base);
+                sum += static_cast<double>(v[r][i].x[j]);
+            }
+        sum = wave_total(sum);
+        if (lane % 32 % Rows == r) {
+            lane_most = most;
+            lane_sum = sum;
+        }
+    }
+    Slope<T> lane_slope = finish_row(a, lane_row, there, lane_most, lane_sum, lane < Rows && counted && first + lane < a.rows);
+    if (lane < Rows && !counted && first + lane < a.rows) empty_row(a, lane_row);
+    if (a.grad == nullptr) return;
+#pragma unroll
+    for (int r = 0; r < Rows; ++r) {
+        if (first + r >= a.rows) continue;
+        Slope<T> slope{from_lane(lane_slope.factor, r), from_lane(lane_slope.by, r)};
+        if (target[r] < 0) slope = {0, 0};
+        T* g = a.grad + (first + r) * a.cols;
+#pragma unroll
+        for (int i = 0; i < Pieces; ++i)
+            if (own + i * kStep < a.cols) store_grad<PastStores>(g, own + i * kStep, a.cols, v[r][i], target[r], slope);
+    }
+}
+
+// Longer rows: a workgroup has one. More: `Pieces` a thread are not all of it.
+template <typename T, int Threads, int Pieces, bool More, bool PastLoads, bool PastStores>
+__global__ __launch_bounds__(Threads) void answer_rows_kernel(AnswerRows<T> a) {
+    constexpr int kWaves = Threads / 64, kCount = Piece<T>::kCount;
     __shared__ T room_most[16];
     __shared__ double room_sum[16];
     __shared__ Slope<T> room_slope;
-    const int wave_at = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) / 64), lane = threadIdx.x % 64;
-    const int wave = wave_at % kWaves;
-    const int64_t row = static_cast<int64_t>(blockIdx.x) * kTeams + wave_at / kWaves;
-    if (row >= a.rows) return;
-    const int64_t target = from_lane(a.targets[row], 0), own = static_cast<int64_t>(wave * 64 + lane) * kCount;
+    const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) / 64), lane = threadIdx.x % 64;
+    const int64_t row = blockIdx.x, target = a.targets[row], own = static_cast<int64_t>(threadIdx.x) * kCount;
     constexpr int64_t kStep = Threads * kCount, kHeld = kStep * Pieces;
-    T* g = a.grad != nullptr ? a.grad + row * a.cols : nullptr;
+    T* g = a.grad + row * a.cols;
     if (!is_target(target, a.cols)) {
-        if (g != nullptr)
-            for (int64_t at = own; at < a.cols; at += kStep) store_grad<Past>(g, at, a.cols, Piece<T>{}, -1, Slope<T>{0, 0});
-        if (wave == 0 && lane == 0) {
-            if (a.losses != nullptr) a.losses[row] = 0;
-            if (a.logps != nullptr) a.logps[row] = 0;
-            if (a.stats != nullptr) {
-                a.stats[2 * row] = 0;
-                a.stats[2 * row + 1] = 1;
-            }
-        }
+        if (a.grad != nullptr)
+            for (int64_t at = own; at < a.cols; at += kStep) store_grad<PastStores>(g, at, a.cols, Piece<T>{}, -1, Slope<T>{0, 0});
+        if (threadIdx.x == 0) empty_row(a, row);
         return;
     }
     const T* z = a.logits + row * a.cols;
     const T lowest = static_cast<T>(-INFINITY);
     Piece<T> v[Pieces];
 #pragma unroll
-    for (int i = 0; i < Pieces; ++i) v[i] = load_piece<Past>(z, own + i * kStep, a.cols, lowest);
+    for (int i = 0; i < Pieces; ++i) v[i] = load_piece<PastLoads>(z, own + i * kStep, a.cols, lowest);
     const T there = z[target];
     T most = lowest;  // a NaN is passed over here and comes through its exponential
 #pragma unroll
     for (int i = 0; i < Pieces; ++i)
 #pragma unroll
         for (int j = 0; j < kCount; ++j) most = fmax(most, v[i].x[j]);
-    for (int64_t at = own + kHeld; at < a.cols; at += kStep) {
-        const Piece<T> p = load_piece(z, at, a.cols, lowest);
+    // what is not held, four pieces at a time
+    constexpr int kMore = 4;
+    const auto rest = [&](auto&& use) {
+        if constexpr (More)
+            for (int64_t at = own + kHeld; at < a.cols; at += kMore * kStep) {
+                Piece<T> p[kMore];
+#pragma unroll
+                for (int i = 0; i < kMore; ++i) p[i] = load_piece(z, at + i * kStep, a.cols, lowest);
+#pragma unroll
+                for (int i = 0; i < kMore; ++i)
+                    if (at + i * kStep < a.cols) use(p[i], at + i * kStep);
+            }
+    };
+    rest([&](const Piece<T>& p, int64_t) {
 #pragma unroll
         for (int j = 0; j < kCount; ++j) most = fmax(most, p.x[j]);
-    }
+    });
     most = wave_most(most);
-    if constexpr (kWaves > 1) {
-        if (lane == 0) room_most[wave] = most;
-        __syncthreads();
-        most = from_lane(most_of_16(room_most[lane % 16 < kWaves ? lane % 16 : 0]), 15);
-    }
+    if (lane == 0) room_most[wave] = most;
+    __syncthreads();
+    most = from_lane(most_of_16(room_most[lane % 16 < kWaves ? lane % 16 : 0]), 15);
     const T base = or_zero(most);
     double sum = 0;
 #pragma unroll
@@ -225,78 +325,136 @@ __global__ __launch_bounds__(group_of(Threads)) void answer_rows_kernel(AnswerRo
             v[i].x[j] = a.t.exp(v[i].x[j] - base);
             sum += static_cast<double>(v[i].x[j]);
         }
-    for (int64_t at = own + kHeld; at < a.cols; at += kStep) {
-        const Piece<T> p = load_piece(z, at, a.cols, lowest);
+    rest([&](const Piece<T>& p, int64_t) {
 #pragma unroll
         for (int j = 0; j < kCount; ++j) sum += static_cast<double>(a.t.exp(p.x[j] - base));
-    }
+    });
     sum = wave_total(sum);
-    if constexpr (kWaves > 1) {
-        if (lane == 0) room_sum[wave] = sum;
-        __syncthreads();
-        sum = from_lane(sum_of_16(lane % 16 < kWaves ? room_sum[lane % 16] : 0.0), 15);
+    if (lane == 0) room_sum[wave] = sum;
+    __syncthreads();
+    sum = from_lane(sum_of_16(lane % 16 < kWaves ? room_sum[lane % 16] : 0.0), 15);
+    // by turns, since the first waves of all workgroups share a SIMD
+    if (wave == static_cast<int>(blockIdx.x % kWaves)) {
+        const Slope<T> slope = finish_row(a, row, there, most, sum, lane == 0);
+        if (lane == 0) room_slope = slope;
     }
-    Slope<T> slope{0, 0};
-    if (wave == 0) {
-        const double lp = (static_cast<double>(there) - static_cast<double>(most)) / a.temperature - log(sum);
-        double loss = 0, derivative = 0;
-        if (a.with_policy) {
-            policy_terms(a.policy, row, lp, loss, derivative);
-            if (g != nullptr) slope = slope_of<T>(derivative * static_cast<double>(a.policy.row_weights[row]), sum, a.temperature);
-        }
-        if (lane == 0) {
-            if (a.losses != nullptr) a.losses[row] = static_cast<T>(loss);
-            if (a.logps != nullptr) a.logps[row] = lp;
-            if (a.stats != nullptr) {
-                a.stats[2 * row] = most;
-                a.stats[2 * row + 1] = static_cast<T>(sum);
-            }
-            if (kWaves > 1) room_slope = slope;
-        }
-    }
-    if (g == nullptr) return;
-    if constexpr (kWaves > 1) {
-        __syncthreads();
-        slope = room_slope;
-    }
+    if (a.grad == nullptr) return;
+    __syncthreads();
+    const Slope<T> slope = room_slope;
 #pragma unroll
     for (int i = 0; i < Pieces; ++i)
-        if (own + i * kStep < a.cols) store_grad<Past>(g, own + i * kStep, a.cols, v[i], target, slope);
-    for (int64_t at = own + kHeld; at < a.cols; at += kStep) {
-        Piece<T> p = load_piece(z, at, a.cols, lowest);
+        if (own + i * kStep < a.cols) store_grad<PastStores>(g, own + i * kStep, a.cols, v[i], target, slope);
+    rest([&](Piece<T>& p, int64_t at) {
 #pragma unroll
         for (int j = 0; j < kCount; ++j) p.x[j] = a.t.exp(p.x[j] - base);
-        store_grad<Past>(g, at, a.cols, p, target, slope);
-    }
+        store_grad<PastStores>(g, at, a.cols, p, target, slope);
+    });
 }
 
-// The gradient from a row's statistics: a workgroup takes `span` columns of a row, the last rows first, whose logits the caches
-// may still hold from kd_token_logps.
-template <typename T, bool PastLoads, bool PastStores>
-__global__ __launch_bounds__(256) void token_logps_grad_kernel(T* out, const T* logits, const T* stats, const int64_t* targets,
-                                                               const T* slopes, int64_t rows, int64_t cols, double temperature,
-                                                               Tempered<T> t, int64_t span, int spans) {
+// Without a gradient no row is held: a workgroup reads a long one in rounds of four pieces a thread, and several share a
+// CU. All exponentials are taken from one base, the largest logit of the first round, so that no sum is moved from one maximum to
+// another (each move is a rounding that all of a sum's terms share); only a row whose largest logit is far above that base is
+// read once more.
+template <typename T>
+__global__ __launch_bounds__(kMostThreads) void answer_forward_kernel(AnswerRows<T> a) {
     constexpr int kCount = Piece<T>::kCount, kPieces = 4;
-    const int64_t row = rows - 1 - blockIdx.x / spans, from = blockIdx.x % spans * span, to = min(from + span, cols);
+    constexpr double kFar = 40;  // e^40 is well inside f32's range
+    __shared__ T room_most[2][16];
+    __shared__ double room_sum[16];
+    const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) / 64), lane = threadIdx.x % 64;
+    const int waves = blockDim.x / 64;
+    const int64_t row = blockIdx.x, target = a.targets[row];
+    if (!is_target(target, a.cols)) {
+        if (threadIdx.x == 0) empty_row(a, row);
+        return;
+    }
+    const T* z = a.logits + row * a.cols;
+    const T there = z[target], lowest = static_cast<T>(-INFINITY);
+    const int64_t own = static_cast<int64_t>(threadIdx.x) * kCount, step = static_cast<int64_t>(blockDim.x) * kCount;
+    const auto load = [&](Piece<T>(&p)[kPieces], int64_t at) {
+#pragma unroll
+        for (int i = 0; i < kPieces; ++i) p[i] = load_piece(z, at + i * step, a.cols, lowest);
+    };
+    const auto most_of = [&](const Piece<T>(&p)[kPieces], T most) {
+#pragma unroll
+        for (int i = 0; i < kPieces; ++i)
+#pragma unroll
+            for (int j = 0; j < kCount; ++j) most = fmax(most, p[i].x[j]);  // passes over NaN, which the sum takes up
+        return most;
+    };
+    const auto over_group = [&](T v, T* room) {
+        v = wave_most(v);
+        if (lane == 0) room[wave] = v;
+        __syncthreads();
+        return from_lane(most_of_16(room[lane % 16 < waves ? lane % 16 : 0]), 15);
+    };
+    Piece<T> p[kPieces], next[kPieces];
+    load(p, own);
+    const T first = over_group(most_of(p, lowest), room_most[0]);
+    T base = or_zero(first), most = lowest;
+    double sum = 0;
+    const auto add = [&](const Piece<T>(&q)[kPieces]) {
+#pragma unroll
+        for (int i = 0; i < kPieces; ++i)
+#pragma unroll
+            for (int j = 0; j < kCount; ++j) sum += static_cast<double>(a.t.exp(q[i].x[j] - base));
+    };
+    for (int64_t at = own; at < a.cols; at += kPieces * step) {
+        const bool more = at + kPieces * step < a.cols;
+        if (more) load(next, at + kPieces * step);
+        most = most_of(p, most);
+        add(p);
+        if (more)
+#pragma unroll
+            for (int i = 0; i < kPieces; ++i) p[i] = next[i];
+    }
+    most = over_group(most, room_most[1]);
+    // the base's own rounding of the difference is the same for the whole workgroup
+    if (!((static_cast<double>(most) - static_cast<double>(base)) * a.inverse <= kFar) && most != lowest) {
+        base = most;
+        sum = 0;
+        for (int64_t at = own; at < a.cols; at += kPieces * step) {
+            load(p, at);
+            add(p);
+        }
+    }
+    sum = wave_total(sum);
+    if (lane == 0) room_sum[wave] = sum;
+    __syncthreads();
+    if (wave != 0) return;
+    sum = from_lane(sum_of_16(lane % 16 < waves ? room_sum[lane % 16] : 0.0), 15);
+    if (base != most && most != lowest) sum *= exp((static_cast<double>(base) - static_cast<double>(most)) * a.inverse);
+    finish_row(a, row, there, most, sum, lane == 0);
+}
+
+// The gradient from a row's statistics: a team of `Threads` (of a workgroup of 256) takes a round of a row, the last rows first, whose logits the caches may still
+// hold from kd_token_logps (1837 x 50257: 126 us, from the first row on 142).
+template <typename T, int Threads, bool Past>
+__global__ __launch_bounds__(256) void token_logps_grad_kernel(T* out, const T* logits, const T* stats, const int64_t* targets,
+                                                               const T* slopes, int64_t rows, int64_t cols, double inverse,
+                                                               Tempered<T> t, int spans) {
+    constexpr int kCount = Piece<T>::kCount, kPieces = 4;
+    constexpr int64_t kStep = Threads * kCount;
+    const int team = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) / 64) / (Threads / 64);
+    const int64_t round = static_cast<int64_t>(blockIdx.x) * (256 / Threads) + team;
+    const int64_t row = rows - 1 - round / spans, at = round % spans * kPieces * kStep + static_cast<int64_t>(threadIdx.x % Threads) * kCount;
+    if (row < 0) return;
     const int64_t target = targets[row];
     const double own = is_target(target, cols) ? static_cast<double>(slopes[row]) : 0.0;
-    const Slope<T> slope = slope_of<T>(own, static_cast<double>(stats[2 * row + 1]), temperature);
+    const Slope<T> slope = slope_of<T>(own, static_cast<double>(stats[2 * row + 1]), inverse);
     const T base = or_zero(stats[2 * row]);
     const T* z = logits + row * cols;
     T* g = out + row * cols;
-    constexpr int64_t kStep = 256 * kCount;
-    for (int64_t at = from + static_cast<int64_t>(threadIdx.x) * kCount; at < to; at += kPieces * kStep) {
-        Piece<T> p[kPieces] = {};
-        if (own != 0)
+    Piece<T> p[kPieces] = {};
+    if (own != 0)
 #pragma unroll
-            for (int i = 0; i < kPieces; ++i) p[i] = load_piece<PastLoads>(z, at + i * kStep, to, base);
+        for (int i = 0; i < kPieces; ++i) p[i] = load_piece(z, at + i * kStep, cols, base);
 #pragma unroll
-        for (int i = 0; i < kPieces; ++i) {
-            if (at + i * kStep >= to) continue;
+    for (int i = 0; i < kPieces; ++i) {
+        if (at + i * kStep >= cols) continue;
 #pragma unroll
-            for (int j = 0; j < kCount; ++j) p[i].x[j] = t.exp(p[i].x[j] - base);
-            store_grad<PastStores>(g, at + i * kStep, to, p[i], target, slope);
-        }
+        for (int j = 0; j < kCount; ++j) p[i].x[j] = t.exp(p[i].x[j] - base);
+        store_grad<Past>(g, at + i * kStep, cols, p[i], target, slope);
     }
 }
 
@@ -311,28 +469,61 @@ int check_rows(const std::string& name, int dtype, int64_t rows, int64_t cols, d
     return KD_OK;
 }
 
-// A team's threads and the 16-byte pieces that each of them holds, by the row's pieces.
+template <int N> using Int = std::integral_constant<int, N>;
+
+// Threads and the 16-byte pieces that each of them holds, by the row's pieces.
 template <typename T> void launch_rows(const AnswerRows<T>& a) {
     const int64_t pieces = (a.cols + Piece<T>::kCount - 1) / Piece<T>::kCount;
-    const bool past = a.rows * a.cols * static_cast<int64_t>(sizeof(T)) > int64_t{96} << 20;
-    const auto one = [&](auto kernel, int threads) {
-        const int teams = group_of(threads) / threads;
-        hipLaunchKernelGGL(kernel, dim3(static_cast<uint32_t>((a.rows + teams - 1) / teams)), dim3(group_of(threads)), 0, stream(), a);
+    // Logits that are read once go past the caches where they would drive the gradient out of them, and so does a gradient that
+    // the last cache's 256 MiB cannot hold. f32 rows of 50257, us: neither / loads / stores / both:
+    //   40 MB 18.5 / 20.3 / 19.8 / 21.7    100 MB 43.1 / 42.1 / 42.7 / 48.4    181 MB 86.5 / 73.0 / 85.4 / 82.8
+    //   281 MB 119 / 107 / 120 / 120    412 MB 170 / 167 / 164 / 163
+    const int64_t bytes = a.rows * a.cols * static_cast<int64_t>(sizeof(T));
+    const bool past_loads = bytes > int64_t{128} << 20, past_stores = bytes > int64_t{320} << 20;
+    if (a.grad == nullptr && pieces > 1024) {
+        hipLaunchKernelGGL((answer_forward_kernel<T>), dim3(static_cast<uint32_t>(a.rows)), dim3(row_threads(a.rows, a.cols)), 0,
+                           stream(), a);
+        return;
+    }
+    const auto with = [&](auto kernel, int64_t groups, int threads) {
+        hipLaunchKernelGGL(kernel, dim3(static_cast<uint32_t>(groups)), dim3(threads), 0, stream(), a);
     };
-    const auto both = [&](auto threads, auto held) {
-        constexpr int kThreads = decltype(threads)::value, kPieces = decltype(held)::value;
-        if (past) one(answer_rows_kernel<T, kThreads, kPieces, true>, kThreads);
-        else one(answer_rows_kernel<T, kThreads, kPieces, false>, kThreads);
+    const auto by_caches = [&](auto launch) {
+        if (past_stores) launch(std::true_type{}, std::true_type{});
+        else if (past_loads) launch(std::true_type{}, std::false_type{});
+        else launch(std::false_type{}, std::false_type{});
     };
-    using std::integral_constant;
-    if (pieces <= 64) both(integral_constant<int, 64>{}, integral_constant<int, 1>{});
-    else if (pieces <= 256) both(integral_constant<int, 64>{}, integral_constant<int, 4>{});
-    else if (pieces <= 1024) both(integral_constant<int, 256>{}, integral_constant<int, 4>{});
-    else if (pieces <= 2048) both(integral_constant<int, 512>{}, integral_constant<int, 4>{});
-    else if (pieces <= 4096) both(integral_constant<int, 1024>{}, integral_constant<int, 4>{});
-    else if (pieces <= 8192) both(integral_constant<int, 1024>{}, integral_constant<int, 8>{});
-    else if (pieces <= 13 * 1024) both(integral_constant<int, 1024>{}, integral_constant<int, 13>{});
-    else both(integral_constant<int, 1024>{}, integral_constant<int, 20>{});
+    if (pieces <= 256) {
+        // Four rows share a wave's f64 functions where there are enough of them: 66667 x 300 44.6 us (one a wave 52.9), but 4096 x 96
+        // 6.3 (5.5) and, with two rows, 33333 x 600 38.5 (36).
+        const auto rows = [&](auto held, auto together) {
+            by_caches([&](auto loads, auto stores) {
+                constexpr int kTogether = decltype(together)::value, kGroup = kShortThreads / 64 * kTogether;
+                with(answer_short_kernel<T, decltype(held)::value, kTogether, decltype(loads)::value, decltype(stores)::value>,
+                     (a.rows + kGroup - 1) / kGroup, kShortThreads);
+            });
+        };
+        const bool many = a.rows >= 64 * compute_units();
+        if (pieces <= 64) many ? rows(Int<1>{}, Int<4>{}) : rows(Int<1>{}, Int<1>{});
+        else if (pieces <= 128) many ? rows(Int<2>{}, Int<4>{}) : rows(Int<2>{}, Int<1>{});
+        else rows(Int<4>{}, Int<1>{});
+        return;
+    }
+    const auto row = [&](auto threads, auto held, auto more) {
+        by_caches([&](auto loads, auto stores) {
+            constexpr int kThreads = decltype(threads)::value;
+            with(answer_rows_kernel<T, kThreads, decltype(held)::value, decltype(more)::value, decltype(loads)::value, decltype(stores)::value>,
+                 a.rows, kThreads);
+        });
+    };
+    if (pieces <= 512) row(Int<256>{}, Int<2>{}, std::false_type{});
+    else if (pieces <= 1024) row(Int<256>{}, Int<4>{}, std::false_type{});
+    else if (pieces <= 2048) row(Int<512>{}, Int<4>{}, std::false_type{});
+    else if (pieces <= 4096) row(Int<1024>{}, Int<4>{}, std::false_type{});
+    else if (pieces <= 5 * 1024) row(Int<1024>{}, Int<5>{}, std::false_type{});
+    else if (pieces <= 8 * 1024) row(Int<1024>{}, Int<8>{}, std::false_type{});
+    else if (pieces <= 13 * 1024) row(Int<1024>{}, Int<13>{}, std::false_type{});
+    else row(Int<1024>{}, Int<14>{}, std::true_type{});
 }
 
 // Whether `out` is neither apart from the logits nor the logits themselves.
@@ -357,7 +548,7 @@ extern "C" int kd_token_logps(int dtype, double* logps, void* stats, const void*
     if (int rc = ensure_device()) return rc;
     const auto launch = [&](auto zero) {
         using T = decltype(zero);
-        AnswerRows<T> a{nullptr, nullptr, static_cast<T*>(stats), logps, static_cast<const T*>(logits), targets, rows, cols, temperature,
+        AnswerRows<T> a{nullptr, nullptr, static_cast<T*>(stats), logps, static_cast<const T*>(logits), targets, rows, cols, 1.0 / temperature,
                         Tempered<T>(temperature), false, {}};
         launch_rows(a);
     };
@@ -378,20 +569,23 @@ extern "C" int kd_token_logps_grad(int dtype, void* out, const void* logits, con
     if (int rc = ensure_device()) return rc;
     const auto launch = [&](auto zero) -> int {
         using T = decltype(zero);
-        // parts of a row to a workgroup, in whole rounds of it
-        const int64_t round = int64_t{256} * 4 * Piece<T>::kCount;
-        const int64_t span = round * std::max<int64_t>(1, std::min<int64_t>((cols + round - 1) / round, 4));
-        const int64_t spans = (cols + span - 1) / span;
-        if (!fits_grid(rows * spans, 256)) return fail(KD_E_INVALID, name + ": too many rows and columns");
-        const auto one = [&](auto kernel) {
-            hipLaunchKernelGGL(kernel, dim3(static_cast<uint32_t>(rows * spans)), dim3(256), 0, stream(), static_cast<T*>(out),
+        // one round a team: with two 2 % slower, with four 20 % (1837 x 50257)
+        const auto one = [&](auto kernel, int threads) -> int {
+            const int64_t span = int64_t{threads} * 4 * Piece<T>::kCount, spans = (cols + span - 1) / span;
+            const int64_t groups = (rows * spans + 256 / threads - 1) / (256 / threads);
+            if (!fits_grid(groups, 256)) return fail(KD_E_INVALID, name + ": too many rows and columns");
+            hipLaunchKernelGGL(kernel, dim3(static_cast<uint32_t>(groups)), dim3(256), 0, stream(), static_cast<T*>(out),
                                static_cast<const T*>(logits), static_cast<const T*>(stats), targets, static_cast<const T*>(slopes),
-                               rows, cols, temperature, Tempered<T>(temperature), span, static_cast<int>(spans));
+                               rows, cols, 1.0 / temperature, Tempered<T>(temperature), static_cast<int>(spans));
+            return KD_OK;
         };
-        const PastCaches past = past_caches(rows * cols * static_cast<int64_t>(sizeof(T)));
-        if (past.grad_stores) one(token_logps_grad_kernel<T, true, true>);
-        else if (past.grad_loads) one(token_logps_grad_kernel<T, true, false>);
-        else one(token_logps_grad_kernel<T, false, false>);
+        // A gradient that goes past the caches leaves the logits in them. With kd_token_logps, f32 rows of 50257, us, through / past:
+        // 50 MB 26.3 / 27.4, 130 MB 69 / 58, 231 MB 134 / 116, 369 MB 202 / 176.
+        const bool past = rows * cols * static_cast<int64_t>(sizeof(T)) > int64_t{96} << 20;
+        const bool brief = cols <= 64 * 4 * Piece<T>::kCount;  // a wave's round
+        if (int rc = brief ? past ? one(token_logps_grad_kernel<T, 64, true>, 64) : one(token_logps_grad_kernel<T, 64, false>, 64)
+                           : past ? one(token_logps_grad_kernel<T, 256, true>, 256) : one(token_logps_grad_kernel<T, 256, false>, 256))
+            return rc;
         KD_LAUNCH_CHECK();
         return KD_OK;
     };
@@ -445,7 +639,7 @@ extern "C" int kd_policy_rows(int dtype, void* losses, double* logps, void* grad
     const auto launch = [&](auto zero) {
         using T = decltype(zero);
         AnswerRows<T> a{static_cast<T*>(losses), static_cast<T*>(grad), nullptr, logps, static_cast<const T*>(logits), targets, rows,
-                        cols, policy->temperature, Tempered<T>(policy->temperature), true,
+                        cols, 1.0 / policy->temperature, Tempered<T>(policy->temperature), true,
                         {policy->old_logps, policy->reference_logps, static_cast<const T*>(policy->advantages),
                          static_cast<const T*>(row_weights), policy->clip_low, policy->clip_high, policy->kl_weight}};
         launch_rows(a);

@@ -139,12 +139,9 @@ def test_the_policy_loss_and_its_gradient(kdb, shape, dtype):
         old, reference = policy_of(rng, lp, targets, shape[1], 0.2, 0.3)
         advantages, weights = rng.normal(size=(2, shape[0])).astype(dtype)
         advantages[::7] = 0
-        one = check_policy(kdb, z, targets, old if given else None, reference if kl else None, advantages, weights, temperature,
-                           0.2, 0.3, kl, in_place=in_place)
-        alone = run_policy(kdb, z, targets, old if given else None, reference if kl else None, advantages, None, temperature,
-                           0.2, 0.3, kl, grad=False)
-        for a, b in zip(one[:2], alone[:2]):
-            np.testing.assert_array_equal(a, b)
+        for how in (dict(in_place=in_place), dict(grad=False)):
+            check_policy(kdb, z, targets, old if given else None, reference if kl else None, advantages, weights, temperature,
+                         0.2, 0.3, kl, **how)
 
 
 @pytest.mark.parametrize("cols", [40, 700, 3000, 50257, 120001])
@@ -193,6 +190,25 @@ def test_masked_logits_and_rows_without_a_distribution(kdb, dtype, cols):
         np.testing.assert_allclose(losses[[0, 1, 3, 9]], loss, rtol=2 * np.finfo(dtype).eps)
         if sign == 1:
             assert (grad[[0, 1, 3, 9]] == 0).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("cols", [5000, 50257])
+def test_rows_that_rise(kdb, dtype, cols):
+    """The largest logits at the end, far above or a little above what comes first, -inf and the type's lowest value ahead."""
+    rng = np.random.default_rng(cols)
+    z, targets = logits_of(rng, 6, cols, dtype)
+    targets[:] = rng.integers(cols - 100, cols, 6)
+    for r, rise in enumerate((30, 60, 1e4)):
+        z[r, cols - 100:] += dtype(rise)
+    z[3, :cols - 50], targets[3] = -np.inf, cols - 3
+    z[4, :cols - 1], targets[4] = np.finfo(dtype).min, cols - 1
+    z[5, cols - 1], targets[5] = np.finfo(dtype).max, cols - 1
+    for temperature in (1.0, 0.05):
+        logps, stats, _, _ = token_logps(kdb, z, targets, temperature)
+        with np.errstate(over="ignore"):
+            same(logps.numpy(), answers.token_logps(z, targets, temperature), logp_tolerance(z, temperature))
+        np.testing.assert_array_equal(stats.numpy()[:, 0], z.max(1))
 
 
 # ---- pairs ----------------------------------------------------------------------------------------
