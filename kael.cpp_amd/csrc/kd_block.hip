@@ -16,19 +16,41 @@ constexpr int kThreads = 256;
 template <typename T> struct Quad {
     T v[4];
 };
-template <typename T> __device__ __forceinline__ Quad<T> load_quad(const T* row, int64_t c, int64_t cols) {
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4), aligned(4)));
+// Past: past the caches.
+template <bool Past = false, typename T> __device__ __forceinline__ Quad<T> load_quad(const T* row, int64_t c) {
     Quad<T> q;
-    if (c + 4 <= cols) {
-        __builtin_memcpy(&q, row + c, sizeof q);
-    } else {
+    if constexpr (Past) {
+        u32x4 raw[sizeof q / 16];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) q.v[e] = c + e < cols ? row[c + e] : T(0);
+        for (int i = 0; i < static_cast<int>(sizeof q / 16); ++i) raw[i] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(row + c) + i);
+        __builtin_memcpy(&q, raw, sizeof q);
+    } else {
+        __builtin_memcpy(&q, row + c, sizeof q);
     }
     return q;
 }
-template <typename T> __device__ __forceinline__ void store_quad(T* row, int64_t c, int64_t cols, const Quad<T>& q) {
-    if (c + 4 <= cols) {
+template <bool Past = false, typename T> __device__ __forceinline__ Quad<T> load_quad(const T* row, int64_t c, int64_t cols) {
+    if (c + 4 <= cols) return load_quad<Past>(row, c);
+    Quad<T> q;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) q.v[e] = c + e < cols ? row[c + e] : T(0);
+    return q;
+}
+template <bool Past = false, typename T> __device__ __forceinline__ void store_quad(T* row, int64_t c, const Quad<T>& q) {
+    if constexpr (Past) {
+        u32x4 raw[sizeof q / 16];
+        __builtin_memcpy(raw, &q, sizeof q);
+#pragma unroll
+        for (int i = 0; i < static_cast<int>(sizeof q / 16); ++i) __builtin_nontemporal_store(raw[i], reinterpret_cast<u32x4*>(row + c) + i);
+    } else {
         __builtin_memcpy(row + c, &q, sizeof q);
+    }
+}
+template <bool Past = false, typename T>
+__device__ __forceinline__ void store_quad(T* row, int64_t c, int64_t cols, const Quad<T>& q) {
+    if (c + 4 <= cols) {
+        store_quad<Past>(row, c, q);
     } else {
 #pragma unroll
         for (int e = 0; e < 4; ++e)
@@ -251,6 +273,11 @@ template <int Threads, int Quads> struct Team {
         const Pair p = exchange({a, b}, room);
         return {from_lane(sum_of_16(p.a), 15), from_lane(sum_of_16(p.b), 15)};
     }
+    __device__ __forceinline__ double sum(double a, Pair* room) const {
+        a = wave_total(a);
+        if constexpr (kWaves == 1) return a;
+        return from_lane(sum_of_16(exchange({a, 0}, room).a), 15);
+    }
     // A row's statistics. A wave's sums are taken about its first value, and the waves' means about wave 0's: see Moments.
     template <typename T>
     __device__ __forceinline__ RowStats stats(int kind, double eps, int cols, const Quad<T> (&v)[Quads], Pair* room) const {
@@ -267,8 +294,7 @@ template <int Threads, int Quads> struct Team {
             }
         const double all = static_cast<double>(cols);
         if (kind == KD_NORM_RMS) {
-            const Pair p = sums(s2, 0.0, room);
-            return {0.0, 1.0 / sqrt(p.a / all + eps)};
+            return {0.0, rsqrt(sum(s2, room) * (1.0 / all) + eps)};
         }
         s1 = wave_total(s1);
         s2 = wave_total(s2);
@@ -281,10 +307,10 @@ template <int Threads, int Quads> struct Team {
             const double d = count > 0 ? p.a - base : 0.0;
             s1 = from_lane(sum_of_16(count * d), 15);
             s2 = from_lane(sum_of_16((count > 0 ? p.b : 0.0) + count * d * d), 15);
-            mean = base + s1 / all;
-            squares = s2 - s1 * (s1 / all);
+            mean = base + s1 * (1.0 / all);
+            squares = s2 - s1 * (s1 * (1.0 / all));
         }
-        return {mean, 1.0 / sqrt((squares < 0 ? 0.0 : squares) / all + eps)};
+        return {mean, rsqrt((squares < 0 ? 0.0 : squares) * (1.0 / all) + eps)};
     }
 };
 
@@ -305,67 +331,138 @@ __device__ __forceinline__ uint32_t kept_bits(const BlockArgs<T>& a, const Team<
     return bits;
 }
 
-template <typename T> __device__ __forceinline__ Quad<T> quad_or(const T* p, int64_t c, int64_t cols, T otherwise) {
+// A row's quads for a kernel whose rows are of whole quads, or of any length. A whole quad is loaded without a branch: behind the
+// row's end it is the last one again, which nothing counts or stores.
+// Offsets in a row are 32 bits without a sign, beside a row's start in scalar registers: one register an address.
+template <typename T> __device__ __forceinline__ const T* place_in(const T* row, int c) {
+    return reinterpret_cast<const T*>(reinterpret_cast<const char*>(row) + static_cast<uint32_t>(c) * static_cast<uint32_t>(sizeof(T)));
+}
+template <typename T> __device__ __forceinline__ T* place_in(T* row, int c) {
+    return reinterpret_cast<T*>(reinterpret_cast<char*>(row) + static_cast<uint32_t>(c) * static_cast<uint32_t>(sizeof(T)));
+}
+template <bool Whole, bool Past = false, typename T> __device__ __forceinline__ Quad<T> take_quad(const T* row, int c, int cols) {
+    if constexpr (Whole) return load_quad<Past>(place_in(row, min(c, cols - 4)), 0);
+    else return load_quad<Past>(place_in(row, c), 0, cols - c);
+}
+template <bool Whole, bool Past = false, typename T> __device__ __forceinline__ Quad<T> quad_or(const T* p, int c, int cols, T otherwise) {
     Quad<T> q{otherwise, otherwise, otherwise, otherwise};
-    if (p != nullptr) q = load_quad(p, c, cols);
+    if (p != nullptr) q = take_quad<Whole, Past>(p, c, cols);
     return q;
 }
+template <bool Whole, bool Past = false, typename T> __device__ __forceinline__ void give_quad(T* row, int c, int cols, const Quad<T>& q) {
+    if constexpr (Whole) {
+        if (c < cols) store_quad<Past>(place_in(row, c), 0, q);
+    } else {
+        store_quad<Past>(place_in(row, c), 0, cols - c, q);
+    }
+}
+
+// Keeps the compiler from holding the f64 forms of a loop's f32 constants, twice the registers, all through the loop.
+__device__ __forceinline__ void converted_late(Quad<float>& q) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) asm volatile("" : "+v"(q.v[e]));
+}
+__device__ __forceinline__ void converted_late(Quad<double>&) {}
 
 constexpr int group_of(int threads) { return threads < 256 ? 256 : threads; }
 
-// A row is read once, held in registers and written once.
-template <typename T, int Threads, int Quads>
+// A row is read once, held in registers and written once. Held: the workgroup takes rows one after another, with the norms'
+// weights and the gate in registers all through (from the L2 they are more bytes than the row) and the next row on its way.
+template <typename T, int Threads, int Quads, bool Whole, bool Held>
 __global__ __launch_bounds__(group_of(Threads)) void block_rows_kernel(T* h, T* y, double* stats, BlockArgs<T> a) {
-    __shared__ Pair room[2][kMostWaves];
-    const Team<Threads, Quads> at;
     constexpr int kTeams = group_of(Threads) / Threads;
     static_assert(kTeams == 1 || Threads == 64, "teams that leave early may not meet at barriers");
-    const int64_t row = static_cast<int64_t>(blockIdx.x) * kTeams + at.team;
-    if (row >= a.rows) return;
+    __shared__ Pair room[2][2][kMostWaves];  // by turns: a row's waves may be ahead of the last ones of the row before
+    const Team<Threads, Quads> at;
     const int cols = static_cast<int>(a.cols);
-    const int64_t base = row * a.cols;
-    Quad<T> v[Quads], r[Quads];
+    const uint32_t step = a.mask.step_now();
+    Quad<T> after_w[Quads], after_b[Quads], before_w[Quads], before_b[Quads], gate[Quads];
+    const auto load_after = [&](int i, int64_t row) {
+        after_w[i] = quad_or<Whole>(a.after.weight, at.column(i), cols, T(1));
+        after_b[i] = quad_or<Whole>(a.after.bias, at.column(i), cols, T(0));
+        gate[i] = quad_or<Whole>(a.gate != nullptr ? a.gate + row * a.gate_step : nullptr, at.column(i), cols, T(1));
+    };
+    const auto load_before = [&](int i) {
+        before_w[i] = quad_or<Whole>(a.before.weight, at.column(i), cols, T(1));
+        before_b[i] = quad_or<Whole>(a.before.bias, at.column(i), cols, T(0));
+    };
+    if constexpr (Held)
 #pragma unroll
-    for (int i = 0; i < Quads; ++i) {
-        v[i] = load_quad(a.x + base, at.column(i), cols);
-        r[i] = quad_or(a.residual != nullptr ? a.residual + base : nullptr, at.column(i), cols, T(0));
-    }
-    const uint32_t bits = kept_bits(a, at, row, a.mask.step_now());
-    const RowStats after = at.stats(a.after.kind, a.after.eps, cols, v, room[0]);
-#pragma unroll
-    for (int i = 0; i < Quads; ++i) {
-        const int c = at.column(i);
-        const Quad<T> gate = quad_or(a.gate != nullptr ? a.gate + row * a.gate_step : nullptr, c, cols, T(1));
-        const Quad<T> w = quad_or(a.after.weight, c, cols, T(1)), b = quad_or(a.after.bias, c, cols, T(0));
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            double n = static_cast<double>(v[i].v[e]);
-            if (a.after.kind != KD_NORM_NONE) n = after.unit(n) * static_cast<double>(w.v[e]) + static_cast<double>(b.v[e]);
-            n = bits >> (4 * i + e) & 1 ? n * a.mask.scale : 0.0;
-            v[i].v[e] = static_cast<T>(a.block_scale * static_cast<double>(gate.v[e]) * n + a.residual_scale * static_cast<double>(r[i].v[e]));
+        for (int i = 0; i < Quads; ++i) {
+            load_after(i, 0);
+            load_before(i);
         }
-        if (h != nullptr) store_quad(h + base, c, cols, v[i]);
-    }
-    RowStats before{0.0, 1.0};
-    if (a.before.kind != KD_NORM_NONE && (y != nullptr || stats != nullptr)) {
-        before = at.stats(a.before.kind, a.before.eps, cols, v, room[1]);
-        if (y != nullptr)
+    Quad<T> next_v[Quads], next_r[Quads];
+    const auto load_row = [&](int64_t row) {
+#pragma unroll
+        for (int i = 0; i < Quads; ++i) {
+            next_v[i] = take_quad<Whole>(a.x + row * a.cols, at.column(i), cols);
+            next_r[i] = quad_or<Whole>(a.residual != nullptr ? a.residual + row * a.cols : nullptr, at.column(i), cols, T(0));
+        }
+    };
+    const int64_t stride = static_cast<int64_t>(gridDim.x) * kTeams;
+    int64_t row = static_cast<int64_t>(blockIdx.x) * kTeams + at.team;
+    if (row >= a.rows) return;
+    load_row(row);
+    for (int turn = 0; row < a.rows; row += stride, turn ^= 1) {
+        const int64_t base = row * a.cols;
+        Quad<T> v[Quads], r[Quads];
+#pragma unroll
+        for (int i = 0; i < Quads; ++i) {
+            v[i] = next_v[i];
+            r[i] = next_r[i];
+        }
+        if constexpr (Held) {
+            if (row + stride < a.rows) load_row(row + stride);
 #pragma unroll
             for (int i = 0; i < Quads; ++i) {
-                const int c = at.column(i);
-                const Quad<T> w = quad_or(a.before.weight, c, cols, T(1)), b = quad_or(a.before.bias, c, cols, T(0));
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    v[i].v[e] = static_cast<T>(before.unit(static_cast<double>(v[i].v[e])) * static_cast<double>(w.v[e]) +
-                                               static_cast<double>(b.v[e]));
-                store_quad(y + base, c, cols, v[i]);
+                converted_late(after_w[i]);
+                converted_late(after_b[i]);
+                converted_late(before_w[i]);
+                converted_late(before_b[i]);
+                converted_late(gate[i]);
+                if (a.gate_step != 0) gate[i] = take_quad<Whole>(a.gate + row * a.gate_step, at.column(i), cols);
             }
-    }
-    if (stats != nullptr && at.wave == 0 && at.lane == 0) {
-        stats[4 * row] = after.mean;
-        stats[4 * row + 1] = after.rate;
-        stats[4 * row + 2] = before.mean;
-        stats[4 * row + 3] = before.rate;
+        }
+        const uint32_t bits = kept_bits(a, at, row, step);
+        const RowStats after = at.stats(a.after.kind, a.after.eps, cols, v, room[turn][0]);
+#pragma unroll
+        for (int i = 0; i < Quads; ++i) {
+            const int c = at.column(i);
+            if constexpr (!Held) load_after(i, row);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                double n = static_cast<double>(v[i].v[e]);
+                if (a.after.kind != KD_NORM_NONE)
+                    n = after.unit(n) * static_cast<double>(after_w[i].v[e]) + static_cast<double>(after_b[i].v[e]);
+                n = bits >> (4 * i + e) & 1 ? n * a.mask.scale : 0.0;
+                v[i].v[e] = static_cast<T>(a.block_scale * static_cast<double>(gate[i].v[e]) * n +
+                                           a.residual_scale * static_cast<double>(r[i].v[e]));
+            }
+            if (h != nullptr) give_quad<Whole>(h + base, c, cols, v[i]);
+        }
+        RowStats before{0.0, 1.0};
+        if (a.before.kind != KD_NORM_NONE && (y != nullptr || stats != nullptr)) {
+            before = at.stats(a.before.kind, a.before.eps, cols, v, room[turn][1]);
+            if (y != nullptr)
+#pragma unroll
+                for (int i = 0; i < Quads; ++i) {
+                    const int c = at.column(i);
+                    if constexpr (!Held) load_before(i);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        v[i].v[e] = static_cast<T>(before.unit(static_cast<double>(v[i].v[e])) * static_cast<double>(before_w[i].v[e]) +
+                                                   static_cast<double>(before_b[i].v[e]));
+                    give_quad<Whole>(y + base, c, cols, v[i]);
+                }
+        }
+        if (stats != nullptr && at.wave == 0 && at.lane == 0) {
+            stats[4 * row] = after.mean;
+            stats[4 * row + 1] = after.rate;
+            stats[4 * row + 2] = before.mean;
+            stats[4 * row + 3] = before.rate;
+        }
+        if constexpr (!Held) break;
     }
 }
 
@@ -424,8 +521,8 @@ __device__ __forceinline__ void before_means(const BackArgs<T>& a, int64_t row, 
     mean = a.b.before.kind == KD_NORM_LAYER ? group_sum(mean, room) / static_cast<double>(a.b.cols) : 0.0;
 }
 
-// Any row length: the gradients of the rows, a workgroup each.
-template <typename T> __global__ __launch_bounds__(kThreads) void block_back_wide_kernel(BackArgs<T> a) {
+// Any row length: the gradients of the rows, a workgroup each, and the means of p and p v, [rows][2], for the sums over rows.
+template <typename T> __global__ __launch_bounds__(kThreads) void block_back_wide_kernel(double* means, BackArgs<T> a) {
     __shared__ double room[kThreads / 64];
     const uint32_t step = a.b.mask.step_now();
     const int64_t cols = a.b.cols;
@@ -434,6 +531,11 @@ template <typename T> __global__ __launch_bounds__(kThreads) void block_back_wid
         const RowStats before = a.before(row), after = a.after(row);
         double mean, along, back_mean = 0, back_along = 0;
         before_means(a, row, room, mean, along);
+        if (means != nullptr && threadIdx.x == 0) {
+            means[2 * row] = mean;
+            means[2 * row + 1] = along;
+        }
+        if (a.x == nullptr && a.residual == nullptr && a.gate == nullptr) continue;
         const auto through = [&](int64_t c, double g) {
             return a.kept(row, c, step) ? a.b.block_scale * gate_at(a.b, row, c) * g * a.b.mask.scale : 0.0;
         };
@@ -461,56 +563,177 @@ template <typename T> __global__ __launch_bounds__(kThreads) void block_back_wid
     }
 }
 
-// The means that the sums over rows need: [rows][2].
-template <typename T> __global__ __launch_bounds__(kThreads) void block_means_kernel(double* means, BackArgs<T> a) {
-    __shared__ double room[kThreads / 64];
-    for (int64_t row = blockIdx.x; row < a.b.rows; row += gridDim.x) {
-        double mean, along;
-        before_means(a, row, room, mean, along);
-        if (threadIdx.x == 0) {
-            means[2 * row] = mean;
-            means[2 * row + 1] = along;
+// The sums over a segment of rows: [segment][sum][cols]. A workgroup takes 256 columns, four a lane, and its waves share the rows.
+template <typename T, bool Whole>
+__global__ __launch_bounds__(kThreads) void block_columns_kernel(T* parts, const double* means, BackArgs<T> a,
+                                                                 int64_t rows_per_segment) {
+    constexpr int kWaves = kThreads / 64;
+    __shared__ double room[kWaves][4][64];
+    const uint32_t step = a.b.mask.step_now();
+    const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) / 64);
+    const int c = static_cast<int>(blockIdx.x) * 256 + 4 * lane, cols = static_cast<int>(a.b.cols);
+    const int64_t from = blockIdx.y * rows_per_segment, to = min(a.b.rows, from + rows_per_segment);
+    const bool normed = a.b.after.kind != KD_NORM_NONE, gate_sum = a.sums[kGate] != nullptr, x_read = normed || gate_sum;
+    const Quad<T> before_w = quad_or<Whole>(a.b.before.weight, c, cols, T(1)), after_w = quad_or<Whole>(a.b.after.weight, c, cols, T(1));
+    const Quad<T> after_b = quad_or<Whole>(a.b.after.bias, c, cols, T(0));
+    Quad<T> gate = quad_or<Whole>(a.b.gate, c, cols, T(1));
+    double sums[kSums][4] = {};
+    if (c < cols)
+        for (int64_t row = from + wave; row < to; row += kWaves) {
+            const int64_t base = row * a.b.cols;
+            const RowStats before = a.before(row), after = a.after(row);
+            const double mean = means[2 * row], along = means[2 * row + 1];
+            Quad<T> x{}, h{}, grad_y{};
+            const Quad<T> grad_h = quad_or<Whole>(a.grad_h != nullptr ? a.grad_h + base : nullptr, c, cols, T(0));
+            if (a.grad_y != nullptr) {
+                grad_y = take_quad<Whole>(a.grad_y + base, c, cols);
+                h = take_quad<Whole>(a.h + base, c, cols);
+            }
+            if (x_read) x = take_quad<Whole>(a.b.x + base, c, cols);
+            if (a.b.gate_step != 0) gate = take_quad<Whole>(a.b.gate + row * a.b.gate_step, c, cols);
+            bool kept[4] = {true, true, true, true};
+            if (a.b.masked) a.b.mask.kept(kept, static_cast<uint32_t>(row), static_cast<uint32_t>(c / 4), step);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                double g = static_cast<double>(grad_h.v[e]);
+                if (a.grad_y != nullptr) {
+                    const double own = static_cast<double>(grad_y.v[e]), v = before.unit(static_cast<double>(h.v[e]));
+                    g += before.rate * (own * static_cast<double>(before_w.v[e]) - mean - v * along);
+                    sums[kBeforeWeight][e] += own * v;
+                    sums[kBeforeBias][e] += own;
+                }
+                const double through = kept[e] ? a.b.block_scale * a.b.mask.scale * g : 0.0;
+                const double u = after.unit(static_cast<double>(x.v[e]));
+                if (gate_sum)
+                    sums[kGate][e] += kept[e] ? through * (normed ? u * static_cast<double>(after_w.v[e]) + static_cast<double>(after_b.v[e]) : u) : 0.0;
+                const double d = through * static_cast<double>(gate.v[e]);
+                if (normed) {
+                    sums[kAfterWeight][e] += d * u;
+                    sums[kAfterBias][e] += d;
+                }
+            }
+        }
+#pragma unroll
+    for (int k = 0; k < kSums; ++k) {
+        if (a.sums[k] == nullptr) continue;
+        __syncthreads();
+#pragma unroll
+        for (int e = 0; e < 4; ++e) room[wave][e][lane] = sums[k][e];
+        __syncthreads();
+        if (wave == 0 && c < cols) {
+            Quad<T> q;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                double total = room[0][e][lane];
+                for (int w = 1; w < kWaves; ++w) total += room[w][e][lane];
+                q.v[e] = static_cast<T>(total);
+            }
+            give_quad<Whole>(parts + (blockIdx.y * kSums + k) * a.b.cols, c, cols, q);
         }
     }
 }
 
-// The sums over a segment of rows: [segment][sum][cols]. A workgroup takes 64 columns, its waves share the rows.
-template <typename T>
-__global__ __launch_bounds__(kThreads) void block_columns_kernel(T* parts, const double* means, BackArgs<T> a,
-                                                                 int64_t rows_per_segment) {
-    __shared__ double room[kThreads / 64][kSums][64];
-    const uint32_t step = a.b.mask.step_now();
-    const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
-    const int64_t c = static_cast<int64_t>(blockIdx.x) * 64 + lane, cols = a.b.cols;
-    const int64_t from = blockIdx.y * rows_per_segment, to = min(a.b.rows, from + rows_per_segment);
-    double sums[kSums] = {};
-    if (c < cols)
-        for (int64_t row = from + wave; row < to; row += kThreads / 64) {
-            const int64_t base = row * cols;
-            const RowStats before = a.before(row), after = a.after(row);
-            const double g = a.total(base, c, before, means[2 * row], means[2 * row + 1]);
-            if (a.grad_y != nullptr) {
-                const double own = static_cast<double>(a.grad_y[base + c]);
-                sums[kBeforeWeight] += own * before.unit(static_cast<double>(a.h[base + c]));
-                sums[kBeforeBias] += own;
-            }
-            if (a.sums[kGate] != nullptr) sums[kGate] += a.b.block_scale * branch_at(a.b, after, row, c, step) * g;
-            if (a.b.after.kind != KD_NORM_NONE) {
-                const double d = a.kept(row, c, step) ? a.b.block_scale * gate_at(a.b, row, c) * g * a.b.mask.scale : 0.0;
-                sums[kAfterWeight] += d * after.unit(static_cast<double>(a.b.x[base + c]));
-                sums[kAfterBias] += d;
+// A long row's gradients, by a workgroup that holds it: what the sums over rows would take of the registers is left to
+// block_columns_kernel, which reads the rows again.
+template <typename T, int Quads, bool Whole>
+__global__ __launch_bounds__(1024) void block_back_row_kernel(double* means, BackArgs<T> a) {
+    __shared__ Pair room[2][kMostWaves];
+    const Team<1024, Quads> at;
+    const int64_t row = blockIdx.x, base = row * a.b.cols;
+    const int cols = static_cast<int>(a.b.cols);
+    const double share = 1.0 / cols;
+    const RowStats before = a.before(row), after = a.after(row);
+    Quad<T> grad_h[Quads], grad_y[Quads], h[Quads];
+    double g[Quads][4], mean = 0, along = 0;
+#pragma unroll
+    for (int i = 0; i < Quads; ++i) {
+        const int c = at.column(i);
+        if (a.grad_y != nullptr) {
+            grad_y[i] = take_quad<Whole>(a.grad_y + base, c, cols);
+            h[i] = take_quad<Whole>(a.h + base, c, cols);
+        }
+        grad_h[i] = quad_or<Whole>(a.grad_h != nullptr ? a.grad_h + base : nullptr, c, cols, T(0));
+    }
+    const uint32_t bits = kept_bits(a.b, at, row, a.b.mask.step_now());
+    if (a.grad_y != nullptr) {
+        double p_sum = 0, pv_sum = 0;
+#pragma unroll
+        for (int i = 0; i < Quads; ++i) {
+            const Quad<T> w = quad_or<Whole>(a.b.before.weight, at.column(i), cols, T(1));
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                if (at.column(i) + e >= cols) continue;
+                const double p = static_cast<double>(grad_y[i].v[e]) * static_cast<double>(w.v[e]);
+                p_sum += p;
+                pv_sum += p * before.unit(static_cast<double>(h[i].v[e]));
             }
         }
+        const Pair s = at.sums(p_sum, pv_sum, room[0]);
+        mean = a.b.before.kind == KD_NORM_LAYER ? s.a * share : 0.0;
+        along = s.b * share;
+    }
+    if (means != nullptr && threadIdx.x == 0) {
+        means[2 * row] = mean;
+        means[2 * row + 1] = along;
+    }
+    if (a.x == nullptr && a.residual == nullptr && a.gate == nullptr) return;
+    const bool normed = a.b.after.kind != KD_NORM_NONE && a.x != nullptr, x_read = normed || a.gate != nullptr;
+    double q_sum = 0, qu_sum = 0;
+    Quad<T> x[Quads];
 #pragma unroll
-    for (int k = 0; k < kSums; ++k) room[wave][k][lane] = sums[k];
-    __syncthreads();
-    if (wave == 0 && c < cols)
+    for (int i = 0; i < Quads; ++i) {
+        const int c = at.column(i);
+        if (x_read) x[i] = take_quad<Whole>(a.b.x + base, c, cols);
+        const Quad<T> before_w = quad_or<Whole>(a.b.before.weight, c, cols, T(1)), after_w = quad_or<Whole>(a.b.after.weight, c, cols, T(1));
+        const Quad<T> gate = quad_or<Whole>(a.b.gate != nullptr ? a.b.gate + row * a.b.gate_step : nullptr, c, cols, T(1));
+        Quad<T> to_residual, to_gate;
 #pragma unroll
-        for (int k = 0; k < kSums; ++k) {
-            double total = room[0][k][lane];
-            for (int w = 1; w < kThreads / 64; ++w) total += room[w][k][lane];
-            parts[(blockIdx.y * kSums + k) * cols + c] = static_cast<T>(total);
+        for (int e = 0; e < 4; ++e) {
+            double own = static_cast<double>(grad_h[i].v[e]);
+            if (a.grad_y != nullptr)
+                own += before.rate * (static_cast<double>(grad_y[i].v[e]) * static_cast<double>(before_w.v[e]) - mean -
+                                      before.unit(static_cast<double>(h[i].v[e])) * along);
+            to_residual.v[e] = static_cast<T>(a.b.residual_scale * own);
+            const double through = bits >> (4 * i + e) & 1 ? a.b.block_scale * a.b.mask.scale * own : 0.0;
+            g[i][e] = through * static_cast<double>(gate.v[e]);
+            if (x_read) {
+                const double u = after.unit(static_cast<double>(x[i].v[e]));
+                if (a.gate != nullptr) {
+                    const Quad<T> b = quad_or<Whole>(a.b.after.bias, c, cols, T(0));
+                    const double n = a.b.after.kind != KD_NORM_NONE ? u * static_cast<double>(after_w.v[e]) + static_cast<double>(b.v[e]) : u;
+                    to_gate.v[e] = static_cast<T>(bits >> (4 * i + e) & 1 ? through * n : 0.0);
+                }
+                if (normed && c + e < cols) {
+                    const double q = g[i][e] * static_cast<double>(after_w.v[e]);
+                    q_sum += q;
+                    qu_sum += q * u;
+                }
+            }
         }
+        if (a.residual != nullptr) give_quad<Whole>(a.residual + base, c, cols, to_residual);
+        if (a.gate != nullptr) give_quad<Whole>(a.gate + base, c, cols, to_gate);
+    }
+    if (a.x == nullptr) return;
+    double back_mean = 0, back_along = 0;
+    if (normed) {
+        const Pair s = at.sums(q_sum, qu_sum, room[1]);
+        back_mean = a.b.after.kind == KD_NORM_LAYER ? s.a * share : 0.0;
+        back_along = s.b * share;
+    }
+#pragma unroll
+    for (int i = 0; i < Quads; ++i) {
+        const int c = at.column(i);
+        const Quad<T> after_w = quad_or<Whole>(normed ? a.b.after.weight : nullptr, c, cols, T(1));
+        Quad<T> to;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            double d = g[i][e];
+            if (normed)
+                d = after.rate * (d * static_cast<double>(after_w.v[e]) - back_mean - after.unit(static_cast<double>(x[i].v[e])) * back_along);
+            to.v[e] = static_cast<T>(d);
+        }
+        give_quad<Whole>(a.x + base, c, cols, to);
+    }
 }
 
 // A team's rows one after another, each read once: the rows' gradients and the sums over the team's rows. Those lie in LDS,
@@ -532,56 +755,57 @@ template <typename T> __device__ __forceinline__ void add_quad(T* place, const Q
     __builtin_memcpy(p, &own, sizeof own);
 }
 
-template <typename T, int Quads> struct BackRow {
+template <typename T, int Quads, bool Whole> struct BackRow {
     Quad<T> x[Quads], h[Quads], grad_h[Quads], grad_y[Quads];
     RowStats after, before;
     template <int Threads> __device__ __forceinline__ void load(const BackArgs<T>& a, const Team<Threads, Quads>& at, int64_t row, bool x_read) {
         const int64_t base = row * a.b.cols;
+        const int cols = static_cast<int>(a.b.cols);
 #pragma unroll
         for (int i = 0; i < Quads; ++i) {
             const int c = at.column(i);
-            if (x_read) x[i] = load_quad(a.b.x + base, c, a.b.cols);
+            if (x_read) x[i] = take_quad<Whole>(a.b.x + base, c, cols);
             if (a.grad_y != nullptr) {
-                h[i] = load_quad(a.h + base, c, a.b.cols);
-                grad_y[i] = load_quad(a.grad_y + base, c, a.b.cols);
+                h[i] = take_quad<Whole>(a.h + base, c, cols);
+                grad_y[i] = take_quad<Whole>(a.grad_y + base, c, cols);
             }
-            grad_h[i] = quad_or(a.grad_h != nullptr ? a.grad_h + base : nullptr, c, a.b.cols, T(0));
+            grad_h[i] = quad_or<Whole>(a.grad_h != nullptr ? a.grad_h + base : nullptr, c, cols, T(0));
         }
-        after = a.after(row);
-        before = a.before(row);
+        // the same for a wave's lanes and constant in this kernel: scalar loads to scalar registers
+        const auto* s = (const __attribute__((address_space(4))) double*)(a.stats + 4 * row);
+        after = {s[0], s[1]};
+        before = {s[2], s[3]};
     }
-    // The statistics, the same for a wave's lanes, to scalar registers.
-    __device__ __forceinline__ void arrived() {
-        after = {from_lane(after.mean, 0), from_lane(after.rate, 0)};
-        before = {from_lane(before.mean, 0), from_lane(before.rate, 0)};
+    __device__ __forceinline__ void converted_late() {
+#pragma unroll
+        for (int i = 0; i < Quads; ++i) {
+            kd::converted_late(x[i]);
+            kd::converted_late(h[i]);
+            kd::converted_late(grad_h[i]);
+            kd::converted_late(grad_y[i]);
+        }
     }
 };
 
-// Keeps the compiler from holding the f64 forms of a loop's f32 constants, twice the registers, all through the loop.
-__device__ __forceinline__ void converted_late(Quad<float>& q) {
-#pragma unroll
-    for (int e = 0; e < 4; ++e) asm volatile("" : "+v"(q.v[e]));
-}
-__device__ __forceinline__ void converted_late(Quad<double>&) {}
-
-template <typename T, int Threads, int Quads, bool Ahead, bool Held>
+template <typename T, int Threads, int Quads, bool Ahead, bool Held, bool Whole>
 __global__ __launch_bounds__(kBackThreads<T>) void block_back_kernel(T* parts, BackArgs<T> a, int64_t rows_per_team, SumPlaces places) {
     constexpr int kTeams = kBackThreads<T> / Threads;
     extern __shared__ __attribute__((aligned(16))) char shared[];
-    __shared__ Pair room[2][kMostWaves];
+    __shared__ Pair room[2][2][kMostWaves];  // by turns: a row's waves may be ahead of the last ones of the row before
     const Team<Threads, Quads> at;
     const int64_t first = (static_cast<int64_t>(blockIdx.x) * kTeams + at.team) * rows_per_team, end = min(a.b.rows, first + rows_per_team);
     const int cols = static_cast<int>(a.b.cols);
+    const double share = 1.0 / cols;
     const uint32_t step = a.b.mask.step_now();
     const bool normed = a.b.after.kind != KD_NORM_NONE, gate_sum = a.sums[kGate] != nullptr;
     const bool branch = gate_sum || a.gate != nullptr, x_read = normed || branch;
     Quad<T> before_w[Quads], after_w[Quads], after_b[Quads], gate[Quads];
     const auto load_weights = [&](int i, int64_t row) {
         const int c = at.column(i);
-        before_w[i] = quad_or(a.b.before.weight, c, cols, T(1));
-        after_w[i] = quad_or(a.b.after.weight, c, cols, T(1));
-        after_b[i] = quad_or(branch ? a.b.after.bias : nullptr, c, cols, T(0));
-        gate[i] = quad_or(a.b.gate != nullptr ? a.b.gate + row * a.b.gate_step : nullptr, c, cols, T(1));
+        before_w[i] = quad_or<Whole>(a.b.before.weight, c, cols, T(1));
+        after_w[i] = quad_or<Whole>(a.b.after.weight, c, cols, T(1));
+        after_b[i] = quad_or<Whole>(branch ? a.b.after.bias : nullptr, c, cols, T(0));
+        gate[i] = quad_or<Whole>(a.b.gate != nullptr ? a.b.gate + row * a.b.gate_step : nullptr, c, cols, T(1));
     };
     if constexpr (Held)
 #pragma unroll
@@ -593,7 +817,7 @@ __global__ __launch_bounds__(kBackThreads<T>) void block_back_kernel(T* parts, B
 #pragma unroll
         for (int i = 0; i < Quads; ++i)
             if (at.column(i) < cols) __builtin_memset(sums + k * padded + at.column(i), 0, 4 * sizeof(T));
-    BackRow<T, Quads> now, next;
+    BackRow<T, Quads, Whole> now, next;
     if (Ahead && first < end) next.load(a, at, first, x_read);
     for (int64_t n = 0; n < rows_per_team; ++n) {
         const int64_t row = first + n, base = row * a.b.cols;
@@ -604,7 +828,6 @@ __global__ __launch_bounds__(kBackThreads<T>) void block_back_kernel(T* parts, B
         } else if (here) {
             now.load(a, at, row, x_read);
         }
-        if (here) now.arrived();
         if constexpr (Held) {
 #pragma unroll
             for (int i = 0; i < Quads; ++i) {
@@ -622,13 +845,15 @@ __global__ __launch_bounds__(kBackThreads<T>) void block_back_kernel(T* parts, B
 #pragma unroll
                 for (int i = 0; i < Quads; ++i) {
                     Quad<T> by_weight;
-                    if constexpr (!Held) before_w[i] = quad_or(a.b.before.weight, at.column(i), cols, T(1));
+                    if constexpr (!Held) before_w[i] = quad_or<Whole>(a.b.before.weight, at.column(i), cols, T(1));
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
                         const double g = static_cast<double>(now.grad_y[i].v[e]), p = g * static_cast<double>(before_w[i].v[e]);
                         const double v = now.before.unit(static_cast<double>(now.h[i].v[e]));
-                        p_sum += p;
-                        pv_sum += p * v;
+                        if (at.column(i) + e < cols) {
+                            p_sum += p;
+                            pv_sum += p * v;
+                        }
                         by_weight.v[e] = static_cast<T>(g * v);
                     }
                     if (at.column(i) < cols) {
@@ -640,17 +865,22 @@ __global__ __launch_bounds__(kBackThreads<T>) void block_back_kernel(T* parts, B
         }
         double mean = 0, along = 0;
         if (a.grad_y != nullptr) {
-            const Pair s = at.sums(p_sum, pv_sum, room[0]);
-            mean = a.b.before.kind == KD_NORM_LAYER ? s.a / cols : 0.0;
-            along = s.b / cols;
+            if (a.b.before.kind == KD_NORM_LAYER) {
+                const Pair s = at.sums(p_sum, pv_sum, room[n & 1][0]);
+                mean = s.a * share;
+                along = s.b * share;
+            } else {
+                along = at.sum(pv_sum, room[n & 1][0]) * share;
+            }
         }
         double q_sum = 0, qu_sum = 0, d[Quads][4];
         if (here) {
+            now.converted_late();
 #pragma unroll
             for (int i = 0; i < Quads; ++i) {
                 const int c = at.column(i);
                 if constexpr (!Held) load_weights(i, row);
-                else if (a.b.gate_step != 0) gate[i] = load_quad(a.b.gate + row * a.b.gate_step, c, cols);
+                else if (a.b.gate_step != 0) gate[i] = take_quad<Whole>(a.b.gate + row * a.b.gate_step, c, cols);
                 Quad<T> to_residual, to_gate, by_weight, by_bias;
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
@@ -681,20 +911,26 @@ __global__ __launch_bounds__(kBackThreads<T>) void block_back_kernel(T* parts, B
                     if (places.at[kAfterBias] >= 0) add_quad(sum_place(kAfterBias, c), by_bias);
                     if (gate_sum) add_quad(sum_place(kGate, c), to_gate);
                 }
-                if (a.residual != nullptr) store_quad(a.residual + base, c, cols, to_residual);
-                if (a.gate != nullptr) store_quad(a.gate + base, c, cols, to_gate);
+                if (a.residual != nullptr) give_quad<Whole>(a.residual + base, c, cols, to_residual);
+                if (a.gate != nullptr) give_quad<Whole>(a.gate + base, c, cols, to_gate);
             }
         }
         if (normed) {
-            const Pair s = at.sums(q_sum, qu_sum, room[1]);
-            mean = a.b.after.kind == KD_NORM_LAYER ? s.a / cols : 0.0;
-            along = s.b / cols;
+            if (a.b.after.kind == KD_NORM_LAYER) {
+                const Pair s = at.sums(q_sum, qu_sum, room[n & 1][1]);
+                mean = s.a * share;
+                along = s.b * share;
+            } else {
+                mean = 0;
+                along = at.sum(qu_sum, room[n & 1][1]) * share;
+            }
         }
         if (here && a.x != nullptr) {
+            now.converted_late();
 #pragma unroll
             for (int i = 0; i < Quads; ++i) {
                 Quad<T> to;
-                if constexpr (!Held) after_w[i] = quad_or(a.b.after.weight, at.column(i), cols, T(1));
+                if constexpr (!Held) after_w[i] = quad_or<Whole>(a.b.after.weight, at.column(i), cols, T(1));
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     double g = d[i][e];
@@ -703,7 +939,7 @@ __global__ __launch_bounds__(kBackThreads<T>) void block_back_kernel(T* parts, B
                                               now.after.unit(static_cast<double>(now.x[i].v[e])) * along);
                     to.v[e] = static_cast<T>(g);
                 }
-                store_quad(a.x + base, at.column(i), cols, to);
+                give_quad<Whole>(a.x + base, at.column(i), cols, to);
             }
         }
     }
@@ -743,6 +979,8 @@ __global__ __launch_bounds__(kJoinWaves * 64) void block_join_kernel(BackArgs<T>
 
 // ---- plans and checks -----------------------------------------------------------------------------
 
+template <int N> using Int = std::integral_constant<int, N>;
+
 // How a backward pass is divided. threads: a row's team, 0 for rows that registers do not hold; segments: parts of the rows
 // whose sums are kept apart.
 struct BackPlan {
@@ -755,21 +993,21 @@ int64_t sums_bytes(int dtype, int64_t cols, int threads, int wanted) {
     return group_threads(dtype) / threads * wanted * ((cols + 3) / 4 * 4) * dtype_size(dtype);
 }
 BackPlan wide_plan(int64_t rows, int64_t cols) {
-    // enough segments to fill the card, at most 64 MiB of them
-    const int64_t most = std::max<int64_t>(1, (int64_t{64} << 20) / (cols * kSums * 8));
-    const int64_t segments = std::max<int64_t>(1, std::min({(rows + 15) / 16, int64_t{1024}, most}));
-    const int64_t each = (rows + segments - 1) / segments;
+    // workgroups of 256 columns, four for each CU, of 16 rows at least
+    const int64_t wanted = (int64_t{4} * compute_units() + (cols + 255) / 256 - 1) / ((cols + 255) / 256);
+    const int64_t segments = std::clamp<int64_t>(wanted, 1, (rows + 15) / 16), each = (rows + segments - 1) / segments;
     return {0, 0, each, (rows + each - 1) / each};
 }
 BackPlan back_plan(int dtype, int64_t rows, int64_t cols, int wanted) {
-    if (cols > (dtype == KD_F32 ? 8192 : 4096)) return wide_plan(rows, cols);
+    if (cols > 4096) return wide_plan(rows, cols);
+    int threads = 64, quads = 1;
     const int group = group_threads(dtype);
-    int threads = 64;
     while (threads < group && threads * 4 < cols) threads *= 2;
+    while (threads * quads * 4 < cols) quads *= 2;
     if (sums_bytes(dtype, cols, threads, wanted) > 159 * 1024) return wide_plan(rows, cols);
-    const int64_t teams = group / threads;
-    const int64_t each = std::clamp<int64_t>((rows + teams * compute_units() - 1) / (teams * compute_units()), 1, 32);
-    return {threads, threads * 4 < cols ? 2 : 1, each, (rows + teams * each - 1) / (teams * each)};
+    const int64_t teams = group / threads, all = teams * compute_units();
+    const int64_t each = std::clamp<int64_t>((rows + all - 1) / all, 1, 32);
+    return {threads, quads, each, (rows + teams * each - 1) / (teams * each)};
 }
 // What the passes of any number of sums need at most.
 int64_t room_of(int dtype, int64_t rows, int64_t cols) {
@@ -782,6 +1020,7 @@ int64_t room_of(int dtype, int64_t rows, int64_t cols) {
     return most;
 }
 
+constexpr int64_t kMostCols = int64_t{1} << 28;  // offsets in a row are 32 bits
 bool fits(int64_t rows, int64_t cols) { return rows <= (int64_t{1} << 40) && cols <= (int64_t{1} << 40) && (cols == 0 || rows <= (int64_t{1} << 46) / cols); }
 
 template <typename T> NormArgs<T> norm_of(const kd_norm& n) {
@@ -810,7 +1049,7 @@ int check_block(const char* what, int dtype, const kd_block* b, Mask& mask) {
     const std::string name(what);
     if (dtype != KD_F32 && dtype != KD_F64) return fail(KD_E_UNSUPPORTED, name + ": dtype must be f32 or f64");
     if (b == nullptr) return fail(KD_E_INVALID, name + ": the block must be given");
-    if (b->rows < 0 || b->cols < 0 || !fits(b->rows, b->cols)) return fail(KD_E_INVALID, name + ": bad number of rows or columns");
+    if (b->rows < 0 || b->cols < 0 || b->cols > kMostCols || !fits(b->rows, b->cols)) return fail(KD_E_INVALID, name + ": bad number of rows or columns");
     for (const kd_norm* n : {&b->after, &b->before}) {
         if (n->kind != KD_NORM_NONE && n->kind != KD_NORM_LAYER && n->kind != KD_NORM_RMS)
             return fail(KD_E_INVALID, name + ": no such norm");
@@ -887,15 +1126,30 @@ extern "C" int kd_block_rows(int dtype, void* h, void* y, double* stats, const k
             hipLaunchKernelGGL(kernel, dim3(static_cast<uint32_t>(groups)), dim3(threads), 0, stream(), static_cast<T*>(h),
                                static_cast<T*>(y), stats, a);
         };
+        const auto rows = [&](auto threads, auto quads, auto held, int64_t groups) {
+            constexpr int kTeam = decltype(threads)::value, kGroup = group_of(kTeam), kQuads = decltype(quads)::value;
+            constexpr bool kHeld = decltype(held)::value;
+            if (b.cols % 4 == 0) one(block_rows_kernel<T, kTeam, kQuads, true, kHeld>, kGroup, groups);
+            else one(block_rows_kernel<T, kTeam, kQuads, false, kHeld>, kGroup, groups);
+        };
+        // Workgroups a CU that hold the weights: as many as fit its registers. They hold them where the weights are more bytes than x and
+        // residual, and where each has some rows; us, weights read / held, both norms and a gate: 32768 x 768 115 / 97, 16384 x 2048
+        // 128 / 104, 8192 x 4096 124 / 106; a layer norm ahead of the next block alone: 91 / 96, 102 / 113, 103 / 109.
+        const auto choose = [&](auto threads, auto quads, int a_unit) {
+            const int weights = 2 * (b.after.kind != KD_NORM_NONE) + 2 * (b.before.kind != KD_NORM_NONE) + (b.gate_rows == 1);
+            const int64_t groups = int64_t{a_unit} * compute_units();
+            if (weights > 2 && b.rows >= 8 * groups) rows(threads, quads, std::true_type{}, groups);
+            else rows(threads, quads, std::false_type{}, b.rows);
+        };
         if (b.rows >= int64_t{1} << 22 || b.cols > 16384)
             one(block_rows_wide_kernel<T>, kThreads, std::min<int64_t>(b.rows, int64_t{compute_units()} * 32));
-        else if (b.cols <= 256) one(block_rows_kernel<T, 64, 1>, 256, (b.rows + 3) / 4);
-        else if (b.cols <= 512) one(block_rows_kernel<T, 64, 2>, 256, (b.rows + 3) / 4);
-        else if (b.cols <= 1024) one(block_rows_kernel<T, 256, 1>, 256, b.rows);
-        else if (b.cols <= 2048) one(block_rows_kernel<T, 256, 2>, 256, b.rows);
-        else if (b.cols <= 4096) one(block_rows_kernel<T, 512, 2>, 512, b.rows);
-        else if (b.cols <= 8192) one(block_rows_kernel<T, 1024, 2>, 1024, b.rows);
-        else one(block_rows_kernel<T, 1024, 4>, 1024, b.rows);
+        else if (b.cols <= 256) rows(Int<64>{}, Int<1>{}, std::false_type{}, (b.rows + 3) / 4);
+        else if (b.cols <= 512) rows(Int<64>{}, Int<2>{}, std::false_type{}, (b.rows + 3) / 4);
+        else if (b.cols <= 1024) choose(Int<256>{}, Int<1>{}, 5);
+        else if (b.cols <= 2048) choose(Int<256>{}, Int<2>{}, 2);
+        else if (b.cols <= 4096) choose(Int<512>{}, Int<2>{}, 1);
+        else if (b.cols <= 8192) rows(Int<1024>{}, Int<2>{}, std::false_type{}, b.rows);
+        else rows(Int<1024>{}, Int<4>{}, std::false_type{}, b.rows);
     };
     if (dtype == KD_F32) launch(0.f);
     else launch(0.0);
@@ -906,7 +1160,7 @@ extern "C" int kd_block_rows(int dtype, void* h, void* y, double* stats, const k
 extern "C" int kd_block_rows_workspace(int64_t* bytes, int dtype, int64_t rows, int64_t cols) {
     const std::string name("kd_block_rows_workspace");
     if (dtype != KD_F32 && dtype != KD_F64) return fail(KD_E_UNSUPPORTED, name + ": dtype must be f32 or f64");
-    if (bytes == nullptr || rows < 0 || cols < 0 || !fits(rows, cols)) return fail(KD_E_INVALID, name + ": bad arguments");
+    if (bytes == nullptr || rows < 0 || cols < 0 || cols > kMostCols || !fits(rows, cols)) return fail(KD_E_INVALID, name + ": bad arguments");
     *bytes = room_of(dtype, rows, cols);
     return KD_OK;
 }
@@ -977,31 +1231,58 @@ extern "C" int kd_block_rows_backward(int dtype, const kd_block_grads* grads, co
         for (int k = 0; k < kSums; ++k) places.at[k] = sums[k] != nullptr ? places.wanted++ : -1;
         const BackPlan plan = b.rows > 0 ? back_plan(dtype, b.rows, b.cols, places.wanted) : BackPlan{0, 0, 0, 0};
         const int64_t column_groups = (b.cols + 63) / 64;
-        if (!fits_grid(column_groups, kJoinWaves * 64) || !fits_grid(plan.segments, kBackThreads<float>))
+        if (!fits_grid(column_groups, kJoinWaves * 64) || !fits_grid(plan.segments, kBackThreads<float>) ||
+            (plan.threads == 0 && plan.segments > 65535))
             return fail(KD_E_INVALID, name + ": too many rows or columns");
         const uint32_t groups = static_cast<uint32_t>(std::min<int64_t>(b.rows, int64_t{compute_units()} * 32));
         double* means = static_cast<double*>(workspace);
         T* parts = summed ? reinterpret_cast<T*>(means + (plan.threads == 0 ? 2 * b.rows : 0)) : nullptr;
-        if (b.rows > 0 && plan.threads == 0 && summed) {
-            hipLaunchKernelGGL((block_means_kernel<T>), dim3(groups), dim3(kThreads), 0, stream(), means, a);
-            hipLaunchKernelGGL((block_columns_kernel<T>), dim3(static_cast<uint32_t>(column_groups), static_cast<uint32_t>(plan.segments)),
-                               dim3(kThreads), 0, stream(), parts, means, a, plan.rows_per_team);
+        if (b.rows > 0 && plan.threads == 0) {
+            const auto rows_of = [&](const BackArgs<T>& which, double* to) {
+                const auto one = [&](auto kernel) {
+                    hipLaunchKernelGGL(kernel, dim3(static_cast<uint32_t>(b.rows)), dim3(1024), 0, stream(), to, which);
+                };
+                const bool whole = b.cols % 4 == 0, two = b.cols <= 8192;
+                if (b.rows >= int64_t{1} << 22 || b.cols > (sizeof(T) == 4 ? 16384 : 8192)) {
+                    hipLaunchKernelGGL((block_back_wide_kernel<T>), dim3(groups), dim3(kThreads), 0, stream(), to, which);
+                    return;
+                }
+                if (two) whole ? one(block_back_row_kernel<T, 2, true>) : one(block_back_row_kernel<T, 2, false>);
+                else if constexpr (sizeof(T) == 4) whole ? one(block_back_row_kernel<T, 4, true>) : one(block_back_row_kernel<T, 4, false>);
+            };
+            // gradients in the place of what the sums read are written last
+            const bool first = !summed || grads->residual == grad_h || grads->residual == grad_y || grads->x == b.x || grads->x == grad_h ||
+                               grads->x == grad_y;
+            if (summed) {
+                BackArgs<T> which = a;
+                if (first) which.x = which.residual = which.gate = nullptr;
+                rows_of(which, means);
+                const dim3 grid(static_cast<uint32_t>((b.cols + 255) / 256), static_cast<uint32_t>(plan.segments));
+                if (b.cols % 4 == 0) hipLaunchKernelGGL((block_columns_kernel<T, true>), grid, dim3(kThreads), 0, stream(), parts, means, a, plan.rows_per_team);
+                else hipLaunchKernelGGL((block_columns_kernel<T, false>), grid, dim3(kThreads), 0, stream(), parts, means, a, plan.rows_per_team);
+            }
+            if (first && by_row) rows_of(a, nullptr);
         }
-        if (b.rows > 0 && plan.threads == 0 && by_row)
-            hipLaunchKernelGGL((block_back_wide_kernel<T>), dim3(groups), dim3(kThreads), 0, stream(), a);
         if (plan.threads != 0) {
             const auto one = [&](auto kernel) {
                 hipLaunchKernelGGL(kernel, dim3(static_cast<uint32_t>(plan.segments)), dim3(kBackThreads<T>),
                                    static_cast<uint32_t>(sums_bytes(dtype, b.cols, plan.threads, places.wanted)), stream(), parts, a,
                                    plan.rows_per_team, places);
             };
+            const auto teams = [&](auto threads, auto quads) {
+                constexpr int kTeam = decltype(threads)::value, kQuads = decltype(quads)::value;
+                constexpr bool kHeld = kQuads == 1;
+                if (b.cols % 4 == 0) one(block_back_kernel<T, kTeam, kQuads, kHeld, kHeld, true>);
+                else one(block_back_kernel<T, kTeam, kQuads, kHeld, kHeld, false>);
+            };
             constexpr int kMost = kBackThreads<T>;
-            if (plan.quads == 2) one(block_back_kernel<T, kMost, 2, false, false>);
-            else if (plan.threads == kMost) one(block_back_kernel<T, kMost, 1, true, true>);
-            else if (plan.threads == 64) one(block_back_kernel<T, 64, 1, true, true>);
-            else if (plan.threads == 128) one(block_back_kernel<T, 128, 1, true, true>);
-            else if (plan.threads == 256) one(block_back_kernel<T, 256, 1, true, true>);
-            else one(block_back_kernel<T, 512, 1, true, true>);
+            if (plan.quads == 2) {
+                if constexpr (sizeof(T) == 8) teams(Int<kMost>{}, Int<2>{});
+            } else if (plan.threads == kMost) teams(Int<kMost>{}, Int<1>{});
+            else if (plan.threads == 64) teams(Int<64>{}, Int<1>{});
+            else if (plan.threads == 128) teams(Int<128>{}, Int<1>{});
+            else if (plan.threads == 256) teams(Int<256>{}, Int<1>{});
+            else teams(Int<512>{}, Int<1>{});
         }
         if (summed)
             hipLaunchKernelGGL((block_join_kernel<T>), dim3(static_cast<uint32_t>(column_groups), kSums), dim3(kJoinWaves * 64), 0,

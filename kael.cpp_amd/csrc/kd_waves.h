@@ -16,8 +16,16 @@ template <int Control, int Rows, typename T> __device__ __forceinline__ T dpp_fr
     __builtin_memcpy(&v, in, sizeof v);
     return v;
 }
+// v + that value, or + 0; within rows of lanes the hardware's own 0 stands in for it.
 template <int Control, int Rows = 0xf> __device__ __forceinline__ double dpp_add(double v) {
-    return v + dpp_from<Control, Rows>(v, 0.0);
+    if constexpr (Rows != 0xf) return v + dpp_from<Control, Rows>(v, 0.0);
+    int2 in;
+    __builtin_memcpy(&in, &v, 8);
+    in.x = __builtin_amdgcn_mov_dpp(in.x, Control, 0xf, 0xf, true);
+    in.y = __builtin_amdgcn_mov_dpp(in.y, Control, 0xf, 0xf, true);
+    double other;
+    __builtin_memcpy(&other, &in, 8);
+    return v + other;
 }
 template <int Control, int Rows = 0xf, typename T> __device__ __forceinline__ T dpp_max(T v) {
     return fmax(v, dpp_from<Control, Rows>(v, v));
