@@ -966,10 +966,20 @@ __global__ __launch_bounds__(kJoinWaves * 64) void block_join_kernel(BackArgs<T>
     T* out = a.sums[blockIdx.y];
     if (out == nullptr) return;
     const int64_t c = static_cast<int64_t>(blockIdx.x) * 64 + lane, cols = a.b.cols;
-    const int64_t run = (segments + kJoinWaves - 1) / kJoinWaves;
+    const int64_t run = (segments + kJoinWaves - 1) / kJoinWaves, end = min(segments, (wave + 1) * run);
     double sum = 0;
-    if (c < cols)
-        for (int64_t s = wave * run; s < min(segments, (wave + 1) * run); ++s) sum += static_cast<double>(parts[(s * kSums + blockIdx.y) * cols + c]);
+    if (c < cols) {
+        const T* own = parts + blockIdx.y * cols + c;
+        int64_t at = wave * run;
+        for (; at + 8 <= end; at += 8) {  // eight loads in flight
+            T part[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) part[i] = own[(at + i) * kSums * cols];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) sum += static_cast<double>(part[i]);
+        }
+        for (; at < end; ++at) sum += static_cast<double>(own[at * kSums * cols]);
+    }
     room[wave][lane] = sum;
     __syncthreads();
     if (wave != 0 || c >= cols) return;
