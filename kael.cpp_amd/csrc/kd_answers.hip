@@ -409,8 +409,8 @@ __global__ __launch_bounds__(kMostThreads) void answer_forward_kernel(AnswerRows
             for (int i = 0; i < kPieces; ++i) p[i] = next[i];
     }
     most = over_group(most, room_most[1]);
-    // the base's own rounding of the difference is the same for the whole workgroup
-    if (!((static_cast<double>(most) - static_cast<double>(base)) * a.inverse <= kFar) && most != lowest) {
+    const bool far = first == lowest || !((static_cast<double>(most) - static_cast<double>(base)) * a.inverse <= kFar);
+    if (far && most != lowest) {
         base = most;
         sum = 0;
         for (int64_t at = own; at < a.cols; at += kPieces * step) {

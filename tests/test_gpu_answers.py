@@ -193,6 +193,25 @@ def test_masked_logits_and_rows_without_a_distribution(kdb, dtype, cols):
 
 
 @pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("cols", [5000, 50257, 100003])
+def test_rows_far_below_zero_behind_masked_ones(kdb, dtype, cols):
+    """Nothing but -inf or the type's lowest value in a row's first thousands, and logits near -1e3 and -1e6 behind them."""
+    rng = np.random.default_rng(cols)
+    z, targets = logits_of(rng, 4, cols, dtype)
+    targets[:] = rng.integers(cols - 100, cols, 4)
+    z[:2, :cols - 100] = -np.inf
+    z[2:, :cols - 100] = np.finfo(dtype).min
+    z[0::2, cols - 100:] -= dtype(1e3)
+    z[1::2, cols - 100:] -= dtype(1e6)
+    logps, stats, _, _ = token_logps(kdb, z, targets, 1.0)
+    with np.errstate(over="ignore"):
+        same(logps.numpy(), answers.token_logps(z, targets, 1.0), logp_tolerance(z, 1.0))
+    np.testing.assert_array_equal(stats.numpy()[:, 0], z.max(1))
+    advantages = np.ones(4, dtype)
+    check_policy(kdb, z, targets, None, None, advantages, advantages, 1.0, 0.2, 0.2, 0.0)
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
 @pytest.mark.parametrize("cols", [5000, 50257])
 def test_rows_that_rise(kdb, dtype, cols):
     """The largest logits at the end, far above or a little above what comes first, -inf and the type's lowest value ahead."""
