@@ -213,13 +213,23 @@ def test_a_block_is_its_definition(kdb, shape, dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
-@pytest.mark.parametrize("shape", [(1, 96), (4096, 64), (5000, 250), (1100, 768), (2500, 1030), (600, 4100), (257, 9000)],
-                         ids=lambda s: "x".join(map(str, s)))
+@pytest.mark.parametrize("shape", [(1, 96), (4096, 64), (5000, 250), (1100, 768), (2500, 1030), (600, 4100), (257, 9000), (300, 4096),
+                                   (9000, 30)], ids=lambda s: "x".join(map(str, s)))
 def test_sums_over_many_rows(kdb, shape, dtype):
+    """Parts of the rows, of each plan; a pass with one exchange a row (a norm on one side) as well as two."""
     rng = np.random.default_rng(shape[0])
-    for after, before, gate, keep in ((R, L, 1, 0.9), (L, R, 2, 1.0)):
+    for after, before, gate, keep in ((R, L, 1, 0.9), (L, R, 2, 1.0), (None, L, 0, 0.9), (R, None, 0, 1.0)):
         case = random_case(rng, *shape, dtype, after, before, gate, keep)
-        check_block(kdb, case, *(rng.normal(size=shape).astype(dtype) for _ in range(2)))
+        grad_h, grad_y = (rng.normal(size=shape).astype(dtype) for _ in range(2))
+        check_block(kdb, case, grad_h, grad_y if before else None)
+
+
+@pytest.mark.parametrize("shape", [(2100, 4096), (4200, 1102), (10300, 520)], ids=lambda s: "x".join(map(str, s)))
+def test_rows_one_after_another(kdb, shape):
+    """As many rows as make the forward kernel hold the weights, with one exchange a row and with two, whole quads and others."""
+    rng = np.random.default_rng(shape[0])
+    for after, before, gate, keep in ((L, L, 1, 1.0), (L, None, 1, 1.0), (R, R, 1, 0.5)):
+        check_block(kdb, random_case(rng, *shape, np.float32, after, before, gate, keep), forward_only=True)
 
 
 @pytest.mark.parametrize("shape", [(5, 96), (5, 768), (5, 4096), (3, 40000)], ids=lambda s: "x".join(map(str, s)))
