@@ -85,8 +85,6 @@ template <typename T> struct NormArgs {
     const T* bias;
     double eps;
     int kind;
-    __device__ __forceinline__ double weight_at(int64_t c) const { return weight != nullptr ? static_cast<double>(weight[c]) : 1.0; }
-    __device__ __forceinline__ double bias_at(int64_t c) const { return bias != nullptr ? static_cast<double>(bias[c]) : 0.0; }
 };
 
 // Mean and 1 / sqrt(mean square + eps) of a row.
@@ -105,136 +103,6 @@ template <typename T> struct BlockArgs {
     Mask mask;
     bool masked;
 };
-
-// Count, mean and sum of squared distances from the mean. A part's sums are taken about one of its own values p, which lies
-// within sqrt(n var) of the mean, so the difference below loses at most a factor n of the rounding; parts are joined by Chan,
-// Golub and LeVeque's formula ("Algorithms for computing the sample variance", 1983).
-struct Moments {
-    double n, mean, squares;
-    __device__ __forceinline__ void join(const Moments& o) {
-        const double total = n + o.n, d = o.mean - mean;
-        if (o.n == 0) return;
-        if (n == 0) {
-            *this = o;
-            return;
-        }
-        mean += d * (o.n / total);
-        squares += o.squares + d * d * (n * o.n / total);
-        n = total;
-    }
-};
-struct MomentSums {
-    double n = 0, p = 0, s1 = 0, s2 = 0;
-    __device__ __forceinline__ void add(double v) {
-        if (n == 0) p = v;
-        const double d = v - p;
-        n += 1;
-        s1 += d;
-        s2 += d * d;
-    }
-    __device__ __forceinline__ Moments moments() const {
-        const double squares = s2 - s1 * (s1 / n);
-        return n > 0 ? Moments{n, p + s1 / n, squares < 0 ? 0.0 : squares} : Moments{0, 0, 0};
-    }
-};
-
-// Sums over the workgroup, the waves' in order; `room` holds a value a wave.
-__device__ __forceinline__ double group_sum(double v, double* room) {
-    const int waves = blockDim.x / 64;
-    v = wave_total(v);
-    __syncthreads();
-    if (threadIdx.x % 64 == 0) room[threadIdx.x / 64] = v;
-    __syncthreads();
-    double total = 0;
-    for (int w = 0; w < waves; ++w) total += room[w];
-    return total;
-}
-
-__device__ __forceinline__ Moments group_moments(Moments m, Moments* room) {
-    const int waves = blockDim.x / 64;
-#pragma unroll
-    for (int d = 32; d > 0; d /= 2) {
-        Moments o;
-        o.n = __shfl_xor(m.n, d);
-        o.mean = __shfl_xor(m.mean, d);
-        o.squares = __shfl_xor(m.squares, d);
-        m.join(o);
-    }
-    __syncthreads();
-    if (threadIdx.x % 64 == 0) room[threadIdx.x / 64] = m;
-    __syncthreads();
-    Moments total = room[0];
-    for (int w = 1; w < waves; ++w) total.join(room[w]);
-    return total;
-}
-
-// The statistics of a row that `value(c)` gives.
-template <typename F> __device__ __forceinline__ RowStats row_stats(int kind, double eps, int64_t cols, Moments* room, F value) {
-    if (kind == KD_NORM_NONE) return {0.0, 1.0};
-    MomentSums sums;
-    if (kind == KD_NORM_LAYER) {
-        for (int64_t c = threadIdx.x; c < cols; c += blockDim.x) sums.add(value(c));
-        const Moments m = group_moments(sums.moments(), room);
-        return {m.mean, 1.0 / sqrt(m.squares / static_cast<double>(cols) + eps)};
-    }
-    double squares = 0;
-    for (int64_t c = threadIdx.x; c < cols; c += blockDim.x) {
-        const double v = value(c);
-        squares += v * v;
-    }
-    return {0.0, 1.0 / sqrt(group_sum(squares, reinterpret_cast<double*>(room)) / static_cast<double>(cols) + eps)};
-}
-
-// The block's output at column c of a row, after its norm and dropout.
-template <typename T>
-__device__ __forceinline__ double branch_at(const BlockArgs<T>& a, const RowStats& s, int64_t row, int64_t c, uint32_t step) {
-    double v = static_cast<double>(a.x[row * a.cols + c]);
-    if (a.after.kind != KD_NORM_NONE) v = s.unit(v) * a.after.weight_at(c) + a.after.bias_at(c);
-    if (a.masked) {
-        bool k[4];
-        a.mask.kept(k, static_cast<uint32_t>(row), static_cast<uint32_t>(c / 4), step);
-        const bool one = c % 4 == 0 ? k[0] : c % 4 == 1 ? k[1] : c % 4 == 2 ? k[2] : k[3];
-        v = one ? v * a.mask.scale : 0.0;
-    }
-    return v;
-}
-template <typename T> __device__ __forceinline__ double gate_at(const BlockArgs<T>& a, int64_t row, int64_t c) {
-    return a.gate != nullptr ? static_cast<double>(a.gate[row * a.gate_step + c]) : 1.0;
-}
-
-// Any row length: a workgroup a row, which is read again in each pass.
-template <typename T>
-__global__ __launch_bounds__(kThreads) void block_rows_wide_kernel(T* h, T* y, double* stats, BlockArgs<T> a) {
-    __shared__ Moments room[kThreads / 64];
-    const uint32_t step = a.mask.step_now();
-    for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
-        const int64_t base = row * a.cols;
-        const RowStats after = row_stats(a.after.kind, a.after.eps, a.cols, room,
-                                         [&](int64_t c) { return static_cast<double>(a.x[base + c]); });
-        const auto sum = [&](int64_t c) {
-            double v = a.block_scale * gate_at(a, row, c) * branch_at(a, after, row, c, step);
-            if (a.residual != nullptr) v += a.residual_scale * static_cast<double>(a.residual[base + c]);
-            return static_cast<T>(v);
-        };
-        // h may take x's or the residual's place, so from then on it is read there; each thread reads what it has written
-        if (h != nullptr)
-            for (int64_t c = threadIdx.x; c < a.cols; c += kThreads) h[base + c] = sum(c);
-        const auto h_at = [&](int64_t c) { return static_cast<double>(h != nullptr ? h[base + c] : sum(c)); };
-        RowStats before{0.0, 1.0};
-        if (a.before.kind != KD_NORM_NONE && (y != nullptr || stats != nullptr)) {
-            before = row_stats(a.before.kind, a.before.eps, a.cols, room, h_at);
-            if (y != nullptr)
-                for (int64_t c = threadIdx.x; c < a.cols; c += kThreads)
-                    y[base + c] = static_cast<T>(before.unit(h_at(c)) * a.before.weight_at(c) + a.before.bias_at(c));
-        }
-        if (stats != nullptr && threadIdx.x == 0) {
-            stats[4 * row] = after.mean;
-            stats[4 * row + 1] = after.rate;
-            stats[4 * row + 2] = before.mean;
-            stats[4 * row + 3] = before.rate;
-        }
-    }
-}
 
 // A team of `Threads` threads has a row: each thread the columns 4 * (thread + i * Threads) .. + 3 for i < Quads.
 struct Pair {
@@ -278,7 +146,30 @@ template <int Threads, int Quads> struct Team {
         if constexpr (kWaves == 1) return a;
         return from_lane(sum_of_16(exchange({a, 0}, room).a), 15);
     }
-    // A row's statistics. A wave's sums are taken about its first value, and the waves' means about wave 0's: see Moments.
+    // A row's statistics from its waves' sums. For a layer norm those are of the distances from one of the wave's own values, the
+    // pivot, and of their squares: a value lies within sqrt(n var) of the mean of n, so var from them loses a factor n of the
+    // rounding at most, and a row of one value has a var of 0. The waves' means are joined in the same way about wave 0's.
+    // of(w): how many values wave w has.
+    template <typename F>
+    __device__ __forceinline__ RowStats stats(int kind, double eps, int cols, double pivot, double s1, double s2, Pair* room, F of) const {
+        const double share = 1.0 / static_cast<double>(cols);
+        if (kind == KD_NORM_RMS) return {0.0, rsqrt(sum(s2, room) * share + eps)};
+        s1 = wave_total(s1);
+        s2 = wave_total(s2);
+        const double n = static_cast<double>(of(wave)), by = n > 0 ? s1 / n : 0.0;
+        double mean = pivot + by, squares = s2 - s1 * by;
+        if constexpr (kWaves > 1) {
+            const Pair p = exchange({mean, squares}, room);
+            const int w = lane % kMostWaves;
+            const double base = from_lane(p.a, 0), count = w < kWaves ? static_cast<double>(of(w)) : 0.0;
+            const double d = count > 0 ? p.a - base : 0.0;
+            s1 = from_lane(sum_of_16(count * d), 15);
+            s2 = from_lane(sum_of_16((count > 0 ? p.b : 0.0) + count * d * d), 15);
+            mean = base + s1 * share;
+            squares = s2 - s1 * (s1 * share);
+        }
+        return {mean, rsqrt((squares < 0 ? 0.0 : squares) * share + eps)};
+    }
     template <typename T>
     __device__ __forceinline__ RowStats stats(int kind, double eps, int cols, const Quad<T> (&v)[Quads], Pair* room) const {
         if (kind == KD_NORM_NONE) return {0.0, 1.0};
@@ -292,25 +183,7 @@ template <int Threads, int Quads> struct Team {
                 s1 += d;
                 s2 += d * d;
             }
-        const double all = static_cast<double>(cols);
-        if (kind == KD_NORM_RMS) {
-            return {0.0, rsqrt(sum(s2, room) * (1.0 / all) + eps)};
-        }
-        s1 = wave_total(s1);
-        s2 = wave_total(s2);
-        const double n = static_cast<double>(held(wave, cols)), by = n > 0 ? s1 / n : 0.0;
-        double mean = pivot + by, squares = s2 - s1 * by;
-        if constexpr (kWaves > 1) {
-            const Pair p = exchange({mean, squares}, room);
-            const int w = lane % kMostWaves;
-            const double base = from_lane(p.a, 0), count = w < kWaves ? static_cast<double>(held(w, cols)) : 0.0;
-            const double d = count > 0 ? p.a - base : 0.0;
-            s1 = from_lane(sum_of_16(count * d), 15);
-            s2 = from_lane(sum_of_16((count > 0 ? p.b : 0.0) + count * d * d), 15);
-            mean = base + s1 * (1.0 / all);
-            squares = s2 - s1 * (s1 * (1.0 / all));
-        }
-        return {mean, rsqrt((squares < 0 ? 0.0 : squares) * (1.0 / all) + eps)};
+        return stats(kind, eps, cols, pivot, s1, s2, room, [&](int w) { return held(w, cols); });
     }
 };
 
@@ -466,6 +339,101 @@ __global__ __launch_bounds__(group_of(Threads)) void block_rows_kernel(T* h, T* 
     }
 }
 
+// Any row length: a workgroup reads a row again in each pass, from the caches for the most part.
+constexpr int kWideThreads = 1024, kWideStep = 4 * kWideThreads;
+
+// How many values of a row of any length a wave of such a workgroup has.
+__device__ __forceinline__ int wide_held(int wave, int cols) {
+    return cols / kWideStep * 256 + min(max(cols % kWideStep - 256 * wave, 0), 256);
+}
+// A row's statistics, from quads that `value(c)` gives.
+template <typename F>
+__device__ __forceinline__ RowStats wide_stats(int kind, double eps, int cols, const Team<kWideThreads, 1>& at, Pair* room, F value) {
+    if (kind == KD_NORM_NONE) return {0.0, 1.0};
+    double pivot = 0, s1 = 0, s2 = 0;
+    for (int c = at.column(0); c < cols; c += kWideStep) {
+        const auto q = value(c);
+        if (kind == KD_NORM_LAYER && c == at.column(0)) pivot = from_lane(static_cast<double>(q.v[0]), 0);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const double d = c + e < cols ? static_cast<double>(q.v[e]) - pivot : 0.0;
+            s1 += d;
+            s2 += d * d;
+        }
+    }
+    return at.stats(kind, eps, cols, pivot, s1, s2, room, [&](int w) { return wide_held(w, cols); });
+}
+
+// Four values of x after their norm, and whether dropout keeps them.
+struct Branch {
+    double u[4], n[4];
+    bool kept[4];
+};
+template <typename T>
+__device__ __forceinline__ Branch branch_at(const BlockArgs<T>& a, const RowStats& s, int64_t row, int c, int cols, uint32_t step, bool x_read) {
+    Branch b{{}, {}, {true, true, true, true}};
+    if (a.masked) a.mask.kept(b.kept, static_cast<uint32_t>(row), static_cast<uint32_t>(c / 4), step);
+    if (!x_read) return b;
+    const Quad<T> x = take_quad<false>(a.x + row * a.cols, c, cols);
+    const Quad<T> w = quad_or<false>(a.after.weight, c, cols, T(1)), bias = quad_or<false>(a.after.bias, c, cols, T(0));
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        b.u[e] = s.unit(static_cast<double>(x.v[e]));
+        b.n[e] = a.after.kind != KD_NORM_NONE ? b.u[e] * static_cast<double>(w.v[e]) + static_cast<double>(bias.v[e]) : b.u[e];
+    }
+    return b;
+}
+template <typename T> __device__ __forceinline__ Quad<T> gate_at(const BlockArgs<T>& a, int64_t row, int c, int cols) {
+    return quad_or<false>(a.gate != nullptr ? a.gate + row * a.gate_step : nullptr, c, cols, T(1));
+}
+
+template <typename T>
+__global__ __launch_bounds__(kWideThreads) void block_rows_wide_kernel(T* h, T* y, double* stats, BlockArgs<T> a) {
+    __shared__ Pair room[2][2][kMostWaves];
+    const Team<kWideThreads, 1> at;
+    const uint32_t step = a.mask.step_now();
+    const int cols = static_cast<int>(a.cols);
+    int turn = 0;
+    for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x, turn ^= 1) {
+        const int64_t base = row * a.cols;
+        const RowStats after = wide_stats(a.after.kind, a.after.eps, cols, at, room[turn][0],
+                                          [&](int c) { return take_quad<false>(a.x + base, c, cols); });
+        const auto sum = [&](int c) {
+            const Branch b = branch_at(a, after, row, c, cols, step, true);
+            const Quad<T> gate = gate_at(a, row, c, cols), r = quad_or<false>(a.residual != nullptr ? a.residual + base : nullptr, c, cols, T(0));
+            Quad<T> q;
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                q.v[e] = static_cast<T>(a.block_scale * static_cast<double>(gate.v[e]) * (b.kept[e] ? b.n[e] * a.mask.scale : 0.0) +
+                                        a.residual_scale * static_cast<double>(r.v[e]));
+            return q;
+        };
+        // h may take x's or the residual's place, so from then on it is read there; each thread reads what it has written
+        if (h != nullptr)
+            for (int c = at.column(0); c < cols; c += kWideStep) give_quad<false>(h + base, c, cols, sum(c));
+        const auto h_at = [&](int c) { return h != nullptr ? take_quad<false>(h + base, c, cols) : sum(c); };
+        RowStats before{0.0, 1.0};
+        if (a.before.kind != KD_NORM_NONE && (y != nullptr || stats != nullptr)) {
+            before = wide_stats(a.before.kind, a.before.eps, cols, at, room[turn][1], h_at);
+            if (y != nullptr)
+                for (int c = at.column(0); c < cols; c += kWideStep) {
+                    Quad<T> q = h_at(c);
+                    const Quad<T> w = quad_or<false>(a.before.weight, c, cols, T(1)), b = quad_or<false>(a.before.bias, c, cols, T(0));
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        q.v[e] = static_cast<T>(before.unit(static_cast<double>(q.v[e])) * static_cast<double>(w.v[e]) + static_cast<double>(b.v[e]));
+                    give_quad<false>(y + base, c, cols, q);
+                }
+        }
+        if (stats != nullptr && threadIdx.x == 0) {
+            stats[4 * row] = after.mean;
+            stats[4 * row + 1] = after.rate;
+            stats[4 * row + 2] = before.mean;
+            stats[4 * row + 3] = before.rate;
+        }
+    }
+}
+
 // ---- its backward pass ----------------------------------------------------------------------------
 //
 // With v the standardized rows of h, u those of x, w the norms' weights: p = grad_y w, G = grad_h + rate (p - mean p -
@@ -487,78 +455,95 @@ template <typename T> struct BackArgs {
 
     __device__ __forceinline__ RowStats after(int64_t row) const { return {stats[4 * row], stats[4 * row + 1]}; }
     __device__ __forceinline__ RowStats before(int64_t row) const { return {stats[4 * row + 2], stats[4 * row + 3]}; }
-    // p and p v at column c
-    __device__ __forceinline__ double weighted(int64_t base, int64_t c) const {
-        return static_cast<double>(grad_y[base + c]) * b.before.weight_at(c);
-    }
-    // G, from the means of p and p v
-    __device__ __forceinline__ double total(int64_t base, int64_t c, const RowStats& s, double mean, double along) const {
-        double g = grad_h != nullptr ? static_cast<double>(grad_h[base + c]) : 0.0;
-        if (grad_y != nullptr) g += s.rate * (weighted(base, c) - mean - s.unit(static_cast<double>(h[base + c])) * along);
-        return g;
-    }
-    __device__ __forceinline__ bool kept(int64_t row, int64_t c, uint32_t step) const {
-        if (!b.masked) return true;
-        bool k[4];
-        b.mask.kept(k, static_cast<uint32_t>(row), static_cast<uint32_t>(c / 4), step);
-        return c % 4 == 0 ? k[0] : c % 4 == 1 ? k[1] : c % 4 == 2 ? k[2] : k[3];
-    }
 };
 
-// The means of p and p v of a row.
-template <typename T>
-__device__ __forceinline__ void before_means(const BackArgs<T>& a, int64_t row, double* room, double& mean, double& along) {
-    mean = along = 0;
-    if (a.grad_y == nullptr) return;
-    const int64_t base = row * a.b.cols;
-    const RowStats s = a.before(row);
-    for (int64_t c = threadIdx.x; c < a.b.cols; c += blockDim.x) {
-        const double p = a.weighted(base, c);
-        mean += p;
-        along += p * s.unit(static_cast<double>(a.h[base + c]));
-    }
-    along = group_sum(along, room) / static_cast<double>(a.b.cols);
-    mean = a.b.before.kind == KD_NORM_LAYER ? group_sum(mean, room) / static_cast<double>(a.b.cols) : 0.0;
-}
-
 // Any row length: the gradients of the rows, a workgroup each, and the means of p and p v, [rows][2], for the sums over rows.
-template <typename T> __global__ __launch_bounds__(kThreads) void block_back_wide_kernel(double* means, BackArgs<T> a) {
-    __shared__ double room[kThreads / 64];
+template <typename T> __global__ __launch_bounds__(kWideThreads) void block_back_wide_kernel(double* means, BackArgs<T> a) {
+    __shared__ Pair room[2][2][kMostWaves];
+    const Team<kWideThreads, 1> at;
     const uint32_t step = a.b.mask.step_now();
-    const int64_t cols = a.b.cols;
-    for (int64_t row = blockIdx.x; row < a.b.rows; row += gridDim.x) {
-        const int64_t base = row * cols;
+    const int cols = static_cast<int>(a.b.cols);
+    const double share = 1.0 / cols;
+    const bool normed = a.b.after.kind != KD_NORM_NONE && a.x != nullptr, x_read = normed || a.gate != nullptr;
+    int turn = 0;
+    for (int64_t row = blockIdx.x; row < a.b.rows; row += gridDim.x, turn ^= 1) {
+        const int64_t base = row * a.b.cols;
         const RowStats before = a.before(row), after = a.after(row);
-        double mean, along, back_mean = 0, back_along = 0;
-        before_means(a, row, room, mean, along);
+        double mean = 0, along = 0, back_mean = 0, back_along = 0;
+        if (a.grad_y != nullptr) {
+            for (int c = at.column(0); c < cols; c += kWideStep) {
+                const Quad<T> grad_y = take_quad<false>(a.grad_y + base, c, cols), h = take_quad<false>(a.h + base, c, cols);
+                const Quad<T> w = quad_or<false>(a.b.before.weight, c, cols, T(1));
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    if (c + e >= cols) continue;
+                    const double p = static_cast<double>(grad_y.v[e]) * static_cast<double>(w.v[e]);
+                    mean += p;
+                    along += p * before.unit(static_cast<double>(h.v[e]));
+                }
+            }
+            const Pair s = at.sums(mean, along, room[turn][0]);
+            mean = a.b.before.kind == KD_NORM_LAYER ? s.a * share : 0.0;
+            along = s.b * share;
+        }
         if (means != nullptr && threadIdx.x == 0) {
             means[2 * row] = mean;
             means[2 * row + 1] = along;
         }
         if (a.x == nullptr && a.residual == nullptr && a.gate == nullptr) continue;
-        const auto through = [&](int64_t c, double g) {
-            return a.kept(row, c, step) ? a.b.block_scale * gate_at(a.b, row, c) * g * a.b.mask.scale : 0.0;
-        };
-        const bool normed = a.b.after.kind != KD_NORM_NONE && a.x != nullptr;
-        if (normed) {
-            for (int64_t c = threadIdx.x; c < cols; c += kThreads) {
-                const double q = through(c, a.total(base, c, before, mean, along)) * a.b.after.weight_at(c);
-                back_mean += q;
-                back_along += q * after.unit(static_cast<double>(a.b.x[base + c]));
+        // G and what it gives of the block's output, for four columns
+        const auto through = [&](int c, const Branch& b, double(&g)[4], double(&d)[4]) {
+            const Quad<T> grad_h = quad_or<false>(a.grad_h != nullptr ? a.grad_h + base : nullptr, c, cols, T(0));
+            const Quad<T> gate = gate_at(a.b, row, c, cols);
+            Quad<T> grad_y{}, h{}, w{};
+            if (a.grad_y != nullptr) {
+                grad_y = take_quad<false>(a.grad_y + base, c, cols);
+                h = take_quad<false>(a.h + base, c, cols);
+                w = quad_or<false>(a.b.before.weight, c, cols, T(1));
             }
-            back_along = group_sum(back_along, room) / static_cast<double>(cols);
-            back_mean = a.b.after.kind == KD_NORM_LAYER ? group_sum(back_mean, room) / static_cast<double>(cols) : 0.0;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                g[e] = static_cast<double>(grad_h.v[e]);
+                if (a.grad_y != nullptr)
+                    g[e] += before.rate * (static_cast<double>(grad_y.v[e]) * static_cast<double>(w.v[e]) - mean -
+                                           before.unit(static_cast<double>(h.v[e])) * along);
+                d[e] = b.kept[e] ? a.b.block_scale * static_cast<double>(gate.v[e]) * g[e] * a.b.mask.scale : 0.0;
+            }
+        };
+        if (normed) {
+            for (int c = at.column(0); c < cols; c += kWideStep) {
+                const Branch b = branch_at(a.b, after, row, c, cols, step, true);
+                const Quad<T> w = quad_or<false>(a.b.after.weight, c, cols, T(1));
+                double g[4], d[4];
+                through(c, b, g, d);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    if (c + e >= cols) continue;
+                    const double q = d[e] * static_cast<double>(w.v[e]);
+                    back_mean += q;
+                    back_along += q * b.u[e];
+                }
+            }
+            const Pair s = at.sums(back_mean, back_along, room[turn][1]);
+            back_mean = a.b.after.kind == KD_NORM_LAYER ? s.a * share : 0.0;
+            back_along = s.b * share;
         }
         // outputs may take the place of what is read at the same element
-        for (int64_t c = threadIdx.x; c < cols; c += kThreads) {
-            const double g = a.total(base, c, before, mean, along);
-            const double branch = a.gate != nullptr ? branch_at(a.b, after, row, c, step) : 0.0;
-            double d = through(c, g);
-            if (normed)
-                d = after.rate * (d * a.b.after.weight_at(c) - back_mean - after.unit(static_cast<double>(a.b.x[base + c])) * back_along);
-            if (a.residual != nullptr) a.residual[base + c] = static_cast<T>(a.b.residual_scale * g);
-            if (a.gate != nullptr) a.gate[base + c] = static_cast<T>(a.b.block_scale * branch * g);
-            if (a.x != nullptr) a.x[base + c] = static_cast<T>(d);
+        for (int c = at.column(0); c < cols; c += kWideStep) {
+            const Branch b = branch_at(a.b, after, row, c, cols, step, x_read);
+            const Quad<T> w = quad_or<false>(a.b.after.weight, c, cols, T(1));
+            double g[4], d[4];
+            through(c, b, g, d);
+            Quad<T> to_x, to_residual, to_gate;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                to_residual.v[e] = static_cast<T>(a.b.residual_scale * g[e]);
+                to_gate.v[e] = static_cast<T>(b.kept[e] ? a.b.block_scale * (b.n[e] * a.b.mask.scale) * g[e] : 0.0);
+                to_x.v[e] = static_cast<T>(normed ? after.rate * (d[e] * static_cast<double>(w.v[e]) - back_mean - b.u[e] * back_along) : d[e]);
+            }
+            if (a.residual != nullptr) give_quad<false>(a.residual + base, c, cols, to_residual);
+            if (a.gate != nullptr) give_quad<false>(a.gate + base, c, cols, to_gate);
+            if (a.x != nullptr) give_quad<false>(a.x + base, c, cols, to_x);
         }
     }
 }
@@ -1152,7 +1137,7 @@ extern "C" int kd_block_rows(int dtype, void* h, void* y, double* stats, const k
             else rows(threads, quads, std::false_type{}, b.rows);
         };
         if (b.rows >= int64_t{1} << 22 || b.cols > 16384)
-            one(block_rows_wide_kernel<T>, kThreads, std::min<int64_t>(b.rows, int64_t{compute_units()} * 32));
+            one(block_rows_wide_kernel<T>, kWideThreads, std::min<int64_t>(b.rows, int64_t{compute_units()} * 16));
         else if (b.cols <= 256) rows(Int<64>{}, Int<1>{}, std::false_type{}, (b.rows + 3) / 4);
         else if (b.cols <= 512) rows(Int<64>{}, Int<2>{}, std::false_type{}, (b.rows + 3) / 4);
         else if (b.cols <= 1024) choose(Int<256>{}, Int<1>{}, 5);
@@ -1244,7 +1229,7 @@ extern "C" int kd_block_rows_backward(int dtype, const kd_block_grads* grads, co
         if (!fits_grid(column_groups, kJoinWaves * 64) || !fits_grid(plan.segments, kBackThreads<float>) ||
             (plan.threads == 0 && plan.segments > 65535))
             return fail(KD_E_INVALID, name + ": too many rows or columns");
-        const uint32_t groups = static_cast<uint32_t>(std::min<int64_t>(b.rows, int64_t{compute_units()} * 32));
+        const uint32_t groups = static_cast<uint32_t>(std::min<int64_t>(b.rows, int64_t{compute_units()} * 16));
         double* means = static_cast<double*>(workspace);
         T* parts = summed ? reinterpret_cast<T*>(means + (plan.threads == 0 ? 2 * b.rows : 0)) : nullptr;
         if (b.rows > 0 && plan.threads == 0) {
@@ -1254,7 +1239,7 @@ extern "C" int kd_block_rows_backward(int dtype, const kd_block_grads* grads, co
                 };
                 const bool whole = b.cols % 4 == 0, two = b.cols <= 8192;
                 if (b.rows >= int64_t{1} << 22 || b.cols > (sizeof(T) == 4 ? 16384 : 8192)) {
-                    hipLaunchKernelGGL((block_back_wide_kernel<T>), dim3(groups), dim3(kThreads), 0, stream(), to, which);
+                    hipLaunchKernelGGL((block_back_wide_kernel<T>), dim3(groups), dim3(kWideThreads), 0, stream(), to, which);
                     return;
                 }
                 if (two) whole ? one(block_back_row_kernel<T, 2, true>) : one(block_back_row_kernel<T, 2, false>);
