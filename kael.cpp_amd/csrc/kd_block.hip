@@ -16,41 +16,19 @@ constexpr int kThreads = 256;
 template <typename T> struct Quad {
     T v[4];
 };
-typedef uint32_t u32x4 __attribute__((ext_vector_type(4), aligned(4)));
-// Past: past the caches.
-template <bool Past = false, typename T> __device__ __forceinline__ Quad<T> load_quad(const T* row, int64_t c) {
+template <typename T> __device__ __forceinline__ Quad<T> load_quad(const T* row, int64_t c, int64_t cols) {
     Quad<T> q;
-    if constexpr (Past) {
-        u32x4 raw[sizeof q / 16];
-#pragma unroll
-        for (int i = 0; i < static_cast<int>(sizeof q / 16); ++i) raw[i] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(row + c) + i);
-        __builtin_memcpy(&q, raw, sizeof q);
-    } else {
-        __builtin_memcpy(&q, row + c, sizeof q);
-    }
-    return q;
-}
-template <bool Past = false, typename T> __device__ __forceinline__ Quad<T> load_quad(const T* row, int64_t c, int64_t cols) {
-    if (c + 4 <= cols) return load_quad<Past>(row, c);
-    Quad<T> q;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) q.v[e] = c + e < cols ? row[c + e] : T(0);
-    return q;
-}
-template <bool Past = false, typename T> __device__ __forceinline__ void store_quad(T* row, int64_t c, const Quad<T>& q) {
-    if constexpr (Past) {
-        u32x4 raw[sizeof q / 16];
-        __builtin_memcpy(raw, &q, sizeof q);
-#pragma unroll
-        for (int i = 0; i < static_cast<int>(sizeof q / 16); ++i) __builtin_nontemporal_store(raw[i], reinterpret_cast<u32x4*>(row + c) + i);
-    } else {
-        __builtin_memcpy(row + c, &q, sizeof q);
-    }
-}
-template <bool Past = false, typename T>
-__device__ __forceinline__ void store_quad(T* row, int64_t c, int64_t cols, const Quad<T>& q) {
     if (c + 4 <= cols) {
-        store_quad<Past>(row, c, q);
+        __builtin_memcpy(&q, row + c, sizeof q);
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) q.v[e] = c + e < cols ? row[c + e] : T(0);
+    }
+    return q;
+}
+template <typename T> __device__ __forceinline__ void store_quad(T* row, int64_t c, int64_t cols, const Quad<T>& q) {
+    if (c + 4 <= cols) {
+        __builtin_memcpy(row + c, &q, sizeof q);
     } else {
 #pragma unroll
         for (int e = 0; e < 4; ++e)
@@ -213,20 +191,24 @@ template <typename T> __device__ __forceinline__ const T* place_in(const T* row,
 template <typename T> __device__ __forceinline__ T* place_in(T* row, int c) {
     return reinterpret_cast<T*>(reinterpret_cast<char*>(row) + static_cast<uint32_t>(c) * static_cast<uint32_t>(sizeof(T)));
 }
-template <bool Whole, bool Past = false, typename T> __device__ __forceinline__ Quad<T> take_quad(const T* row, int c, int cols) {
-    if constexpr (Whole) return load_quad<Past>(place_in(row, min(c, cols - 4)), 0);
-    else return load_quad<Past>(place_in(row, c), 0, cols - c);
-}
-template <bool Whole, bool Past = false, typename T> __device__ __forceinline__ Quad<T> quad_or(const T* p, int c, int cols, T otherwise) {
-    Quad<T> q{otherwise, otherwise, otherwise, otherwise};
-    if (p != nullptr) q = take_quad<Whole, Past>(p, c, cols);
-    return q;
-}
-template <bool Whole, bool Past = false, typename T> __device__ __forceinline__ void give_quad(T* row, int c, int cols, const Quad<T>& q) {
+template <bool Whole, typename T> __device__ __forceinline__ Quad<T> take_quad(const T* row, int c, int cols) {
     if constexpr (Whole) {
-        if (c < cols) store_quad<Past>(place_in(row, c), 0, q);
+        Quad<T> q;
+        __builtin_memcpy(&q, place_in(row, min(c, cols - 4)), sizeof q);
+        return q;
     } else {
-        store_quad<Past>(place_in(row, c), 0, cols - c, q);
+        return load_quad(place_in(row, c), 0, cols - c);
+    }
+}
+template <bool Whole, typename T> __device__ __forceinline__ Quad<T> quad_or(const T* p, int c, int cols, T otherwise) {
+    if (p != nullptr) return take_quad<Whole>(p, c, cols);
+    return {otherwise, otherwise, otherwise, otherwise};
+}
+template <bool Whole, typename T> __device__ __forceinline__ void give_quad(T* row, int c, int cols, const Quad<T>& q) {
+    if constexpr (Whole) {
+        if (c < cols) __builtin_memcpy(place_in(row, c), &q, sizeof q);
+    } else {
+        store_quad(place_in(row, c), 0, cols - c, q);
     }
 }
 
@@ -591,7 +573,7 @@ __global__ __launch_bounds__(kThreads) void block_columns_kernel(T* parts, const
                 const double u = after.unit(static_cast<double>(x.v[e]));
                 if (gate_sum)
                     sums[kGate][e] += kept[e] ? through * (normed ? u * static_cast<double>(after_w.v[e]) + static_cast<double>(after_b.v[e]) : u) : 0.0;
-                const double d = through * static_cast<double>(gate.v[e]);
+                const double d = kept[e] ? through * static_cast<double>(gate.v[e]) : 0.0;
                 if (normed) {
                     sums[kAfterWeight][e] += d * u;
                     sums[kAfterBias][e] += d;
@@ -680,7 +662,7 @@ __global__ __launch_bounds__(1024) void block_back_row_kernel(double* means, Bac
                                       before.unit(static_cast<double>(h[i].v[e])) * along);
             to_residual.v[e] = static_cast<T>(a.b.residual_scale * own);
             const double through = bits >> (4 * i + e) & 1 ? a.b.block_scale * a.b.mask.scale * own : 0.0;
-            g[i][e] = through * static_cast<double>(gate.v[e]);
+            g[i][e] = bits >> (4 * i + e) & 1 ? through * static_cast<double>(gate.v[e]) : 0.0;
             if (x_read) {
                 const double u = after.unit(static_cast<double>(x[i].v[e]));
                 if (a.gate != nullptr) {
@@ -724,7 +706,6 @@ __global__ __launch_bounds__(1024) void block_back_row_kernel(double* means, Bac
 // A team's rows one after another, each read once: the rows' gradients and the sums over the team's rows. Those lie in LDS,
 // [team][wanted sum][cols up to a quad], where each thread adds to the places of its own columns: in registers they took 20 a
 // quad (40 in f64), and the row spilled. Ahead: a row is loaded while the one before it is worked on.
-// Held: the norms' weights and the gate stay in registers.
 template <typename T> constexpr int kBackThreads = std::is_same_v<T, float> ? 1024 : 512;
 
 struct SumPlaces {
@@ -772,7 +753,7 @@ template <typename T, int Quads, bool Whole> struct BackRow {
     }
 };
 
-template <typename T, int Threads, int Quads, bool Ahead, bool Held, bool Whole>
+template <typename T, int Threads, int Quads, bool Held, bool Whole>
 __global__ __launch_bounds__(kBackThreads<T>) void block_back_kernel(T* parts, BackArgs<T> a, int64_t rows_per_team, SumPlaces places) {
     constexpr int kTeams = kBackThreads<T> / Threads;
     extern __shared__ __attribute__((aligned(16))) char shared[];
@@ -803,11 +784,11 @@ __global__ __launch_bounds__(kBackThreads<T>) void block_back_kernel(T* parts, B
         for (int i = 0; i < Quads; ++i)
             if (at.column(i) < cols) __builtin_memset(sums + k * padded + at.column(i), 0, 4 * sizeof(T));
     BackRow<T, Quads, Whole> now, next;
-    if (Ahead && first < end) next.load(a, at, first, x_read);
+    if (Held && first < end) next.load(a, at, first, x_read);
     for (int64_t n = 0; n < rows_per_team; ++n) {
         const int64_t row = first + n, base = row * a.b.cols;
         const bool here = row < end;  // the same for all threads of a team; the teams meet at the barriers
-        if constexpr (Ahead) {
+        if constexpr (Held) {
             now = next;
             if (row + 1 < end) next.load(a, at, row + 1, x_read);
         } else if (here) {
@@ -1136,7 +1117,9 @@ extern "C" int kd_block_rows(int dtype, void* h, void* y, double* stats, const k
             if (weights > 2 && b.rows >= 8 * groups) rows(threads, quads, std::true_type{}, groups);
             else rows(threads, quads, std::false_type{}, b.rows);
         };
-        if (b.rows >= int64_t{1} << 22 || b.cols > 16384)
+        // rows that a launch of a workgroup for each (or for four short ones) can have
+        const int64_t most = b.cols <= 512 ? int64_t{1} << 25 : b.cols <= 2048 ? int64_t{1} << 23 : int64_t{1} << 21;
+        if (b.rows > most || b.cols > 16384)
             one(block_rows_wide_kernel<T>, kWideThreads, std::min<int64_t>(b.rows, int64_t{compute_units()} * 16));
         else if (b.cols <= 256) rows(Int<64>{}, Int<1>{}, std::false_type{}, (b.rows + 3) / 4);
         else if (b.cols <= 512) rows(Int<64>{}, Int<2>{}, std::false_type{}, (b.rows + 3) / 4);
@@ -1238,7 +1221,7 @@ extern "C" int kd_block_rows_backward(int dtype, const kd_block_grads* grads, co
                     hipLaunchKernelGGL(kernel, dim3(static_cast<uint32_t>(b.rows)), dim3(1024), 0, stream(), to, which);
                 };
                 const bool whole = b.cols % 4 == 0, two = b.cols <= 8192;
-                if (b.rows >= int64_t{1} << 22 || b.cols > (sizeof(T) == 4 ? 16384 : 8192)) {
+                if (b.rows > int64_t{1} << 21 || b.cols > (sizeof(T) == 4 ? 16384 : 8192)) {
                     hipLaunchKernelGGL((block_back_wide_kernel<T>), dim3(groups), dim3(kWideThreads), 0, stream(), to, which);
                     return;
                 }
@@ -1267,8 +1250,8 @@ extern "C" int kd_block_rows_backward(int dtype, const kd_block_grads* grads, co
             const auto teams = [&](auto threads, auto quads) {
                 constexpr int kTeam = decltype(threads)::value, kQuads = decltype(quads)::value;
                 constexpr bool kHeld = kQuads == 1;
-                if (b.cols % 4 == 0) one(block_back_kernel<T, kTeam, kQuads, kHeld, kHeld, true>);
-                else one(block_back_kernel<T, kTeam, kQuads, kHeld, kHeld, false>);
+                if (b.cols % 4 == 0) one(block_back_kernel<T, kTeam, kQuads, kHeld, true>);
+                else one(block_back_kernel<T, kTeam, kQuads, kHeld, false>);
             };
             constexpr int kMost = kBackThreads<T>;
             if (plan.quads == 2) {

@@ -272,6 +272,30 @@ def test_what_is_not_finite_stays_in_its_row(kdb):
     assert np.isfinite(np.delete(grads["x"], 3, 0)).all() and np.isnan(grads["residual"][3]).all()
 
 
+@pytest.mark.parametrize("cols", [90, 1100, 6000, 9001, 20003])
+def test_dropped_places_of_an_infinite_gate_have_no_gradient(kdb, cols):
+    rng = np.random.default_rng(cols)
+    case = random_case(rng, 3, cols, np.float64, R, None, 2, 0.5)
+    out = ~block.kept(3, cols, 0.5, **case.counter)
+    grad = rng.normal(size=(3, cols))
+    want = case.backward(case.sum()[0], grad, None)
+    case.gate[out] = np.inf
+    run = Run(kdb, case)
+    run.forward()
+    got = run.backward(grad, None)
+    for name in ("x", "gate", "after_weight", "after_bias"):
+        check(got[name], *want[name], 2.0 ** -52, 4 * noise(case) + 2.0 ** -48, name)
+
+
+def test_millions_of_short_rows(kdb):
+    """More rows than a launch has workgroups of 1024 threads."""
+    rng = np.random.default_rng(11)
+    rows, cols = (1 << 22) + 3, 5
+    case = random_case(rng, rows, cols, np.float32, None, R, 0, 1.0)
+    grad = rng.normal(size=(rows, cols)).astype(np.float32)
+    check_block(kdb, case, grad, grad)
+
+
 @pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
 @pytest.mark.parametrize("shape", [(4, 100), (3, 4096), (2, 40001)], ids=lambda s: "x".join(map(str, s)))
 def test_in_place(kdb, shape, dtype):
