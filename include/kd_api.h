@@ -593,8 +593,7 @@ typedef struct kd_norm {
  *   y = before(h)
  * gate is NULL (1), one row of [cols] (gate_rows = 1) or a row for each row (gate_rows = rows); gate_rows is 0 without a
  * gate. residual may be NULL: h = block_scale * gate * a. With all but x left out it is an embedding's dropout and the
- * first norm; with one row a decoding step's. kael composes the same from dropout, add and LayerNorm (reference
- * src/nn/transformer.cpp:149-165). */
+ * first norm; with one row a decoding step's. cols <= 2^28. kael composes the same from dropout, add and LayerNorm. */
 typedef struct kd_block {
     const void* x;
     const void* residual;

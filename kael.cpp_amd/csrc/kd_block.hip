@@ -1,6 +1,7 @@
 // kd_block.hip - dropout with a mask from a counter, and the end of a transformer's block (a norm of its output, dropout, a
 // gate, the residual sum, the norm ahead of the next block) with its backward pass.
 #include <algorithm>
+#include <iterator>
 
 #include "kd_counter.h"
 #include "kd_internal.h"
@@ -1202,11 +1203,12 @@ extern "C" int kd_block_rows_backward(int dtype, const kd_block_grads* grads, co
         const Memory ins[] = {{x_read ? b.x : nullptr, bytes}, {grad_h, bytes}, {grad_y, bytes},
                               {grad_y != nullptr ? h : nullptr, bytes}, {b.gate, b.gate_rows * row_bytes}, {stats, b.rows * 32},
                               {b.after.kind != KD_NORM_NONE ? b.after.weight : nullptr, row_bytes},
+                              {b.after.kind != KD_NORM_NONE && grads->gate != nullptr ? b.after.bias : nullptr, row_bytes},
                               {b.before.kind != KD_NORM_NONE ? b.before.weight : nullptr, row_bytes}};
-        for (int i = 0; i < 8; ++i) {
+        for (int i = 0; i < static_cast<int>(std::size(outs)); ++i) {
             for (int j = 0; j < i; ++j)
                 if (overlap(outs[i].at, outs[i].bytes, outs[j].at, outs[j].bytes)) return fail(KD_E_INVALID, name + ": outputs overlap");
-            for (int j = 0; j < 8; ++j) {
+            for (int j = 0; j < static_cast<int>(std::size(ins)); ++j) {
                 // an element's own place
                 const bool same = outs[i].at == ins[j].at && ((i == 0 && j <= 2) || (i == 1 && (j == 1 || j == 2)));
                 if (!same && overlap(outs[i].at, outs[i].bytes, ins[j].at, ins[j].bytes))
@@ -1248,8 +1250,9 @@ extern "C" int kd_block_rows_backward(int dtype, const kd_block_grads* grads, co
                 else if constexpr (sizeof(T) == 4) whole ? one(block_back_row_kernel<T, 4, true>) : one(block_back_row_kernel<T, 4, false>);
             };
             // gradients in the place of what the sums read are written last
-            const bool first = !summed || grads->residual == grad_h || grads->residual == grad_y || grads->x == b.x || grads->x == grad_h ||
-                               grads->x == grad_y;
+            const auto in_place = [](const void* out, const void* in) { return out != nullptr && out == in; };
+            const bool first = !summed || in_place(grads->residual, grad_h) || in_place(grads->residual, grad_y) || in_place(grads->x, b.x) ||
+                               in_place(grads->x, grad_h) || in_place(grads->x, grad_y);
             if (summed) {
                 BackArgs<T> which = a;
                 if (first) which.x = which.residual = which.gate = nullptr;

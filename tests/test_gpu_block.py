@@ -410,3 +410,11 @@ def test_offsets_past_32_bits(kdb):
     kdb.call("block_rows_backward", kd.F32, kd.BlockGrads(x=far[2].ptr, residual=far[1].ptr), b, far[2].ptr, stats.ptr, far[1].ptr, None, None, 0)
     np.testing.assert_array_equal(last(far[1]), grads["residual"])
     np.testing.assert_array_equal(last(far[2]), grads["x"])
+
+
+@pytest.mark.parametrize("cols", [4065, 4068, 4069, 4072])
+def test_sums_that_fill_the_local_memory(kdb, cols):
+    """Five f64 sums of rows that just fit a workgroup's local memory, and of rows that just do not."""
+    rng = np.random.default_rng(cols)
+    case = random_case(rng, 300, cols, np.float64, L, R, 1, 0.9)
+    check_block(kdb, case, *(rng.normal(size=(300, cols)) for _ in range(2)))

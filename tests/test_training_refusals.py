@@ -132,3 +132,10 @@ def test_bad_policies(lib):
         (6, policy(**c), INVALID) for c in (dict(advantages=None), dict(temperature=0.0), dict(temperature=INF), dict(low=-0.1), dict(low=1.1),
                                             dict(low=NAN), dict(high=-0.1), dict(high=INF), dict(kl=-1.0), dict(kl=NAN))], "kd_policy_rows:")
     assert lib.lib.kd_policy_rows(kd.F32, None, None, None, None, None, policy(), None, 0, 8) == 0
+
+
+def test_an_output_over_the_first_norms_bias(lib):
+    assert backward(lib, block(), kd.BlockGrads(x=at(4), gate=at(15))) == INVALID
+    assert backward(lib, block(), kd.BlockGrads(after_bias=at(4), gate=at(15))) == INVALID
+    assert lib.error().startswith("kd_block_rows_backward:")
+    assert lib.lib.kd_block_rows(kd.F32, at(8), at(9), at(10), block(cols=(1 << 28) + 4)) == INVALID
