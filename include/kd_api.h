@@ -639,7 +639,7 @@ typedef struct kd_block_grads {
  * an input or another output otherwise.
  * Summed gradients pass through `workspace` (device, 16-byte aligned, as many bytes as kd_block_rows_workspace says; not
  * needed where none of them is wanted). Calls that may run at the same time (streams, graphs) need workspaces of their own.
- * The same arguments and contents give the same bits. */
+ * A workspace for some number of rows serves fewer rows of the same length too. The same arguments and contents give the same bits. */
 int kd_block_rows_backward(int dtype, const kd_block_grads* grads, const kd_block* block, const void* h,
                            const double* stats, const void* grad_h, const void* grad_y, void* workspace,
                            int64_t workspace_bytes);

@@ -223,6 +223,18 @@ template <bool Whole, typename T> __device__ __forceinline__ void give_quad(T* r
     }
 }
 
+// The same past the caches.
+template <bool Whole, typename T> __device__ __forceinline__ void give_quad_past(T* row, int c, int cols, const Quad<T>& q) {
+    typedef T Four __attribute__((ext_vector_type(4), aligned(sizeof(T))));
+    if (Whole ? c < cols : c + 4 <= cols) {
+        Four four;
+        __builtin_memcpy(&four, &q, sizeof q);
+        __builtin_nontemporal_store(four, reinterpret_cast<Four*>(place_in(row, c)));
+    } else if constexpr (!Whole) {
+        store_quad(place_in(row, c), 0, cols - c, q);
+    }
+}
+
 // Keeps the compiler from holding the f64 forms of a loop's f32 constants, twice the registers, all through the loop.
 __device__ __forceinline__ void converted_late(Quad<float>& q) {
 #pragma unroll
@@ -438,7 +450,7 @@ __global__ __launch_bounds__(kWideThreads) void block_rows_wide_kernel(T* h, T* 
 // sums: rows of up to 4096. The parts' sums are 5 % more where each team has many rows, and a second kernel adds them in order, so that no
 // result depends on what runs first. f32: 8192 x 4096, both norms and a gate, 170 to 205 + 6 us (805 MB at 3.9 to 4.7 TB/s, vector ALU busy
 // 0.70); a layer norm alone 148 + 5; 32768 x 1024 160 + 5; 4096 x 256 10.5 + 3.8, where it is a chain of launch, loads and two
-// exchanges. 4096 x 8192 with all sums: the row's kernel 220, the sums' 125 to 131 us.
+// exchanges. 4096 x 8192 with all sums: the row's kernel 214, the sums' 102 us.
 
 enum Sum { kAfterWeight, kAfterBias, kBeforeWeight, kBeforeBias, kGate, kSums };
 
@@ -549,22 +561,23 @@ template <typename T> __global__ __launch_bounds__(kWideThreads) void block_back
 }
 
 // The sums over a segment of rows: [segment][sum][cols]. A workgroup takes 256 columns, four a lane, and its waves share the rows.
+// All segments go from the last rows to the first ones, since the last cache may still hold the last ones from the rows' kernel (4096 x 8192,
+// both norms and a gate, 122 us from the first row on, 111 so, 104 where the gradients went past the caches as well).
 template <typename T, bool Whole>
-__global__ __launch_bounds__(kThreads) void block_columns_kernel(T* parts, const double* means, BackArgs<T> a,
-                                                                 int64_t rows_per_segment) {
+__global__ __launch_bounds__(kThreads) void block_columns_kernel(T* parts, const double* means, BackArgs<T> a) {
     constexpr int kWaves = kThreads / 64;
     __shared__ double room[kWaves][4][64];
     const uint32_t step = a.b.mask.step_now();
     const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) / 64);
     const int c = static_cast<int>(blockIdx.x) * 256 + 4 * lane, cols = static_cast<int>(a.b.cols);
-    const int64_t from = blockIdx.y * rows_per_segment, to = min(a.b.rows, from + rows_per_segment);
     const bool normed = a.b.after.kind != KD_NORM_NONE, gate_sum = a.sums[kGate] != nullptr, x_read = normed || gate_sum;
     const Quad<T> before_w = quad_or<Whole>(a.b.before.weight, c, cols, T(1)), after_w = quad_or<Whole>(a.b.after.weight, c, cols, T(1));
     const Quad<T> after_b = quad_or<Whole>(a.b.after.bias, c, cols, T(0));
     Quad<T> gate = quad_or<Whole>(a.b.gate, c, cols, T(1));
     double sums[kSums][4] = {};
     if (c < cols)
-        for (int64_t row = from + wave; row < to; row += kWaves) {
+        for (int64_t row = a.b.rows - 1 - (static_cast<int64_t>(wave) * gridDim.y + blockIdx.y); row >= 0;
+             row -= static_cast<int64_t>(kWaves) * gridDim.y) {
             const int64_t base = row * a.b.cols;
             const RowStats before = a.before(row), after = a.after(row);
             const double mean = means[2 * row], along = means[2 * row + 1];
@@ -619,14 +632,18 @@ __global__ __launch_bounds__(kThreads) void block_columns_kernel(T* parts, const
 }
 
 // A long row's gradients, by a workgroup that holds it: what the sums over rows would take of the registers is left to
-// block_columns_kernel, which reads the rows again (4096 x 8192: 161 + 101 us for a layer norm; in one kernel, which spilled, 421 to 480).
-template <typename T, int Quads, bool Whole>
+// block_columns_kernel, which reads the rows again (4096 x 8192: 165 + 80 us for a layer norm; in one kernel, which spilled, 421 to 480).
+template <typename T, int Quads, bool Whole, bool Past>
 __global__ __launch_bounds__(1024) void block_back_row_kernel(double* means, BackArgs<T> a) {
     __shared__ Pair room[2][kMostWaves];
     const Team<1024, Quads> at;
     const int64_t row = blockIdx.x, base = row * a.b.cols;
     const int cols = static_cast<int>(a.b.cols);
     const double share = 1.0 / cols;
+    const auto give = [&](T* out, int c, const Quad<T>& q) {
+        if constexpr (Past) give_quad_past<Whole>(out, c, cols, q);
+        else give_quad<Whole>(out, c, cols, q);
+    };
     const RowStats before = a.before(row), after = a.after(row);
     Quad<T> grad_h[Quads], grad_y[Quads], h[Quads];
     double g[Quads][4], mean = 0, along = 0;
@@ -695,8 +712,8 @@ __global__ __launch_bounds__(1024) void block_back_row_kernel(double* means, Bac
                 }
             }
         }
-        if (a.residual != nullptr) give_quad<Whole>(a.residual + base, c, cols, to_residual);
-        if (a.gate != nullptr) give_quad<Whole>(a.gate + base, c, cols, to_gate);
+        if (a.residual != nullptr) give(a.residual + base, c, to_residual);
+        if (a.gate != nullptr) give(a.gate + base, c, to_gate);
     }
     if (a.x == nullptr) return;
     double back_mean = 0, back_along = 0;
@@ -717,7 +734,7 @@ __global__ __launch_bounds__(1024) void block_back_row_kernel(double* means, Bac
                 d = after.rate * (d * static_cast<double>(after_w.v[e]) - back_mean - after.unit(static_cast<double>(x[i].v[e])) * back_along);
             to.v[e] = static_cast<T>(d);
         }
-        give_quad<Whole>(a.x + base, c, cols, to);
+        give(a.x + base, c, to);
     }
 }
 
@@ -982,6 +999,7 @@ template <int N> using Int = std::integral_constant<int, N>;
 struct BackPlan {
     int threads, quads;
     int64_t rows_per_team, segments;
+    int64_t most;  // segments that no smaller number of rows passes, so that a workspace serves those too
 };
 int group_threads(int dtype) { return dtype == KD_F32 ? kBackThreads<float> : kBackThreads<double>; }
 // Bytes of LDS that `wanted` sums take for teams of `threads`.
@@ -989,10 +1007,11 @@ int64_t sums_bytes(int dtype, int64_t cols, int threads, int wanted) {
     return group_threads(dtype) / threads * wanted * ((cols + 3) / 4 * 4) * dtype_size(dtype);
 }
 BackPlan wide_plan(int64_t rows, int64_t cols) {
-    // workgroups of 256 columns, four for each CU, of 16 rows at least
-    const int64_t wanted = (int64_t{4} * compute_units() + (cols + 255) / 256 - 1) / ((cols + 255) / 256);
-    const int64_t segments = std::clamp<int64_t>(wanted, 1, (rows + 15) / 16), each = (rows + segments - 1) / segments;
-    return {0, 0, each, (rows + each - 1) / each};
+    // Workgroups of 256 columns, of 16 rows at least, and four for each CU at most, as many as it has at once: with one round more of a few
+    // of them 8192 x 5120 took 168 us instead of 113, 2000 x 20000 215 instead of 133.
+    const int64_t wanted = int64_t{4} * compute_units() / ((cols + 255) / 256);
+    const int64_t segments = std::clamp<int64_t>(wanted, 1, (rows + 15) / 16);
+    return {0, 0, 0, segments, segments};
 }
 BackPlan back_plan(int dtype, int64_t rows, int64_t cols, int wanted) {
     if (cols > 4096) return wide_plan(rows, cols);
@@ -1002,8 +1021,10 @@ BackPlan back_plan(int dtype, int64_t rows, int64_t cols, int wanted) {
     while (threads * quads * 4 < cols) quads *= 2;
     if (sums_bytes(dtype, cols, threads, wanted) > 159 * 1024) return wide_plan(rows, cols);
     const int64_t teams = group / threads, all = teams * compute_units();
-    const int64_t each = std::clamp<int64_t>((rows + all - 1) / all, 1, 32);
-    return {threads, quads, each, (rows + teams * each - 1) / (teams * each)};
+    // a CU has one workgroup at a time: as few rounds as parts of 32 rows allow, all of them full
+    const int64_t rounds = (rows + 32 * all - 1) / (32 * all), each = (rows + rounds * all - 1) / (rounds * all);
+    return {threads, quads, each, (rows + teams * each - 1) / (teams * each),
+            std::min(rounds * compute_units(), (rows + teams - 1) / teams)};
 }
 // What the passes of any number of sums need at most.
 int64_t room_of(int dtype, int64_t rows, int64_t cols) {
@@ -1011,7 +1032,7 @@ int64_t room_of(int dtype, int64_t rows, int64_t cols) {
     int64_t most = 0;
     for (int wanted = 1; wanted <= kSums; ++wanted) {
         const BackPlan plan = back_plan(dtype, rows, cols, wanted);
-        most = std::max(most, (plan.threads == 0 ? rows * 16 : 0) + plan.segments * kSums * cols * dtype_size(dtype));
+        most = std::max(most, (plan.threads == 0 ? rows * 16 : 0) + plan.most * kSums * cols * dtype_size(dtype));
     }
     return most;
 }
@@ -1228,7 +1249,7 @@ extern "C" int kd_block_rows_backward(int dtype, const kd_block_grads* grads, co
         SumPlaces places;
         places.wanted = 0;
         for (int k = 0; k < kSums; ++k) places.at[k] = sums[k] != nullptr ? places.wanted++ : -1;
-        const BackPlan plan = b.rows > 0 ? back_plan(dtype, b.rows, b.cols, places.wanted) : BackPlan{0, 0, 0, 0};
+        const BackPlan plan = b.rows > 0 ? back_plan(dtype, b.rows, b.cols, places.wanted) : BackPlan{};
         const int64_t column_groups = (b.cols + 63) / 64;
         if (!fits_grid(column_groups, kJoinWaves * 64) || !fits_grid(plan.segments, kBackThreads<float>) ||
             (plan.threads == 0 && plan.segments > 65535))
@@ -1241,13 +1262,26 @@ extern "C" int kd_block_rows_backward(int dtype, const kd_block_grads* grads, co
                 const auto one = [&](auto kernel) {
                     hipLaunchKernelGGL(kernel, dim3(static_cast<uint32_t>(b.rows)), dim3(1024), 0, stream(), to, which);
                 };
-                const bool whole = b.cols % 4 == 0, two = b.cols <= 8192;
+                const auto by_whole = [&](auto quads, auto past) {
+                    constexpr int kQuads = decltype(quads)::value;
+                    constexpr bool kPast = decltype(past)::value;
+                    if (b.cols % 4 == 0) one(block_back_row_kernel<T, kQuads, true, kPast>);
+                    else one(block_back_row_kernel<T, kQuads, false, kPast>);
+                };
+                // Gradients go past the caches where they and the inputs are more than the last one's 256 MiB: the sums' kernel finds
+                // more of its inputs there. Both kernels, us, through / past: f32, both norms and a gate, 4096 x 8192 332 / 325, a layer
+                // norm alone 254 / 244, 8192 x 5120 337 / 331; f64 2000 x 8192 366 / 352.
+                const bool past = to != nullptr && 6 * b.rows * b.cols * static_cast<int64_t>(sizeof(T)) > int64_t{256} << 20;
+                const auto by_past = [&](auto quads) {
+                    if (past) by_whole(quads, std::true_type{});
+                    else by_whole(quads, std::false_type{});
+                };
                 if (b.rows > int64_t{1} << 21 || b.cols > (sizeof(T) == 4 ? 16384 : 8192)) {
                     hipLaunchKernelGGL((block_back_wide_kernel<T>), dim3(groups), dim3(kWideThreads), 0, stream(), to, which);
                     return;
                 }
-                if (two) whole ? one(block_back_row_kernel<T, 2, true>) : one(block_back_row_kernel<T, 2, false>);
-                else if constexpr (sizeof(T) == 4) whole ? one(block_back_row_kernel<T, 4, true>) : one(block_back_row_kernel<T, 4, false>);
+                if (b.cols <= 8192) by_past(Int<2>{});
+                else if constexpr (sizeof(T) == 4) by_past(Int<4>{});
             };
             // gradients in the place of what the sums read are written last
             const auto in_place = [](const void* out, const void* in) { return out != nullptr && out == in; };
@@ -1258,8 +1292,8 @@ extern "C" int kd_block_rows_backward(int dtype, const kd_block_grads* grads, co
                 if (first) which.x = which.residual = which.gate = nullptr;
                 rows_of(which, means);
                 const dim3 grid(static_cast<uint32_t>((b.cols + 255) / 256), static_cast<uint32_t>(plan.segments));
-                if (b.cols % 4 == 0) hipLaunchKernelGGL((block_columns_kernel<T, true>), grid, dim3(kThreads), 0, stream(), parts, means, a, plan.rows_per_team);
-                else hipLaunchKernelGGL((block_columns_kernel<T, false>), grid, dim3(kThreads), 0, stream(), parts, means, a, plan.rows_per_team);
+                if (b.cols % 4 == 0) hipLaunchKernelGGL((block_columns_kernel<T, true>), grid, dim3(kThreads), 0, stream(), parts, means, a);
+                else hipLaunchKernelGGL((block_columns_kernel<T, false>), grid, dim3(kThreads), 0, stream(), parts, means, a);
             }
             if (first && by_row) rows_of(a, nullptr);
         }

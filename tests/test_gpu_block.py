@@ -418,3 +418,12 @@ def test_sums_that_fill_the_local_memory(kdb, cols):
     rng = np.random.default_rng(cols)
     case = random_case(rng, 300, cols, np.float64, L, R, 1, 0.9)
     check_block(kdb, case, *(rng.normal(size=(300, cols)) for _ in range(2)))
+
+
+@pytest.mark.parametrize("shape", [(8193, 4096), (8705, 1100), (33000, 520), (140001, 31), (4100, 5120), (900, 16001)],
+                         ids=lambda s: "x".join(map(str, s)))
+def test_sums_of_more_rows_than_one_round(kdb, shape):
+    """Parts of the rows in two rounds and more; segments that are not as many as the rows' parts; gradients past the caches."""
+    rng = np.random.default_rng(shape[0])
+    case = random_case(rng, *shape, np.float32, R, L, 1, 0.9)
+    check_block(kdb, case, *(rng.normal(size=shape).astype(np.float32) for _ in range(2)))

@@ -139,3 +139,14 @@ def test_an_output_over_the_first_norms_bias(lib):
     assert backward(lib, block(), kd.BlockGrads(after_bias=at(4), gate=at(15))) == INVALID
     assert lib.error().startswith("kd_block_rows_backward:")
     assert lib.lib.kd_block_rows(kd.F32, at(8), at(9), at(10), block(cols=(1 << 28) + 4)) == INVALID
+
+
+@pytest.mark.parametrize("dtype", [kd.F32, kd.F64])
+@pytest.mark.parametrize("cols", [1, 30, 256, 1000, 1537, 2048, 4068, 4096, 5120, 20000])
+def test_a_workspace_serves_fewer_rows(lib, cols, dtype):
+    n = ctypes.c_int64()
+    last = 0
+    for rows in [*range(0, 1200), *range(1200, 70000, 37), 1 << 20, (1 << 20) + 1, 1 << 30]:
+        assert lib.lib.kd_block_rows_workspace(ctypes.byref(n), dtype, rows, cols) == 0
+        assert n.value >= last, rows
+        last = n.value
