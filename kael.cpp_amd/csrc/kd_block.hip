@@ -93,46 +93,45 @@ template <typename T> struct BlockArgs {
     bool masked;
 };
 
-// A team of `Threads` threads has a row: each thread the columns 4 * (thread + i * Threads) .. + 3 for i < Quads.
+// A team of `threads` threads has a row: each thread the columns 4 * (thread + i * threads) .. + 3 for i < Quads.
 struct Pair {
     double a, b;
 };
 constexpr int kMostWaves = 16;
 
-template <int Threads, int Quads> struct Team {
-    static constexpr int kWaves = Threads / 64;
-    int team, wave, lane;  // wave: its place in the team
-    __device__ __forceinline__ Team() {
+template <int Quads> struct Team {
+    int threads, waves, team, wave, lane;  // wave: its place in the team
+    __device__ __forceinline__ explicit Team(int threads_) : threads(threads_), waves(threads_ / 64) {
         const int wave_at = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) / 64);
-        team = wave_at / kWaves;
-        wave = wave_at % kWaves;
+        team = wave_at / waves;
+        wave = wave_at % waves;
         lane = threadIdx.x % 64;
     }
-    __device__ __forceinline__ int column(int i) const { return 4 * (wave * 64 + lane + i * Threads); }
+    __device__ __forceinline__ int column(int i) const { return 4 * (wave * 64 + lane + i * threads); }
     // How many of a row's values the team's wave w holds.
-    __device__ __forceinline__ static int held(int w, int cols) {
+    __device__ __forceinline__ int held(int w, int cols) const {
         int n = 0;
 #pragma unroll
-        for (int i = 0; i < Quads; ++i) n += min(max(cols - 4 * (w * 64 + i * Threads), 0), 256);
+        for (int i = 0; i < Quads; ++i) n += min(max(cols - 4 * (w * 64 + i * threads), 0), 256);
         return n;
     }
-    // Lane w < kWaves gets wave w's pair; one barrier, so a team's next exchange takes another room.
+    // Lane w < waves gets wave w's pair; one barrier, so a team's next exchange takes another room.
     __device__ __forceinline__ Pair exchange(Pair own, Pair* room) const {
-        if (lane == 0) room[team * kWaves + wave] = own;
+        if (lane == 0) room[team * waves + wave] = own;
         __syncthreads();
         const int w = lane % kMostWaves;
-        return w < kWaves ? room[team * kWaves + w] : Pair{0, 0};
+        return w < waves ? room[team * waves + w] : Pair{0, 0};
     }
     __device__ __forceinline__ Pair sums(double a, double b, Pair* room) const {
         a = wave_total(a);
         b = wave_total(b);
-        if constexpr (kWaves == 1) return {a, b};
+        if (waves == 1) return {a, b};
         const Pair p = exchange({a, b}, room);
         return {from_lane(sum_of_16(p.a), 15), from_lane(sum_of_16(p.b), 15)};
     }
     __device__ __forceinline__ double sum(double a, Pair* room) const {
         a = wave_total(a);
-        if constexpr (kWaves == 1) return a;
+        if (waves == 1) return a;
         return from_lane(sum_of_16(exchange({a, 0}, room).a), 15);
     }
     // A row's statistics from its waves' sums. For a layer norm those are of the distances from one of the wave's own values, the
@@ -147,10 +146,10 @@ template <int Threads, int Quads> struct Team {
         s2 = wave_total(s2);
         const double n = static_cast<double>(of(wave)), by = n > 0 ? s1 / n : 0.0;
         double mean = pivot + by, squares = s2 - s1 * by;
-        if constexpr (kWaves > 1) {
+        if (waves > 1) {
             const Pair p = exchange({mean, squares}, room);
             const int w = lane % kMostWaves;
-            const double base = from_lane(p.a, 0), count = w < kWaves ? static_cast<double>(of(w)) : 0.0;
+            const double base = from_lane(p.a, 0), count = w < waves ? static_cast<double>(of(w)) : 0.0;
             const double d = count > 0 ? p.a - base : 0.0;
             s1 = from_lane(sum_of_16(count * d), 15);
             s2 = from_lane(sum_of_16((count > 0 ? p.b : 0.0) + count * d * d), 15);
@@ -177,8 +176,8 @@ template <int Threads, int Quads> struct Team {
 };
 
 // Whether a thread's values are kept, a bit each.
-template <typename T, int Threads, int Quads>
-__device__ __forceinline__ uint32_t kept_bits(const BlockArgs<T>& a, const Team<Threads, Quads>& at, int64_t row, uint32_t step) {
+template <typename T, int Quads>
+__device__ __forceinline__ uint32_t kept_bits(const BlockArgs<T>& a, const Team<Quads>& at, int64_t row, uint32_t step) {
     uint32_t bits = ~0u;
     if (a.masked) {
         bits = 0;
@@ -242,16 +241,15 @@ __device__ __forceinline__ void converted_late(Quad<float>& q) {
 }
 __device__ __forceinline__ void converted_late(Quad<double>&) {}
 
-constexpr int group_of(int threads) { return threads < 256 ? 256 : threads; }
-
 // A row is read once, held in registers and written once. Held: the workgroup takes rows one after another, with the norms'
 // weights and the gate in registers all through (from the L2 they are more bytes than the row) and the next row on its way.
-template <typename T, int Threads, int Quads, bool Whole, bool Held>
-__global__ __launch_bounds__(group_of(Threads)) void block_rows_kernel(T* h, T* y, double* stats, BlockArgs<T> a) {
-    constexpr int kTeams = group_of(Threads) / Threads;
-    static_assert(kTeams == 1 || Threads == 64, "teams that leave early may not meet at barriers");
+// Most: the workgroup's threads at most, all of them a row's, as many waves as the row needs (All: that is all of them, which the
+// compiler then knows); 64: a workgroup of four such rows, whose waves leave when they are done and so may not meet at barriers.
+template <typename T, int Most, int Quads, bool Whole, bool Held, bool All>
+__global__ __launch_bounds__(Most == 64 ? 256 : Most) void block_rows_kernel(T* h, T* y, double* stats, BlockArgs<T> a) {
+    constexpr int kTeams = Most == 64 ? 4 : 1;
     __shared__ Pair room[2][2][kMostWaves];  // by turns: a row's waves may be ahead of the last ones of the row before
-    const Team<Threads, Quads> at;
+    const Team<Quads> at(All ? Most : blockDim.x);
     const int cols = static_cast<int>(a.cols);
     const uint32_t step = a.mask.step_now();
     Quad<T> after_w[Quads], after_b[Quads], before_w[Quads], before_b[Quads], gate[Quads];
@@ -354,7 +352,7 @@ __device__ __forceinline__ int wide_held(int wave, int cols) {
 }
 // A row's statistics, from quads that `value(c)` gives.
 template <typename F>
-__device__ __forceinline__ RowStats wide_stats(int kind, double eps, int cols, const Team<kWideThreads, 1>& at, Pair* room, F value) {
+__device__ __forceinline__ RowStats wide_stats(int kind, double eps, int cols, const Team<1>& at, Pair* room, F value) {
     if (kind == KD_NORM_NONE) return {0.0, 1.0};
     double pivot = 0, s1 = 0, s2 = 0;
     for (int c = at.column(0); c < cols; c += kWideStep) {
@@ -396,7 +394,7 @@ template <typename T> __device__ __forceinline__ Quad<T> gate_at(const BlockArgs
 template <typename T>
 __global__ __launch_bounds__(kWideThreads) void block_rows_wide_kernel(T* h, T* y, double* stats, BlockArgs<T> a) {
     __shared__ Pair room[2][2][kMostWaves];
-    const Team<kWideThreads, 1> at;
+    const Team<1> at(kWideThreads);
     const uint32_t step = a.mask.step_now();
     const int cols = static_cast<int>(a.cols);
     int turn = 0;
@@ -472,7 +470,7 @@ template <typename T> struct BackArgs {
 // Any row length: the gradients of the rows, a workgroup each, and the means of p and p v, [rows][2], for the sums over rows.
 template <typename T> __global__ __launch_bounds__(kWideThreads) void block_back_wide_kernel(double* means, BackArgs<T> a) {
     __shared__ Pair room[2][2][kMostWaves];
-    const Team<kWideThreads, 1> at;
+    const Team<1> at(kWideThreads);
     const uint32_t step = a.b.mask.step_now();
     const int cols = static_cast<int>(a.b.cols);
     const double share = 1.0 / cols;
@@ -636,7 +634,7 @@ __global__ __launch_bounds__(kThreads) void block_columns_kernel(T* parts, const
 template <typename T, int Quads, bool Whole, bool Past>
 __global__ __launch_bounds__(1024) void block_back_row_kernel(double* means, BackArgs<T> a) {
     __shared__ Pair room[2][kMostWaves];
-    const Team<1024, Quads> at;
+    const Team<Quads> at(blockDim.x);
     const int64_t row = blockIdx.x, base = row * a.b.cols;
     const int cols = static_cast<int>(a.b.cols);
     const double share = 1.0 / cols;
@@ -761,7 +759,7 @@ template <typename T> __device__ __forceinline__ void add_quad(T* place, const Q
 template <typename T, int Quads, bool Whole> struct BackRow {
     Quad<T> x[Quads], h[Quads], grad_h[Quads], grad_y[Quads];
     RowStats after, before;
-    template <int Threads> __device__ __forceinline__ void load(const BackArgs<T>& a, const Team<Threads, Quads>& at, int64_t row, bool x_read) {
+    __device__ __forceinline__ void load(const BackArgs<T>& a, const Team<Quads>& at, int64_t row, bool x_read) {
         const int64_t base = row * a.b.cols;
         const int cols = static_cast<int>(a.b.cols);
 #pragma unroll
@@ -790,13 +788,14 @@ template <typename T, int Quads, bool Whole> struct BackRow {
     }
 };
 
+// Threads: a team's, 0: as many as are given.
 template <typename T, int Threads, int Quads, bool Held, bool Whole>
-__global__ __launch_bounds__(kBackThreads<T>) void block_back_kernel(T* parts, BackArgs<T> a, int64_t rows_per_team, SumPlaces places) {
-    constexpr int kTeams = kBackThreads<T> / Threads;
+__global__ __launch_bounds__(kBackThreads<T>) void block_back_kernel(T* parts, BackArgs<T> a, int threads, int64_t rows_per_team, SumPlaces places) {
     extern __shared__ __attribute__((aligned(16))) char shared[];
     __shared__ Pair room[2][2][kMostWaves];  // by turns: a row's waves may be ahead of the last ones of the row before
-    const Team<Threads, Quads> at;
-    const int64_t first = (static_cast<int64_t>(blockIdx.x) * kTeams + at.team) * rows_per_team, end = min(a.b.rows, first + rows_per_team);
+    const Team<Quads> at(Threads != 0 ? Threads : threads);
+    const int teams = static_cast<int>(blockDim.x) / threads;
+    const int64_t first = (static_cast<int64_t>(blockIdx.x) * teams + at.team) * rows_per_team, end = min(a.b.rows, first + rows_per_team);
     const int cols = static_cast<int>(a.b.cols);
     const double share = 1.0 / cols;
     const uint32_t step = a.b.mask.step_now();
@@ -952,9 +951,9 @@ __global__ __launch_bounds__(kBackThreads<T>) void block_back_kernel(T* parts, B
         if (places.at[k] < 0) continue;
         T* out = parts + (static_cast<int64_t>(blockIdx.x) * kSums + k) * cols;
         const T* own = reinterpret_cast<const T*>(shared) + places.at[k] * padded;
-        for (int c = threadIdx.x; c < cols; c += kBackThreads<T>) {
+        for (int c = threadIdx.x; c < cols; c += blockDim.x) {
             double total = static_cast<double>(own[c]);
-            for (int t = 1; t < kTeams; ++t) total += static_cast<double>(own[t * places.wanted * padded + c]);
+            for (int t = 1; t < teams; ++t) total += static_cast<double>(own[t * places.wanted * padded + c]);
             out[c] = static_cast<T>(total);
         }
     }
@@ -994,36 +993,35 @@ __global__ __launch_bounds__(kJoinWaves * 64) void block_join_kernel(BackArgs<T>
 
 template <int N> using Int = std::integral_constant<int, N>;
 
-// How a backward pass is divided. threads: a row's team, 0 for rows that registers do not hold; segments: parts of the rows
-// whose sums are kept apart.
+// How a backward pass is divided. threads: a row's team, 0 for rows that registers do not hold; teams: of a workgroup; segments:
+// parts of the rows whose sums are kept apart.
 struct BackPlan {
     int threads, quads;
-    int64_t rows_per_team, segments;
+    int64_t teams, rows_per_team, segments;
     int64_t most;  // segments that no smaller number of rows passes, so that a workspace serves those too
 };
-int group_threads(int dtype) { return dtype == KD_F32 ? kBackThreads<float> : kBackThreads<double>; }
-// Bytes of LDS that `wanted` sums take for teams of `threads`.
-int64_t sums_bytes(int dtype, int64_t cols, int threads, int wanted) {
-    return group_threads(dtype) / threads * wanted * ((cols + 3) / 4 * 4) * dtype_size(dtype);
-}
+// Threads of a team that holds a row in `quads` quads a thread: as many waves as that takes, so that none is idle (32768 x 768 176 us in teams of
+// four waves, three of them at work, 158 in teams of three; 20000 x 1280 207 and 150).
+int team_threads(int64_t cols, int quads) { return static_cast<int>((cols + 256 * quads - 1) / (256 * quads) * 64); }
+int most_threads(int dtype) { return dtype == KD_F32 ? kBackThreads<float> : kBackThreads<double>; }
+// Bytes of LDS that `wanted` sums take for `teams`.
+int64_t sums_bytes(int dtype, int64_t cols, int64_t teams, int wanted) { return teams * wanted * ((cols + 3) / 4 * 4) * dtype_size(dtype); }
 BackPlan wide_plan(int64_t rows, int64_t cols) {
     // Workgroups of 256 columns, of 16 rows at least, and four for each CU at most, as many as it has at once: with one round more of a few
     // of them 8192 x 5120 took 168 us instead of 113, 2000 x 20000 215 instead of 133.
     const int64_t wanted = int64_t{4} * compute_units() / ((cols + 255) / 256);
     const int64_t segments = std::clamp<int64_t>(wanted, 1, (rows + 15) / 16);
-    return {0, 0, 0, segments, segments};
+    return {0, 0, 0, 0, segments, segments};
 }
 BackPlan back_plan(int dtype, int64_t rows, int64_t cols, int wanted) {
     if (cols > 4096) return wide_plan(rows, cols);
-    int threads = 64, quads = 1;
-    const int group = group_threads(dtype);
-    while (threads < group && threads * 4 < cols) threads *= 2;
-    while (threads * quads * 4 < cols) quads *= 2;
-    if (sums_bytes(dtype, cols, threads, wanted) > 159 * 1024) return wide_plan(rows, cols);
-    const int64_t teams = group / threads, all = teams * compute_units();
+    const int quads = cols <= 4 * most_threads(dtype) ? 1 : 2, threads = team_threads(cols, quads);
+    const int64_t teams = most_threads(dtype) / threads;
+    if (sums_bytes(dtype, cols, teams, wanted) > 159 * 1024) return wide_plan(rows, cols);
+    const int64_t all = teams * compute_units();
     // a CU has one workgroup at a time: as few rounds as parts of 32 rows allow, all of them full
     const int64_t rounds = (rows + 32 * all - 1) / (32 * all), each = (rows + rounds * all - 1) / (rounds * all);
-    return {threads, quads, each, (rows + teams * each - 1) / (teams * each),
+    return {threads, quads, teams, each, (rows + teams * each - 1) / (teams * each),
             std::min(rounds * compute_units(), (rows + teams - 1) / teams)};
 }
 // What the passes of any number of sums need at most.
@@ -1143,32 +1141,40 @@ extern "C" int kd_block_rows(int dtype, void* h, void* y, double* stats, const k
             hipLaunchKernelGGL(kernel, dim3(static_cast<uint32_t>(groups)), dim3(threads), 0, stream(), static_cast<T*>(h),
                                static_cast<T*>(y), stats, a);
         };
-        const auto rows = [&](auto threads, auto quads, auto held, int64_t groups) {
-            constexpr int kTeam = decltype(threads)::value, kGroup = group_of(kTeam), kQuads = decltype(quads)::value;
+        const auto rows = [&](auto most, auto quads, auto held, int threads, int64_t groups) {
+            constexpr int kMost = decltype(most)::value, kQuads = decltype(quads)::value;
             constexpr bool kHeld = decltype(held)::value;
-            if (b.cols % 4 == 0) one(block_rows_kernel<T, kTeam, kQuads, true, kHeld>, kGroup, groups);
-            else one(block_rows_kernel<T, kTeam, kQuads, false, kHeld>, kGroup, groups);
+            if (b.cols % 4 != 0) one(block_rows_kernel<T, kMost, kQuads, false, kHeld, kMost == 64>, threads, groups);
+            else if (kMost == 64 || threads == kMost) one(block_rows_kernel<T, kMost, kQuads, true, kHeld, true>, threads, groups);
+            else one(block_rows_kernel<T, kMost, kQuads, true, kHeld, false>, threads, groups);
         };
-        // Workgroups a CU that hold the weights: as many as fit its registers. They hold them where the weights are more bytes than x and
+        // Workgroups a CU that hold the weights: as many as fit its registers, `waves` a CU. They hold them where the weights are more bytes than x and
         // residual, and where each has some rows; us, weights read / held, both norms and a gate: 32768 x 768 115 / 97, 16384 x 2048
         // 128 / 104, 8192 x 4096 124 / 106; a layer norm ahead of the next block alone: 91 / 96, 102 / 113, 103 / 109.
-        const auto choose = [&](auto threads, auto quads, int a_unit) {
+        const auto choose = [&](auto most, auto quads, int waves) {
             const int weights = 2 * (b.after.kind != KD_NORM_NONE) + 2 * (b.before.kind != KD_NORM_NONE) + (b.gate_rows == 1);
-            const int64_t groups = int64_t{a_unit} * compute_units();
-            if (weights > 2 && b.rows >= 8 * groups) rows(threads, quads, std::true_type{}, groups);
-            else rows(threads, quads, std::false_type{}, b.rows);
+            const int threads = team_threads(b.cols, decltype(quads)::value);
+            const int64_t groups = int64_t{waves * 64 / threads} * compute_units();
+            if (weights > 2 && b.rows >= 8 * groups) rows(most, quads, std::true_type{}, threads, groups);
+            else rows(most, quads, std::false_type{}, threads, b.rows);
         };
+        // Quads a thread: so few registers that a CU has two workgroups of rows at least, but few enough threads that the barriers wait for few; one row a CU,
+        // of many threads, where there are no more rows. us, a layer norm with dropout / both norms and a gate: 16384 x 2560 two quads 148 / 194,
+        // three 141 / 137; 7000 x 6144 two 132 / 164, three 138 / 177, four 174 / 212; 4096 x 8192 two 124 / 163, four 115 / 142.
         // rows that a launch of a workgroup for each (or for four short ones) can have
-        const int64_t most = b.cols <= 512 ? int64_t{1} << 25 : b.cols <= 2048 ? int64_t{1} << 23 : int64_t{1} << 21;
-        if (b.rows > most || b.cols > 16384)
+        const int64_t limit = b.cols <= 512 ? int64_t{1} << 25 : b.cols <= 2048 ? int64_t{1} << 23 : int64_t{1} << 21;
+        if (b.rows > limit || b.cols > 16384)
             one(block_rows_wide_kernel<T>, kWideThreads, std::min<int64_t>(b.rows, int64_t{compute_units()} * 16));
-        else if (b.cols <= 256) rows(Int<64>{}, Int<1>{}, std::false_type{}, (b.rows + 3) / 4);
-        else if (b.cols <= 512) rows(Int<64>{}, Int<2>{}, std::false_type{}, (b.rows + 3) / 4);
-        else if (b.cols <= 1024) choose(Int<256>{}, Int<1>{}, 5);
-        else if (b.cols <= 2048) choose(Int<256>{}, Int<2>{}, 2);
-        else if (b.cols <= 4096) choose(Int<512>{}, Int<2>{}, 1);
-        else if (b.cols <= 8192) rows(Int<1024>{}, Int<2>{}, std::false_type{}, b.rows);
-        else rows(Int<1024>{}, Int<4>{}, std::false_type{}, b.rows);
+        else if (b.cols <= 256) rows(Int<64>{}, Int<1>{}, std::false_type{}, 256, (b.rows + 3) / 4);
+        else if (b.cols <= 512) rows(Int<64>{}, Int<2>{}, std::false_type{}, 256, (b.rows + 3) / 4);
+        else if (b.cols <= 1024) choose(Int<256>{}, Int<1>{}, 20);
+        else if (sizeof(T) == 4 && b.cols > 2048 && b.cols <= 12 * 256) choose(Int<256>{}, Int<3>{}, 8);
+        else if (b.cols <= 4096) choose(Int<512>{}, Int<2>{}, sizeof(T) == 4 ? 12 : 8);
+        else if (b.cols <= 6144 || (b.cols <= 8192 && b.rows <= compute_units()))
+            rows(Int<1024>{}, Int<2>{}, std::false_type{}, team_threads(b.cols, 2), b.rows);
+        else if (b.cols <= 8192) rows(Int<512>{}, Int<4>{}, std::false_type{}, team_threads(b.cols, 4), b.rows);
+        else if (b.cols <= 12288) rows(Int<1024>{}, Int<3>{}, std::false_type{}, team_threads(b.cols, 3), b.rows);
+        else rows(Int<1024>{}, Int<4>{}, std::false_type{}, team_threads(b.cols, 4), b.rows);
     };
     if (dtype == KD_F32) launch(0.f);
     else launch(0.0);
@@ -1259,14 +1265,14 @@ extern "C" int kd_block_rows_backward(int dtype, const kd_block_grads* grads, co
         T* parts = summed ? reinterpret_cast<T*>(means + (plan.threads == 0 ? 2 * b.rows : 0)) : nullptr;
         if (b.rows > 0 && plan.threads == 0) {
             const auto rows_of = [&](const BackArgs<T>& which, double* to) {
-                const auto one = [&](auto kernel) {
-                    hipLaunchKernelGGL(kernel, dim3(static_cast<uint32_t>(b.rows)), dim3(1024), 0, stream(), to, which);
+                const auto one = [&](auto kernel, int quads) {
+                    hipLaunchKernelGGL(kernel, dim3(static_cast<uint32_t>(b.rows)), dim3(team_threads(b.cols, quads)), 0, stream(), to, which);
                 };
                 const auto by_whole = [&](auto quads, auto past) {
                     constexpr int kQuads = decltype(quads)::value;
                     constexpr bool kPast = decltype(past)::value;
-                    if (b.cols % 4 == 0) one(block_back_row_kernel<T, kQuads, true, kPast>);
-                    else one(block_back_row_kernel<T, kQuads, false, kPast>);
+                    if (b.cols % 4 == 0) one(block_back_row_kernel<T, kQuads, true, kPast>, kQuads);
+                    else one(block_back_row_kernel<T, kQuads, false, kPast>, kQuads);
                 };
                 // Gradients go past the caches where they and the inputs are more than the last one's 256 MiB: the sums' kernel finds
                 // more of its inputs there. Both kernels, us, through / past: f32, both norms and a gate, 4096 x 8192 332 / 325, a layer
@@ -1299,24 +1305,25 @@ extern "C" int kd_block_rows_backward(int dtype, const kd_block_grads* grads, co
         }
         if (plan.threads != 0) {
             const auto one = [&](auto kernel) {
-                hipLaunchKernelGGL(kernel, dim3(static_cast<uint32_t>(plan.segments)), dim3(kBackThreads<T>),
-                                   static_cast<uint32_t>(sums_bytes(dtype, b.cols, plan.threads, places.wanted)), stream(), parts, a,
+                hipLaunchKernelGGL(kernel, dim3(static_cast<uint32_t>(plan.segments)), dim3(static_cast<uint32_t>(plan.teams * plan.threads)),
+                                   static_cast<uint32_t>(sums_bytes(dtype, b.cols, plan.teams, places.wanted)), stream(), parts, a, plan.threads,
                                    plan.rows_per_team, places);
             };
-            const auto teams = [&](auto threads, auto quads) {
+            // what the compiler knows of a team saves 3 %
+            const auto by_whole = [&](auto threads, auto quads) {
                 constexpr int kTeam = decltype(threads)::value, kQuads = decltype(quads)::value;
                 constexpr bool kHeld = kQuads == 1;
                 if (b.cols % 4 == 0) one(block_back_kernel<T, kTeam, kQuads, kHeld, true>);
                 else one(block_back_kernel<T, kTeam, kQuads, kHeld, false>);
             };
-            constexpr int kMost = kBackThreads<T>;
             if (plan.quads == 2) {
-                if constexpr (sizeof(T) == 8) teams(Int<kMost>{}, Int<2>{});
-            } else if (plan.threads == kMost) teams(Int<kMost>{}, Int<1>{});
-            else if (plan.threads == 64) teams(Int<64>{}, Int<1>{});
-            else if (plan.threads == 128) teams(Int<128>{}, Int<1>{});
-            else if (plan.threads == 256) teams(Int<256>{}, Int<1>{});
-            else teams(Int<512>{}, Int<1>{});
+                if constexpr (sizeof(T) == 8) by_whole(Int<0>{}, Int<2>{});
+            } else if (plan.threads == 64) by_whole(Int<64>{}, Int<1>{});
+            else if (plan.threads == 256) by_whole(Int<256>{}, Int<1>{});
+            else if (plan.threads == 512) by_whole(Int<512>{}, Int<1>{});
+            else if (plan.threads == 1024) {
+                if constexpr (sizeof(T) == 4) by_whole(Int<1024>{}, Int<1>{});
+            } else by_whole(Int<0>{}, Int<1>{});
         }
         if (summed)
             hipLaunchKernelGGL((block_join_kernel<T>), dim3(static_cast<uint32_t>(column_groups), kSums), dim3(kJoinWaves * 64), 0,

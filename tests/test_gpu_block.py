@@ -427,3 +427,20 @@ def test_sums_of_more_rows_than_one_round(kdb, shape):
     rng = np.random.default_rng(shape[0])
     case = random_case(rng, *shape, np.float32, R, L, 1, 0.9)
     check_block(kdb, case, *(rng.normal(size=shape).astype(np.float32) for _ in range(2)))
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("cols", [769, 1001, 1281, 1285, 1793, 2305, 2561, 4097, 5121, 6145, 7169, 8193, 12289, 16384, 640, 1280, 2560, 5120, 12292])
+def test_teams_of_any_number_of_waves(kdb, cols, dtype):
+    """Rows that need one wave more, and whole quads; many rows and few, which divide otherwise."""
+    rng = np.random.default_rng(cols)
+    for rows, (after, before, gate, keep) in ((3, (L, R, 1, 0.9)), (300, (R, L, 1, 0.8)), (290, (None, L, 0, 0.7))):
+        case = random_case(rng, rows, cols, dtype, after, before, gate, keep)
+        check_block(kdb, case, *(rng.normal(size=(rows, cols)).astype(dtype) for _ in range(2)))
+
+
+@pytest.mark.parametrize("shape", [(12400, 640), (16400, 1281), (8300, 1797), (8200, 2304), (4100, 2572)], ids=lambda s: "x".join(map(str, s)))
+def test_rows_one_after_another_in_teams_of_any_number_of_waves(kdb, shape):
+    rng = np.random.default_rng(shape[1])
+    for after, before, gate in ((L, L, 1), (R, R, 1), (L, R, 2)):
+        check_block(kdb, random_case(rng, *shape, np.float32, after, before, gate, 0.9), forward_only=True)
