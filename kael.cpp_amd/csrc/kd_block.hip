@@ -756,7 +756,33 @@ template <typename T> __device__ __forceinline__ void add_quad(T* place, const Q
     __builtin_memcpy(p, &own, sizeof own);
 }
 
+// A quad of a row of any length without a branch: one behind the row's end, or over it, is loaded from the last four values, and `settled`
+// moves them to their places once they are there. What is in the other places nothing counts or stores.
+template <typename T> __device__ __forceinline__ Quad<T> raw_quad(const T* row, int c, int cols) {
+    Quad<T> q;
+    if (cols >= 4) {
+        __builtin_memcpy(&q, place_in(row, min(c, cols - 4)), sizeof q);
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) q.v[e] = row[min(c + e, cols - 1)];
+    }
+    return q;
+}
+template <typename T> __device__ __forceinline__ void settled(Quad<T>& q, int c, int cols) {
+    const int by = cols < 4 ? 0 : c - min(c, cols - 4);
+    const bool one = by & 1, two = by & 2;
+    const T v0 = one ? q.v[1] : q.v[0], v1 = one ? q.v[2] : q.v[1], v2 = one ? q.v[3] : q.v[2];
+    q = {two ? v2 : v0, two ? q.v[3] : v1, v2, q.v[3]};
+}
+
+// kLate: f64 rows that are not of whole quads, whose quads are two loads each (6610 x 454 57 us with branches, 47 without; in f32 the
+// moves cost more than the branches, 7000 x 4095 174 and 192).
 template <typename T, int Quads, bool Whole> struct BackRow {
+    static constexpr bool kLate = !Whole && sizeof(T) == 8;
+    __device__ __forceinline__ static Quad<T> take(const T* row, int c, int cols) {
+        if constexpr (kLate) return raw_quad(row, c, cols);
+        else return take_quad<Whole>(row, c, cols);
+    }
     Quad<T> x[Quads], h[Quads], grad_h[Quads], grad_y[Quads];
     RowStats after, before;
     __device__ __forceinline__ void load(const BackArgs<T>& a, const Team<Quads>& at, int64_t row, bool x_read) {
@@ -765,17 +791,28 @@ template <typename T, int Quads, bool Whole> struct BackRow {
 #pragma unroll
         for (int i = 0; i < Quads; ++i) {
             const int c = at.column(i);
-            if (x_read) x[i] = take_quad<Whole>(a.b.x + base, c, cols);
+            if (x_read) x[i] = take(a.b.x + base, c, cols);
             if (a.grad_y != nullptr) {
-                h[i] = take_quad<Whole>(a.h + base, c, cols);
-                grad_y[i] = take_quad<Whole>(a.grad_y + base, c, cols);
+                h[i] = take(a.h + base, c, cols);
+                grad_y[i] = take(a.grad_y + base, c, cols);
             }
-            grad_h[i] = quad_or<Whole>(a.grad_h != nullptr ? a.grad_h + base : nullptr, c, cols, T(0));
+            if (a.grad_h != nullptr) grad_h[i] = take(a.grad_h + base, c, cols);
+            else grad_h[i] = {};
         }
         // the same for a wave's lanes and constant in this kernel: scalar loads to scalar registers
         const auto* s = (const __attribute__((address_space(4))) double*)(a.stats + 4 * row);
         after = {s[0], s[1]};
         before = {s[2], s[3]};
+    }
+    __device__ __forceinline__ void settle(const Team<Quads>& at, int cols) {
+        if constexpr (kLate)
+#pragma unroll
+            for (int i = 0; i < Quads; ++i) {
+                settled(x[i], at.column(i), cols);
+                settled(h[i], at.column(i), cols);
+                settled(grad_h[i], at.column(i), cols);
+                settled(grad_y[i], at.column(i), cols);
+            }
     }
     __device__ __forceinline__ void converted_late() {
 #pragma unroll
@@ -843,6 +880,7 @@ __global__ __launch_bounds__(kBackThreads<T>) void block_back_kernel(T* parts, B
         uint32_t bits = 0;
         if (here) {
             bits = kept_bits(a.b, at, row, step);
+            now.settle(at, cols);
             if (a.grad_y != nullptr) {
 #pragma unroll
                 for (int i = 0; i < Quads; ++i) {
@@ -1149,13 +1187,13 @@ extern "C" int kd_block_rows(int dtype, void* h, void* y, double* stats, const k
             else one(block_rows_kernel<T, kMost, kQuads, true, kHeld, false>, threads, groups);
         };
         // Workgroups a CU that hold the weights: as many as fit its registers, `waves` a CU. They hold them where the weights are more bytes than x and
-        // residual, and where each has some rows; us, weights read / held, both norms and a gate: 32768 x 768 115 / 97, 16384 x 2048
+        // residual, and where each has two rows or more, in f64 (2000 x 2263 46 / 53) eight; us, weights read / held, both norms and a gate: 32768 x 768 115 / 97, 16384 x 2048
         // 128 / 104, 8192 x 4096 124 / 106; a layer norm ahead of the next block alone: 91 / 96, 102 / 113, 103 / 109.
         const auto choose = [&](auto most, auto quads, int waves) {
             const int weights = 2 * (b.after.kind != KD_NORM_NONE) + 2 * (b.before.kind != KD_NORM_NONE) + (b.gate_rows == 1);
             const int threads = team_threads(b.cols, decltype(quads)::value);
             const int64_t groups = int64_t{waves * 64 / threads} * compute_units();
-            if (weights > 2 && b.rows >= 8 * groups) rows(most, quads, std::true_type{}, threads, groups);
+            if (weights > 2 && b.rows >= (sizeof(T) == 4 ? 2 : 8) * groups) rows(most, quads, std::true_type{}, threads, groups);
             else rows(most, quads, std::false_type{}, threads, b.rows);
         };
         // Quads a thread: so few registers that a CU has two workgroups of rows at least, but few enough threads that the barriers wait for few; one row a CU,
