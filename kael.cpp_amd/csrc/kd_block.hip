@@ -66,8 +66,8 @@ __global__ __launch_bounds__(kThreads) void counter_dropout_kernel(T* out, const
 // Bound by the bytes: x and residual read once, h and y written once, from registers in between. A row's arithmetic is f64,
 // whose operations cost what f32's do here (packed ones aside); a thread's dropout words are made while its loads are on their
 // way. Rows of up to 512 belong to a wave, which needs no barrier, longer ones to a workgroup with one barrier a norm.
-// f32, a layer norm with dropout: 4096 x 256 7.2 us, 32768 x 1024 102 us (5.2 TB/s), 8192 x 4096 105 us (5.1 TB/s); RMS norms on both sides
-// with a gate: 8192 x 4096 100 to 120 us, vector ALU busy 0.59 of the cycles; one row of 768 2.9 us, 16 rows 3.6 us.
+// f32, a layer norm with dropout: 4096 x 256 7.2 us, 32768 x 768 79 us, 32768 x 1024 102 us (5.2 TB/s), 8192 x 4096 105 us (5.1 TB/s); RMS norms on
+// both sides with a gate: 8192 x 4096 100 to 120 us, vector ALU busy 0.59 of the cycles; one row of 768 2.9 us, 16 rows 3.6 us.
 
 template <typename T> struct NormArgs {
     const T* weight;
@@ -446,7 +446,7 @@ __global__ __launch_bounds__(kWideThreads) void block_rows_wide_kernel(T* h, T* 
 //
 // Bound by the bytes: x, h, grad_h and grad_y read once, two gradients written once, where a team's registers hold a row and LDS its
 // sums: rows of up to 4096. The parts' sums are 5 % more where each team has many rows, and a second kernel adds them in order, so that no
-// result depends on what runs first. f32: 8192 x 4096, both norms and a gate, 170 to 205 + 6 us (805 MB at 3.9 to 4.7 TB/s, vector ALU busy
+// result depends on what runs first. f32: 8192 x 4096, both norms and a gate, 170 to 217 + 6 us (805 MB at 3.7 to 4.7 TB/s, vector ALU busy
 // 0.70); a layer norm alone 148 + 5; 32768 x 1024 160 + 5; 4096 x 256 10.5 + 3.8, where it is a chain of launch, loads and two
 // exchanges. 4096 x 8192 with all sums: the row's kernel 214, the sums' 102 us.
 
@@ -831,7 +831,7 @@ __global__ __launch_bounds__(kBackThreads<T>) void block_back_kernel(T* parts, B
     extern __shared__ __attribute__((aligned(16))) char shared[];
     __shared__ Pair room[2][2][kMostWaves];  // by turns: a row's waves may be ahead of the last ones of the row before
     const Team<Quads> at(Threads != 0 ? Threads : threads);
-    const int teams = static_cast<int>(blockDim.x) / threads;
+    const int group = Threads != 0 ? kBackThreads<T> : static_cast<int>(blockDim.x), teams = group / at.threads;
     const int64_t first = (static_cast<int64_t>(blockIdx.x) * teams + at.team) * rows_per_team, end = min(a.b.rows, first + rows_per_team);
     const int cols = static_cast<int>(a.b.cols);
     const double share = 1.0 / cols;
@@ -989,7 +989,7 @@ __global__ __launch_bounds__(kBackThreads<T>) void block_back_kernel(T* parts, B
         if (places.at[k] < 0) continue;
         T* out = parts + (static_cast<int64_t>(blockIdx.x) * kSums + k) * cols;
         const T* own = reinterpret_cast<const T*>(shared) + places.at[k] * padded;
-        for (int c = threadIdx.x; c < cols; c += blockDim.x) {
+        for (int c = threadIdx.x; c < cols; c += group) {
             double total = static_cast<double>(own[c]);
             for (int t = 1; t < teams; ++t) total += static_cast<double>(own[t * places.wanted * padded + c]);
             out[c] = static_cast<T>(total);
@@ -1187,8 +1187,9 @@ extern "C" int kd_block_rows(int dtype, void* h, void* y, double* stats, const k
             else one(block_rows_kernel<T, kMost, kQuads, true, kHeld, false>, threads, groups);
         };
         // Workgroups a CU that hold the weights: as many as fit its registers, `waves` a CU. They hold them where the weights are more bytes than x and
-        // residual, and where each has two rows or more, in f64 (2000 x 2263 46 / 53) eight; us, weights read / held, both norms and a gate: 32768 x 768 115 / 97, 16384 x 2048
-        // 128 / 104, 8192 x 4096 124 / 106; a layer norm ahead of the next block alone: 91 / 96, 102 / 113, 103 / 109.
+        // residual, and where each has two rows or more, in f64 (2000 x 2263 46 / 53) eight; us, weights read / held, both
+        // norms and a gate: 32768 x 768 95 / 83, 16384 x 2048 122 / 105, 16384 x 2560 187 / 138, 8192 x 4096 121 / 106; a layer norm ahead of
+        // the next block alone: 78 / 84, 104 / 108, 143 / 135, 104 / 111.
         const auto choose = [&](auto most, auto quads, int waves) {
             const int weights = 2 * (b.after.kind != KD_NORM_NONE) + 2 * (b.before.kind != KD_NORM_NONE) + (b.gate_rows == 1);
             const int threads = team_threads(b.cols, decltype(quads)::value);
