@@ -356,16 +356,17 @@ __global__ __launch_bounds__(Threads) void answer_rows_kernel(AnswerRows<T> a) {
     });
 }
 
-// Without a gradient no row is held: a workgroup reads a long one in rounds of four pieces a thread, and several share a
-// CU. All exponentials are taken from one base, the largest logit of the first round, so that no sum is moved from one maximum to
-// another (each move is a rounding that all of a sum's terms share); only a row whose largest logit is far above that base, or
-// that begins with nothing but -inf, is read once more. 1433 rows of 50257 of 1908: 57 to 64 us (288 MB at 4.5 to 5.1 TB/s); held in
-// registers, one workgroup a CU, 69.
+// Without a gradient no row is held: a workgroup reads a long one in rounds of four pieces a thread, and a CU's eight waves a SIMD
+// have the next loads on their way while one computes. A wave takes its exponentials from the largest logit that it has seen: an f32
+// exponential's error grows with the distance from its base, so a confident target has to be that base, whose exponential is
+// exactly 1 (with the largest logit of a row's first round as the base of all, targets 12 to 39 above it were 4e-7 to 2e-6 off and above 0).
+// A round that holds a larger one moves the sum there first, in f64, whose rounding does not count beside f32's; that is seldom: a
+// wave's k-th round does so with a chance of 1 / k. 1433 rows of 50257 of 1908: 59 to 62 us (288 MB at 4.6 to 4.9 TB/s); held in
+// registers, one workgroup a CU, 69. f64: 500 x 50257 41 us (4.9 TB/s).
 template <typename T>
 __global__ __launch_bounds__(kMostThreads) void answer_forward_kernel(AnswerRows<T> a) {
     constexpr int kCount = Piece<T>::kCount, kPieces = 4;
-    constexpr double kFar = 40;  // e^40 is well inside f32's range
-    __shared__ T room_most[2][16];
+    __shared__ T room_most[16];
     __shared__ double room_sum[16];
     const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) / 64), lane = threadIdx.x % 64;
     const int waves = blockDim.x / 64;
@@ -377,59 +378,42 @@ __global__ __launch_bounds__(kMostThreads) void answer_forward_kernel(AnswerRows
     const T* z = a.logits + row * a.cols;
     const T there = z[target], lowest = static_cast<T>(-INFINITY);
     const int64_t own = static_cast<int64_t>(threadIdx.x) * kCount, step = static_cast<int64_t>(blockDim.x) * kCount;
-    const auto load = [&](Piece<T>(&p)[kPieces], int64_t at) {
+    T base = lowest;
+    double sum = 0;
+    // the same rounds for all lanes: what is behind the row's end is -inf
+    for (int64_t from = 0; from < a.cols; from += kPieces * step) {
+        Piece<T> p[kPieces];
 #pragma unroll
-        for (int i = 0; i < kPieces; ++i) p[i] = load_piece(z, at + i * step, a.cols, lowest);
-    };
-    const auto most_of = [&](const Piece<T>(&p)[kPieces], T most) {
+        for (int i = 0; i < kPieces; ++i) p[i] = load_piece(z, from + own + i * step, a.cols, lowest);
+        T most = base;
 #pragma unroll
         for (int i = 0; i < kPieces; ++i)
 #pragma unroll
             for (int j = 0; j < kCount; ++j) most = fmax(most, p[i].x[j]);  // passes over NaN, which the sum takes up
-        return most;
-    };
-    const auto over_group = [&](T v, T* room) {
-        v = wave_most(v);
-        if (lane == 0) room[wave] = v;
-        __syncthreads();
-        return from_lane(most_of_16(room[lane % 16 < waves ? lane % 16 : 0]), 15);
-    };
-    Piece<T> p[kPieces], next[kPieces];
-    load(p, own);
-    const T first = over_group(most_of(p, lowest), room_most[0]);
-    T base = or_zero(first), most = lowest;
-    double sum = 0;
-    const auto add = [&](const Piece<T>(&q)[kPieces]) {
+        if (__any(most > base)) {
+            most = wave_most(most);
+            if (base != lowest) sum *= exp((static_cast<double>(base) - static_cast<double>(most)) * a.inverse);
+            base = most;
+        }
+        const T from_base = or_zero(base);
 #pragma unroll
         for (int i = 0; i < kPieces; ++i)
 #pragma unroll
-            for (int j = 0; j < kCount; ++j) sum += static_cast<double>(a.t.exp(q[i].x[j] - base));
-    };
-    for (int64_t at = own; at < a.cols; at += kPieces * step) {
-        const bool more = at + kPieces * step < a.cols;
-        if (more) load(next, at + kPieces * step);
-        most = most_of(p, most);
-        add(p);
-        if (more)
-#pragma unroll
-            for (int i = 0; i < kPieces; ++i) p[i] = next[i];
-    }
-    most = over_group(most, room_most[1]);
-    const bool far = first == lowest || !((static_cast<double>(most) - static_cast<double>(base)) * a.inverse <= kFar);
-    if (far && most != lowest) {
-        base = most;
-        sum = 0;
-        for (int64_t at = own; at < a.cols; at += kPieces * step) {
-            load(p, at);
-            add(p);
-        }
+            for (int j = 0; j < kCount; ++j) sum += static_cast<double>(a.t.exp(p[i].x[j] - from_base));
     }
     sum = wave_total(sum);
-    if (lane == 0) room_sum[wave] = sum;
+    if (lane == 0) {
+        room_most[wave] = base;
+        room_sum[wave] = sum;
+    }
     __syncthreads();
     if (wave != 0) return;
-    sum = from_lane(sum_of_16(lane % 16 < waves ? room_sum[lane % 16] : 0.0), 15);
-    if (base != most && most != lowest) sum *= exp((static_cast<double>(base) - static_cast<double>(most)) * a.inverse);
+    const int w = lane % 16 < waves ? lane % 16 : 0;
+    base = room_most[w];
+    const T most = from_lane(most_of_16(base), 15);
+    sum = lane % 16 < waves ? room_sum[w] : 0.0;
+    if (base != most) sum *= exp((static_cast<double>(base) - static_cast<double>(most)) * a.inverse);
+    sum = from_lane(sum_of_16(sum), 15);
     finish_row(a, row, there, most, sum, lane == 0);
 }
 
