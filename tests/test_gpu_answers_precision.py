@@ -5,7 +5,7 @@ import pytest
 
 import answers
 import kd
-from test_gpu_answers import run_policy, same, token_logps
+from test_gpu_answers import grad_tolerance, run_policy, same, token_logps
 
 pytestmark = pytest.mark.gpu
 
@@ -91,3 +91,48 @@ def test_no_lean_over_many_rows(kdb, shape):
         for lp in (token_logps(kdb, z, targets, temperature)[0].numpy(),
                    run_policy(kdb, z, targets, None, None, weights, weights, temperature, 0.2, 0.2, 0.0)[1]):
             assert abs((lp - want).mean()) <= bound, ((lp - want).mean(), bound)
+
+
+def held(kdb, z, targets, temperature, kl, advantages, moved, away):
+    """A policy whose old and reference log-probabilities stand `moved` below and `away` above the ones that the call gives."""
+    rows = len(z)
+    weights = np.ones(rows, z.dtype)
+    _, lp, _ = run_policy(kdb, z, targets, None, None, advantages, weights, temperature, 0.2, 0.3, 0.0)
+    old, reference = lp - moved, lp + away
+    losses, again, grad = run_policy(kdb, z, targets, old, reference, advantages, weights, temperature, 0.2, 0.3, kl)
+    np.testing.assert_array_equal(again, lp)
+    return losses, grad, lp - old, reference - lp
+
+
+@pytest.mark.parametrize("shape", [(90, 40), (30, 700), (15, 3001), (15, 9000)], ids=lambda s: "x".join(map(str, s)))
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+def test_a_model_that_is_still_close_to_its_reference(kdb, dtype, shape):
+    """exp(d) - d - 1 is d^2 / 2 and its derivative d for small d. expm1 is good to one step; the difference, the weight and
+    the result are half a step each."""
+    rng = np.random.default_rng(shape[1])
+    rows, cols = shape
+    z = (2 * rng.normal(size=shape)).astype(dtype)
+    targets = rng.integers(0, cols, rows)
+    away = np.resize([1e-8, -1e-8, 3e-7, -1e-6, 1e-4, -1e-2, 0.3, -2, 20, -40, 0, 7e-9, -1.1e-8, 1e-7, 3e-3], rows)
+    losses, grad, _, d = held(kdb, z, targets, 0.8, 0.3, np.zeros(rows, dtype), 0.0, away)
+    e = np.expm1(d.astype(np.longdouble))
+    want = 0.3 * (e - d)
+    off = 0.3 * 2.0 ** -52 * np.abs(e) + (2.0 ** -52 + np.finfo(dtype).eps / 2) * np.abs(want) + np.finfo(dtype).tiny
+    same(losses, want.astype(np.float64), off.astype(np.float64))
+    slopes = (-0.3 * e).astype(np.float64)
+    same(grad, answers.token_logps_grad(z, targets, slopes, 0.8), grad_tolerance(z, targets, slopes, 0.8))
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+def test_ratios_near_and_far_from_one_beside_a_reference(kdb, dtype):
+    """A ratio is good to two steps (an exponential's one and two halves) however small or large it is; f32's one rounding more."""
+    rng = np.random.default_rng(1)
+    moved = np.array([-600, -80, -40, -3, -0.5, -1e-9, 0, 1e-9, 0.1, 0.5, 3, 40, 80])
+    rows = len(moved)
+    z = (2 * rng.normal(size=(rows, 50))).astype(dtype)
+    targets = rng.integers(0, 50, rows)
+    advantages = np.where(moved <= 0, 1, -1).astype(dtype)  # where no clip holds the ratio
+    losses, _, moved, _ = held(kdb, z, targets, 1.0, 0.1, advantages, moved, 0.0)
+    want = -np.exp(moved.astype(np.longdouble)) * advantages
+    off = (2.0 ** -51 + np.finfo(dtype).eps / 2) * np.abs(want) + np.finfo(dtype).tiny * (dtype is np.float32)
+    same(losses, want.astype(np.float64), off.astype(np.float64))
