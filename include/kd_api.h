@@ -610,8 +610,8 @@ typedef struct kd_block {
 } kd_block;
 
 /* Writes h, y and stats, each of which may be NULL where it is not wanted: h [rows][cols]; y [rows][cols], NULL if
- * before.kind is KD_NORM_NONE; stats [rows][4] f64, which the backward pass reads: mean and 1 / sqrt(mean square + eps) of
- * `after`, then of `before` (0 and 1 for KD_NORM_NONE). y is the norm of h as it is stored (rounded to dtype). A row is
+ * before.kind is KD_NORM_NONE; stats [rows][4] f64 (aligned to 8 bytes), which the backward pass reads: mean and
+ * 1 / sqrt(mean square + eps) of `after`, then of `before` (0 and 1 for KD_NORM_NONE). y is the norm of h as it is stored (rounded to dtype). A row is
  * computed in 64 bits and rounded once. h may be x or residual, y may be x or residual; no output overlaps an input or another
  * output otherwise. f32 or f64. */
 int kd_block_rows(int dtype, void* h, void* y, double* stats, const kd_block* block);
@@ -650,7 +650,9 @@ int kd_block_rows_workspace(int64_t* bytes, int dtype, int64_t rows, int64_t col
  * kd_token_logps_grad reads. A target outside 0 .. cols - 1 is none (a prompt's token, padding): its row of logits is not
  * read, logps is 0 and stats are 0 and 1. logps are f64, since sums over long answers cancel against the reference's;
  * the exponentials are dtype's, their sum f64. A logit of -inf has no part; a row of nothing else, of NaN or of +inf is NaN.
- * dtype f32 or f64, rows contiguous; 1e-6 <= temperature <= 1e6, rows at most 2^22 - 4, cols below 2^31. */
+ * dtype f32 or f64, rows contiguous; 1e-6 <= temperature <= 1e6, rows at most 2^22 - 4, cols below 2^31. In this call and the
+ * three below no output overlaps an input or another output, but for the places that they name, and every operand is
+ * aligned to its elements. */
 int kd_token_logps(int dtype, double* logps, void* stats, const void* logits, const int64_t* targets, int64_t rows,
                    int64_t cols, double temperature);
 
@@ -669,7 +671,8 @@ int kd_token_logps_grad(int dtype, void* out, const void* logits, const void* st
  *   slopes[r] = weights[p] * the derivative of losses[p] with respect to logps[r], for kd_token_logps_grad; 0 for
  *   rows without a target and for rows outside every sequence
  * losses [pairs], rewards [pairs][2], slopes [rows] and weights [pairs] are dtype's, sums f64. 0 <= smoothing < 0.5,
- * 0 < beta <= 1e6, pairs below 2^22. rewards may be NULL. No pairs: slopes are 0. */
+ * 0 < beta <= 1e6, pairs below 2^22. rewards may be NULL; f64 slopes may be logps or reference. No pairs: slopes are 0, and
+ * nothing else is read or written. */
 int kd_preference_pairs(int dtype, void* losses, void* rewards, void* slopes, const double* logps,
                         const double* reference, const int64_t* targets, const int64_t* starts, const void* weights,
                         int64_t pairs, int64_t rows, int64_t cols, double beta, double smoothing);
@@ -682,8 +685,8 @@ int kd_preference_pairs(int dtype, void* losses, void* rewards, void* slopes, co
  * has neither term nor derivative, whatever w is. A row without a target (as there) has loss, lp and gradient 0.
  * old_logps and reference_logps f64 [rows] (old_logps NULL: lp itself, w = 1, for answers that this very model sampled;
  * reference_logps NULL or kl_weight 0: no second term); advantages and row_weights dtype [rows]. logps (f64 [rows], may be NULL) receives
- * lp. grad may be NULL (then row_weights is not read) and may be logits. clip_low is 0 .. 1, clip_high and kl_weight
- * are 0 .. 1e6; sizes and temperature as in kd_token_logps. */
+ * lp. grad may be NULL (then row_weights is not read) and may be logits; losses may be advantages or row_weights, logps may be
+ * old_logps or reference_logps. clip_low is 0 .. 1, clip_high and kl_weight are 0 .. 1e6; sizes and temperature as in kd_token_logps. */
 typedef struct kd_policy {
     const double* old_logps;
     const double* reference_logps;

@@ -1,6 +1,7 @@
 // kd_answers.hip - training on sampled answers and on pairs of them: the targets' log-probabilities with their gradient, the
 // preference loss of pairs, and the clipped policy loss with its gradient.
 #include <algorithm>
+#include <initializer_list>
 
 #include "kd_counter.h"
 #include "kd_internal.h"
@@ -520,10 +521,27 @@ template <typename T> void launch_rows(const AnswerRows<T>& a) {
     else row(Int<1024>{}, Int<14>{}, std::true_type{});
 }
 
-// Whether `out` is neither apart from the logits nor the logits themselves.
-bool crosses(const void* out, const void* logits, int dtype, int64_t rows, int64_t cols) {
-    const int64_t bytes = rows * cols * dtype_size(dtype);
-    return out != logits && overlap(out, bytes, logits, bytes);
+struct Operand {
+    const void* at;
+    int64_t count, size;  // of its elements
+    int same = -1;        // of an input: the output that may stand in its very place, since it reads an element before it writes it
+};
+// Refuses an operand that is not aligned to its elements, and an output that has a byte in common with another operand.
+int check_operands(const std::string& name, std::initializer_list<Operand> outs, std::initializer_list<Operand> ins) {
+    const auto crosses = [](const Operand& a, const Operand& b) { return overlap(a.at, a.count * a.size, b.at, b.count * b.size); };
+    for (const auto* operands : {&outs, &ins})
+        for (const Operand& o : *operands)
+            if (reinterpret_cast<uintptr_t>(o.at) % static_cast<uintptr_t>(o.size) != 0)
+                return fail(KD_E_INVALID, name + ": an operand is not aligned to its elements");
+    int place = 0;
+    for (const Operand& out : outs) {
+        for (const Operand& other : outs)
+            if (&out != &other && crosses(out, other)) return fail(KD_E_INVALID, name + ": outputs overlap");
+        for (const Operand& in : ins)
+            if (!(in.same == place && out.at == in.at) && crosses(out, in)) return fail(KD_E_INVALID, name + ": an output overlaps an input");
+        ++place;
+    }
+    return KD_OK;
 }
 
 } // namespace
@@ -539,6 +557,8 @@ extern "C" int kd_token_logps(int dtype, double* logps, void* stats, const void*
     if (rows == 0) return KD_OK;
     if (logps == nullptr || stats == nullptr || logits == nullptr || targets == nullptr)
         return fail(KD_E_INVALID, name + ": every operand must be given");
+    const int64_t size = dtype_size(dtype);
+    if (int rc = check_operands(name, {{logps, rows, 8}, {stats, 2 * rows, size}}, {{logits, rows * cols, size}, {targets, rows, 8}})) return rc;
     if (int rc = ensure_device()) return rc;
     const auto launch = [&](auto zero) {
         using T = decltype(zero);
@@ -559,7 +579,10 @@ extern "C" int kd_token_logps_grad(int dtype, void* out, const void* logits, con
     if (rows == 0) return KD_OK;
     if (out == nullptr || logits == nullptr || stats == nullptr || targets == nullptr || slopes == nullptr)
         return fail(KD_E_INVALID, name + ": every operand must be given");
-    if (crosses(out, logits, dtype, rows, cols)) return fail(KD_E_INVALID, name + ": out overlaps the logits");
+    const int64_t size = dtype_size(dtype);
+    if (int rc = check_operands(name, {{out, rows * cols, size}},
+                                {{logits, rows * cols, size, 0}, {stats, 2 * rows, size}, {targets, rows, 8}, {slopes, rows, size}}))
+        return rc;
     if (int rc = ensure_device()) return rc;
     const auto launch = [&](auto zero) -> int {
         using T = decltype(zero);
@@ -598,6 +621,11 @@ extern "C" int kd_preference_pairs(int dtype, void* losses, void* rewards, void*
     if ((pairs > 0 && (losses == nullptr || starts == nullptr || weights == nullptr)) ||
         (rows > 0 && (slopes == nullptr || logps == nullptr || targets == nullptr)))
         return fail(KD_E_INVALID, name + ": every operand but rewards and reference must be given");
+    const int64_t size = dtype_size(dtype), read = pairs > 0 ? rows : 0;  // without pairs the slopes alone are written
+    const int same = dtype == KD_F64 ? 2 : -1;
+    if (int rc = check_operands(name, {{losses, pairs, size}, {rewards, 2 * pairs, size}, {slopes, rows, size}},
+                                {{logps, read, 8, same}, {reference, read, 8, same}, {targets, read, 8}, {starts, 2 * pairs + 1, 8}, {weights, pairs, size}}))
+        return rc;
     if (int rc = ensure_device()) return rc;
     const auto launch = [&](auto zero) {
         using T = decltype(zero);
@@ -628,7 +656,12 @@ extern "C" int kd_policy_rows(int dtype, void* losses, double* logps, void* grad
     if (losses == nullptr || logits == nullptr || targets == nullptr || policy->advantages == nullptr ||
         (grad != nullptr && row_weights == nullptr))
         return fail(KD_E_INVALID, name + ": losses, logits, targets, advantages and, for a gradient, row_weights must be given");
-    if (grad != nullptr && crosses(grad, logits, dtype, rows, cols)) return fail(KD_E_INVALID, name + ": grad overlaps the logits");
+    const int64_t size = dtype_size(dtype);
+    if (int rc = check_operands(name, {{losses, rows, size}, {logps, rows, 8}, {grad, rows * cols, size}},
+                                {{logits, rows * cols, size, 2}, {targets, rows, 8}, {policy->old_logps, rows, 8, 1},
+                                 {policy->reference_logps, rows, 8, 1}, {policy->advantages, rows, size, 0},
+                                 {grad != nullptr ? row_weights : nullptr, rows, size, 0}}))
+        return rc;
     if (int rc = ensure_device()) return rc;
     const auto launch = [&](auto zero) {
         using T = decltype(zero);

@@ -1156,6 +1156,7 @@ extern "C" int kd_block_rows(int dtype, void* h, void* y, double* stats, const k
     if (y != nullptr && b.before.kind == KD_NORM_NONE) return fail(KD_E_INVALID, name + ": y needs a norm");
     if (b.rows == 0 || b.cols == 0) return KD_OK;
     if (b.x == nullptr) return fail(KD_E_INVALID, name + ": x must be given");
+    if (reinterpret_cast<uintptr_t>(stats) % 8 != 0) return fail(KD_E_INVALID, name + ": stats must be aligned to 8 bytes");
     const int64_t bytes = b.rows * b.cols * dtype_size(dtype), row_bytes = b.cols * dtype_size(dtype);
     for (void* out : {h, y})
         for (const void* in : {b.x, b.residual})
@@ -1251,7 +1252,8 @@ extern "C" int kd_block_rows_backward(int dtype, const kd_block_grads* grads, co
     if (!summed && (!by_row || b.rows == 0)) return KD_OK;
     int64_t needed = 0;
     if (b.rows > 0) {
-        if (stats == nullptr) return fail(KD_E_INVALID, name + ": stats must be given");
+        if (stats == nullptr || reinterpret_cast<uintptr_t>(stats) % 8 != 0)
+            return fail(KD_E_INVALID, name + ": stats must be given, aligned to 8 bytes");
         if (b.x == nullptr && (b.after.kind != KD_NORM_NONE || grads->gate != nullptr))
             return fail(KD_E_INVALID, name + ": x must be given");
         if (h == nullptr && grad_y != nullptr) return fail(KD_E_INVALID, name + ": h must be given");

@@ -150,3 +150,50 @@ def test_a_workspace_serves_fewer_rows(lib, cols, dtype):
         assert lib.lib.kd_block_rows_workspace(ctypes.byref(n), dtype, rows, cols) == 0
         assert n.value >= last, rows
         last = n.value
+
+
+def crossing(lib, f, good, rows, name):
+    """`rows`: (argument, other argument, offset) triples of which one lies over the other's bytes."""
+    for place, other, by in rows:
+        args = list(good)
+        args[place] = args[other] + by
+        assert f(*args) == INVALID, (place, other, by)
+        assert lib.error().startswith(name), lib.error()
+
+
+def test_outputs_of_the_losses_over_their_operands(lib):
+    """10 rows of 8 in f32: 320 bytes of logits, 80 of stats, targets and log-probabilities, 40 of a number a row."""
+    crossing(lib, lib.lib.kd_token_logps, [kd.F32, at(0), at(1), at(2), at(3), 10, 8, 1.0],
+             ((1, 2, 0), (1, 3, 0), (1, 3, 312), (2, 3, 76), (2, 3, 0), (2, 1, 76), (2, 4, -72), (1, 4, 72), (1, 2, -72)), "kd_token_logps:")
+    crossing(lib, lib.lib.kd_token_logps_grad, [kd.F32, at(0), at(1), at(2), at(3), at(4), 10, 8, 1.0],
+             ((1, 3, 0), (1, 3, 76), (1, 4, 0), (1, 4, -316), (1, 5, 36), (1, 5, 0)), "kd_token_logps_grad:")
+    pairs = [kd.F32, at(0), at(1), at(2), at(3), at(4), at(5), at(6), at(7), 3, 10, 8, 0.1, 0.1]
+    crossing(lib, lib.lib.kd_preference_pairs, pairs, [(1, 2, 0), (1, 3, 36), (2, 3, -20), (3, 2, 20)] + [
+        (i, j, 0) for i in (1, 2, 3) for j in range(4, 9)], "kd_preference_pairs:")
+    pairs[0] = kd.F64
+    crossing(lib, lib.lib.kd_preference_pairs, pairs, ((3, 4, 8), (3, 5, -8), (3, 6, 0), (1, 4, 0)), "kd_preference_pairs:")
+
+    def policy(lib, losses, logps, grad, logits, targets, old, reference, advantages, weights):
+        return lib.lib.kd_policy_rows(kd.F32, losses, logps, grad, logits, targets, kd.Policy(old, reference, advantages, 1.0, 0.2, 0.2, 0.1),
+                                      weights, 10, 8)
+
+    good = [lib] + [at(i) for i in range(9)]
+    crossing(lib, policy, good, ((1, 2, 0), (1, 2, 76), (2, 1, -76 + 4), (1, 3, 316), (3, 1, 36), (3, 2, 0), (1, 4, 0), (2, 4, 312), (3, 4, 4),
+                                 (3, 5, 0), (1, 5, 0), (2, 5, 0), (3, 6, 0), (3, 7, 0), (3, 8, 0), (3, 9, 0), (2, 6, 8), (2, 7, -8), (2, 8, 0),
+                                 (2, 9, 0), (1, 8, 4), (1, 9, -4), (1, 6, 0), (1, 7, 0)), "kd_policy_rows:")
+
+
+def test_misaligned_operands_of_the_losses(lib):
+    for f, good, places, name in (
+            (lib.lib.kd_token_logps, [kd.F64, at(0), at(1), at(2), at(3), 10, 8, 1.0], (1, 2, 3, 4), "kd_token_logps:"),
+            (lib.lib.kd_token_logps_grad, [kd.F64, at(0), at(1), at(2), at(3), at(4), 10, 8, 1.0], (1, 2, 3, 4, 5), "kd_token_logps_grad:"),
+            (lib.lib.kd_preference_pairs, [kd.F64] + [at(i) for i in range(8)] + [3, 10, 8, 0.1, 0.1], range(1, 9), "kd_preference_pairs:")):
+        refused(lib, f, good, [(i, good[i] + 4, INVALID) for i in places], name)
+    assert lib.lib.kd_token_logps(kd.F32, at(0), at(1) + 2, at(2), at(3), 10, 8, 1.0) == INVALID
+
+
+def test_misaligned_statistics_of_a_block(lib):
+    assert lib.lib.kd_block_rows(kd.F32, at(8), at(9), at(10) + 4, block()) == INVALID
+    assert lib.error().startswith("kd_block_rows:")
+    assert backward(lib, block(), stats=at(9) + 4) == INVALID
+    assert lib.error().startswith("kd_block_rows_backward:")
