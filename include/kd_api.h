@@ -558,7 +558,8 @@ int kd_layer_norm_rows_backward(int dtype, void* grad_in, void* grad_weight, voi
  * element is kept where its word is below keep * 2^32, rounded to the nearest whole number. So the mask needs no memory: the
  * same counter gives it again in the backward pass, and in parts of the tensor's rows, in any order. A program gives each
  * of a step's dropouts a stream of its own. more_steps (device, may be NULL for 0) is read when the kernels run, so a
- * captured step draws a new mask at every replay whose program counts it up, ahead of the step or behind it. */
+ * captured step draws a new mask at every replay whose program counts it up, ahead of the step or behind it; no output of the
+ * calls that read it overlaps it. */
 typedef struct kd_counter {
     uint64_t seed;
     uint32_t stream;

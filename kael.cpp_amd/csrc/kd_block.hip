@@ -1134,6 +1134,7 @@ extern "C" int kd_counter_dropout(int dtype, void* out, const void* in, int64_t 
     if (out == nullptr || in == nullptr) return fail(KD_E_INVALID, name + ": in and out must be given");
     const int64_t bytes = rows * cols * dtype_size(dtype);
     if (out != in && overlap(out, bytes, in, bytes)) return fail(KD_E_INVALID, name + ": out overlaps in");
+    if (overlap(out, bytes, mask.more_steps, 8)) return fail(KD_E_INVALID, name + ": out overlaps more_steps");
     if (int rc = ensure_device()) return rc;
     const int64_t quads = (cols + 3) / 4;
     const uint32_t groups = static_cast<uint32_t>(
@@ -1163,6 +1164,7 @@ extern "C" int kd_block_rows(int dtype, void* h, void* y, double* stats, const k
             if (out != in && overlap(out, bytes, in, bytes)) return fail(KD_E_INVALID, name + ": an output overlaps an input");
     for (void* out : {h, y, static_cast<void*>(stats)}) {
         const int64_t size = out == stats ? b.rows * 32 : bytes;
+        if (overlap(out, size, mask.more_steps, 8)) return fail(KD_E_INVALID, name + ": an output overlaps more_steps");
         if (overlap(out, size, b.gate, b.gate_rows * row_bytes)) return fail(KD_E_INVALID, name + ": an output overlaps the gate");
         for (const kd_norm* n : {&b.after, &b.before})
             for (const void* in : {n->weight, n->bias})
@@ -1272,7 +1274,7 @@ extern "C" int kd_block_rows_backward(int dtype, const kd_block_grads* grads, co
                               {grad_y != nullptr ? h : nullptr, bytes}, {b.gate, b.gate_rows * row_bytes}, {stats, b.rows * 32},
                               {b.after.kind != KD_NORM_NONE ? b.after.weight : nullptr, row_bytes},
                               {b.after.kind != KD_NORM_NONE && grads->gate != nullptr ? b.after.bias : nullptr, row_bytes},
-                              {b.before.kind != KD_NORM_NONE ? b.before.weight : nullptr, row_bytes}};
+                              {b.before.kind != KD_NORM_NONE ? b.before.weight : nullptr, row_bytes}, {mask.more_steps, 8}};
         for (int i = 0; i < static_cast<int>(std::size(outs)); ++i) {
             for (int j = 0; j < i; ++j)
                 if (overlap(outs[i].at, outs[i].bytes, outs[j].at, outs[j].bytes)) return fail(KD_E_INVALID, name + ": outputs overlap");

@@ -197,3 +197,19 @@ def test_misaligned_statistics_of_a_block(lib):
     assert lib.error().startswith("kd_block_rows:")
     assert backward(lib, block(), stats=at(9) + 4) == INVALID
     assert lib.error().startswith("kd_block_rows_backward:")
+
+
+def test_outputs_over_a_masks_step(lib):
+    """The step is read by every workgroup, while others write."""
+    counter = kd.Counter(1, 2, 3, 0, at(20))
+    for by in (-4, 0, 4):
+        assert lib.lib.kd_counter_dropout(kd.F32, at(20) + by, at(1), 10, 8, 0.5, counter) == INVALID
+        assert lib.error().startswith("kd_counter_dropout:")
+        masked = block(counter=counter)
+        for args in ((at(20) + by, at(9), at(10)), (at(8), at(20) - 316, at(10)), (at(8), at(9), at(20) - 312)):
+            assert lib.lib.kd_block_rows(kd.F32, *args, masked) == INVALID
+            assert lib.error().startswith("kd_block_rows:")
+        for grads in (kd.BlockGrads(x=at(20) + by), kd.BlockGrads(residual=at(20) - 316), kd.BlockGrads(before_bias=at(20) + by)):
+            assert backward(lib, masked, grads) == INVALID
+            assert lib.error().startswith("kd_block_rows_backward:")
+        assert backward(lib, masked, room=at(20) - 16) == INVALID
