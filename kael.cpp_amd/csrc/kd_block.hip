@@ -1185,9 +1185,14 @@ extern "C" int kd_block_rows(int dtype, void* h, void* y, double* stats, const k
         const auto rows = [&](auto most, auto quads, auto held, int threads, int64_t groups) {
             constexpr int kMost = decltype(most)::value, kQuads = decltype(quads)::value;
             constexpr bool kHeld = decltype(held)::value;
-            if (b.cols % 4 != 0) one(block_rows_kernel<T, kMost, kQuads, false, kHeld, kMost == 64>, threads, groups);
-            else if (kMost == 64 || threads == kMost) one(block_rows_kernel<T, kMost, kQuads, true, kHeld, true>, threads, groups);
-            else one(block_rows_kernel<T, kMost, kQuads, true, kHeld, false>, threads, groups);
+            if (b.cols % 4 != 0) {
+                one(block_rows_kernel<T, kMost, kQuads, false, kHeld, kMost == 64>, threads, groups);
+            } else if constexpr (kMost == 64) {
+                one(block_rows_kernel<T, kMost, kQuads, true, kHeld, true>, threads, groups);
+            } else {
+                if (threads == kMost) one(block_rows_kernel<T, kMost, kQuads, true, kHeld, true>, threads, groups);
+                else one(block_rows_kernel<T, kMost, kQuads, true, kHeld, false>, threads, groups);
+            }
         };
         // Workgroups a CU that hold the weights: as many as fit its registers, `waves` a CU. They hold them where the weights are more bytes than x and
         // residual, and where each has two rows or more, in f64 (2000 x 2263 46 / 53) eight; us, weights read / held, both
@@ -1210,8 +1215,15 @@ extern "C" int kd_block_rows(int dtype, void* h, void* y, double* stats, const k
         else if (b.cols <= 256) rows(Int<64>{}, Int<1>{}, std::false_type{}, 256, (b.rows + 3) / 4);
         else if (b.cols <= 512) rows(Int<64>{}, Int<2>{}, std::false_type{}, 256, (b.rows + 3) / 4);
         else if (b.cols <= 1024) choose(Int<256>{}, Int<1>{}, 20);
-        else if (sizeof(T) == 4 && b.cols > 2048 && b.cols <= 12 * 256) choose(Int<256>{}, Int<3>{}, 8);
-        else if (b.cols <= 4096) choose(Int<512>{}, Int<2>{}, sizeof(T) == 4 ? 12 : 8);
+        else if (b.cols <= 2048) choose(Int<512>{}, Int<2>{}, sizeof(T) == 4 ? 12 : 8);
+        else if (b.cols <= 4096) {
+            if constexpr (sizeof(T) == 4) {
+                if (b.cols <= 12 * 256) choose(Int<256>{}, Int<3>{}, 8);
+                else choose(Int<512>{}, Int<2>{}, 12);
+            } else {
+                choose(Int<512>{}, Int<2>{}, 8);
+            }
+        }
         else if (b.cols <= 6144 || (b.cols <= 8192 && b.rows <= compute_units()))
             rows(Int<1024>{}, Int<2>{}, std::false_type{}, team_threads(b.cols, 2), b.rows);
         else if (b.cols <= 8192) rows(Int<512>{}, Int<4>{}, std::false_type{}, team_threads(b.cols, 4), b.rows);
