@@ -3,7 +3,6 @@
 #include <algorithm>
 #include <initializer_list>
 
-#include "kd_counter.h"
 #include "kd_internal.h"
 #include "kd_logits.h"
 #include "kd_waves.h"

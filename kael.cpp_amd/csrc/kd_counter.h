@@ -56,11 +56,4 @@ inline int mask_of(Mask& mask, const char* what, const kd_counter* counter, doub
     return KD_OK;
 }
 
-// Whether two pieces of memory have a byte in common.
-inline bool overlap(const void* a, int64_t a_bytes, const void* b, int64_t b_bytes) {
-    const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
-    return a != nullptr && b != nullptr && a_bytes > 0 && b_bytes > 0 && x < y + static_cast<uint64_t>(b_bytes) &&
-           y < x + static_cast<uint64_t>(a_bytes);
-}
-
 } // namespace kd

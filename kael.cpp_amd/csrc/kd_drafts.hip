@@ -10,6 +10,12 @@ namespace kd {
 
 namespace {
 
+__device__ __forceinline__ double wave_sum(double v) {
+#pragma unroll
+    for (int m = 32; m > 0; m /= 2) v += __shfl_xor(v, m);
+    return v;
+}
+
 // ---- verification ---------------------------------------------------------------------------------
 //
 // One workgroup a sequence: it finds the first draft that is not accepted, reads that one row (the target's and the draft's)
@@ -310,6 +316,26 @@ __global__ __launch_bounds__(kVerifyWaves * kVerifyWaves) void verify_entry_kern
 // index, its logit and the f64 exponentials and logarithms.
 
 constexpr int kMaxKept = 1024;
+constexpr int kNarrow = 256;        // columns up to which a wave holds a row
+constexpr int kNarrowRows = 4;      // rows of such a workgroup
+
+__device__ __forceinline__ double wave_max(double v) {
+#pragma unroll
+    for (int m = 32; m > 0; m /= 2) v = max_na(v, __shfl_xor(v, m));
+    return v;
+}
+
+// exp(x / T) from x and c = kScale / T. f32: the hardware's power of two, whose argument's rounding is no worse than that of
+// the quotient itself.
+template <typename T> struct Exp;
+template <> struct Exp<float> {
+    static constexpr double kScale = 1.4426950408889634074;
+    __device__ static __forceinline__ float of(float x, float c) { return __builtin_amdgcn_exp2f(x * c); }
+};
+template <> struct Exp<double> {
+    static constexpr double kScale = 1.0;
+    __device__ static __forceinline__ double of(double x, double c) { return std::exp(x * c); }
+};
 
 // A row's kept entries as one wave sees them: the largest teacher logit, the log of the sum of exponentials, and whether there
 // is any entry.
@@ -349,6 +375,30 @@ template <typename T> struct Teacher {
                 sum += share == 0 ? 0 : share * (own - student);
             }
         return temperature * temperature * wave_sum(sum);
+    }
+};
+
+// A thread's running maximum and its sum of exp((z - largest) / T).
+template <typename T> struct Running {
+    T largest = -INFINITY;
+    double sum = 0;
+    template <int N> __device__ __forceinline__ void add(const T (&x)[N], T c) {
+        T most = largest;
+#pragma unroll
+        for (int i = 0; i < N; ++i) most = fmax(most, x[i]);
+        const T base = or_zero(most);  // nothing but -inf so far: every exponential is 0
+        if (most != largest) sum *= static_cast<double>(Exp<T>::of(largest - base, c));
+        largest = most;
+#pragma unroll
+        for (int i = 0; i < N; ++i) sum += static_cast<double>(Exp<T>::of(x[i] - base, c));
+    }
+    // the same over a wave
+    __device__ __forceinline__ void over_wave(T c) {
+        T most = largest;
+#pragma unroll
+        for (int m = 32; m > 0; m /= 2) most = fmax(most, __shfl_xor(most, m));
+        sum = wave_sum(sum * static_cast<double>(Exp<T>::of(largest - or_zero(most), c)));
+        largest = most;
     }
 };
 
@@ -551,6 +601,20 @@ int check_distill(const char* what, int dtype, int64_t rows, int64_t cols, int64
     if (!(temperature >= 1e-6 && temperature <= 1e6))
         return fail(KD_E_INVALID, name + ": temperature must be between 1e-6 and 1e6");
     return KD_OK;
+}
+
+// What goes past the caches, by the bytes of the logits: the 256 MiB of the last one hold small logits between the loss, its
+// gradient and the gradient's reader; larger ones only drive each other out. Loss and gradient together, f32 rows of 50257,
+// logits that were not in the caches, in us: nothing past them / loads past them in both / loads and stores past them in the
+// gradient alone:
+//   80 MB 52 / 56 / 57    110 MB 82 / 76 / 74    160 MB 125 / 102 / 107    230 MB 169 / 134 / 167
+//   300 MB 216 / 183 / 171    412 MB 284 / 272 / 242    800 MB 531 / 557 / 502
+struct PastCaches {
+    bool loss_loads, grad_loads, grad_stores;
+};
+PastCaches past_caches(int64_t bytes) {
+    const bool large = bytes > int64_t{96} << 20, huge = bytes > int64_t{256} << 20;
+    return {large && !huge, large, huge};
 }
 
 } // namespace

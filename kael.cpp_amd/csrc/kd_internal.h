@@ -35,6 +35,13 @@ hipStream_t stream();
 int device_ordinal();
 int compute_units();
 
+// Whether two pieces of memory have a byte in common.
+inline bool overlap(const void* a, int64_t a_bytes, const void* b, int64_t b_bytes) {
+    const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+    return a != nullptr && b != nullptr && a_bytes > 0 && b_bytes > 0 && x < y + static_cast<uint64_t>(b_bytes) &&
+           y < x + static_cast<uint64_t>(a_bytes);
+}
+
 // Whether a launch of `groups` workgroups in x is one: its work items are counted in 32 bits.
 inline bool fits_grid(int64_t groups, int64_t threads) { return groups < (int64_t{1} << 32) / threads; }
 
