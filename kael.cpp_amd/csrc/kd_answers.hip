@@ -132,7 +132,8 @@ __device__ __forceinline__ void policy_terms(const Policy<T>& a, int64_t row, do
 //
 // The log-probability of a row's target, and with `policy` the row's loss and gradient. A row is read once and held in the
 // registers of its team (a wave, or a workgroup): its largest logit, then the exponentials in the logits' places and their sum,
-// then the gradient from them. What a team's registers do not hold of a long row is read again, from the caches for the most part.
+// then the gradient from them. What a team's registers do not hold of a long row is read twice more, from the caches for the most
+// part: f32 600 x 151936 191 us (693 MB, 3.6 TB/s of what the call has to move), f64 600 x 50257 154 (458 MB, 3.0).
 // Bound by the logits read and the gradient written, f32: 2048 rows of 50257 162 us (782 MB at 4.8 TB/s, the rate of a copy;
 // vector ALU busy 0.26), 3333 x 6000 29 us; 4096 x 96 5.8 us, a launch and a chain of a target, its row, two sums and four f64 functions.
 // f64: 301 x 10007 12.2 us.

@@ -342,8 +342,9 @@ __global__ __launch_bounds__(Most == 64 ? 256 : Most) void block_rows_kernel(T* 
     }
 }
 
-// Any row length: a workgroup reads a row again in each pass, from the caches for the most part. 1500 x 20000 with both norms and
-// a gate 208 us (2.3 TB/s of what the call has to move), one row of 20000 24 us.
+// Any row length, and more rows than a launch of a workgroup for each can have: a workgroup reads a row again in each pass, from the
+// caches for the most part. 1500 x 20000 with both norms and a gate 208 to 220 us (2.2 to 2.3 TB/s of what the call has to move), one row
+// of 20000 24 us.
 constexpr int kWideThreads = 1024, kWideStep = 4 * kWideThreads;
 
 // How many values of a row of any length a wave of such a workgroup has.
@@ -448,7 +449,7 @@ __global__ __launch_bounds__(kWideThreads) void block_rows_wide_kernel(T* h, T* 
 // sums: rows of up to 4096. The parts' sums are 5 % more where each team has many rows, and a second kernel adds them in order, so that no
 // result depends on what runs first. f32: 8192 x 4096, both norms and a gate, 170 to 217 + 6 us (805 MB at 3.7 to 4.7 TB/s, vector ALU busy
 // 0.70); a layer norm alone 148 + 5; 32768 x 1024 160 + 5; 4096 x 256 10.5 + 3.8, where it is a chain of launch, loads and two
-// exchanges. 4096 x 8192 with all sums: the row's kernel 214, the sums' 102 us.
+// exchanges. With all sums the row's kernel and the sums' take 204 to 217 + 97 to 106 us for 4096 x 8192, 311 to 332 + 129 to 147 for 8192 x 5120.
 
 enum Sum { kAfterWeight, kAfterBias, kBeforeWeight, kBeforeBias, kGate, kSums };
 
@@ -630,7 +631,8 @@ __global__ __launch_bounds__(kThreads) void block_columns_kernel(T* parts, const
 }
 
 // A long row's gradients, by a workgroup that holds it: what the sums over rows would take of the registers is left to
-// block_columns_kernel, which reads the rows again (4096 x 8192: 165 + 80 us for a layer norm; in one kernel, which spilled, 421 to 480).
+// block_columns_kernel, which reads the rows again (4096 x 8192: 167 + 80 us for a layer norm; in one kernel, which spilled, 421 to 480).
+// Four quads a thread, rows past 8192, spill too: 24 to 34 of the 128 registers that 16 waves may have.
 template <typename T, int Quads, bool Whole, bool Past>
 __global__ __launch_bounds__(1024) void block_back_row_kernel(double* means, BackArgs<T> a) {
     __shared__ Pair room[2][kMostWaves];
@@ -1046,7 +1048,8 @@ int most_threads(int dtype) { return dtype == KD_F32 ? kBackThreads<float> : kBa
 int64_t sums_bytes(int dtype, int64_t cols, int64_t teams, int wanted) { return teams * wanted * ((cols + 3) / 4 * 4) * dtype_size(dtype); }
 BackPlan wide_plan(int64_t rows, int64_t cols) {
     // Workgroups of 256 columns, of 16 rows at least, and four for each CU at most, as many as it has at once: with one round more of a few
-    // of them 8192 x 5120 took 168 us instead of 113, 2000 x 20000 215 instead of 133.
+    // of them, a layer norm alone / both norms and a gate, 8192 x 5120 took 162 / 205 us instead of 106 / 138, 2000 x 20000 174 / 216
+    // instead of 112 / 138.
     const int64_t wanted = int64_t{4} * compute_units() / ((cols + 255) / 256);
     const int64_t segments = std::clamp<int64_t>(wanted, 1, (rows + 15) / 16);
     return {0, 0, 0, 0, segments, segments};
@@ -1330,8 +1333,8 @@ extern "C" int kd_block_rows_backward(int dtype, const kd_block_grads* grads, co
                     else one(block_back_row_kernel<T, kQuads, false, kPast>, kQuads);
                 };
                 // Gradients go past the caches where they and the inputs are more than the last one's 256 MiB: the sums' kernel finds
-                // more of its inputs there. Both kernels, us, through / past: f32, both norms and a gate, 4096 x 8192 332 / 325, a layer
-                // norm alone 254 / 244, 8192 x 5120 337 / 331; f64 2000 x 8192 366 / 352.
+                // more of its inputs there. Both kernels, us, through / past: both norms and a gate, f32 4096 x 8192 335 / 320, 8192 x 5120
+                // 480 / 470, f64 2000 x 8192 293 / 281; a layer norm alone, f32 4096 x 8192 258 / 247, 8192 x 5120 346 / 348.
                 const bool past = to != nullptr && 6 * b.rows * b.cols * static_cast<int64_t>(sizeof(T)) > int64_t{256} << 20;
                 const auto by_past = [&](auto quads) {
                     if (past) by_whole(quads, std::true_type{});
