@@ -364,8 +364,8 @@ __global__ __launch_bounds__(Threads) void answer_rows_kernel(AnswerRows<T> a) {
 // exponential's error grows with the distance from its base, so a confident target has to be that base, whose exponential is
 // exactly 1 (with the largest logit of a row's first round as the base of all, targets 12 to 39 above it were 4e-7 to 2e-6 off and above 0).
 // A round that holds a larger one moves the sum there first, in f64, whose rounding does not count beside f32's; that is seldom: a
-// wave's k-th round does so with a chance of 1 / k. 1433 rows of 50257 of 1908: 59 to 62 us (288 MB at 4.6 to 4.9 TB/s); held in
-// registers, one workgroup a CU, 69. f64: 500 x 50257 41 us (4.9 TB/s).
+// wave's k-th round does so with a chance of 1 / k. 1433 rows of 50257 of 1908: 61 to 66 us, by the machine (288 MB at 4.4 to 4.7 TB/s); held
+// in registers, one workgroup a CU, 69. f64: 500 x 50257 41 us (4.9 TB/s).
 template <typename T>
 __global__ __launch_bounds__(kMostThreads) void answer_forward_kernel(AnswerRows<T> a) {
     constexpr int kCount = Piece<T>::kCount, kPieces = 4;
